@@ -508,6 +508,104 @@ int32_t mhsa_encoder_fill(const mhsa_encoder* enc, int32_t* filled_out_host);
 int32_t mhsa_encoder_step(mhsa_encoder* enc, float* x_inout, const void* pos_emb, int32_t pos_len,
                           const mhsa_stream_mask* mask, const int32_t* valid_host, void* hip_stream);
 
+/* ---- 8-bit block-scaled projections and experts ---------------------------- */
+
+/* No counterpart in the reference (its quantized layers are affine).
+ *
+ * Format: OCP e4m3 codes (uint8) with a power of two for each block of 128:
+ * value = code * 2^(s - 127), s one byte. A weight [N, K] has one s for each
+ * 128 x 128 block, scales [ceil(N/128), ceil(K/128)]; activations are rounded
+ * in the call, one s for each row's 128 inputs. s is the smallest s >= 0 with
+ * max |v| <= 448 * 2^(s - 127) over the block's finite values (127 for a block
+ * of zeros), codes are rounded to nearest even, and an infinity or a NaN
+ * becomes a NaN.
+ *
+ * Weight handles are written by the load calls alone. Forward calls are const:
+ * their scratch memory is the caller's workspace (device, 16-byte aligned,
+ * no contents before or after), so calls on one handle may overlap on
+ * different streams or threads with a workspace each, and a call may be
+ * captured into a HIP graph, whose replays then need that workspace. Forward
+ * calls run on the GPU that was current at loading, which is to be current
+ * again, and on a stream of it. Loading waits for the GPU; no call that reads
+ * the handle may run at the same time. Weight pointers may be host or device
+ * memory. */
+
+/* y = W q(x) + b. */
+typedef struct mhsa_fp8_linear mhsa_fp8_linear;
+/* Any in_dim up to 32768 and any out_dim, up to 2 GiB of weights. */
+int32_t mhsa_fp8_linear_create(int32_t in_dim, int32_t out_dim, int32_t use_bias, mhsa_fp8_linear** out);
+void mhsa_fp8_linear_destroy(mhsa_fp8_linear* linear);
+/* weight [out_dim, in_dim] and bias [out_dim] (NULL without one) in data_dtype
+ * (MHSA_F32 / MHSA_BF16 / MHSA_F16), rounded to codes here. */
+int32_t mhsa_fp8_linear_load(mhsa_fp8_linear* linear, int32_t data_dtype, const void* weight, const void* bias);
+/* The weight as codes [out_dim, in_dim] and scales [ceil(out_dim/128),
+ * ceil(in_dim/128)]; a scale byte of 255 makes its block NaN. bias f32. */
+int32_t mhsa_fp8_linear_load_codes(mhsa_fp8_linear* linear, const uint8_t* codes, const uint8_t* scales,
+                                   const float* bias);
+/* The weight as held, in load_codes' layout (host or device memory). Waits for
+ * the GPU. */
+int32_t mhsa_fp8_linear_read_codes(const mhsa_fp8_linear* linear, uint8_t* codes, uint8_t* scales);
+/* Workspace bytes of a forward of `rows` rows (0 for few rows, -1 for bad
+ * arguments). */
+int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* linear, int32_t rows);
+/* x [rows, in_dim] in x_dtype and out [rows, out_dim] in out_dtype (MHSA_F32 or
+ * MHSA_BF16 each), device, rows x_stride and out_stride elements apart (>= the
+ * row); x, out and the workspace must not overlap. rows may be 0. Products of
+ * an f32 out are exact and summed in f32; for a bf16 out they go through the
+ * fp8 matrix unit, whose sums are off by some 1e-5 of the result (at most 9e-4 of
+ * their terms' magnitudes). A row's low bits may depend on the number of
+ * rows. */
+int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* linear, const void* x, int32_t x_dtype, int32_t rows,
+                                int64_t x_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
+                                int64_t workspace_bytes, void* hip_stream);
+
+/* Routing of frames to experts from the gate's logits [rows, n_experts]
+ * (MHSA_F32 or MHSA_BF16, device, rows `stride` elements apart):
+ *   s = softmax(logits) or sigmoid(logits); c = s + bias (bias [n_experts]
+ *   device f32 or NULL); of n_groups equal runs of experts, the topk_groups
+ *   with the largest sums of their two best c; in them the top_k experts by
+ *   c, best first; weights = scale * s, divided by the chosen s's sum when
+ *   renormalize.
+ * Scores are formed and compared in 64 bits; ties go to the lower index. An
+ * expert whose logit is -inf or NaN, or whose c is not above -inf, is not
+ * chosen: where fewer than top_k are left, the last indices are -1 and their
+ * weights 0 (a frame whose logits are all -inf chooses no expert).
+ * indices int32 and weights f32 [rows, top_k], device. n_experts <= 512,
+ * n_groups <= 64, top_k <= 32 and at most the experts of topk_groups groups.
+ * rows may be 0. */
+#define MHSA_ROUTE_SOFTMAX 0
+#define MHSA_ROUTE_SIGMOID 1
+int32_t mhsa_route(const void* logits, int32_t dtype, int32_t rows, int32_t n_experts, int64_t stride, int32_t score,
+                   const float* bias, int32_t n_groups, int32_t topk_groups, int32_t top_k, int32_t renormalize,
+                   float scale, int32_t* indices, float* weights, void* hip_stream);
+
+/* FeedForward by experts: out = residual + res_scale * sum_j weights[r, j] *
+ * FF_e(x_r), e = indices[r, j], FF_e(x) = W2_e q(silu(W1_e q(x) + b1_e)) + b2_e,
+ * W1 [n_experts, ff_dim, d_model], W2 [n_experts, d_model, ff_dim]; d_model and
+ * ff_dim multiples of 64 up to 32768, at most 1024 experts. An index outside
+ * [0, n_experts) adds nothing (mhsa_route's -1); an expert may come twice. */
+typedef struct mhsa_experts mhsa_experts;
+int32_t mhsa_experts_create(int32_t n_experts, int32_t d_model, int32_t ff_dim, int32_t use_bias, mhsa_experts** out);
+void mhsa_experts_destroy(mhsa_experts* experts);
+/* Weights and biases (b1 [n_experts, ff_dim], b2 [n_experts, d_model]; NULL
+ * without) as mhsa_fp8_linear_load and mhsa_fp8_linear_load_codes take them,
+ * the experts' matrices back to back. */
+int32_t mhsa_experts_load(mhsa_experts* experts, int32_t data_dtype, const void* weight1, const void* bias1,
+                          const void* weight2, const void* bias2);
+int32_t mhsa_experts_load_codes(mhsa_experts* experts, const uint8_t* codes1, const uint8_t* scales1,
+                                const float* bias1, const uint8_t* codes2, const uint8_t* scales2, const float* bias2);
+/* Workspace bytes of a forward (-1 for bad arguments). Rows run in parts of
+ * up to 2^18 frame and expert pairs, which bounds it. */
+int64_t mhsa_experts_workspace(const mhsa_experts* experts, int32_t rows, int32_t top_k);
+/* x, residual (or NULL) and out [rows, d_model] in dtype (MHSA_F32 or
+ * MHSA_BF16), indices int32 and weights f32 [rows, top_k], all device. out may
+ * be the residual (the block's half step), and must not overlap anything else.
+ * top_k <= 32; rows may be 0. Sums go through the fp8 matrix unit in either
+ * dtype. */
+int32_t mhsa_experts_forward(const mhsa_experts* experts, const void* x, int32_t dtype, int32_t rows,
+                             const int32_t* indices, const float* weights, int32_t top_k, const void* residual,
+                             float res_scale, void* out, void* workspace, int64_t workspace_bytes, void* hip_stream);
+
 /* ---- encoder-level streaming ---------------------------------------------- */
 
 /* The per-chunk layer loop of ConformerEncoder::forward_streaming

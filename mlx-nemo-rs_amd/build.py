@@ -27,7 +27,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmhsa_hip.so")
 SOURCES = ["gemm.hip", "attention.hip", "misc.hip", "mhsa_api.hip", "block_api.hip", "encoder_api.hip", "conv.hip",
-           "checkpoint.cpp"]
+           "fp8_gemm.hip", "experts.hip", "fp8_api.hip", "checkpoint.cpp"]
 ARCH = "gfx950"
 
 

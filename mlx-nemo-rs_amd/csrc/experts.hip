@@ -1,0 +1,311 @@
+// Routing of frames to experts, and the bookkeeping around the experts'
+// products (fp8_gemm.hip): pairs of frame and expert sorted by expert, and
+// the weighted sum of a frame's experts.
+#include <algorithm>
+
+#include "fp8_common.hpp"
+#include "fp8_kernels.hpp"
+
+namespace mhsa {
+namespace {
+
+// ---------------------------------------------------------------------------
+// Routing: s_e = softmax(x)_e or sigmoid(x_e); the choice score c_e = s_e +
+// bias_e; the groups with the largest sums of their two best c; in them the
+// top_k experts by c, ties to the lower index; w_j = s_e / sum of the chosen
+// s. Scores are formed and compared in 64 bits: two experts' scores often
+// differ by less than f32 resolves, and the choice between them is then not a
+// matter of the order of a sum.
+//
+// One wave per row, expert e in lane e % 64.
+// ---------------------------------------------------------------------------
+
+constexpr double kNone = -__builtin_inf();
+
+__device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor(v, o, 64); }
+
+// the better of two candidates in (v, i): larger value, then lower index
+__device__ __forceinline__ void better(double& v, int& i, double v2, int i2) {
+  if (v2 > v || (v2 == v && i2 < i)) {
+    v = v2;
+    i = i2;
+  }
+}
+
+template <typename T, int EPL>
+__global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
+  __shared__ double tab[4][EPL * 64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wv;
+  const bool live = row < p.rows;
+  const T* x = reinterpret_cast<const T*>(p.logits) + (live ? row : 0) * p.ld;
+  double s[EPL], c[EPL];
+  double mx = kNone;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int e = lane + 64 * i;
+    const double v = e < p.experts ? (double)(float)x[e] : kNone;
+    c[i] = v > kNone ? v : kNone;  // (a NaN is no score)
+    mx = c[i] > mx ? c[i] : mx;
+  }
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) s[i] = c[i] > kNone ? 1.0 / (1.0 + exp(-c[i])) : 0.0;
+  } else {
+    for (int o = 32; o > 0; o >>= 1) {
+      const double t = shfl_xor_d(mx, o);
+      mx = t > mx ? t : mx;
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      s[i] = c[i] > kNone ? (c[i] == mx ? 1.0 : exp(c[i] - mx)) : 0.0;
+      sum += s[i];
+    }
+    for (int o = 32; o > 0; o >>= 1) sum += shfl_xor_d(sum, o);
+    if (sum > 0.0) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) s[i] /= sum;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int e = lane + 64 * i;
+    const double v = p.bias && e < p.experts ? s[i] + (double)p.bias[e] : s[i];
+    c[i] = c[i] > kNone && v > kNone ? v : kNone;
+  }
+  if (p.groups > 1) {
+    const int size = p.experts / p.groups;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) tab[wv][lane + 64 * i] = c[i];
+    __syncthreads();
+    double best = kNone;
+    if (lane < p.groups) {
+      double a = kNone, b = kNone;  // the two largest
+      for (int e = 0; e < size; ++e) {
+        const double v = tab[wv][lane * size + e];
+        if (v > a) {
+          b = a;
+          a = v;
+        } else if (v > b) {
+          b = v;
+        }
+      }
+      best = b > kNone ? a + b : a;
+    }
+    int before = 0;  // groups ahead of this lane's
+    for (int g = 0; g < p.groups; ++g) {
+      const double v = __shfl(best, g, 64);
+      before += v > best || (v == best && g < lane) ? 1 : 0;
+    }
+    const uint64_t kept = __ballot(lane < p.groups && before < p.topk_groups);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int g = (lane + 64 * i) / size;
+      if (g >= p.groups || !(kept >> g & 1)) c[i] = kNone;
+    }
+  }
+  int idx = -1;
+  double wj = 0.0, total = 0.0;
+  for (int j = 0; j < p.top_k; ++j) {
+    double v = kNone;
+    int at = 1 << 30;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (c[i] > kNone) better(v, at, c[i], lane + 64 * i);
+    for (int o = 32; o > 0; o >>= 1) better(v, at, shfl_xor_d(v, o), __shfl_xor(at, o, 64));
+    if (!(v > kNone)) break;
+    double mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (lane + 64 * i == at) {
+        mine = s[i];
+        c[i] = kNone;
+      }
+    const double sj = __shfl(mine, at & 63, 64);
+    total += sj;
+    if (lane == j) {
+      idx = at;
+      wj = sj;
+    }
+  }
+  if (p.renormalize) wj = total > 0.0 ? wj / total : 0.0;
+  if (live && lane < p.top_k) {
+    p.idx[row * p.top_k + lane] = idx;
+    p.w[row * p.top_k + lane] = (float)(wj * (double)p.scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Pairs by expert
+// ---------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024, kPlanPer = 16, kPlanChunk = kPlanThreads * kPlanPer;
+constexpr int kPlanExperts = 1024;
+
+// Counts of one chunk of pairs per expert.
+__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int* idx, int pairs, int experts, int* hist) {
+  __shared__ int cnt[kPlanExperts];
+  cnt[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int p = blockIdx.x * kPlanChunk + i * kPlanThreads + threadIdx.x;
+    const int e = p < pairs ? idx[p] : -1;
+    if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < experts) hist[blockIdx.x * experts + threadIdx.x] = cnt[threadIdx.x];
+}
+
+// Slots of one chunk's pairs (hist null: there is one chunk, counted here) and
+// the tile list. The order of an expert's pairs among its slots is that of
+// the atomics and may change from call to call: no result depends on it, as a
+// slot's row is computed from that row alone.
+__global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* idx, int pairs, int experts,
+                                                                    int tile_rows, const int* hist, int* pair,
+                                                                    int* tile, int* n_tiles) {
+  __shared__ int cursor[kPlanExperts], slots[2][kPlanExperts], tiles[2][kPlanExperts];
+  const int t = threadIdx.x;
+  int mine[kPlanPer];
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int p = blockIdx.x * kPlanChunk + i * kPlanThreads + t;
+    mine[i] = p < pairs ? idx[p] : -1;
+    if (mine[i] >= experts) mine[i] = -1;
+  }
+  int total = 0, before = 0;
+  if (hist) {
+    if (t < experts)
+      for (int c = 0; c < (int)gridDim.x; ++c) {
+        const int h = hist[c * experts + t];
+        total += h;
+        before += c < (int)blockIdx.x ? h : 0;
+      }
+  } else {
+    cursor[t] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i)
+      if (mine[i] >= 0) atomicAdd(&cursor[mine[i]], 1);
+    __syncthreads();
+    total = cursor[t];
+  }
+  const int nt = (total + tile_rows - 1) / tile_rows;
+  slots[0][t] = total;
+  tiles[0][t] = nt;
+  __syncthreads();
+  int cur = 0;
+  for (int o = 1; o < kPlanThreads; o *= 2, cur ^= 1) {  // inclusive sums
+    slots[cur ^ 1][t] = slots[cur][t] + (t >= o ? slots[cur][t - o] : 0);
+    tiles[cur ^ 1][t] = tiles[cur][t] + (t >= o ? tiles[cur][t - o] : 0);
+    __syncthreads();
+  }
+  const int slot0 = slots[cur][t] - total, tile0 = tiles[cur][t] - nt;
+  cursor[t] = slot0 + before;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i)
+    if (mine[i] >= 0) pair[atomicAdd(&cursor[mine[i]], 1)] = blockIdx.x * kPlanChunk + i * kPlanThreads + t;
+  if (blockIdx.x == 0) {
+    if (t == kPlanThreads - 1) *n_tiles = tiles[cur][t];
+    for (int i = 0; i < nt; ++i) {
+      int* e = tile + 4 * (tile0 + i);
+      e[0] = t;
+      e[1] = slot0 + i * tile_rows;
+      e[2] = min(tile_rows, total - i * tile_rows);
+      e[3] = 0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The experts' weighted sum, 8 columns to a thread, in the order of the
+// choices.
+// ---------------------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const float* y, const int* idx, const float* w, int64_t rows,
+                                                      int top_k, int experts, int D, const T* residual,
+                                                      float res_scale, T* out) {
+  const int per = D / 8;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= rows * per) return;
+  const int64_t row = id / per;
+  const int col = (int)(id % per) * 8;
+  float f[8] = {};
+  for (int j = 0; j < top_k; ++j) {
+    const int e = idx[row * top_k + j];
+    if (e < 0 || e >= experts) continue;
+    const float wj = w[row * top_k + j];
+    const floatx4* src = reinterpret_cast<const floatx4*>(y + (row * top_k + j) * D + col);
+    const floatx4 a = src[0], b = src[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = __builtin_fmaf(wj, a[i], f[i]);
+      f[i + 4] = __builtin_fmaf(wj, b[i], f[i + 4]);
+    }
+  }
+  T v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] *= res_scale;
+  if (residual) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      reinterpret_cast<u32x4*>(v)[i] = reinterpret_cast<const u32x4*>(residual + row * D + col)[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] += (float)v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (T)f[i];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    reinterpret_cast<u32x4*>(out + row * D + col)[i] = reinterpret_cast<const u32x4*>(v)[i];
+}
+
+}  // namespace
+
+hipError_t route(const RouteParams& p, hipStream_t s) {
+  if (p.rows <= 0 || p.experts <= 0 || p.experts > kRouteMaxExperts || p.top_k <= 0 || p.top_k > kRouteMaxK ||
+      p.top_k > p.experts || p.groups <= 0 || p.groups > kRouteMaxGroups || p.experts % p.groups ||
+      p.topk_groups <= 0 || p.topk_groups > p.groups)
+    return hipErrorInvalidValue;
+  const int64_t grid = (p.rows + 3) / 4;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (p.experts <= 64) route_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
+    else if (p.experts <= 128) route_kernel<T, 2><<<(unsigned)grid, 256, 0, s>>>(p);
+    else if (p.experts <= 256) route_kernel<T, 4><<<(unsigned)grid, 256, 0, s>>>(p);
+    else route_kernel<T, 8><<<(unsigned)grid, 256, 0, s>>>(p);
+  };
+  if (p.dt == kBF16) go(bf16{});
+  else go(float{});
+  return hipGetLastError();
+}
+
+int64_t plan_scratch_ints(int64_t pairs, int experts) { return (pairs + kPlanChunk - 1) / kPlanChunk * experts; }
+
+hipError_t experts_plan(const int* idx, int pairs, int experts, int tile_rows, int* pair, int* tile, int* n_tiles,
+                        int* scratch, hipStream_t s) {
+  if (pairs <= 0 || experts <= 0 || experts > kPlanExperts || tile_rows <= 0) return hipErrorInvalidValue;
+  const int chunks = (pairs + kPlanChunk - 1) / kPlanChunk;
+  if (chunks > 1) plan_count_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, experts, scratch);
+  plan_scatter_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, experts, tile_rows, chunks > 1 ? scratch : nullptr,
+                                                      pair, tile, n_tiles);
+  return hipGetLastError();
+}
+
+hipError_t experts_combine(DType dt, const float* y, const int* idx, const float* w, int64_t rows, int top_k,
+                           int experts, int D, const void* residual, float res_scale, void* out, hipStream_t s) {
+  const int64_t grid = (rows * (D / 8) + 255) / 256;
+  if (rows <= 0 || D <= 0 || D % 8 || grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (dt == kBF16)
+    combine_kernel<bf16><<<(unsigned)grid, 256, 0, s>>>(y, idx, w, rows, top_k, experts, D,
+                                                        static_cast<const bf16*>(residual), res_scale, static_cast<bf16*>(out));
+  else
+    combine_kernel<float><<<(unsigned)grid, 256, 0, s>>>(y, idx, w, rows, top_k, experts, D,
+                                                         static_cast<const float*>(residual), res_scale, static_cast<float*>(out));
+  return hipGetLastError();
+}
+
+}  // namespace mhsa

@@ -1,0 +1,551 @@
+// C ABI of the 8-bit block-scaled projection, the routing of frames to
+// experts and the experts' FeedForward. The handles hold weights alone, laid
+// out once at loading; a forward call takes its scratch memory from the
+// caller, so calls on one handle may run at once on different streams, and
+// captured graphs share nothing.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "fp8_kernels.hpp"
+#include "host_common.hpp"
+#include "kernels.hpp"
+
+using mhsa::DType;
+
+namespace {
+
+// n weight matrices [N, K] in the kernels' format.
+struct Fp8Weights {
+  int n = 0, N = 0, K = 0;
+  bool use_bias = false, loaded = false;
+  DevBuf codes, scales, bias;
+  int64_t stride() const { return (int64_t)N * mhsa::fp8_kp(K); }
+  int64_t scale_stride() const { return (int64_t)((N + 127) / 128) * mhsa::fp8_kbp(K); }
+  int64_t scale_in() const { return (int64_t)((N + 127) / 128) * ((K + 127) / 128); }
+};
+
+// Whether p is memory of the current GPU (true) or host memory (false).
+int32_t on_device(const void* p, bool* yes) {
+  hipPointerAttribute_t a{};
+  *yes = false;
+  if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+    (void)hipGetLastError();  // memory that HIP does not know: the host's
+    return MHSA_OK;
+  }
+  if (a.type != hipMemoryTypeDevice) return MHSA_OK;
+  int dev = 0;
+  HIPCHK(hipGetDevice(&dev));
+  if (a.device != dev) return fail(MHSA_EINVAL, "the tensor is on GPU %d, the current GPU is %d", a.device, dev);
+  *yes = true;
+  return MHSA_OK;
+}
+
+int32_t load_bias(Fp8Weights& w, int data_dtype, const void* bias) {
+  if (!w.use_bias) return MHSA_OK;
+  const size_t n = (size_t)w.n * w.N, es = data_dtype == MHSA_F32 ? 4 : 2;
+  std::vector<char> raw(n * es);
+  std::vector<float> f(n);
+  HIPCHK(hipMemcpy(raw.data(), bias, raw.size(), hipMemcpyDefault));
+  for (size_t i = 0; i < n; ++i) f[i] = load_host(data_dtype, raw.data(), i);
+  HIPCHK(w.bias.ensure(n * 4));
+  HIPCHK(hipMemcpy(w.bias.p, f.data(), n * 4, hipMemcpyHostToDevice));
+  return MHSA_OK;
+}
+
+// From floats (codes null) or from codes and scale bytes; host or device
+// memory. Everything queued on the GPU comes first: a forward may still read
+// the old weights, and device tensors may still be being written.
+int32_t load_weights(Fp8Weights& w, int data_dtype, const void* weight, const uint8_t* codes, const uint8_t* scales,
+                     const void* bias) {
+  if (codes ? !scales : !weight) return fail(MHSA_EINVAL, "null weight pointer");
+  if (w.use_bias != (bias != nullptr))
+    return fail(MHSA_EINVAL, w.use_bias ? "a bias is expected" : "the layer was created without a bias");
+  if (!codes && !float_dtype(data_dtype)) return fail(MHSA_ENOTSUP, "weight dtype %d not supported (f32, bf16, f16)", data_dtype);
+  bool dev = false, sdev = false;
+  if (int32_t rc = on_device(codes ? codes : weight, &dev)) return rc;
+  if (codes)
+    if (int32_t rc = on_device(scales, &sdev)) return rc;
+  if (codes && dev != sdev) return fail(MHSA_EINVAL, "codes and scales are to be both on the host or both on the GPU");
+  HIPCHK(hipDeviceSynchronize());
+  w.loaded = false;
+  HIPCHK(w.codes.ensure(w.n * w.stride()));
+  HIPCHK(w.scales.ensure(w.n * w.scale_stride()));
+  const int64_t es = codes ? 1 : data_dtype == MHSA_F32 ? 4 : 2, mat = (int64_t)w.N * w.K * es;
+  uint8_t* dc = static_cast<uint8_t*>(w.codes.p);
+  uint8_t* ds = static_cast<uint8_t*>(w.scales.p);
+  const uint8_t* src = codes ? codes : static_cast<const uint8_t*>(weight);
+  DevBuf stage, sstage;
+  if (!dev) {
+    HIPCHK(stage.ensure(mat));
+    if (codes) HIPCHK(sstage.ensure(w.scale_in()));
+  }
+  // device tensors: as many matrices to a launch as its grid takes; host ones
+  // one by one through the staging buffer
+  const int step = dev ? 1024 : 1;
+  for (int i = 0; i < w.n; i += step) {
+    const int m = std::min(step, w.n - i);
+    const uint8_t* from = src + i * mat;
+    const uint8_t* sfrom = codes ? scales + i * w.scale_in() : nullptr;
+    if (!dev) {
+      HIPCHK(hipMemcpy(stage.p, from, mat, hipMemcpyHostToDevice));
+      from = static_cast<const uint8_t*>(stage.p);
+      if (codes) {
+        HIPCHK(hipMemcpy(sstage.p, sfrom, w.scale_in(), hipMemcpyHostToDevice));
+        sfrom = static_cast<const uint8_t*>(sstage.p);
+      }
+    }
+    if (codes)
+      HIPCHK(mhsa::fp8_pad_weight(from, sfrom, m, w.N, w.K, dc + i * w.stride(), ds + i * w.scale_stride(), nullptr));
+    else
+      HIPCHK(mhsa::fp8_quantize_weight(data_dtype, from, m, w.N, w.K, dc + i * w.stride(), ds + i * w.scale_stride(), nullptr));
+    HIPCHK(hipStreamSynchronize(nullptr));
+  }
+  if (int32_t rc = load_bias(w, codes ? MHSA_F32 : data_dtype, bias)) return rc;
+  w.loaded = true;
+  return MHSA_OK;
+}
+
+// Weights are where they were loaded.
+int32_t check_device(int device) {
+  int dev = 0;
+  HIPCHK(hipGetDevice(&dev));
+  if (dev != device) return fail(MHSA_EINVAL, "the weights are on GPU %d, the current GPU is %d", device, dev);
+  return MHSA_OK;
+}
+
+bool act_dtype(int32_t d, DType* out) {
+  *out = d == MHSA_BF16 ? mhsa::kBF16 : mhsa::kF32;
+  return d == MHSA_F32 || d == MHSA_BF16;
+}
+
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+// Hands out 256-byte aligned pieces of a workspace (or only adds them up).
+struct Arena {
+  char* base;
+  int64_t used = 0;
+  explicit Arena(void* p) : base(static_cast<char*>(p)) {}
+  template <typename T> T* take(int64_t n) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used = align_up(used + n * (int64_t)sizeof(T), 256);
+    return p;
+  }
+};
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// The projection
+// ---------------------------------------------------------------------------
+
+struct mhsa_fp8_linear {
+  Fp8Weights w;
+  int device = -1;
+};
+
+namespace {
+
+struct LinearPlan {
+  bool few = false;
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
+  int64_t bytes = 0;
+};
+
+LinearPlan linear_plan(const Fp8Weights& w, int64_t rows, void* ws) {
+  LinearPlan p;
+  p.few = mhsa::fp8_few_rows(rows, w.N, w.K);
+  if (p.few) return p;
+  Arena a(ws);
+  p.codes = a.take<uint8_t>(rows * mhsa::fp8_kp(w.K));
+  p.scales = a.take<uint8_t>(rows * mhsa::fp8_kbp(w.K));
+  p.bytes = a.used;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t mhsa_fp8_linear_create(int32_t in_dim, int32_t out_dim, int32_t use_bias, mhsa_fp8_linear** out) {
+  if (!out) return fail(MHSA_EINVAL, "null output pointer");
+  *out = nullptr;
+  if (in_dim <= 0 || out_dim <= 0) return fail(MHSA_EINVAL, "in_dim %d and out_dim %d must be positive", in_dim, out_dim);
+  if (in_dim > mhsa::kFp8MaxK) return fail(MHSA_ENOTSUP, "in_dim %d exceeds %d", in_dim, mhsa::kFp8MaxK);
+  if ((int64_t)out_dim * mhsa::fp8_kp(in_dim) > INT32_MAX)
+    return fail(MHSA_ENOTSUP, "a weight of %d x %d exceeds 2 GiB", out_dim, in_dim);
+  mhsa_fp8_linear* h = new (std::nothrow) mhsa_fp8_linear();
+  if (!h) return fail(MHSA_ENOMEM, "out of host memory");
+  h->w.n = 1;
+  h->w.N = out_dim;
+  h->w.K = in_dim;
+  h->w.use_bias = use_bias != 0;
+  *out = h;
+  return MHSA_OK;
+}
+
+void mhsa_fp8_linear_destroy(mhsa_fp8_linear* h) { delete h; }
+
+int32_t mhsa_fp8_linear_load(mhsa_fp8_linear* h, int32_t data_dtype, const void* weight, const void* bias) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  if (int32_t rc = load_weights(h->w, data_dtype, weight, nullptr, nullptr, bias)) return rc;
+  HIPCHK(hipGetDevice(&h->device));
+  return MHSA_OK;
+}
+
+int32_t mhsa_fp8_linear_load_codes(mhsa_fp8_linear* h, const uint8_t* codes, const uint8_t* scales, const float* bias) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  if (!codes) return fail(MHSA_EINVAL, "null weight pointer");
+  if (int32_t rc = load_weights(h->w, MHSA_F32, nullptr, codes, scales, bias)) return rc;
+  HIPCHK(hipGetDevice(&h->device));
+  return MHSA_OK;
+}
+
+int32_t mhsa_fp8_linear_read_codes(const mhsa_fp8_linear* h, uint8_t* codes, uint8_t* scales) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  if (!codes || !scales) return fail(MHSA_EINVAL, "null output pointer");
+  if (!h->w.loaded) return fail(MHSA_EINVAL, "no weights are loaded");
+  if (int32_t rc = check_device(h->device)) return rc;
+  DevBuf c, s;
+  const int64_t n = (int64_t)h->w.N * h->w.K;
+  HIPCHK(c.ensure(n));
+  HIPCHK(s.ensure(h->w.scale_in()));
+  HIPCHK(mhsa::fp8_unpad_weight(static_cast<const uint8_t*>(h->w.codes.p), static_cast<const uint8_t*>(h->w.scales.p),
+                                h->w.N, h->w.K, static_cast<uint8_t*>(c.p), static_cast<uint8_t*>(s.p), nullptr));
+  HIPCHK(hipStreamSynchronize(nullptr));
+  HIPCHK(hipMemcpy(codes, c.p, n, hipMemcpyDefault));
+  HIPCHK(hipMemcpy(scales, s.p, h->w.scale_in(), hipMemcpyDefault));
+  return MHSA_OK;
+}
+
+int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* h, int32_t rows) {
+  if (!h || rows < 0) return -1;
+  return rows == 0 ? 0 : linear_plan(h->w, rows, nullptr).bytes;
+}
+
+int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t x_dtype, int32_t rows,
+                                int64_t x_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
+                                int64_t workspace_bytes, void* hs) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  const Fp8Weights& w = h->w;
+  DType xd, od;
+  if (!act_dtype(x_dtype, &xd) || !act_dtype(out_dtype, &od))
+    return fail(MHSA_ENOTSUP, "dtypes %d and %d not supported (f32, bf16)", x_dtype, out_dtype);
+  if (rows < 0) return fail(MHSA_EINVAL, "rows must not be negative (got %d)", rows);
+  if (rows == 0) return MHSA_OK;
+  if (!x || !out) return fail(MHSA_EINVAL, "null tensor pointer");
+  const int xs = mhsa::dtype_size(xd), os = mhsa::dtype_size(od);
+  if (reinterpret_cast<uintptr_t>(x) % xs || reinterpret_cast<uintptr_t>(out) % os)
+    return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
+  if (x_stride < w.K || out_stride < w.N)
+    return fail(MHSA_EINVAL, "row strides %lld and %lld are shorter than the rows (%d, %d)", (long long)x_stride,
+                (long long)out_stride, w.K, w.N);
+  if (x_stride > (int64_t)1 << 40 || out_stride > (int64_t)1 << 40) return fail(MHSA_EINVAL, "row strides exceed 2^40");
+  if (!w.loaded) return fail(MHSA_EINVAL, "no weights are loaded");
+  const LinearPlan plan = linear_plan(w, rows, workspace);
+  if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes))
+    return fail(MHSA_EINVAL, "%d rows need a 16-byte aligned workspace of %lld bytes", rows, (long long)plan.bytes);
+  const int64_t xn = ((rows - 1) * x_stride + w.K) * xs, on = ((rows - 1) * out_stride + w.N) * os;
+  if (overlap(x, xn, out, on) || overlap(workspace, plan.bytes, x, xn) || overlap(workspace, plan.bytes, out, on))
+    return fail(MHSA_EINVAL, "x, out and the workspace must not overlap");
+  if (int32_t rc = check_device(h->device)) return rc;
+  hipStream_t s = static_cast<hipStream_t>(hs);
+  mhsa::Fp8Gemm p;
+  p.w = static_cast<const uint8_t*>(w.codes.p);
+  p.ws = static_cast<const uint8_t*>(w.scales.p);
+  p.bias = w.use_bias ? static_cast<const float*>(w.bias.p) : nullptr;
+  p.M = rows;
+  p.N = w.N;
+  p.K = w.K;
+  p.out = out;
+  p.out_dt = od;
+  p.ldo = out_stride;
+  if (plan.few) {
+    p.x = x;
+    p.x_dt = xd;
+    p.ldx = x_stride;
+    HIPCHK(mhsa::fp8_gemm_few(p, s));
+    return MHSA_OK;
+  }
+  HIPCHK(mhsa::fp8_quantize_rows(xd, x, x_stride, rows, w.K, plan.codes, plan.scales, s));
+  p.a = plan.codes;
+  p.as = plan.scales;
+  p.a_rows = rows;
+  HIPCHK(mhsa::fp8_gemm_tile(p, s));
+  return MHSA_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Routing
+// ---------------------------------------------------------------------------
+
+extern "C" int32_t mhsa_route(const void* logits, int32_t dtype, int32_t rows, int32_t n_experts, int64_t stride,
+                              int32_t score, const float* bias, int32_t n_groups, int32_t topk_groups, int32_t top_k,
+                              int32_t renormalize, float scale, int32_t* indices, float* weights, void* hs) {
+  mhsa::RouteParams p;
+  if (!act_dtype(dtype, &p.dt)) return fail(MHSA_ENOTSUP, "dtype %d not supported (f32, bf16)", dtype);
+  if (score != MHSA_ROUTE_SOFTMAX && score != MHSA_ROUTE_SIGMOID)
+    return fail(MHSA_ENOTSUP, "score %d not supported (softmax, sigmoid)", score);
+  if (rows < 0 || n_experts <= 0) return fail(MHSA_EINVAL, "bad shape: %d rows, %d experts", rows, n_experts);
+  if (n_experts > mhsa::kRouteMaxExperts) return fail(MHSA_ENOTSUP, "%d experts exceed %d", n_experts, mhsa::kRouteMaxExperts);
+  if (n_groups <= 0 || n_experts % n_groups)
+    return fail(MHSA_EINVAL, "%d experts do not divide into %d groups", n_experts, n_groups);
+  if (n_groups > mhsa::kRouteMaxGroups) return fail(MHSA_ENOTSUP, "%d groups exceed %d", n_groups, mhsa::kRouteMaxGroups);
+  if (topk_groups <= 0 || topk_groups > n_groups)
+    return fail(MHSA_EINVAL, "topk_groups %d is not in [1, %d]", topk_groups, n_groups);
+  if (top_k <= 0 || top_k > topk_groups * (n_experts / n_groups))
+    return fail(MHSA_EINVAL, "top_k %d is not in [1, %d], the experts of %d groups", top_k,
+                topk_groups * (n_experts / n_groups), topk_groups);
+  if (top_k > mhsa::kRouteMaxK) return fail(MHSA_ENOTSUP, "top_k %d exceeds %d", top_k, mhsa::kRouteMaxK);
+  if (stride < n_experts) return fail(MHSA_EINVAL, "row stride %lld is shorter than a row", (long long)stride);
+  if (!std::isfinite(scale)) return fail(MHSA_EINVAL, "scale must be finite");
+  if (rows == 0) return MHSA_OK;
+  if (!logits || !indices || !weights) return fail(MHSA_EINVAL, "null tensor pointer");
+  if (reinterpret_cast<uintptr_t>(logits) % mhsa::dtype_size(p.dt) || reinterpret_cast<uintptr_t>(indices) % 4 ||
+      reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(bias) % 4)
+    return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
+  p.logits = logits;
+  p.ld = stride;
+  p.rows = rows;
+  p.experts = n_experts;
+  p.top_k = top_k;
+  p.sigmoid = score == MHSA_ROUTE_SIGMOID;
+  p.groups = n_groups;
+  p.topk_groups = topk_groups;
+  p.renormalize = renormalize != 0;
+  p.scale = scale;
+  p.bias = bias;
+  p.idx = indices;
+  p.w = weights;
+  HIPCHK(mhsa::route(p, static_cast<hipStream_t>(hs)));
+  return MHSA_OK;
+}
+
+// ---------------------------------------------------------------------------
+// The experts' FeedForward
+// ---------------------------------------------------------------------------
+
+struct mhsa_experts {
+  Fp8Weights lin[2];  // linear1 [E, F, D], linear2 [E, D, F]
+  int E = 0, D = 0, F = 0;
+  int device = -1;
+};
+
+namespace {
+
+constexpr int kMaxExperts = 1024, kMaxTopK = 32;
+constexpr int kFewPairs = 64;  // up to these no list of pairs is built
+constexpr int64_t kMaxPairs = 1 << 18;
+
+// How a call runs, and its pieces of the workspace. Rows go in runs of
+// `step`, each through the same buffers, which bounds them.
+struct ExpertsPlan {
+  int64_t step = 0;
+  int tile_rows = 0;  // 0: no list; 16: few-row kernel; else tiles
+  int max_tiles = 0;
+  int *pair = nullptr, *tile = nullptr, *n_tiles = nullptr, *scratch = nullptr;
+  uint8_t *xc = nullptr, *xs = nullptr, *hc = nullptr, *hsc = nullptr;
+  float *h = nullptr, *y = nullptr;
+  int64_t bytes = 0;
+};
+
+ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void* ws) {
+  ExpertsPlan p;
+  const int64_t dp = mhsa::fp8_kp(e->D), fp = mhsa::fp8_kp(e->F);
+  const int64_t most = std::min({kMaxPairs / top_k, INT32_MAX / (fp * top_k), INT32_MAX / dp});
+  p.step = std::min(rows, most);
+  const int64_t pairs = p.step * top_k;
+  Arena a(ws);
+  if (rows * top_k > kFewPairs) {
+    p.tile_rows = mhsa::fp8_group_rows(pairs, e->E);
+    p.max_tiles = (int)(pairs / p.tile_rows + std::min<int64_t>(pairs, e->E));
+    p.pair = a.take<int>(pairs);
+    p.tile = a.take<int>(4 * (int64_t)p.max_tiles);
+    p.n_tiles = a.take<int>(1);
+    p.scratch = a.take<int>(mhsa::plan_scratch_ints(pairs, e->E));
+  }
+  if (p.tile_rows > 16) {
+    p.xc = a.take<uint8_t>(p.step * dp);
+    p.xs = a.take<uint8_t>(p.step * mhsa::fp8_kbp(e->D));
+    p.hc = a.take<uint8_t>(pairs * fp);
+    p.hsc = a.take<uint8_t>(pairs * mhsa::fp8_kbp(e->F));
+  } else {
+    p.h = a.take<float>(pairs * e->F);
+  }
+  p.y = a.take<float>(pairs * e->D);
+  p.bytes = a.used;
+  return p;
+}
+
+int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* x, DType dt, int64_t rows,
+                    const int32_t* idx, const float* weights, int top_k, const void* residual, float res_scale,
+                    void* out, hipStream_t s) {
+  const int pairs = (int)(rows * top_k);
+  mhsa::Fp8Gemm g[2];
+  for (int i = 0; i < 2; ++i) {
+    const Fp8Weights& w = e->lin[i];
+    g[i].w = static_cast<const uint8_t*>(w.codes.p);
+    g[i].ws = static_cast<const uint8_t*>(w.scales.p);
+    g[i].w_stride = w.stride();
+    g[i].ws_stride = w.scale_stride();
+    g[i].bias = w.use_bias ? static_cast<const float*>(w.bias.p) : nullptr;
+    g[i].N = w.N;
+    g[i].K = w.K;
+    g[i].M = pairs;
+    g[i].ldo = w.N;
+    g[i].g.top_k = top_k;
+    g[i].g.experts = e->E;
+    g[i].g.pairs = pairs;
+    if (plan.tile_rows) {
+      g[i].g.tile = plan.tile;
+      g[i].g.n_tiles = plan.n_tiles;
+      g[i].g.max_tiles = (int)(pairs / plan.tile_rows + std::min(pairs, e->E));
+      g[i].g.tile_rows = plan.tile_rows;
+      g[i].g.pair = plan.pair;
+    } else {
+      g[i].g.idx = idx;
+    }
+  }
+  g[1].epilogue = mhsa::kFp8Pair;
+  g[1].out = plan.y;
+  if (plan.tile_rows)
+    HIPCHK(mhsa::experts_plan(idx, pairs, e->E, plan.tile_rows, plan.pair, plan.tile, plan.n_tiles, plan.scratch, s));
+  if (plan.tile_rows > 16) {
+    HIPCHK(mhsa::fp8_quantize_rows(dt, x, e->D, rows, e->D, plan.xc, plan.xs, s));
+    g[0].a = plan.xc;
+    g[0].as = plan.xs;
+    g[0].a_rows = rows;
+    g[0].rows = mhsa::Fp8Gemm::kByFrame;
+    g[0].epilogue = mhsa::kFp8HiddenQ;
+    g[0].out_codes = plan.hc;
+    g[0].out_scales = plan.hsc;
+    HIPCHK(mhsa::fp8_gemm_tile(g[0], s));
+    g[1].a = plan.hc;
+    g[1].as = plan.hsc;
+    g[1].a_rows = pairs;
+    HIPCHK(mhsa::fp8_gemm_tile(g[1], s));
+  } else {
+    g[0].x = x;
+    g[0].x_dt = dt;
+    g[0].ldx = e->D;
+    g[0].rows = mhsa::Fp8Gemm::kByFrame;
+    g[0].epilogue = mhsa::kFp8HiddenF32;
+    g[0].out = plan.h;
+    HIPCHK(mhsa::fp8_gemm_few(g[0], s));
+    g[1].x = plan.h;
+    g[1].x_dt = mhsa::kF32;
+    g[1].ldx = e->F;
+    g[1].rows = mhsa::Fp8Gemm::kByPair;
+    HIPCHK(mhsa::fp8_gemm_few(g[1], s));
+  }
+  HIPCHK(mhsa::experts_combine(dt, plan.y, idx, weights, rows, top_k, e->E, e->D, residual, res_scale, out, s));
+  return MHSA_OK;
+}
+
+int32_t experts_loaded(mhsa_experts* h) {
+  HIPCHK(hipGetDevice(&h->device));
+  return MHSA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t mhsa_experts_create(int32_t n_experts, int32_t d_model, int32_t ff_dim, int32_t use_bias, mhsa_experts** out) {
+  if (!out) return fail(MHSA_EINVAL, "null output pointer");
+  *out = nullptr;
+  if (n_experts <= 0 || d_model <= 0 || ff_dim <= 0 || d_model % 64 || ff_dim % 64)
+    return fail(MHSA_EINVAL, "n_experts %d must be positive, d_model %d and ff_dim %d positive multiples of 64", n_experts,
+                d_model, ff_dim);
+  if (n_experts > kMaxExperts || d_model > mhsa::kFp8MaxK || ff_dim > mhsa::kFp8MaxK)
+    return fail(MHSA_ENOTSUP, "n_experts %d, d_model %d, ff_dim %d exceed %d, %d, %d", n_experts, d_model, ff_dim,
+                kMaxExperts, mhsa::kFp8MaxK, mhsa::kFp8MaxK);
+  mhsa_experts* h = new (std::nothrow) mhsa_experts();
+  if (!h) return fail(MHSA_ENOMEM, "out of host memory");
+  h->E = n_experts;
+  h->D = d_model;
+  h->F = ff_dim;
+  for (int i = 0; i < 2; ++i) {
+    h->lin[i].n = n_experts;
+    h->lin[i].N = i == 0 ? ff_dim : d_model;
+    h->lin[i].K = i == 0 ? d_model : ff_dim;
+    h->lin[i].use_bias = use_bias != 0;
+  }
+  *out = h;
+  return MHSA_OK;
+}
+
+void mhsa_experts_destroy(mhsa_experts* h) { delete h; }
+
+int32_t mhsa_experts_load(mhsa_experts* h, int32_t data_dtype, const void* weight1, const void* bias1,
+                          const void* weight2, const void* bias2) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  if (!weight1 || !weight2) return fail(MHSA_EINVAL, "null weight pointer");
+  if (int32_t rc = load_weights(h->lin[0], data_dtype, weight1, nullptr, nullptr, bias1)) return rc;
+  if (int32_t rc = load_weights(h->lin[1], data_dtype, weight2, nullptr, nullptr, bias2)) return rc;
+  return experts_loaded(h);
+}
+
+int32_t mhsa_experts_load_codes(mhsa_experts* h, const uint8_t* codes1, const uint8_t* scales1, const float* bias1,
+                                const uint8_t* codes2, const uint8_t* scales2, const float* bias2) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  if (!codes1 || !codes2) return fail(MHSA_EINVAL, "null weight pointer");
+  if (int32_t rc = load_weights(h->lin[0], MHSA_F32, nullptr, codes1, scales1, bias1)) return rc;
+  if (int32_t rc = load_weights(h->lin[1], MHSA_F32, nullptr, codes2, scales2, bias2)) return rc;
+  return experts_loaded(h);
+}
+
+int64_t mhsa_experts_workspace(const mhsa_experts* h, int32_t rows, int32_t top_k) {
+  if (!h || rows < 0 || top_k <= 0 || top_k > kMaxTopK) return -1;
+  return rows == 0 ? 0 : experts_layout(h, rows, top_k, nullptr).bytes;
+}
+
+int32_t mhsa_experts_forward(const mhsa_experts* h, const void* x, int32_t dtype, int32_t rows, const int32_t* indices,
+                             const float* weights, int32_t top_k, const void* residual, float res_scale, void* out,
+                             void* workspace, int64_t workspace_bytes, void* hs) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  DType dt;
+  if (!act_dtype(dtype, &dt)) return fail(MHSA_ENOTSUP, "dtype %d not supported (f32, bf16)", dtype);
+  if (rows < 0) return fail(MHSA_EINVAL, "rows must not be negative (got %d)", rows);
+  if (top_k <= 0 || top_k > kMaxTopK) return fail(MHSA_EINVAL, "top_k %d is not in [1, %d]", top_k, kMaxTopK);
+  if (rows == 0) return MHSA_OK;
+  if (!x || !indices || !weights || !out) return fail(MHSA_EINVAL, "null tensor pointer");
+  if (!aligned16(x) || !aligned16(out) || !aligned16(residual))
+    return fail(MHSA_EINVAL, "device tensors must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(indices) % 4 || reinterpret_cast<uintptr_t>(weights) % 4)
+    return fail(MHSA_EINVAL, "indices and weights must be aligned to their elements");
+  if (!h->lin[0].loaded || !h->lin[1].loaded) return fail(MHSA_EINVAL, "no weights are loaded");
+  const ExpertsPlan plan = experts_layout(h, rows, top_k, workspace);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes)
+    return fail(MHSA_EINVAL, "%d rows of %d experts need a 16-byte aligned workspace of %lld bytes", rows, top_k,
+                (long long)plan.bytes);
+  const int64_t es = mhsa::dtype_size(dt), n = (int64_t)rows * h->D * es, np = (int64_t)rows * top_k * 4;
+  if (overlap(x, n, out, n) || (residual && residual != out && overlap(residual, n, out, n)) ||
+      overlap(indices, np, out, n) || overlap(weights, np, out, n))
+    return fail(MHSA_EINVAL, "out must not overlap another tensor, but may be the residual");
+  for (const void* t : {x, static_cast<const void*>(out), residual})
+    if (t && overlap(workspace, plan.bytes, t, n)) return fail(MHSA_EINVAL, "the workspace must not overlap a tensor");
+  if (overlap(workspace, plan.bytes, indices, np) || overlap(workspace, plan.bytes, weights, np))
+    return fail(MHSA_EINVAL, "the workspace must not overlap a tensor");
+  if (int32_t rc = check_device(h->device)) return rc;
+  for (int64_t r = 0; r < rows; r += plan.step) {
+    const int64_t m = std::min<int64_t>(plan.step, rows - r), at = r * h->D * es;
+    const int32_t rc = experts_run(h, plan, static_cast<const char*>(x) + at, dt, m, indices + r * top_k,
+                                   weights + r * top_k, top_k, residual ? static_cast<const char*>(residual) + at : nullptr,
+                                   res_scale, static_cast<char*>(out) + at, static_cast<hipStream_t>(hs));
+    if (rc) return rc;
+  }
+  return MHSA_OK;
+}
+
+}  // extern "C"

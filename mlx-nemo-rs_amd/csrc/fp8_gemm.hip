@@ -1,0 +1,708 @@
+// Products of e4m3 codes with a power of two for each block of 128
+// (fp8_kernels.hpp has the format): y = (2^s_x q_x) (2^s_w q_w)^T.
+//
+// The scaled fp8 MFMA multiplies codes and applies both powers of two inside
+// the instruction, so a chain over K needs no work between blocks. It adds
+// products in groups of 8, in which it drops what lies under 2^-13 of the
+// largest product's power of two: a sum is off by at most 7 * 2^-13 of its
+// terms' magnitudes (measured: 1.4e-5 of the result in the 2-norm for normally
+// distributed values, 5.5e-5 for codes spread over the whole exponent range,
+// at any K; the running sum keeps its 24 bits). That is far under half a step
+// of a bf16 result (2e-3 in the 2-norm) or of e4m3 codes. An f32 result keeps
+// f32 sums: there the codes go to the bf16 matrix cores, which hold them and
+// their products exactly (1e-7), at half the rate.
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/relpos_mhsa.h"
+#include "fp8_common.hpp"
+#include "fp8_kernels.hpp"
+#include "quant.hpp"
+
+namespace mhsa {
+namespace {
+
+#include "gemm_tile.hpp"
+
+// ---------------------------------------------------------------------------
+// Rounding to codes
+// ---------------------------------------------------------------------------
+
+// 8 values of row x from column c on, zero past K.
+template <typename T>
+__device__ __forceinline__ void load8(const T* x, int c, int K, bool vec, float v[8]) {
+  if (vec && c + 8 <= K) {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      reinterpret_cast<u32x4*>(t)[i] = reinterpret_cast<const u32x4*>(x + c)[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)x[c + i] : 0.f;
+  }
+}
+
+// A wave rounds 4 blocks of a row, 16 lanes of 8 values to a block.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int64_t rows, int K, bool vec,
+                                                            uint8_t* codes, uint8_t* scales) {
+  const int kb = (K + 127) / 128, items = (kb + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= rows * items) return;
+  const int64_t row = id / items;
+  const int lane = threadIdx.x & 63, blk = (int)(id % items) * 4 + (lane >> 4);
+  float v[8];
+  load8(x + row * ldx, blk * 128 + (lane & 15) * 8, blk < kb ? K : 0, vec, v);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fp8_mag(v[i]));
+#pragma unroll
+  for (int o = 1; o < 16; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (blk >= kb) return;
+  const int s = fp8_scale_byte(m);
+  const float inv = fp8_inverse_scale(s);
+  const u32x2 q = {fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                   fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+  *reinterpret_cast<u32x2*>(codes + row * ((int64_t)kb * 128) + blk * 128 + (lane & 15) * 8) = q;
+  if ((lane & 15) == 0) scales[row * (items * 4) + blk] = (uint8_t)s;
+}
+
+// One workgroup per 128 x 128 block of a weight matrix.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_weight_kernel(const T* w, int N, int K, uint8_t* codes,
+                                                              uint8_t* scales) {
+  const int kb = (K + 127) / 128, kbp = (kb + 3) / 4 * 4, nb = (N + 127) / 128;
+  const int bk = blockIdx.x, bn = blockIdx.y;
+  w += (int64_t)blockIdx.z * N * K;
+  codes += (int64_t)blockIdx.z * N * (kb * 128);
+  scales += (int64_t)blockIdx.z * nb * kbp;
+  __shared__ float part[4];
+  float v[64];
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    const int at = i * 256 + threadIdx.x, n = bn * 128 + at / 128, k = bk * 128 + at % 128;
+    v[i] = n < N && k < K ? (float)w[(int64_t)n * K + k] : 0.f;
+    m = fmaxf(m, fp8_mag(v[i]));
+  }
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  const int s = fp8_scale_byte(m);
+  const float inv = fp8_inverse_scale(s);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    const int at = i * 256 + threadIdx.x, n = bn * 128 + at / 128, k = bk * 128 + at % 128;
+    if (n < N) codes[(int64_t)n * (kb * 128) + k] = (uint8_t)fp8_pack4(v[i] * inv, 0.f, 0.f, 0.f);
+  }
+  if (threadIdx.x == 0) scales[bn * kbp + bk] = (uint8_t)s;
+}
+
+// Codes [rows, K] <-> [rows, Kp] and scale bytes [blocks, kb] <-> [blocks,
+// kbp], 16 codes of a padded row to a thread. A scale byte of 255 says that
+// its block is not a number: the block's codes then say so.
+__global__ __launch_bounds__(256) void pad_weight_kernel(const uint8_t* w, const uint8_t* ws, int64_t rows, int N,
+                                                         int K, bool vec, uint8_t* codes, uint8_t* scales) {
+  const int kb = (K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4, nb = (N + 127) / 128;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at < rows * (kp / 16)) {
+    const int64_t n = at / (kp / 16), blk = n / N * nb + n % N / 128;
+    const int k = (int)(at % (kp / 16)) * 16;
+    const bool nan = ws[blk * kb + k / 128] == 255;
+    uint8_t v[16];
+    if (vec && !nan) {
+      *reinterpret_cast<u32x4*>(v) = *reinterpret_cast<const u32x4*>(w + n * K + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = k + i < K ? (nan ? 0x7F : w[n * K + k + i]) : 0;
+    }
+    *reinterpret_cast<u32x4*>(codes + n * kp + k) = *reinterpret_cast<const u32x4*>(v);
+  }
+  if (at < rows / N * nb * kbp) {
+    const int64_t n = at / kbp;
+    const int k = (int)(at % kbp);
+    const uint8_t s = k < kb ? ws[n * kb + k] : 127;
+    scales[at] = s == 255 ? 127 : s;
+  }
+}
+__global__ __launch_bounds__(256) void unpad_weight_kernel(const uint8_t* codes, const uint8_t* scales, int64_t N,
+                                                           int K, int64_t nb, uint8_t* w, uint8_t* ws) {
+  const int kb = (K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at < N * K) w[at] = codes[at / K * kp + at % K];
+  if (at < nb * kb) ws[at] = scales[at / kb * kbp + at % kb];
+}
+
+// ---------------------------------------------------------------------------
+// Few rows
+//
+// Weights are read once and everything else is small: a workgroup computes 16
+// output columns of up to 16 rows, its NW waves take every NW-th block of 128
+// inputs, and their sums are added in wave order at the end. One 16x16x128 MFMA
+// covers a block: lane l holds 32 inputs, 32 (l / 16) on, of weight row l % 16
+// and of activation row l % 16. The activations are rounded to codes in these
+// registers (the block's maximum is one over 4 lanes), so there is no other
+// launch.
+// ---------------------------------------------------------------------------
+
+// 32 values of row x from column c on, zero past K.
+template <typename T>
+__device__ __forceinline__ void load32(const T* x, int c, int K, bool vec, float v[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load8(x, c + 8 * i, K, vec, v + 8 * i);
+}
+
+// Stores one value in the output's type.
+__device__ __forceinline__ void store_as(DType dt, void* out, int64_t at, float v) {
+  if (dt == kBF16) reinterpret_cast<bf16*>(out)[at] = (bf16)v;
+  else reinterpret_cast<float*>(out)[at] = v;
+}
+
+template <typename TX, int NW, bool EXACT>
+__global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
+  __shared__ float red[NW][16][20];
+  __shared__ int dst[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c4 = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  // row r of this workgroup: its expert, its source row and its output row
+  int expert = 0, src = -1, to = -1;
+  if (p.g.tile) {
+    if ((int)blockIdx.y >= *p.g.n_tiles) return;
+    const int* t = p.g.tile + 4 * blockIdx.y;
+    expert = t[0];
+    if (r < t[2]) to = p.g.pair[t[1] + r];
+  } else if (p.g.idx) {
+    // up to 64 pairs, one to a lane: the pairs of pair y's expert, of which y
+    // is to be the first of a run of 16
+    const int mine = lane < p.g.pairs ? p.g.idx[lane] : -1;
+    expert = __shfl(mine, (int)blockIdx.y, 64);
+    if (expert < 0 || expert >= p.g.experts) return;
+    uint64_t same = __ballot(mine == expert);
+    const int before = __popcll(same & (((uint64_t)1 << blockIdx.y) - 1));
+    if (before % 16) return;
+    for (int i = 0; i < before + r; ++i) same &= same - 1;
+    if (same) to = __builtin_ctzll(same);
+  } else {
+    const int row = blockIdx.y * 16 + r;
+    if (row < p.M) src = to = row;
+  }
+  if ((p.g.tile || p.g.idx) && to >= 0) src = p.rows == Fp8Gemm::kByFrame ? to / p.g.top_k : to;
+  if (threadIdx.x < 16) dst[r] = to;
+
+  const int kb = (p.K + 127) / 128, kbp = (kb + 3) / 4 * 4;
+  const uint8_t* wrow = p.w + expert * p.w_stride + (int64_t)min(n0 + r, p.N - 1) * (kb * 128) + 32 * c4;
+  const uint8_t* wsc = p.ws + expert * p.ws_stride + (int64_t)(n0 / 128) * kbp;
+  const TX* xrow = reinterpret_cast<const TX*>(p.x) + (int64_t)max(src, 0) * p.ldx;
+  const int K = src >= 0 ? p.K : 0;
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int b = w; b < kb; b += NW) {
+    const u32x4 w0 = *reinterpret_cast<const u32x4*>(wrow + b * 128), w1 = *reinterpret_cast<const u32x4*>(wrow + b * 128 + 16);
+    const int sw = wsc[b];
+    float v[32];
+    load32(xrow, b * 128 + 32 * c4, K, vec, v);
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m = fmaxf(m, fp8_mag(v[i]));
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const int s = fp8_scale_byte(m);
+    const float inv = fp8_inverse_scale(s);
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = fp8_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+    if constexpr (EXACT) {
+      // element group j of every lane's 32: the same inputs of both operands
+      floatx4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x4 wj = j < 2 ? w0 : w1;
+        part = mma16(fp8_to_bf16(wj[2 * (j & 1)], wj[2 * (j & 1) + 1]), fp8_to_bf16(q[2 * j], q[2 * j + 1]), part);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += __builtin_ldexpf(part[e], s + sw - 254);
+    } else {
+      i32x8 a, x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[i] = (int)w0[i];
+        a[i + 4] = (int)w1[i];
+        x[i] = (int)q[i];
+        x[i + 4] = (int)q[i + 4];
+      }
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, acc, 0, 0, 0, sw, 0, s);
+    }
+  }
+  // lane: row l % 16, columns 4 (l / 16) + [0, 4)
+  *reinterpret_cast<floatx4*>(&red[w][r][4 * c4]) = acc;
+  __syncthreads();
+  if (threadIdx.x >= 256) return;
+  const int row = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15), out = dst[row];
+  if (out < 0 || n >= p.N) return;
+  float v = red[0][row][threadIdx.x & 15];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) v += red[i][row][threadIdx.x & 15];
+  if (p.bias) v += p.bias[(int64_t)expert * p.N + n];
+  if (p.epilogue == kFp8HiddenF32) v = silu_value<float>(v);
+  store_as(p.epilogue == kFp8Out ? p.out_dt : kF32, p.out, (int64_t)out * p.ldo + n, v);
+}
+
+// ---------------------------------------------------------------------------
+// Tiles
+//
+// A workgroup of 4 waves (2 x 2) computes a BM x BN tile from LDS stages of
+// 128 inputs, one block: rows of 128 bytes whose eight 16-byte chunks are
+// stored XOR-permuted by (row / 2) % 8 (the 32 rows of a fragment read then
+// lie on all 64 banks), filled by direct-to-LDS loads that run NS - 1 stages
+// ahead. A 32x32x64 MFMA takes 32 bytes of each operand from a lane; the weight
+// is its first operand, so a lane's accumulators hold four consecutive output
+// columns of one row. Row scales come with the stages, 4 stages to a word;
+// the weight's scale is one byte per wave and stage, read from a lane of a
+// register that holds all of them.
+// ---------------------------------------------------------------------------
+
+template <int BM, int BN, int NS_>
+struct Fp8Cfg {
+  static constexpr int NS = NS_, DIST = NS - 1;
+  static constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
+  static constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  static constexpr int NA = BM / 32, NB = BN / 32;  // 1 KB loads per wave and stage
+  static constexpr int OP = WN * 4 + 16;            // pitch of a staged output row
+  static constexpr int STG = 4 * 32 * OP, AMAX = 2 * BM * 4;
+  static constexpr int SCALES = NS * STAGE;         // two words a row behind the stages
+  static constexpr int LOOP = SCALES + 2 * BM * 4;
+  static constexpr int LDS = LOOP > STG + AMAX ? LOOP : STG + AMAX;
+  static_assert(LDS <= 160 * 1024, "tile exceeds LDS");
+};
+
+template <int BM, int BN, int NS, bool EXACT, int EPI>
+__device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
+  using C = Fp8Cfg<BM, BN, NS>;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w >> 1, wn = w & 1;
+  const int kb = (p.K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4;
+
+  // contiguous tile ranges per XCD, walked 8 row tiles at a time
+  const bool grouped = p.g.tile != nullptr;
+  const int tilesM = grouped ? *p.g.n_tiles : (p.M + BM - 1) / BM, tilesN = (p.N + BN - 1) / BN;
+  const int nt = tilesM * tilesN, per = (nt + 7) / 8;
+  const int at = (int)(blockIdx.x / 8u), T = (int)(blockIdx.x % 8u) * per + at;
+  if (at >= per || T >= nt) return;
+  constexpr int GM = 8;
+  const int gsz = GM * tilesN, first = T / gsz * GM, gm = min(tilesM - first, GM);
+  const int tm = first + (T % gsz) % gm, n0 = (T % gsz) / gm * BN;
+  int expert = 0, m0 = tm * BM, rows = min(p.M - m0, BM);
+  if (grouped) {
+    expert = p.g.tile[4 * tm];
+    m0 = p.g.tile[4 * tm + 1];
+    rows = p.g.tile[4 * tm + 2];
+  }
+
+  // activations: this tile's rows, or gathered ones (rows past the tile's
+  // repeat its last; their results are not stored)
+  const bool gather = grouped && p.rows == Fp8Gemm::kByFrame;
+  const uint8_t* ab = p.a + (gather ? 0 : (int64_t)m0 * kp);
+  const uint8_t* sb = p.as + (gather ? 0 : (int64_t)m0 * kbp);
+  const int64_t arows = gather ? p.a_rows : rows;
+  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ab, (short)0, (int)(uint32_t)(arows * kp), kRawBuffer);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, (int)(uint32_t)(arows * kbp), kRawBuffer);
+  auto source = [&](int row) -> uint32_t {
+    row = min(row, rows - 1);
+    return gather ? (uint32_t)(p.g.pair[m0 + row] / p.g.top_k) : (uint32_t)row;
+  };
+  int aoff[C::NA];
+#pragma unroll
+  for (int g = 0; g < C::NA; ++g) {
+    const int pos = (w * C::NA + g) * 64 + lane, row = pos >> 3;
+    aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((pos & 7) ^ ((row >> 1) & 7)));
+  }
+  const int srow = (w * 64) % BM;
+  const int soff = (int)(source(srow + lane) * (uint32_t)kbp);
+  const uint8_t* wb = p.w + expert * p.w_stride + (int64_t)n0 * kp;
+  const __amdgpu_buffer_rsrc_t rb =
+      __builtin_amdgcn_make_buffer_rsrc((void*)wb, (short)0, min(p.N - n0, BN) * kp, kRawBuffer);
+  int boff[C::NB];
+#pragma unroll
+  for (int g = 0; g < C::NB; ++g) {
+    const int pos = (w * C::NB + g) * 64 + lane, row = pos >> 3;
+    boff[g] = row * kp + 16 * ((pos & 7) ^ ((row >> 1) & 7));
+  }
+  // the weight scales of this wave's 128-column block, a word of 4 to a lane
+  const int wblk = min((n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
+  const uint32_t wword = *reinterpret_cast<const uint32_t*>(p.ws + expert * p.ws_stride + (int64_t)wblk * kbp +
+                                                            4 * min(lane, kbp / 4 - 1));
+  auto issue = [&](int kt, int buf) {
+    char* S = smem + buf * C::STAGE;
+#pragma unroll
+    for (int g = 0; g < C::NA; ++g)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(S + (w * C::NA + g) * 1024), 16, aoff[g], kt * 128, 0, 0);
+#pragma unroll
+    for (int g = 0; g < C::NB; ++g)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(S + C::ABYTES + (w * C::NB + g) * 1024), 16, boff[g],
+                                               kt * 128, 0, 0);
+    // (a word is loaded again by each of its stages, and by two waves of a
+    // tile of under 256 rows: always the same bytes)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((kt >> 2) & 1) * BM * 4 + srow * 4), 4,
+                                             soff, kt & ~3, 0, 0);
+  };
+  constexpr int LOADS = C::NA + C::NB + 1;
+  auto landed = [&](int behind) {  // this wave's loads but the last `behind` stages' are in LDS
+    switch (behind) {
+      case 0: __builtin_amdgcn_s_waitcnt(7 << 4); break;
+      case 1: __builtin_amdgcn_s_waitcnt((LOADS & 15) | ((LOADS >> 4) << 14) | (7 << 4)); break;
+      default: __builtin_amdgcn_s_waitcnt(((2 * LOADS) & 15) | (((2 * LOADS) >> 4) << 14) | (7 << 4)); break;
+    }
+  };
+  static_assert(C::DIST >= 1 && C::DIST <= 3 && 2 * LOADS < 64, "wait counts");
+
+  const int arow = (wm * C::WM + (lane & 31)) * 128;
+  const int brow = C::ABYTES + (wn * C::WN + (lane & 31)) * 128;
+  floatx16 acc[C::TN][C::TM];
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
+  int xs[C::TM], xn[C::TM];
+  auto scales_of = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+      xn[i] = *reinterpret_cast<const int*>(smem + C::SCALES + ((kt >> 2) & 1) * BM * 4 +
+                                            (wm * C::WM + 32 * i + (lane & 31)) * 4) >> (8 * (kt & 3));
+  };
+  auto chunk = [&](int base, int c) { return base + 16 * (c ^ ((lane >> 1) & 7)); };
+
+#pragma unroll
+  for (int st = 0; st < C::DIST; ++st) issue(min(st, kb - 1), st);
+  landed(C::DIST - 1);
+  asm volatile("s_barrier" ::: "memory");
+
+  if constexpr (!EXACT) {
+    i32x8 fa[2][C::TM], fb[2][C::TN];
+    auto rd = [&](const char* S, int s, int b) {
+      const int c = 4 * s + 2 * half;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        reinterpret_cast<u32x4*>(&fa[b][i])[0] = *reinterpret_cast<const u32x4*>(S + chunk(arow, c) + i * 4096);
+        reinterpret_cast<u32x4*>(&fa[b][i])[1] = *reinterpret_cast<const u32x4*>(S + chunk(arow, c + 1) + i * 4096);
+      }
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        reinterpret_cast<u32x4*>(&fb[b][j])[0] = *reinterpret_cast<const u32x4*>(S + chunk(brow, c) + j * 4096);
+        reinterpret_cast<u32x4*>(&fb[b][j])[1] = *reinterpret_cast<const u32x4*>(S + chunk(brow, c + 1) + j * 4096);
+      }
+    };
+    scales_of(0);
+    rd(smem, 0, 0);
+    for (int kt = 0; kt < kb; ++kt) {
+      const char* S = smem + kt % NS * C::STAGE;
+      // the buffer that stage kt + DIST fills was last read in stage kt - 1
+      issue(min(kt + C::DIST, kb - 1), (kt + C::DIST) % NS);
+      const int ws = __builtin_amdgcn_readlane((int)wword, kt >> 2) >> (8 * (kt & 3));
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) xs[i] = xn[i];
+      rd(S, 1, 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[0][j], fa[0][i], acc[j][i], 0, 0, 0, ws, 0, xs[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      landed(C::DIST - 1);
+      asm volatile("s_barrier" ::: "memory");
+      scales_of(min(kt + 1, kb - 1));
+      rd(smem + (kt + 1) % NS * C::STAGE, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[1][j], fa[1][i], acc[j][i], 0, 0, 0, ws, 0, xs[i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    // exact products and f32 sums: per block on the bf16 cores, then added
+    // with the block's power of two
+    for (int kt = 0; kt < kb; ++kt) {
+      const char* S = smem + kt % NS * C::STAGE;
+      issue(min(kt + C::DIST, kb - 1), (kt + C::DIST) % NS);
+      const int ws = (__builtin_amdgcn_readlane((int)wword, kt >> 2) >> (8 * (kt & 3))) & 255;
+      scales_of(kt);
+      floatx16 part[C::TN][C::TM];
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) part[j][i] = floatx16{};
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        u32x4 fa[C::TM], fb[C::TN];
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) fa[i] = *reinterpret_cast<const u32x4*>(S + chunk(arow, 2 * t + half) + i * 4096);
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) fb[j] = *reinterpret_cast<const u32x4*>(S + chunk(brow, 2 * t + half) + j * 4096);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          bf16x8 xa[C::TM], xb[C::TN];
+#pragma unroll
+          for (int i = 0; i < C::TM; ++i) xa[i] = fp8_to_bf16(fa[i][2 * u], fa[i][2 * u + 1]);
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[j][2 * u], fb[j][2 * u + 1]);
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i) part[j][i] = mma32(xb[j], xa[i], part[j][i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int e = (xn[i] & 255) + ws - 254;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[j][i][r] += __builtin_ldexpf(part[j][i][r], e);
+      }
+      landed(C::DIST - 1);
+      asm volatile("s_barrier" ::: "memory");
+    }
+  }
+  // the clamped loads of the last stages still write LDS: all of them are to
+  // have landed before the epilogue reuses it
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+
+  // lane: row 32 i + lane % 32 of the wave's block, columns 32 j + 8 q +
+  // 4 (lane / 32) + [0, 4)
+  const int col0 = n0 + wn * C::WN;
+  char* st = smem + w * 32 * C::OP;
+  if constexpr (EPI == kFp8HiddenQ) {
+    // silu, then codes: the block's 128 columns of a row lie in one wave
+    // (both lane halves) or in the two of a row of waves
+    float* amax = reinterpret_cast<float*>(smem + C::STG);
+    float top[C::TM];
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) top[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = col0 + 32 * j + 8 * q + 4 * half;
+        floatx4 b = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias && col < p.N) b = *reinterpret_cast<const floatx4*>(p.bias + (int64_t)expert * p.N + col);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = silu_value<float>(acc[j][i][4 * q + e] + b[e]);
+            acc[j][i][4 * q + e] = v;
+            top[i] = fmaxf(top[i], fp8_mag(v));
+          }
+      }
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor(top[i], 32, 64));
+      if (C::WN < 128 && half == 0) amax[wn * BM + wm * C::WM + 32 * i + lane] = top[i];
+    }
+    if constexpr (C::WN < 128) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int r = wm * C::WM + 32 * i + (lane & 31);
+        top[i] = fmaxf(amax[r], amax[BM + r]);
+      }
+    }
+    const int np = (p.N + 127) / 128 * 128, nbp = (np / 128 + 3) / 4 * 4;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const int s = fp8_scale_byte(top[i]);
+      const float inv = fp8_inverse_scale(s);
+      constexpr int HP = C::WN + 16;
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint32_t*>(st + (lane & 31) * HP + 32 * j + 8 * q + 4 * half) =
+              fp8_pack4(acc[j][i][4 * q] * inv, acc[j][i][4 * q + 1] * inv, acc[j][i][4 * q + 2] * inv,
+                        acc[j][i][4 * q + 3] * inv);
+      const int row0 = wm * C::WM + 32 * i;
+#pragma unroll
+      for (int it = 0; it < C::WN / 32; ++it) {
+        const int id = it * 64 + lane, r = id / (C::WN / 16), c = id % (C::WN / 16) * 16;
+        if (row0 + r < rows && col0 + c < np)
+          *reinterpret_cast<u32x4*>(p.out_codes + (int64_t)(m0 + row0 + r) * np + col0 + c) =
+              *reinterpret_cast<const u32x4*>(st + r * HP + c);
+      }
+      if (half == 0 && col0 % 128 == 0 && col0 < np && row0 + lane < rows)
+        p.out_scales[(int64_t)(m0 + row0 + lane) * nbp + col0 / 128] = (uint8_t)s;
+    }
+  } else {
+    const bool b16 = EPI == kFp8Out && p.out_dt == kBF16;
+    const int V = b16 ? 8 : 4;  // columns of a 16-byte store
+    const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldo % V == 0;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<floatx4*>(st + (lane & 31) * C::OP + (32 * j + 8 * q + 4 * half) * 4) =
+              floatx4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+      const int runs = C::WN / V;
+      for (int id = lane; id < 32 * runs; id += 64) {
+        const int r = id / runs, c = id % runs * V, col = col0 + c, row = wm * C::WM + 32 * i + r;
+        if (row >= rows || col >= p.N) continue;
+        const int64_t orow = EPI == kFp8Pair ? p.g.pair[m0 + row] : m0 + row;
+        float f[8];
+        *reinterpret_cast<floatx4*>(f) = *reinterpret_cast<const floatx4*>(st + r * C::OP + c * 4);
+        if (b16) *reinterpret_cast<floatx4*>(f + 4) = *reinterpret_cast<const floatx4*>(st + r * C::OP + c * 4 + 16);
+        if (p.bias) {
+          const float* b = p.bias + (int64_t)expert * p.N + col;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < V && col + e < p.N) f[e] += b[e];
+        }
+        if (vec && col + V <= p.N) {
+          if (b16) {
+            bf16x8 v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (bf16)f[e];
+            *reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(p.out) + orow * p.ldo + col) = v;
+          } else {
+            *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(p.out) + orow * p.ldo + col) =
+                floatx4{f[0], f[1], f[2], f[3]};
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < V && col + e < p.N) store_as(b16 ? kBF16 : kF32, p.out, orow * p.ldo + col + e, f[e]);
+        }
+      }
+    }
+  }
+}
+
+template <int BM, int BN, int NS, bool EXACT, int EPI>
+__global__ __launch_bounds__(256, 1) void fp8_tile_kernel(Fp8Gemm p) {
+  __shared__ __attribute__((aligned(1024))) char smem[Fp8Cfg<BM, BN, NS>::LDS];
+  fp8_tile_body<BM, BN, NS, EXACT, EPI>(p, smem);
+}
+
+template <int BM, int BN, int NS, bool EXACT, int EPI>
+hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
+  const int64_t tm = p.g.tile ? p.g.max_tiles : (p.M + BM - 1) / BM;
+  const int64_t nt = tm * ((p.N + BN - 1) / BN);
+  if (p.g.tile && p.g.tile_rows != BM) return hipErrorInvalidValue;
+  if (nt > (int64_t)1 << 28) return hipErrorInvalidValue;
+  fp8_tile_kernel<BM, BN, NS, EXACT, EPI><<<(unsigned)((nt + 7) / 8 * 8), 256, 0, s>>>(p);
+  return hipGetLastError();
+}
+
+bool bad_gemm(const Fp8Gemm& p) {
+  return p.N <= 0 || p.K <= 0 || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);
+}
+
+}  // namespace
+
+hipError_t fp8_quantize_rows(DType dt, const void* x, int64_t ldx, int64_t rows, int K, uint8_t* codes,
+                             uint8_t* scales, hipStream_t s) {
+  if (rows <= 0 || K <= 0 || K > kFp8MaxK) return hipErrorInvalidValue;
+  const int64_t items = rows * (fp8_kbp(K) / 4), grid = (items + 3) / 4;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const int es = dtype_size(dt);
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx * es % 16 == 0;
+  if (dt == kBF16)
+    quantize_rows_kernel<bf16><<<(unsigned)grid, 256, 0, s>>>(static_cast<const bf16*>(x), ldx, rows, K, vec, codes, scales);
+  else
+    quantize_rows_kernel<float><<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(x), ldx, rows, K, vec, codes, scales);
+  return hipGetLastError();
+}
+
+hipError_t fp8_quantize_weight(int data_dtype, const void* w, int n_mats, int N, int K, uint8_t* codes,
+                               uint8_t* scales, hipStream_t s) {
+  if (N <= 0 || K <= 0 || n_mats <= 0 || n_mats > 65535 || (N + 127) / 128 > 65535) return hipErrorInvalidValue;
+  const dim3 grid((K + 127) / 128, (N + 127) / 128, n_mats);
+  switch (data_dtype) {
+    case MHSA_F32: quantize_weight_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(w), N, K, codes, scales); break;
+    case MHSA_BF16: quantize_weight_kernel<<<grid, 256, 0, s>>>(static_cast<const bf16*>(w), N, K, codes, scales); break;
+    case MHSA_F16: quantize_weight_kernel<<<grid, 256, 0, s>>>(static_cast<const _Float16*>(w), N, K, codes, scales); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t fp8_pad_weight(const uint8_t* w, const uint8_t* ws, int n_mats, int N, int K, uint8_t* codes,
+                          uint8_t* scales, hipStream_t s) {
+  if (N <= 0 || K <= 0 || n_mats <= 0) return hipErrorInvalidValue;
+  const int64_t rows = (int64_t)n_mats * N, nb = (int64_t)n_mats * ((N + 127) / 128);
+  const int64_t grid = (std::max(rows * fp8_kp(K) / 16, nb * fp8_kbp(K)) + 255) / 256;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const bool vec = K % 128 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  pad_weight_kernel<<<(unsigned)grid, 256, 0, s>>>(w, ws, rows, N, K, vec, codes, scales);
+  return hipGetLastError();
+}
+
+hipError_t fp8_unpad_weight(const uint8_t* codes, const uint8_t* scales, int N, int K, uint8_t* w, uint8_t* ws,
+                            hipStream_t s) {
+  const int64_t grid = ((int64_t)N * K + 255) / 256;
+  if (N <= 0 || K <= 0 || grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  unpad_weight_kernel<<<(unsigned)grid, 256, 0, s>>>(codes, scales, N, K, (N + 127) / 128, w, ws);
+  return hipGetLastError();
+}
+
+bool fp8_few_rows(int64_t M, int N, int K) {
+  (void)N;
+  (void)K;
+  return M <= 64;
+}
+
+hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
+  if (bad_gemm(p) || !p.x) return hipErrorInvalidValue;
+  const int64_t groups = p.g.tile ? p.g.max_tiles : p.g.idx ? p.g.pairs : (p.M + 15) / 16;
+  if (groups <= 0 || groups > 65535 || (p.g.idx && p.g.pairs > 64) || (p.g.tile && p.g.tile_rows != 16)) return hipErrorInvalidValue;
+  const dim3 grid((p.N + 15) / 16, (unsigned)groups);
+  const int es = dtype_size(p.x_dt);
+  const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * es % 16 == 0;
+  const bool exact = p.epilogue == kFp8Out && p.out_dt == kF32;
+  auto go = [&](auto tx, auto nw) {
+    using TX = decltype(tx);
+    constexpr int NW = decltype(nw)::value;
+    if (exact) fp8_few_kernel<TX, NW, true><<<grid, NW * 64, 0, s>>>(p, vec);
+    else fp8_few_kernel<TX, NW, false><<<grid, NW * 64, 0, s>>>(p, vec);
+  };
+  auto by_type = [&](auto nw) {
+    if (p.x_dt == kBF16) go(bf16{}, nw);
+    else go(float{}, nw);
+  };
+  if (p.K > 2048) by_type(std::integral_constant<int, 16>{});
+  else by_type(std::integral_constant<int, 8>{});
+  return hipGetLastError();
+}
+
+int fp8_group_rows(int64_t pairs, int experts) {
+  const int64_t mean = pairs / experts;
+  return mean < 24 ? 16 : mean < 192 ? 128 : 256;
+}
+
+hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
+  if (bad_gemm(p) || !p.a || !p.as) return hipErrorInvalidValue;
+  if (p.g.tile) {
+    if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll) return hipErrorInvalidValue;
+    if (p.epilogue == kFp8HiddenQ)
+      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8HiddenQ>(p, s)
+                                  : launch_tile<128, 128, 2, false, kFp8HiddenQ>(p, s);
+    if (p.epilogue == kFp8Pair)
+      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8Pair>(p, s)
+                                  : launch_tile<128, 128, 2, false, kFp8Pair>(p, s);
+    return hipErrorInvalidValue;
+  }
+  if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
+  const int64_t t128 = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128), t256 = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (p.out_dt == kF32)
+    return t128 >= 128 ? launch_tile<128, 128, 2, true, kFp8Out>(p, s) : launch_tile<64, 64, 3, true, kFp8Out>(p, s);
+  if (t256 >= 128) return launch_tile<256, 256, 2, false, kFp8Out>(p, s);
+  return t128 >= 128 ? launch_tile<128, 128, 2, false, kFp8Out>(p, s) : launch_tile<64, 64, 4, false, kFp8Out>(p, s);
+}
+
+}  // namespace mhsa

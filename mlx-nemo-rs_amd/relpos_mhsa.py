@@ -57,6 +57,10 @@ EXPORTS = (
     "mhsa_debug_position_scores", "mhsa_debug_top_keys", "mhsa_profile_enable", "mhsa_profile_repeat",
     "mhsa_profile_reset", "mhsa_profile_count",
     "mhsa_profile_entry",
+    "mhsa_fp8_linear_create", "mhsa_fp8_linear_destroy", "mhsa_fp8_linear_load", "mhsa_fp8_linear_load_codes",
+    "mhsa_fp8_linear_read_codes", "mhsa_fp8_linear_workspace", "mhsa_fp8_linear_forward", "mhsa_route",
+    "mhsa_experts_create", "mhsa_experts_destroy", "mhsa_experts_load", "mhsa_experts_load_codes",
+    "mhsa_experts_workspace", "mhsa_experts_forward",
 )
 
 
@@ -201,6 +205,23 @@ def library(path: str = LIB_PATH) -> ctypes.CDLL:
         "mhsa_profile_count": (I, [VP]),
         "mhsa_profile_entry": (I, [VP, I, P(ctypes.c_char_p), P(ctypes.c_double), PI]),
     }
+    L = ctypes.c_int64
+    sig.update({
+        "mhsa_fp8_linear_create": (I, [I, I, I, P(VP)]),
+        "mhsa_fp8_linear_destroy": (None, [VP]),
+        "mhsa_fp8_linear_load": (I, [VP, I, VP, VP]),
+        "mhsa_fp8_linear_load_codes": (I, [VP, VP, VP, VP]),
+        "mhsa_fp8_linear_read_codes": (I, [VP, VP, VP]),
+        "mhsa_fp8_linear_workspace": (L, [VP, I]),
+        "mhsa_fp8_linear_forward": (I, [VP, VP, I, I, L, VP, I, L, VP, L, VP]),
+        "mhsa_route": (I, [VP, I, I, I, L, I, VP, I, I, I, I, F, VP, VP, VP]),
+        "mhsa_experts_create": (I, [I, I, I, I, P(VP)]),
+        "mhsa_experts_destroy": (None, [VP]),
+        "mhsa_experts_load": (I, [VP, I, VP, VP, VP, VP]),
+        "mhsa_experts_load_codes": (I, [VP, VP, VP, VP, VP, VP, VP]),
+        "mhsa_experts_workspace": (L, [VP, I, I]),
+        "mhsa_experts_forward": (I, [VP, VP, I, I, VP, VP, I, VP, F, VP, VP, L, VP]),
+    })
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -477,6 +498,263 @@ class FeedForward(_Profiled):
         out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
         _check(self._lib.mhsa_ffn_debug_linear(self._h, which, 1 if promoted else 0, _dptr(x.contiguous()), rows,
                                                _dptr(out), _stream_ptr()))
+        return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit block-scaled projections, routing and experts
+# ---------------------------------------------------------------------------
+
+def _weight_data(a, shape, name, kinds):
+    """(owner to keep alive, pointer, dtype code) of a weight tensor: numpy or
+    torch, host or GPU, of one of `kinds` ("codes": uint8 or float8_e4m3fn)."""
+    import torch
+    if isinstance(a, np.ndarray):
+        a = torch.from_numpy(np.ascontiguousarray(a))
+    if not isinstance(a, torch.Tensor):
+        raise MhsaError(MHSA_EINVAL, f"{name}: expected a numpy array or a tensor")
+    a = a.detach().contiguous()
+    if tuple(a.shape) != tuple(shape):
+        raise MhsaError(MHSA_EINVAL, f"{name}: expected shape {tuple(shape)}, got {tuple(a.shape)}")
+    codes = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+    if kinds == "codes":
+        if a.dtype not in (torch.uint8, torch.float8_e4m3fn):
+            raise MhsaError(MHSA_ENOTSUP, f"{name}: expected uint8 (or float8_e4m3fn), got {a.dtype}")
+        return a, a.data_ptr(), None
+    if a.dtype not in codes or (kinds == "f32" and a.dtype != torch.float32):
+        raise MhsaError(MHSA_ENOTSUP, f"{name}: dtype {a.dtype} not supported")
+    return a, a.data_ptr(), codes[a.dtype]
+
+
+def _load_floats(pairs):
+    """The pointers of (weight, bias) tensors of one float dtype."""
+    keep, ptrs, dtype = [], [], None
+    for (w, wshape, wname), (b, bshape, bname) in pairs:
+        a, ptr, code = _weight_data(w, wshape, wname, "float")
+        if dtype not in (None, code):
+            raise MhsaError(MHSA_EINVAL, f"{wname}: the weights are of different dtypes")
+        dtype = code
+        keep.append(a)
+        ptrs.append(ptr)
+        if b is None:
+            ptrs.append(None)
+            continue
+        if isinstance(b, np.ndarray):
+            import torch
+            b = torch.from_numpy(np.ascontiguousarray(b))
+        a, ptr, _ = _weight_data(b.to(a.dtype), bshape, bname, "float")
+        keep.append(a)
+        ptrs.append(ptr)
+    return keep, ptrs, dtype
+
+
+def _load_codes(groups):
+    """The pointers of (codes, scales, bias) tensors."""
+    keep, ptrs = [], []
+    for (c, cshape, cname), (s, sshape, sname), (b, bshape, bname) in groups:
+        for a, shape, name, kind in ((c, cshape, cname, "codes"), (s, sshape, sname, "codes"), (b, bshape, bname, "f32")):
+            if a is None:
+                ptrs.append(None)
+                continue
+            a, ptr, _ = _weight_data(a, shape, name, kind)
+            keep.append(a)
+            ptrs.append(ptr)
+    return keep, ptrs
+
+
+def _blocks(n: int) -> int:
+    return (n + 127) // 128
+
+
+class _OnDevice:
+    """The GPU of `x` made current for a call, and torch's stream on it."""
+
+    def __init__(self, x):
+        self._x = x
+
+    def __enter__(self):
+        import torch
+        self._before = torch.cuda.current_device()
+        dev = self._x.get_device()
+        if dev != self._before:
+            torch.cuda.set_device(dev)
+        return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+    def __exit__(self, *exc):
+        import torch
+        if self._x.get_device() != self._before:
+            torch.cuda.set_device(self._before)
+
+
+def _rows_of(x, width: int):
+    """(rows, row stride) of x [..., width] whose rows are evenly spaced with
+    contiguous elements; raises for others."""
+    import torch
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1 or x.shape[-1] != width:
+        raise MhsaError(MHSA_EINVAL, f"expected a GPU tensor [..., {width}]")
+    rows = x.numel() // width
+    if x.is_contiguous():
+        return rows, width
+    lead = [(n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
+    if rows and (x.stride(-1) == 1 or width == 1):
+        if not lead:
+            return rows, width
+        if lead[-1][1] >= width and all(a[1] == b[1] * b[0] for a, b in zip(lead, lead[1:])):
+            return rows, lead[-1][1]
+    raise MhsaError(MHSA_EINVAL, "rows must be evenly spaced and their elements contiguous")
+
+
+class Fp8Linear:
+    """y = W q(x) + b with e4m3 weights in 128 x 128 blocks, each with a power
+    of two, and activations rounded the same way per row and 128 inputs
+    (mhsa_fp8_linear_*)."""
+
+    def __init__(self, in_dim: int, out_dim: int, use_bias: bool = False):
+        lib = library()
+        h = ctypes.c_void_p()
+        _check(lib.mhsa_fp8_linear_create(in_dim, out_dim, 1 if use_bias else 0, ctypes.byref(h)))
+        self._h, self._lib = h, lib
+        self.in_dim, self.out_dim = in_dim, out_dim
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            self._lib.mhsa_fp8_linear_destroy(h)
+            self._h = None
+
+    def load(self, weight, bias=None) -> None:
+        """weight [out, in] (float32, bfloat16 or float16), rounded to codes."""
+        keep, ptrs, dtype = _load_floats([((weight, (self.out_dim, self.in_dim), "weight"),
+                                           (bias, (self.out_dim,), "bias"))])
+        _check(self._lib.mhsa_fp8_linear_load(self._h, dtype, *ptrs))
+
+    def load_codes(self, codes, scales, bias=None) -> None:
+        """codes [out, in] (uint8 or float8_e4m3fn), scales [ceil(out/128),
+        ceil(in/128)] uint8 (value = code * 2^(scale - 127)), bias float32."""
+        keep, ptrs = _load_codes([((codes, (self.out_dim, self.in_dim), "codes"),
+                                   (scales, (_blocks(self.out_dim), _blocks(self.in_dim)), "scales"),
+                                   (bias, (self.out_dim,), "bias"))])
+        _check(self._lib.mhsa_fp8_linear_load_codes(self._h, *ptrs))
+
+    def read_codes(self):
+        """(codes, scales) as load_codes takes them, uint8 on the host."""
+        codes = np.empty((self.out_dim, self.in_dim), np.uint8)
+        scales = np.empty((_blocks(self.out_dim), _blocks(self.in_dim)), np.uint8)
+        _check(self._lib.mhsa_fp8_linear_read_codes(self._h, codes.ctypes.data, scales.ctypes.data))
+        return codes, scales
+
+    def forward(self, x, out_dtype=None, out=None):
+        """x [..., in] float32 or bfloat16, rows evenly spaced; the result in
+        out_dtype (x's by default), or in `out` [..., out]."""
+        import torch
+        rows, ldx = _rows_of(x, self.in_dim)
+        xd = _dtype_code(x.dtype)
+        if out is None:
+            out = torch.empty((*x.shape[:-1], self.out_dim), device=x.device,
+                              dtype=x.dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
+            ldo = self.out_dim
+        else:
+            n, ldo = _rows_of(out, self.out_dim)
+            if n != rows or out.device != x.device or (out_dtype is not None and _dtype_code(out_dtype) != _dtype_code(out.dtype)):
+                raise MhsaError(MHSA_EINVAL, f"out: expected {rows} rows on {x.device}")
+        with _OnDevice(x) as stream:
+            need = self._lib.mhsa_fp8_linear_workspace(self._h, rows)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
+            _check(self._lib.mhsa_fp8_linear_forward(self._h, x.data_ptr(), xd, rows, ldx, out.data_ptr(),
+                                                     _dtype_code(out.dtype), ldo, ws.data_ptr() if need > 0 else None,
+                                                     max(need, 0), stream))
+        return out
+
+
+ROUTE_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def route(logits, top_k: int, score: str = "softmax", bias=None, n_groups: int = 1, topk_groups: int = 1,
+          renormalize: bool = False, scale: float = 1.0):
+    """(indices int32, weights float32) [..., top_k] of the experts that the
+    gate's logits [..., n_experts] choose (mhsa_route): by score plus bias,
+    within the topk_groups best of n_groups groups; -1 where none is left."""
+    import torch
+    if score not in ROUTE_SCORES:
+        raise MhsaError(MHSA_ENOTSUP, f"score `{score}` (only softmax and sigmoid are supported)")
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
+        raise MhsaError(MHSA_EINVAL, "expected a GPU tensor [..., n_experts]")
+    n = logits.shape[-1]
+    rows, ld = _rows_of(logits, n)
+    if bias is not None and (bias.device != logits.device or bias.dtype != torch.float32 or tuple(bias.shape) != (n,)
+                             or not bias.is_contiguous()):
+        raise MhsaError(MHSA_EINVAL, f"bias: expected a contiguous float32 tensor [{n}] on {logits.device}")
+    shape = (*logits.shape[:-1], top_k if top_k > 0 else 0)
+    idx = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    w = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    with _OnDevice(logits) as stream:
+        _check(library().mhsa_route(logits.data_ptr(), _dtype_code(logits.dtype), rows, n, ld, ROUTE_SCORES[score],
+                                    None if bias is None else bias.data_ptr(), n_groups, topk_groups, top_k,
+                                    1 if renormalize else 0, float(scale), idx.data_ptr(), w.data_ptr(), stream))
+    return idx, w
+
+
+class ExpertFeedForward:
+    """FeedForward by experts, linear2(silu(linear1(x))) of the experts that
+    `route` chose for each frame, weighted and summed; weights and activations
+    as Fp8Linear's (mhsa_experts_*)."""
+
+    def __init__(self, n_experts: int, d_model: int, ff_dim: int, use_bias: bool = False):
+        lib = library()
+        h = ctypes.c_void_p()
+        _check(lib.mhsa_experts_create(n_experts, d_model, ff_dim, 1 if use_bias else 0, ctypes.byref(h)))
+        self._h, self._lib = h, lib
+        self.n_experts, self.d_model, self.ff_dim = n_experts, d_model, ff_dim
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            self._lib.mhsa_experts_destroy(h)
+            self._h = None
+
+    def load(self, weight1, weight2, bias1=None, bias2=None) -> None:
+        """weight1 [n_experts, ff_dim, d_model], weight2 [n_experts, d_model,
+        ff_dim] of one float dtype, rounded to codes."""
+        e, d, f = self.n_experts, self.d_model, self.ff_dim
+        keep, ptrs, dtype = _load_floats([((weight1, (e, f, d), "weight1"), (bias1, (e, f), "bias1")),
+                                          ((weight2, (e, d, f), "weight2"), (bias2, (e, d), "bias2"))])
+        _check(self._lib.mhsa_experts_load(self._h, dtype, *ptrs))
+
+    def load_codes(self, codes1, scales1, codes2, scales2, bias1=None, bias2=None) -> None:
+        """The experts' matrices as Fp8Linear.load_codes takes them, stacked."""
+        e, d, f = self.n_experts, self.d_model, self.ff_dim
+        keep, ptrs = _load_codes([((codes1, (e, f, d), "codes1"), (scales1, (e, _blocks(f), _blocks(d)), "scales1"),
+                                   (bias1, (e, f), "bias1")),
+                                  ((codes2, (e, d, f), "codes2"), (scales2, (e, _blocks(d), _blocks(f)), "scales2"),
+                                   (bias2, (e, d), "bias2"))])
+        _check(self._lib.mhsa_experts_load_codes(self._h, *ptrs))
+
+    def forward(self, x, indices, weights, residual=None, res_scale: float = 1.0, out=None):
+        """residual + res_scale * sum_j weights[..., j] * FF_indices[..., j](x);
+        x, residual and out [..., d_model] contiguous, float32 or bfloat16;
+        indices int32 and weights float32 [..., top_k] as `route` gives them.
+        out may be the residual."""
+        import torch
+        if not isinstance(x, torch.Tensor) or not x.is_cuda or not x.is_contiguous() or x.dim() < 1 or x.shape[-1] != self.d_model:
+            raise MhsaError(MHSA_EINVAL, f"expected a contiguous GPU tensor [..., {self.d_model}]")
+        dtype = _dtype_code(x.dtype)
+        top_k = indices.shape[-1] if indices.dim() else 0
+        for t, want, name in ((indices, torch.int32, "indices"), (weights, torch.float32, "weights")):
+            if t.dtype != want or t.device != x.device or not t.is_contiguous() or t.shape != (*x.shape[:-1], top_k):
+                raise MhsaError(MHSA_EINVAL, f"{name}: expected contiguous {want} [..., top_k] beside x")
+        for t in (residual, out):
+            if t is not None and (t.dtype != x.dtype or t.device != x.device or t.shape != x.shape or not t.is_contiguous()):
+                raise MhsaError(MHSA_EINVAL, "residual and out are to be like x")
+        if out is None:
+            out = torch.empty_like(x)
+        rows = x.numel() // self.d_model
+        with _OnDevice(x) as stream:
+            need = self._lib.mhsa_experts_workspace(self._h, rows, top_k)
+            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
+            _check(self._lib.mhsa_experts_forward(self._h, x.data_ptr(), dtype, rows, indices.data_ptr(),
+                                                  weights.data_ptr(), top_k,
+                                                  None if residual is None else residual.data_ptr(), float(res_scale),
+                                                  out.data_ptr(), ws.data_ptr(), max(need, 0), stream))
         return out
 
 
