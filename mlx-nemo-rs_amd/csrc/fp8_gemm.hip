@@ -252,23 +252,27 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
 // ---------------------------------------------------------------------------
 // Tiles
 //
-// A workgroup of 4 waves (2 x 2) computes a BM x BN tile from LDS stages of
-// 128 inputs, one block: rows of 128 bytes whose eight 16-byte chunks are
-// stored XOR-permuted by (row / 2) % 8 (the 32 rows of a fragment read then
-// lie on all 64 banks), filled by direct-to-LDS loads that run NS - 1 stages
-// ahead. A 32x32x64 MFMA takes 32 bytes of each operand from a lane; the weight
-// is its first operand, so a lane's accumulators hold four consecutive output
-// columns of one row. Row scales come with the stages, 4 stages to a word;
-// the weight's scale is one byte per wave and stage, read from a lane of a
-// register that holds all of them.
+// A workgroup of 4 waves (2 x 2) computes a BM x BN tile from a ring of NS LDS
+// stages of 64 inputs: rows of 64 bytes whose four 16-byte chunks are stored
+// XOR-permuted by (row / 4) % 4 (the 16 rows that a fragment read takes at a
+// time then lie on all 64 banks), filled by direct-to-LDS loads. A 32x32x64
+// MFMA takes 32 bytes of each operand from a lane; the weight is its first
+// operand, so a lane's accumulators hold four consecutive output columns of
+// one row. A stage's fragments are read into registers while the MFMAs of the
+// stage before run, so a stage's buffer is free again one stage later and
+// loads run NS - 1 stages ahead of their wait (with stages of 128 inputs and
+// two buffers they had half a stage, and a 256 x 256 tile's stage took 2.2
+// us where its MFMAs take 0.85). Row scales come with the stages, 8 stages to a
+// word; the weight's scale is one byte per wave and block, read from a lane
+// of a register that holds all of them.
 // ---------------------------------------------------------------------------
 
 template <int BM, int BN, int NS_>
 struct Fp8Cfg {
-  static constexpr int NS = NS_, DIST = NS - 1;
+  static constexpr int NS = NS_;
   static constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
-  static constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
-  static constexpr int NA = BM / 32, NB = BN / 32;  // 1 KB loads per wave and stage
+  static constexpr int ABYTES = BM * 64, STAGE = (BM + BN) * 64;
+  static constexpr int NA = BM / 64, NB = BN / 64;  // 1 KB loads per wave and stage
   static constexpr int OP = WN * 4 + 16;            // pitch of a staged output row
   static constexpr int STG = 4 * 32 * OP, AMAX = 2 * BM * 4;
   static constexpr int SCALES = NS * STAGE;         // two words a row behind the stages
@@ -277,13 +281,13 @@ struct Fp8Cfg {
   static_assert(LDS <= 160 * 1024, "tile exceeds LDS");
 };
 
-template <int BM, int BN, int NS, bool EXACT, int EPI>
+template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
 __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   using C = Fp8Cfg<BM, BN, NS>;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w >> 1, wn = w & 1;
-  const int kb = (p.K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4;
+  const int kb = (p.K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4, nk = 2 * kb;
 
   // contiguous tile ranges per XCD, walked 8 row tiles at a time
   const bool grouped = p.g.tile != nullptr;
@@ -313,11 +317,12 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     row = min(row, rows - 1);
     return gather ? (uint32_t)(p.g.pair[m0 + row] / p.g.top_k) : (uint32_t)row;
   };
+  // load g of wave w fills 16 LDS rows: lane l row l / 4, stored chunk l % 4
   int aoff[C::NA];
 #pragma unroll
   for (int g = 0; g < C::NA; ++g) {
-    const int pos = (w * C::NA + g) * 64 + lane, row = pos >> 3;
-    aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((pos & 7) ^ ((row >> 1) & 7)));
+    const int row = (w * C::NA + g) * 16 + (lane >> 2);
+    aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 3) ^ ((row >> 2) & 3)));
   }
   const int srow = (w * 64) % BM;
   const int soff = (int)(source(srow + lane) * (uint32_t)kbp);
@@ -327,149 +332,139 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   int boff[C::NB];
 #pragma unroll
   for (int g = 0; g < C::NB; ++g) {
-    const int pos = (w * C::NB + g) * 64 + lane, row = pos >> 3;
-    boff[g] = row * kp + 16 * ((pos & 7) ^ ((row >> 1) & 7));
+    const int row = (w * C::NB + g) * 16 + (lane >> 2);
+    boff[g] = row * kp + 16 * ((lane & 3) ^ ((row >> 2) & 3));
   }
   // the weight scales of this wave's 128-column block, a word of 4 to a lane
   const int wblk = min((n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
   const uint32_t wword = *reinterpret_cast<const uint32_t*>(p.ws + expert * p.ws_stride + (int64_t)wblk * kbp +
                                                             4 * min(lane, kbp / 4 - 1));
-  auto issue = [&](int kt, int buf) {
-    char* S = smem + buf * C::STAGE;
-#pragma unroll
-    for (int g = 0; g < C::NA; ++g)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(S + (w * C::NA + g) * 1024), 16, aoff[g], kt * 128, 0, 0);
-#pragma unroll
-    for (int g = 0; g < C::NB; ++g)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(S + C::ABYTES + (w * C::NB + g) * 1024), 16, boff[g],
-                                               kt * 128, 0, 0);
-    // (a word is loaded again by each of its stages, and by two waves of a
-    // tile of under 256 rows: always the same bytes)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((kt >> 2) & 1) * BM * 4 + srow * 4), 4,
-                                             soff, kt & ~3, 0, 0);
-  };
   constexpr int LOADS = C::NA + C::NB + 1;
-  auto landed = [&](int behind) {  // this wave's loads but the last `behind` stages' are in LDS
-    switch (behind) {
-      case 0: __builtin_amdgcn_s_waitcnt(7 << 4); break;
-      case 1: __builtin_amdgcn_s_waitcnt((LOADS & 15) | ((LOADS >> 4) << 14) | (7 << 4)); break;
-      default: __builtin_amdgcn_s_waitcnt(((2 * LOADS) & 15) | (((2 * LOADS) >> 4) << 14) | (7 << 4)); break;
-    }
+  auto issue1 = [&](int g, int kt) {  // load g of stage kt
+    char* S = smem + kt % NS * C::STAGE;
+    const int k = min(kt, nk - 1);  // (past the end: the last stage again, unread)
+    if (g < C::NA)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(S + (w * C::NA + g) * 1024), 16, aoff[g], k * 64, 0, 0);
+    else if (g < C::NA + C::NB)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(S + C::ABYTES + (w * C::NB + g - C::NA) * 1024), 16,
+                                               boff[g - C::NA], k * 64, 0, 0);
+    else  // a word is loaded again by each of its stages, and by two waves of
+          // a tile of under 256 rows: always the same bytes
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((k >> 3) & 1) * BM * 4 + srow * 4), 4,
+                                               soff, (k >> 3) * 4, 0, 0);
   };
-  static_assert(C::DIST >= 1 && C::DIST <= 3 && 2 * LOADS < 64, "wait counts");
+  auto landed = [&]() {  // the last NS - 2 stages' loads may still be in flight
+    constexpr int vm = (NS - 2) * LOADS;
+    static_assert(NS >= 2 && vm < 64, "wait count");
+    __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));  // lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+  };
 
-  const int arow = (wm * C::WM + (lane & 31)) * 128;
-  const int brow = C::ABYTES + (wn * C::WN + (lane & 31)) * 128;
-  floatx16 acc[C::TN][C::TM];
+  const int arow = (wm * C::WM + (lane & 31)) * 64;
+  const int brow = C::ABYTES + (wn * C::WN + (lane & 31)) * 64;
+  int off[2];  // this lane's two chunks of a row
+#pragma unroll
+  for (int u = 0; u < 2; ++u) off[u] = 16 * ((2 * half + u) ^ ((lane >> 2) & 3));
+  u32x4 fa[2][C::TM][2], fb[2][C::TN][2];
+  int xs[2][C::TM], ws[2];
+  auto rd = [&](int kt, int b) {  // fragments and scales of stage kt (past the end: of the last, unused)
+    const char* S = smem + kt % NS * C::STAGE;
+    const int k = min(kt, nk - 1);
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) fa[b][i][u] = *reinterpret_cast<const u32x4*>(S + arow + off[u] + i * 2048);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) fb[b][j][u] = *reinterpret_cast<const u32x4*>(S + brow + off[u] + j * 2048);
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+      xs[b][i] = *reinterpret_cast<const int*>(smem + C::SCALES + ((k >> 3) & 1) * BM * 4 +
+                                               (wm * C::WM + 32 * i + (lane & 31)) * 4) >> (8 * ((k >> 1) & 3));
+    ws[b] = __builtin_amdgcn_readlane((int)wword, k >> 3) >> (8 * ((k >> 1) & 3));
+  };
+  floatx16 acc[C::TN][C::TM], part[EXACT ? C::TN : 1][EXACT ? C::TM : 1];
 #pragma unroll
   for (int j = 0; j < C::TN; ++j)
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
-  int xs[C::TM], xn[C::TM];
-  auto scales_of = [&](int kt) {
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i)
-      xn[i] = *reinterpret_cast<const int*>(smem + C::SCALES + ((kt >> 2) & 1) * BM * 4 +
-                                            (wm * C::WM + 32 * i + (lane & 31)) * 4) >> (8 * (kt & 3));
-  };
-  auto chunk = [&](int base, int c) { return base + 16 * (c ^ ((lane >> 1) & 7)); };
 
+  // stage kt: its fragments are in set kt % 2
+  auto stage = [&](int kt, int par) {
+    landed();  // stage kt + 1, everywhere; stage kt's buffer has been read
+    rd(kt + 1, par ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int NM = C::TM * C::TN;
+    // the loads of stage kt + NS, into stage kt's buffer, between the MFMAs
+    constexpr int PER = (LOADS + NM - 1) / NM;
+    if constexpr (!EXACT) {
 #pragma unroll
-  for (int st = 0; st < C::DIST; ++st) issue(min(st, kb - 1), st);
-  landed(C::DIST - 1);
-  asm volatile("s_barrier" ::: "memory");
-
-  if constexpr (!EXACT) {
-    i32x8 fa[2][C::TM], fb[2][C::TN];
-    auto rd = [&](const char* S, int s, int b) {
-      const int c = 4 * s + 2 * half;
+      for (int m = 0; m < NM; ++m) {
+        const int j = m / C::TM, i = m % C::TM;
+        auto whole = [](const u32x4* f) {
+          return i32x8{(int)f[0][0], (int)f[0][1], (int)f[0][2], (int)f[0][3],
+                       (int)f[1][0], (int)f[1][1], (int)f[1][2], (int)f[1][3]};
+        };
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[par][j]), whole(fa[par][i]), acc[j][i], 0, 0, 0,
+                                                                    ws[par], 0, xs[par][i]);
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        reinterpret_cast<u32x4*>(&fa[b][i])[0] = *reinterpret_cast<const u32x4*>(S + chunk(arow, c) + i * 4096);
-        reinterpret_cast<u32x4*>(&fa[b][i])[1] = *reinterpret_cast<const u32x4*>(S + chunk(arow, c + 1) + i * 4096);
+        for (int g = m * PER; g < (m + 1) * PER; ++g)
+          if (g < LOADS) issue1(g, kt + NS);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+      // exact products and f32 sums: per block on the bf16 cores, then added
+      // with the block's power of two
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) {
-        reinterpret_cast<u32x4*>(&fb[b][j])[0] = *reinterpret_cast<const u32x4*>(S + chunk(brow, c) + j * 4096);
-        reinterpret_cast<u32x4*>(&fb[b][j])[1] = *reinterpret_cast<const u32x4*>(S + chunk(brow, c + 1) + j * 4096);
-      }
-    };
-    scales_of(0);
-    rd(smem, 0, 0);
-    for (int kt = 0; kt < kb; ++kt) {
-      const char* S = smem + kt % NS * C::STAGE;
-      // the buffer that stage kt + DIST fills was last read in stage kt - 1
-      issue(min(kt + C::DIST, kb - 1), (kt + C::DIST) % NS);
-      const int ws = __builtin_amdgcn_readlane((int)wword, kt >> 2) >> (8 * (kt & 3));
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i) xs[i] = xn[i];
-      rd(S, 1, 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[0][j], fa[0][i], acc[j][i], 0, 0, 0, ws, 0, xs[i]);
-      __builtin_amdgcn_sched_barrier(0);
-      landed(C::DIST - 1);
-      asm volatile("s_barrier" ::: "memory");
-      scales_of(min(kt + 1, kb - 1));
-      rd(smem + (kt + 1) % NS * C::STAGE, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[1][j], fa[1][i], acc[j][i], 0, 0, 0, ws, 0, xs[i]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  } else {
-    // exact products and f32 sums: per block on the bf16 cores, then added
-    // with the block's power of two
-    for (int kt = 0; kt < kb; ++kt) {
-      const char* S = smem + kt % NS * C::STAGE;
-      issue(min(kt + C::DIST, kb - 1), (kt + C::DIST) % NS);
-      const int ws = (__builtin_amdgcn_readlane((int)wword, kt >> 2) >> (8 * (kt & 3))) & 255;
-      scales_of(kt);
-      floatx16 part[C::TN][C::TM];
-#pragma unroll
-      for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i) part[j][i] = floatx16{};
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        u32x4 fa[C::TM], fb[C::TN];
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i) fa[i] = *reinterpret_cast<const u32x4*>(S + chunk(arow, 2 * t + half) + i * 4096);
-#pragma unroll
-        for (int j = 0; j < C::TN; ++j) fb[j] = *reinterpret_cast<const u32x4*>(S + chunk(brow, 2 * t + half) + j * 4096);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          bf16x8 xa[C::TM], xb[C::TN];
-#pragma unroll
-          for (int i = 0; i < C::TM; ++i) xa[i] = fp8_to_bf16(fa[i][2 * u], fa[i][2 * u + 1]);
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[j][2 * u], fb[j][2 * u + 1]);
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-            for (int i = 0; i < C::TM; ++i) part[j][i] = mma32(xb[j], xa[i], part[j][i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const int e = (xn[i] & 255) + ws - 254;
+      for (int g = 0; g < LOADS; ++g) issue1(g, kt + NS);
+      if (par == 0) {
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[j][i][r] += __builtin_ldexpf(part[j][i][r], e);
+          for (int i = 0; i < C::TM; ++i) part[j][i] = floatx16{};
       }
-      landed(C::DIST - 1);
-      asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        bf16x8 xa[C::TM], xb[C::TN];
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) xa[i] = fp8_to_bf16(fa[par][i][u >> 1][2 * (u & 1)], fa[par][i][u >> 1][2 * (u & 1) + 1]);
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[par][j][u >> 1][2 * (u & 1)], fb[par][j][u >> 1][2 * (u & 1) + 1]);
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int i = 0; i < C::TM; ++i) part[j][i] = mma32(xb[j], xa[i], part[j][i]);
+      }
+      if (par == 1) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+          const int e = (xs[par][i] & 255) + (ws[par] & 255) - 254;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[j][i][r] += __builtin_ldexpf(part[j][i][r], e);
+        }
+      }
     }
+  };
+#pragma unroll
+  for (int st = 0; st < NS; ++st)
+#pragma unroll
+    for (int g = 0; g < LOADS; ++g) issue1(g, st);
+  {
+    constexpr int vm = (NS - 1) * LOADS;
+    static_assert(vm < 64, "wait count");
+    __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));
+    asm volatile("s_barrier" ::: "memory");
   }
-  // the clamped loads of the last stages still write LDS: all of them are to
-  // have landed before the epilogue reuses it
+  rd(0, 0);
+  for (int kt = 0; kt < nk; kt += 2) {
+    stage(kt, 0);
+    stage(kt + 1, 1);
+  }
+  // the loads past the end still write LDS: all of them are to have landed
+  // before the epilogue reuses it
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
 
@@ -538,9 +533,16 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
         p.out_scales[(int64_t)(m0 + row0 + lane) * nbp + col0 / 128] = (uint8_t)s;
     }
   } else {
-    const bool b16 = EPI == kFp8Out && p.out_dt == kBF16;
-    const int V = b16 ? 8 : 4;  // columns of a 16-byte store
-    const bool vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ldo % V == 0;
+    // 32 rows at a time through LDS, so that a store is 16 bytes of a run of
+    // the row. A lane has the same columns of every row it stores.
+    constexpr int V = 16 / sizeof(TOut), RUNS = C::WN / V, RPI = 64 / RUNS;
+    static_assert(64 % RUNS == 0, "whole rows a store");
+    const int c = lane % RUNS * V, col = col0 + c;
+    TOut* out = reinterpret_cast<TOut*>(p.out);
+    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.ldo % V == 0 && col + V <= p.N;
+    float b[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = p.bias && col + e < p.N ? p.bias[(int64_t)expert * p.N + col + e] : 0.f;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
 #pragma unroll
@@ -549,53 +551,46 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<floatx4*>(st + (lane & 31) * C::OP + (32 * j + 8 * q + 4 * half) * 4) =
               floatx4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-      const int runs = C::WN / V;
-      for (int id = lane; id < 32 * runs; id += 64) {
-        const int r = id / runs, c = id % runs * V, col = col0 + c, row = wm * C::WM + 32 * i + r;
-        if (row >= rows || col >= p.N) continue;
-        const int64_t orow = EPI == kFp8Pair ? p.g.pair[m0 + row] : m0 + row;
-        float f[8];
-        *reinterpret_cast<floatx4*>(f) = *reinterpret_cast<const floatx4*>(st + r * C::OP + c * 4);
-        if (b16) *reinterpret_cast<floatx4*>(f + 4) = *reinterpret_cast<const floatx4*>(st + r * C::OP + c * 4 + 16);
-        if (p.bias) {
-          const float* b = p.bias + (int64_t)expert * p.N + col;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < V && col + e < p.N) f[e] += b[e];
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int r = it * RPI + lane / RUNS, row = wm * C::WM + 32 * i + r;
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+          const floatx4 t = *reinterpret_cast<const floatx4*>(st + r * C::OP + (c + e) * 4);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) f[e + u] = t[u] + b[e + u];
         }
-        if (vec && col + V <= p.N) {
-          if (b16) {
-            bf16x8 v;
+        if (row >= rows || col >= p.N) continue;
+        TOut* to = out + (EPI == kFp8Pair ? (int64_t)p.g.pair[m0 + row] : (int64_t)(m0 + row)) * p.ldo + col;
+        if (vec) {
+          TOut v[V];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (bf16)f[e];
-            *reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(p.out) + orow * p.ldo + col) = v;
-          } else {
-            *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(p.out) + orow * p.ldo + col) =
-                floatx4{f[0], f[1], f[2], f[3]};
-          }
+          for (int e = 0; e < V; ++e) v[e] = (TOut)f[e];
+          *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(v);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < V && col + e < p.N) store_as(b16 ? kBF16 : kF32, p.out, orow * p.ldo + col + e, f[e]);
+          for (int e = 0; e < V; ++e)
+            if (col + e < p.N) to[e] = (TOut)f[e];
         }
       }
     }
   }
 }
 
-template <int BM, int BN, int NS, bool EXACT, int EPI>
+template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
 __global__ __launch_bounds__(256, 1) void fp8_tile_kernel(Fp8Gemm p) {
   __shared__ __attribute__((aligned(1024))) char smem[Fp8Cfg<BM, BN, NS>::LDS];
-  fp8_tile_body<BM, BN, NS, EXACT, EPI>(p, smem);
+  fp8_tile_body<BM, BN, NS, EXACT, EPI, TOut>(p, smem);
 }
 
-template <int BM, int BN, int NS, bool EXACT, int EPI>
+template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
 hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
   const int64_t tm = p.g.tile ? p.g.max_tiles : (p.M + BM - 1) / BM;
   const int64_t nt = tm * ((p.N + BN - 1) / BN);
   if (p.g.tile && p.g.tile_rows != BM) return hipErrorInvalidValue;
   if (nt > (int64_t)1 << 28) return hipErrorInvalidValue;
-  fp8_tile_kernel<BM, BN, NS, EXACT, EPI><<<(unsigned)((nt + 7) / 8 * 8), 256, 0, s>>>(p);
+  fp8_tile_kernel<BM, BN, NS, EXACT, EPI, TOut><<<(unsigned)((nt + 7) / 8 * 8), 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
@@ -690,19 +685,25 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
   if (p.g.tile) {
     if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll) return hipErrorInvalidValue;
     if (p.epilogue == kFp8HiddenQ)
-      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8HiddenQ>(p, s)
-                                  : launch_tile<128, 128, 2, false, kFp8HiddenQ>(p, s);
+      return p.g.tile_rows == 256 ? launch_tile<256, 256, 4, false, kFp8HiddenQ, float>(p, s)
+                                  : launch_tile<128, 128, 4, false, kFp8HiddenQ, float>(p, s);
     if (p.epilogue == kFp8Pair)
-      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8Pair>(p, s)
-                                  : launch_tile<128, 128, 2, false, kFp8Pair>(p, s);
+      return p.g.tile_rows == 256 ? launch_tile<256, 256, 4, false, kFp8Pair, float>(p, s)
+                                  : launch_tile<128, 128, 4, false, kFp8Pair, float>(p, s);
     return hipErrorInvalidValue;
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
-  const int64_t t128 = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128), t256 = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   if (p.out_dt == kF32)
-    return t128 >= 128 ? launch_tile<128, 128, 2, true, kFp8Out>(p, s) : launch_tile<64, 64, 3, true, kFp8Out>(p, s);
-  if (t256 >= 128) return launch_tile<256, 256, 2, false, kFp8Out>(p, s);
-  return t128 >= 128 ? launch_tile<128, 128, 2, false, kFp8Out>(p, s) : launch_tile<64, 64, 4, false, kFp8Out>(p, s);
+    return tiles(128, 128) >= 128 ? launch_tile<128, 128, 4, true, kFp8Out, float>(p, s)
+                                  : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
+  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256);
+  if (t256 >= 128) {
+    if ((t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256) return launch_tile<192, 256, 4, false, kFp8Out, bf16>(p, s);
+    return launch_tile<256, 256, 4, false, kFp8Out, bf16>(p, s);
+  }
+  return tiles(128, 128) >= 128 ? launch_tile<128, 128, 4, false, kFp8Out, bf16>(p, s)
+                                : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
 }
 
 }  // namespace mhsa
