@@ -366,23 +366,22 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) off[u] = 16 * ((2 * half + u) ^ ((lane >> 2) & 3));
   u32x4 fa[2][C::TM][2], fb[2][C::TN][2];
-  int xs[2][C::TM], ws[2];
-  auto rd = [&](int kt, int b) {  // fragments and scales of stage kt (past the end: of the last, unused)
+  int xw[2][C::TM];
+  // read r of stage kt into set b: its fragments (the weight's first, then the
+  // rows'), then the row scales (past the end: of the last stage, unused)
+  constexpr int READS = 2 * (C::TM + C::TN) + C::TM;
+  auto rd1 = [&](int r, int kt, int b) {
     const char* S = smem + kt % NS * C::STAGE;
-    const int k = min(kt, nk - 1);
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) fa[b][i][u] = *reinterpret_cast<const u32x4*>(S + arow + off[u] + i * 2048);
-#pragma unroll
-    for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) fb[b][j][u] = *reinterpret_cast<const u32x4*>(S + brow + off[u] + j * 2048);
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i)
-      xs[b][i] = *reinterpret_cast<const int*>(smem + C::SCALES + ((k >> 3) & 1) * BM * 4 +
-                                               (wm * C::WM + 32 * i + (lane & 31)) * 4) >> (8 * ((k >> 1) & 3));
-    ws[b] = __builtin_amdgcn_readlane((int)wword, k >> 3) >> (8 * ((k >> 1) & 3));
+    if (r < 2 * C::TN) {
+      fb[b][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + brow + off[r % 2] + r / 2 * 2048);
+    } else if (r < 2 * (C::TM + C::TN)) {
+      r -= 2 * C::TN;
+      fa[b][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + arow + off[r % 2] + r / 2 * 2048);
+    } else {
+      const int i = r - 2 * (C::TM + C::TN), k = min(kt, nk - 1);
+      xw[b][i] = *reinterpret_cast<const int*>(smem + C::SCALES + ((k >> 3) & 1) * BM * 4 +
+                                               (wm * C::WM + 32 * i + (lane & 31)) * 4);
+    }
   };
   floatx16 acc[C::TN][C::TM], part[EXACT ? C::TN : 1][EXACT ? C::TM : 1];
 #pragma unroll
@@ -390,34 +389,46 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
 
-  // stage kt: its fragments are in set kt % 2
+  // Stage kt, whose fragments are in set kt % 2 (par). After the barrier its
+  // MFMAs start at once; the reads of stage kt + 1's fragments and the loads
+  // of stage kt + NS, into stage kt's buffer, are placed between them (issued
+  // ahead of the MFMAs, the reads filled the wave's queue of 15 and held the
+  // first MFMA back).
   auto stage = [&](int kt, int par) {
     landed();  // stage kt + 1, everywhere; stage kt's buffer has been read
-    rd(kt + 1, par ^ 1);
+    const int sh = 8 * ((kt >> 1) & 3), ws = __builtin_amdgcn_readlane((int)wword, kt >> 3) >> sh;
+    int xs[C::TM];
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) xs[i] = xw[par][i] >> sh;
     __builtin_amdgcn_sched_barrier(0);
-    constexpr int NM = C::TM * C::TN;
-    // the loads of stage kt + NS, into stage kt's buffer, between the MFMAs
-    constexpr int PER = (LOADS + NM - 1) / NM;
+    // MFMA m of NMF; reads go behind the first MFMAs, loads behind the later
+    constexpr int NMF = EXACT ? 4 * C::TM * C::TN : C::TM * C::TN;
+    constexpr int RPM = (READS + (NMF + 1) / 2 - 1) / ((NMF + 1) / 2), LPM = (LOADS + (NMF + 1) / 2 - 1) / ((NMF + 1) / 2);
+    auto between = [&](int m) {
+#pragma unroll
+      for (int r = m * RPM; r < (m + 1) * RPM; ++r)
+        if (r < READS) rd1(r, kt + 1, par ^ 1);
+      const int l = m - NMF / 2;
+#pragma unroll
+      for (int g = l * LPM; g < (l + 1) * LPM; ++g)
+        if (g >= 0 && g < LOADS) issue1(g, kt + NS);
+      __builtin_amdgcn_sched_barrier(0);
+    };
     if constexpr (!EXACT) {
 #pragma unroll
-      for (int m = 0; m < NM; ++m) {
+      for (int m = 0; m < NMF; ++m) {
         const int j = m / C::TM, i = m % C::TM;
         auto whole = [](const u32x4* f) {
           return i32x8{(int)f[0][0], (int)f[0][1], (int)f[0][2], (int)f[0][3],
                        (int)f[1][0], (int)f[1][1], (int)f[1][2], (int)f[1][3]};
         };
         acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[par][j]), whole(fa[par][i]), acc[j][i], 0, 0, 0,
-                                                                    ws[par], 0, xs[par][i]);
-#pragma unroll
-        for (int g = m * PER; g < (m + 1) * PER; ++g)
-          if (g < LOADS) issue1(g, kt + NS);
-        __builtin_amdgcn_sched_barrier(0);
+                                                                    ws, 0, xs[i]);
+        between(m);
       }
     } else {
       // exact products and f32 sums: per block on the bf16 cores, then added
       // with the block's power of two
-#pragma unroll
-      for (int g = 0; g < LOADS; ++g) issue1(g, kt + NS);
       if (par == 0) {
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
@@ -432,14 +443,16 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 #pragma unroll
         for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[par][j][u >> 1][2 * (u & 1)], fb[par][j][u >> 1][2 * (u & 1) + 1]);
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-          for (int i = 0; i < C::TM; ++i) part[j][i] = mma32(xb[j], xa[i], part[j][i]);
+        for (int m = 0; m < C::TM * C::TN; ++m) {
+          const int j = m / C::TM, i = m % C::TM;
+          part[j][i] = mma32(xb[j], xa[i], part[j][i]);
+          between(u * C::TM * C::TN + m);
+        }
       }
       if (par == 1) {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i) {
-          const int e = (xs[par][i] & 255) + (ws[par] & 255) - 254;
+          const int e = (xs[i] & 255) + (ws & 255) - 254;
 #pragma unroll
           for (int j = 0; j < C::TN; ++j)
 #pragma unroll
@@ -458,7 +471,8 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));
     asm volatile("s_barrier" ::: "memory");
   }
-  rd(0, 0);
+#pragma unroll
+  for (int r = 0; r < READS; ++r) rd1(r, 0, 0);
   for (int kt = 0; kt < nk; kt += 2) {
     stage(kt, 0);
     stage(kt + 1, 1);
