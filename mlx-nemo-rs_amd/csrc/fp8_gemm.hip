@@ -253,26 +253,26 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
 // Tiles
 //
 // A workgroup of 4 waves (2 x 2) computes a BM x BN tile from a ring of NS LDS
-// stages of 64 inputs: rows of 64 bytes whose four 16-byte chunks are stored
-// XOR-permuted by (row / 4) % 4 (the 16 rows that a fragment read takes at a
-// time then lie on all 64 banks), filled by direct-to-LDS loads. A 32x32x64
-// MFMA takes 32 bytes of each operand from a lane; the weight is its first
-// operand, so a lane's accumulators hold four consecutive output columns of
-// one row. A stage's fragments are read into registers while the MFMAs of the
-// stage before run, so a stage's buffer is free again one stage later and
-// loads run NS - 1 stages ahead of their wait (with stages of 128 inputs and
-// two buffers they had half a stage, and a 256 x 256 tile's stage took 2.2
-// us where its MFMAs take 0.85). Row scales come with the stages, 8 stages to a
-// word; the weight's scale is one byte per wave and block, read from a lane
-// of a register that holds all of them.
+// stages of 128 inputs, one block: rows of 128 bytes whose eight 16-byte
+// chunks are stored XOR-permuted by (row / 2) % 8 (the 16 rows that a fragment
+// read takes at a time then lie on all 64 banks), filled by direct-to-LDS
+// loads of whole 128-byte lines. A 32x32x64 MFMA takes 32 bytes of each
+// operand from a lane; the weight is its first operand, so a lane's
+// accumulators hold four consecutive output columns of one row. A stage is two
+// halves of 64 inputs. A half's fragments are read into registers between the
+// MFMAs of the half before, so all of a stage has been read when its second
+// half begins: there is the stage's one barrier, behind which the loads that
+// refill its buffer are issued. Row scales come with the stages, 4 stages to a
+// word; the weight's scale is one byte per wave and stage, read from a lane of
+// a register that holds all of them.
 // ---------------------------------------------------------------------------
 
 template <int BM, int BN, int NS_>
 struct Fp8Cfg {
   static constexpr int NS = NS_;
   static constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
-  static constexpr int ABYTES = BM * 64, STAGE = (BM + BN) * 64;
-  static constexpr int NA = BM / 64, NB = BN / 64;  // 1 KB loads per wave and stage
+  static constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  static constexpr int NA = BM / 32, NB = BN / 32;  // 1 KB loads per wave and stage
   static constexpr int OP = WN * 4 + 16;            // pitch of a staged output row
   static constexpr int STG = 4 * 32 * OP, AMAX = 2 * BM * 4;
   static constexpr int SCALES = NS * STAGE;         // two words a row behind the stages
@@ -287,7 +287,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w >> 1, wn = w & 1;
-  const int kb = (p.K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4, nk = 2 * kb;
+  const int kb = (p.K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4;
 
   // contiguous tile ranges per XCD, walked 8 row tiles at a time
   const bool grouped = p.g.tile != nullptr;
@@ -317,12 +317,12 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     row = min(row, rows - 1);
     return gather ? (uint32_t)(p.g.pair[m0 + row] / p.g.top_k) : (uint32_t)row;
   };
-  // load g of wave w fills 16 LDS rows: lane l row l / 4, stored chunk l % 4
+  // load g of wave w fills 8 LDS rows: lane l row l / 8, stored chunk l % 8
   int aoff[C::NA];
 #pragma unroll
   for (int g = 0; g < C::NA; ++g) {
-    const int row = (w * C::NA + g) * 16 + (lane >> 2);
-    aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 3) ^ ((row >> 2) & 3)));
+    const int row = (w * C::NA + g) * 8 + (lane >> 3);
+    aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 7) ^ ((row >> 1) & 7)));
   }
   const int srow = (w * 64) % BM;
   const int soff = (int)(source(srow + lane) * (uint32_t)kbp);
@@ -332,8 +332,8 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   int boff[C::NB];
 #pragma unroll
   for (int g = 0; g < C::NB; ++g) {
-    const int row = (w * C::NB + g) * 16 + (lane >> 2);
-    boff[g] = row * kp + 16 * ((lane & 3) ^ ((row >> 2) & 3));
+    const int row = (w * C::NB + g) * 8 + (lane >> 3);
+    boff[g] = row * kp + 16 * ((lane & 7) ^ ((row >> 1) & 7));
   }
   // the weight scales of this wave's 128-column block, a word of 4 to a lane
   const int wblk = min((n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
@@ -342,16 +342,16 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   constexpr int LOADS = C::NA + C::NB + 1;
   auto issue1 = [&](int g, int kt) {  // load g of stage kt
     char* S = smem + kt % NS * C::STAGE;
-    const int k = min(kt, nk - 1);  // (past the end: the last stage again, unread)
+    const int k = min(kt, kb - 1);  // (past the end: the last stage again, unread)
     if (g < C::NA)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(S + (w * C::NA + g) * 1024), 16, aoff[g], k * 64, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(S + (w * C::NA + g) * 1024), 16, aoff[g], k * 128, 0, 0);
     else if (g < C::NA + C::NB)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(S + C::ABYTES + (w * C::NB + g - C::NA) * 1024), 16,
-                                               boff[g - C::NA], k * 64, 0, 0);
+                                               boff[g - C::NA], k * 128, 0, 0);
     else  // a word is loaded again by each of its stages, and by two waves of
           // a tile of under 256 rows: always the same bytes
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((k >> 3) & 1) * BM * 4 + srow * 4), 4,
-                                               soff, (k >> 3) * 4, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((k >> 2) & 1) * BM * 4 + srow * 4), 4,
+                                               soff, k & ~3, 0, 0);
   };
   auto landed = [&]() {  // the last NS - 2 stages' loads may still be in flight
     constexpr int vm = (NS - 2) * LOADS;
@@ -360,27 +360,28 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     asm volatile("s_barrier" ::: "memory");
   };
 
-  const int arow = (wm * C::WM + (lane & 31)) * 64;
-  const int brow = C::ABYTES + (wn * C::WN + (lane & 31)) * 64;
-  int off[2];  // this lane's two chunks of a row
+  const int arow = (wm * C::WM + (lane & 31)) * 128;
+  const int brow = C::ABYTES + (wn * C::WN + (lane & 31)) * 128;
+  int off[2][2];  // this lane's two chunks of a row in either half
 #pragma unroll
-  for (int u = 0; u < 2; ++u) off[u] = 16 * ((2 * half + u) ^ ((lane >> 2) & 3));
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) off[h][u] = 16 * ((4 * h + 2 * half + u) ^ ((lane >> 1) & 7));
   u32x4 fa[2][C::TM][2], fb[2][C::TN][2];
-  int xw[2][C::TM];
-  // read r of stage kt into set b: its fragments (the weight's first, then the
-  // rows'), then the row scales (past the end: of the last stage, unused)
-  constexpr int READS = 2 * (C::TM + C::TN) + C::TM;
-  auto rd1 = [&](int r, int kt, int b) {
+  int xw[C::TM];
+  // read r of half h of stage kt into set h: its fragments (the weight's
+  // first, then the rows'), then the row scales (past the end: unused)
+  constexpr int FRAGS = 2 * (C::TM + C::TN);
+  auto rd1 = [&](int r, int kt, int h) {
     const char* S = smem + kt % NS * C::STAGE;
     if (r < 2 * C::TN) {
-      fb[b][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + brow + off[r % 2] + r / 2 * 2048);
-    } else if (r < 2 * (C::TM + C::TN)) {
+      fb[h][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + brow + off[h][r % 2] + r / 2 * 4096);
+    } else if (r < FRAGS) {
       r -= 2 * C::TN;
-      fa[b][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + arow + off[r % 2] + r / 2 * 2048);
+      fa[h][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + arow + off[h][r % 2] + r / 2 * 4096);
     } else {
-      const int i = r - 2 * (C::TM + C::TN), k = min(kt, nk - 1);
-      xw[b][i] = *reinterpret_cast<const int*>(smem + C::SCALES + ((k >> 3) & 1) * BM * 4 +
-                                               (wm * C::WM + 32 * i + (lane & 31)) * 4);
+      xw[r - FRAGS] = *reinterpret_cast<const int*>(smem + C::SCALES + ((min(kt, kb - 1) >> 2) & 1) * BM * 4 +
+                                                    (wm * C::WM + 32 * (r - FRAGS) + (lane & 31)) * 4);
     }
   };
   floatx16 acc[C::TN][C::TM], part[EXACT ? C::TN : 1][EXACT ? C::TM : 1];
@@ -389,29 +390,35 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
 
-  // Stage kt, whose fragments are in set kt % 2 (par). After the barrier its
-  // MFMAs start at once; the reads of stage kt + 1's fragments and the loads
-  // of stage kt + NS, into stage kt's buffer, are placed between them (issued
-  // ahead of the MFMAs, the reads filled the wave's queue of 15 and held the
-  // first MFMA back).
-  auto stage = [&](int kt, int par) {
-    landed();  // stage kt + 1, everywhere; stage kt's buffer has been read
-    const int sh = 8 * ((kt >> 1) & 3), ws = __builtin_amdgcn_readlane((int)wword, kt >> 3) >> sh;
-    int xs[C::TM];
+  int ws = 0, xs[C::TM];
+  // Half h of stage kt, whose fragments are in set h. The reads of the next
+  // half's fragments and, in the second half, the loads of stage kt + NS are
+  // placed between the MFMAs (issued ahead of them, the reads filled the
+  // wave's queue of 15 and held the first MFMA back).
+  auto step = [&](int kt, auto hc) {
+    constexpr int h = decltype(hc)::value;
+    if constexpr (h == 0) {
+      const int sh = 8 * (kt & 3);
+      ws = __builtin_amdgcn_readlane((int)wword, kt >> 2) >> sh;
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) xs[i] = xw[par][i] >> sh;
+      for (int i = 0; i < C::TM; ++i) xs[i] = xw[i] >> sh;
+    } else {
+      landed();  // stage kt + 1, everywhere; stage kt's buffer has been read
+    }
     __builtin_amdgcn_sched_barrier(0);
-    // MFMA m of NMF; reads go behind the first MFMAs, loads behind the later
     constexpr int NMF = EXACT ? 4 * C::TM * C::TN : C::TM * C::TN;
-    constexpr int RPM = (READS + (NMF + 1) / 2 - 1) / ((NMF + 1) / 2), LPM = (LOADS + (NMF + 1) / 2 - 1) / ((NMF + 1) / 2);
+    constexpr int READS = FRAGS + (h == 1 ? C::TM : 0);
+    constexpr int SLOTS = (NMF + 1) / 2;  // behind the first MFMAs the reads, behind all the loads
+    constexpr int RPM = (READS + SLOTS - 1) / SLOTS, LPM = (LOADS + NMF - 1) / NMF;
     auto between = [&](int m) {
+      if constexpr (h == 1) {
+#pragma unroll
+        for (int g = m * LPM; g < (m + 1) * LPM; ++g)
+          if (g < LOADS) issue1(g, kt + NS);
+      }
 #pragma unroll
       for (int r = m * RPM; r < (m + 1) * RPM; ++r)
-        if (r < READS) rd1(r, kt + 1, par ^ 1);
-      const int l = m - NMF / 2;
-#pragma unroll
-      for (int g = l * LPM; g < (l + 1) * LPM; ++g)
-        if (g >= 0 && g < LOADS) issue1(g, kt + NS);
+        if (r < READS) rd1(r, kt + h, h ^ 1);
       __builtin_amdgcn_sched_barrier(0);
     };
     if constexpr (!EXACT) {
@@ -422,14 +429,14 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
           return i32x8{(int)f[0][0], (int)f[0][1], (int)f[0][2], (int)f[0][3],
                        (int)f[1][0], (int)f[1][1], (int)f[1][2], (int)f[1][3]};
         };
-        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[par][j]), whole(fa[par][i]), acc[j][i], 0, 0, 0,
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[h][j]), whole(fa[h][i]), acc[j][i], 0, 0, 0,
                                                                     ws, 0, xs[i]);
         between(m);
       }
     } else {
       // exact products and f32 sums: per block on the bf16 cores, then added
       // with the block's power of two
-      if (par == 0) {
+      if constexpr (h == 0) {
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
 #pragma unroll
@@ -439,9 +446,9 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       for (int u = 0; u < 4; ++u) {
         bf16x8 xa[C::TM], xb[C::TN];
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i) xa[i] = fp8_to_bf16(fa[par][i][u >> 1][2 * (u & 1)], fa[par][i][u >> 1][2 * (u & 1) + 1]);
+        for (int i = 0; i < C::TM; ++i) xa[i] = fp8_to_bf16(fa[h][i][u >> 1][2 * (u & 1)], fa[h][i][u >> 1][2 * (u & 1) + 1]);
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[par][j][u >> 1][2 * (u & 1)], fb[par][j][u >> 1][2 * (u & 1) + 1]);
+        for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[h][j][u >> 1][2 * (u & 1)], fb[h][j][u >> 1][2 * (u & 1) + 1]);
 #pragma unroll
         for (int m = 0; m < C::TM * C::TN; ++m) {
           const int j = m / C::TM, i = m % C::TM;
@@ -449,7 +456,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
           between(u * C::TM * C::TN + m);
         }
       }
-      if (par == 1) {
+      if constexpr (h == 1) {
 #pragma unroll
         for (int i = 0; i < C::TM; ++i) {
           const int e = (xs[i] & 255) + (ws & 255) - 254;
@@ -472,10 +479,10 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     asm volatile("s_barrier" ::: "memory");
   }
 #pragma unroll
-  for (int r = 0; r < READS; ++r) rd1(r, 0, 0);
-  for (int kt = 0; kt < nk; kt += 2) {
-    stage(kt, 0);
-    stage(kt + 1, 1);
+  for (int r = 0; r < FRAGS + C::TM; ++r) rd1(r, 0, 0);
+  for (int kt = 0; kt < kb; ++kt) {
+    step(kt, std::integral_constant<int, 0>{});
+    step(kt, std::integral_constant<int, 1>{});
   }
   // the loads past the end still write LDS: all of them are to have landed
   // before the epilogue reuses it
@@ -699,24 +706,24 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
   if (p.g.tile) {
     if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll) return hipErrorInvalidValue;
     if (p.epilogue == kFp8HiddenQ)
-      return p.g.tile_rows == 256 ? launch_tile<256, 256, 4, false, kFp8HiddenQ, float>(p, s)
-                                  : launch_tile<128, 128, 4, false, kFp8HiddenQ, float>(p, s);
+      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8HiddenQ, float>(p, s)
+                                  : launch_tile<128, 128, 2, false, kFp8HiddenQ, float>(p, s);
     if (p.epilogue == kFp8Pair)
-      return p.g.tile_rows == 256 ? launch_tile<256, 256, 4, false, kFp8Pair, float>(p, s)
-                                  : launch_tile<128, 128, 4, false, kFp8Pair, float>(p, s);
+      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8Pair, float>(p, s)
+                                  : launch_tile<128, 128, 2, false, kFp8Pair, float>(p, s);
     return hipErrorInvalidValue;
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
   auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   if (p.out_dt == kF32)
-    return tiles(128, 128) >= 128 ? launch_tile<128, 128, 4, true, kFp8Out, float>(p, s)
+    return tiles(128, 128) >= 128 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s)
                                   : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
   const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256);
   if (t256 >= 128) {
-    if ((t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256) return launch_tile<192, 256, 4, false, kFp8Out, bf16>(p, s);
-    return launch_tile<256, 256, 4, false, kFp8Out, bf16>(p, s);
+    if ((t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256) return launch_tile<192, 256, 2, false, kFp8Out, bf16>(p, s);
+    return launch_tile<256, 256, 2, false, kFp8Out, bf16>(p, s);
   }
-  return tiles(128, 128) >= 128 ? launch_tile<128, 128, 4, false, kFp8Out, bf16>(p, s)
+  return tiles(128, 128) >= 128 ? launch_tile<128, 128, 2, false, kFp8Out, bf16>(p, s)
                                 : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
 }
 
