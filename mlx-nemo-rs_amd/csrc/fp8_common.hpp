@@ -22,14 +22,18 @@ __device__ __forceinline__ int fp8_scale_byte(float m) {
   const int s = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   return u == 0 ? 127 : (s > 0 ? s : 0);
 }
-// 2^(127 - s), s <= 247: exact, so scaling loses nothing that e4m3 could hold.
-__device__ __forceinline__ float fp8_inverse_scale(int s) {
-  return __builtin_bit_cast(float, (uint32_t)(254 - s) << 23);
+// 2^(s - 127); the smallest, 2^-127, is a subnormal.
+__device__ __forceinline__ float fp8_scale(int s) {
+  return __builtin_bit_cast(float, s > 0 ? (uint32_t)s << 23 : 0x00400000u);
 }
-// Four values to codes (round to nearest even; past 448 and NaN: NaN).
-__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+// Four values over a power of two to codes, in one step of rounding (to
+// nearest even; past 448 and NaN: NaN).
+__device__ __forceinline__ uint32_t fp8_pack4_scaled(float a, float b, float c, float d, float scale) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  s16x2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, r);
 }
 // Eight codes (two words) as bf16, exactly.
 __device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t lo, uint32_t hi) {

@@ -62,9 +62,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t 
   for (int o = 1; o < 16; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
   if (blk >= kb) return;
   const int s = fp8_scale_byte(m);
-  const float inv = fp8_inverse_scale(s);
-  const u32x2 q = {fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                   fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+  const float scale = fp8_scale(s);
+  const u32x2 q = {fp8_pack4_scaled(v[0], v[1], v[2], v[3], scale), fp8_pack4_scaled(v[4], v[5], v[6], v[7], scale)};
   *reinterpret_cast<u32x2*>(codes + row * ((int64_t)kb * 128) + blk * 128 + (lane & 15) * 8) = q;
   if ((lane & 15) == 0) scales[row * (items * 4) + blk] = (uint8_t)s;
 }
@@ -92,11 +91,11 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* w, int N,
   __syncthreads();
   m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
   const int s = fp8_scale_byte(m);
-  const float inv = fp8_inverse_scale(s);
+  const float scale = fp8_scale(s);
 #pragma unroll
   for (int i = 0; i < 64; ++i) {
     const int at = i * 256 + threadIdx.x, n = bn * 128 + at / 128, k = bk * 128 + at % 128;
-    if (n < N) codes[(int64_t)n * (kb * 128) + k] = (uint8_t)fp8_pack4(v[i] * inv, 0.f, 0.f, 0.f);
+    if (n < N) codes[(int64_t)n * (kb * 128) + k] = (uint8_t)fp8_pack4_scaled(v[i], 0.f, 0.f, 0.f, scale);
   }
   if (threadIdx.x == 0) scales[bn * kbp + bk] = (uint8_t)s;
 }
@@ -209,10 +208,10 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = fmaxf(m, __shfl_xor(m, 32, 64));
     const int s = fp8_scale_byte(m);
-    const float inv = fp8_inverse_scale(s);
+    const float scale = fp8_scale(s);
     uint32_t q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = fp8_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+    for (int i = 0; i < 8; ++i) q[i] = fp8_pack4_scaled(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
     if constexpr (EXACT) {
       // element group j of every lane's 32: the same inputs of both operands
       floatx4 part = {0.f, 0.f, 0.f, 0.f};
@@ -339,7 +338,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   const int wblk = min((n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
   const uint32_t wword = *reinterpret_cast<const uint32_t*>(p.ws + expert * p.ws_stride + (int64_t)wblk * kbp +
                                                             4 * min(lane, kbp / 4 - 1));
-  constexpr int LOADS = C::NA + C::NB + 1;
+  constexpr int LOADS = C::NA + C::NB + 1, EARLY = (LOADS * 2 + 2) / 3;
   auto issue1 = [&](int g, int kt) {  // load g of stage kt
     char* S = smem + kt % NS * C::STAGE;
     const int k = min(kt, kb - 1);  // (past the end: the last stage again, unread)
@@ -392,9 +391,12 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 
   int ws = 0, xs[C::TM];
   // Half h of stage kt, whose fragments are in set h. The reads of the next
-  // half's fragments and, in the second half, the loads of stage kt + NS are
-  // placed between the MFMAs (issued ahead of them, the reads filled the
-  // wave's queue of 15 and held the first MFMA back).
+  // half's fragments and the loads that refill the buffer are placed between
+  // the MFMAs (issued ahead of them, the reads filled the wave's queue of 15
+  // and held the first MFMA back). The loads, stage kt + NS's, begin behind the
+  // second half's barrier and end in the next stage's first half: in one half
+  // they came at the rate at which a CU takes lines from its L1, and waves
+  // stood at their issue.
   auto step = [&](int kt, auto hc) {
     constexpr int h = decltype(hc)::value;
     if constexpr (h == 0) {
@@ -409,12 +411,18 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     constexpr int NMF = EXACT ? 4 * C::TM * C::TN : C::TM * C::TN;
     constexpr int READS = FRAGS + (h == 1 ? C::TM : 0);
     constexpr int SLOTS = (NMF + 1) / 2;  // behind the first MFMAs the reads, behind all the loads
-    constexpr int RPM = (READS + SLOTS - 1) / SLOTS, LPM = (LOADS + NMF - 1) / NMF;
+    constexpr int RPM = (READS + SLOTS - 1) / SLOTS;
     auto between = [&](int m) {
+      // load g behind MFMA g NMF / EARLY of the second half, the rest in the
+      // first MFMAs of the next
       if constexpr (h == 1) {
 #pragma unroll
-        for (int g = m * LPM; g < (m + 1) * LPM; ++g)
-          if (g < LOADS) issue1(g, kt + NS);
+        for (int g = 0; g < EARLY; ++g)
+          if (g * NMF / EARLY == m) issue1(g, kt + NS);
+      } else {
+#pragma unroll
+        for (int g = EARLY; g < LOADS; ++g)
+          if ((g - EARLY) * SLOTS / (LOADS - EARLY) == m) issue1(g, kt - 1 + NS);
       }
 #pragma unroll
       for (int r = m * RPM; r < (m + 1) * RPM; ++r)
@@ -471,9 +479,9 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 #pragma unroll
   for (int st = 0; st < NS; ++st)
 #pragma unroll
-    for (int g = 0; g < LOADS; ++g) issue1(g, st);
+    for (int g = 0; g < (st == NS - 1 ? EARLY : LOADS); ++g) issue1(g, st);
   {
-    constexpr int vm = (NS - 1) * LOADS;
+    constexpr int vm = (NS - 2) * LOADS + EARLY;
     static_assert(vm < 64, "wait count");
     __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));
     asm volatile("s_barrier" ::: "memory");
@@ -513,11 +521,18 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
           for (int e = 0; e < 4; ++e) {
             const float v = silu_value<float>(acc[j][i][4 * q + e] + b[e]);
             acc[j][i][4 * q + e] = v;
-            top[i] = fmaxf(top[i], fp8_mag(v));
+            top[i] = fmaxf(top[i], __builtin_fabsf(v));
           }
       }
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
+      if (!(top[i] < __builtin_inff())) {  // an infinity does not count (a NaN never did): again, without
+        top[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top[i] = fmaxf(top[i], fp8_mag(acc[j][i][r]));
+      }
       top[i] = fmaxf(top[i], __shfl_xor(top[i], 32, 64));
       if (C::WN < 128 && half == 0) amax[wn * BM + wm * C::WM + 32 * i + lane] = top[i];
     }
@@ -533,15 +548,14 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
       const int s = fp8_scale_byte(top[i]);
-      const float inv = fp8_inverse_scale(s);
+      const float scale = fp8_scale(s);
       constexpr int HP = C::WN + 16;
 #pragma unroll
       for (int j = 0; j < C::TN; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<uint32_t*>(st + (lane & 31) * HP + 32 * j + 8 * q + 4 * half) =
-              fp8_pack4(acc[j][i][4 * q] * inv, acc[j][i][4 * q + 1] * inv, acc[j][i][4 * q + 2] * inv,
-                        acc[j][i][4 * q + 3] * inv);
+              fp8_pack4_scaled(acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3], scale);
       const int row0 = wm * C::WM + 32 * i;
 #pragma unroll
       for (int it = 0; it < C::WN / 32; ++it) {
