@@ -191,7 +191,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* i
     total = cursor[t];
   }
   const int nt = (total + tile_rows - 1) / tile_rows;
-  slots[0][t] = total;
+  const int mul = (total + 15) / 16 * 16;  // slots taken
+  slots[0][t] = mul;
   tiles[0][t] = nt;
   __syncthreads();
   int cur = 0;
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* i
     tiles[cur ^ 1][t] = tiles[cur][t] + (t >= o ? tiles[cur][t - o] : 0);
     __syncthreads();
   }
-  const int slot0 = slots[cur][t] - total, tile0 = tiles[cur][t] - nt;
+  const int slot0 = slots[cur][t] - mul, tile0 = tiles[cur][t] - nt;
   cursor[t] = slot0 + before;
   __syncthreads();
 #pragma unroll

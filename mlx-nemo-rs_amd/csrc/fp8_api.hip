@@ -45,15 +45,18 @@ int32_t on_device(const void* p, bool* yes) {
   return MHSA_OK;
 }
 
+// The bias, or zeros without one, and kBiasTail zeros behind it.
+constexpr int kBiasTail = 32;
 int32_t load_bias(Fp8Weights& w, int data_dtype, const void* bias) {
-  if (!w.use_bias) return MHSA_OK;
   const size_t n = (size_t)w.n * w.N, es = data_dtype == MHSA_F32 ? 4 : 2;
-  std::vector<char> raw(n * es);
-  std::vector<float> f(n);
-  HIPCHK(hipMemcpy(raw.data(), bias, raw.size(), hipMemcpyDefault));
-  for (size_t i = 0; i < n; ++i) f[i] = load_host(data_dtype, raw.data(), i);
-  HIPCHK(w.bias.ensure(n * 4));
-  HIPCHK(hipMemcpy(w.bias.p, f.data(), n * 4, hipMemcpyHostToDevice));
+  std::vector<float> f(n + kBiasTail, 0.f);
+  if (w.use_bias) {
+    std::vector<char> raw(n * es);
+    HIPCHK(hipMemcpy(raw.data(), bias, raw.size(), hipMemcpyDefault));
+    for (size_t i = 0; i < n; ++i) f[i] = load_host(data_dtype, raw.data(), i);
+  }
+  HIPCHK(w.bias.ensure(f.size() * 4));
+  HIPCHK(hipMemcpy(w.bias.p, f.data(), f.size() * 4, hipMemcpyHostToDevice));
   return MHSA_OK;
 }
 
@@ -261,7 +264,7 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t
   mhsa::Fp8Gemm p;
   p.w = static_cast<const uint8_t*>(w.codes.p);
   p.ws = static_cast<const uint8_t*>(w.scales.p);
-  p.bias = w.use_bias ? static_cast<const float*>(w.bias.p) : nullptr;
+  p.bias = static_cast<const float*>(w.bias.p);
   p.M = rows;
   p.N = w.N;
   p.K = w.K;
@@ -353,6 +356,7 @@ struct ExpertsPlan {
   int64_t step = 0;
   int tile_rows = 0;  // 0: no list; 16: few-row kernel; else tiles
   int max_tiles = 0;
+  int64_t slots = 0;
   int *pair = nullptr, *tile = nullptr, *n_tiles = nullptr, *scratch = nullptr;
   uint8_t *xc = nullptr, *xs = nullptr, *hc = nullptr, *hsc = nullptr;
   float *h = nullptr, *y = nullptr;
@@ -369,7 +373,7 @@ ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void*
   if (rows * top_k > kFewPairs) {
     p.tile_rows = mhsa::fp8_group_rows(pairs, e->E);
     p.max_tiles = (int)(pairs / p.tile_rows + std::min<int64_t>(pairs, e->E));
-    p.pair = a.take<int>(pairs);
+    p.pair = a.take<int>(mhsa::expert_slots(pairs, e->E));
     p.tile = a.take<int>(4 * (int64_t)p.max_tiles);
     p.n_tiles = a.take<int>(1);
     p.scratch = a.take<int>(mhsa::plan_scratch_ints(pairs, e->E));
@@ -377,8 +381,9 @@ ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void*
   if (p.tile_rows > 16) {
     p.xc = a.take<uint8_t>(p.step * dp);
     p.xs = a.take<uint8_t>(p.step * mhsa::fp8_kbp(e->D));
-    p.hc = a.take<uint8_t>(pairs * fp);
-    p.hsc = a.take<uint8_t>(pairs * mhsa::fp8_kbp(e->F));
+    p.slots = mhsa::expert_slots(pairs, e->E);
+    p.hc = a.take<uint8_t>(p.slots * fp);
+    p.hsc = a.take<uint8_t>(p.slots * (fp / 128));
   } else {
     p.h = a.take<float>(pairs * e->F);
   }
@@ -398,7 +403,8 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
     g[i].ws = static_cast<const uint8_t*>(w.scales.p);
     g[i].w_stride = w.stride();
     g[i].ws_stride = w.scale_stride();
-    g[i].bias = w.use_bias ? static_cast<const float*>(w.bias.p) : nullptr;
+    g[i].bias = static_cast<const float*>(w.bias.p);
+    g[i].zeros = g[i].bias + (int64_t)w.n * w.N;
     g[i].N = w.N;
     g[i].K = w.K;
     g[i].M = pairs;
@@ -429,10 +435,10 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
     g[0].epilogue = mhsa::kFp8HiddenQ;
     g[0].out_codes = plan.hc;
     g[0].out_scales = plan.hsc;
+    g[0].slots = g[1].slots = plan.slots;
     HIPCHK(mhsa::fp8_gemm_tile(g[0], s));
     g[1].a = plan.hc;
     g[1].as = plan.hsc;
-    g[1].a_rows = pairs;
     HIPCHK(mhsa::fp8_gemm_tile(g[1], s));
   } else {
     g[0].x = x;

@@ -12,6 +12,7 @@
 // f32 sums: there the codes go to the bf16 matrix cores, which hold them and
 // their products exactly (1e-7), at half the rate.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "../../include/relpos_mhsa.h"
@@ -274,10 +275,11 @@ struct Fp8Cfg {
   static constexpr int NA = BM / 32, NB = BN / 32;  // 1 KB loads per wave and stage
   static constexpr int OP = WN * 4 + 16;            // pitch of a staged output row
   static constexpr int STG = 4 * 32 * OP, AMAX = 2 * BM * 4;
-  static constexpr int SCALES = NS * STAGE;         // two words a row behind the stages
+  static constexpr int SCALES = NS * STAGE;         // two words a row (or 256 bytes a stage) behind the stages
   static constexpr int LOOP = SCALES + 2 * BM * 4;
   static constexpr int LDS = LOOP > STG + AMAX ? LOOP : STG + AMAX;
   static_assert(LDS <= 160 * 1024, "tile exceeds LDS");
+  static_assert(BM <= 256 && (BM < 128 || NS * 256 <= 2 * BM * 4), "scales");
 };
 
 template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
@@ -308,10 +310,13 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   // repeat its last; their results are not stored)
   const bool gather = grouped && p.rows == Fp8Gemm::kByFrame;
   const uint8_t* ab = p.a + (gather ? 0 : (int64_t)m0 * kp);
-  const uint8_t* sb = p.as + (gather ? 0 : (int64_t)m0 * kbp);
+  // row scales: a word of 4 blocks to a row, or (HT) by block, bytes of
+  // consecutive slots
+  constexpr bool HT = EPI == kFp8Pair;
+  const uint8_t* sb = HT ? p.as + m0 : p.as + (gather ? 0 : (int64_t)m0 * kbp);
   const int64_t arows = gather ? p.a_rows : rows;
   const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ab, (short)0, (int)(uint32_t)(arows * kp), kRawBuffer);
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, (int)(uint32_t)(arows * kbp), kRawBuffer);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, (int)(uint32_t)(HT ? kb * p.slots - m0 : arows * kbp), kRawBuffer);
   auto source = [&](int row) -> uint32_t {
     row = min(row, rows - 1);
     return gather ? (uint32_t)(p.g.pair[m0 + row] / p.g.top_k) : (uint32_t)row;
@@ -324,7 +329,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 7) ^ ((row >> 1) & 7)));
   }
   const int srow = (w * 64) % BM;
-  const int soff = (int)(source(srow + lane) * (uint32_t)kbp);
+  const int soff = HT ? 4 * lane : (int)(source(srow + lane) * (uint32_t)kbp);
   const uint8_t* wb = p.w + expert * p.w_stride + (int64_t)n0 * kp;
   const __amdgpu_buffer_rsrc_t rb =
       __builtin_amdgcn_make_buffer_rsrc((void*)wb, (short)0, min(p.N - n0, BN) * kp, kRawBuffer);
@@ -347,6 +352,9 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     else if (g < C::NA + C::NB)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(S + C::ABYTES + (w * C::NB + g - C::NA) * 1024), 16,
                                                boff[g - C::NA], k * 128, 0, 0);
+    else if (HT)  // 256 rows' bytes, by every wave; rows past the slots read as 0
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + kt % NS * 256), 4, soff,
+                                               (int)(k * p.slots), 0, 0);
     else  // a word is loaded again by each of its stages, and by two waves of
           // a tile of under 256 rows: always the same bytes
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((k >> 2) & 1) * BM * 4 + srow * 4), 4,
@@ -378,6 +386,9 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     } else if (r < FRAGS) {
       r -= 2 * C::TN;
       fa[h][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + arow + off[h][r % 2] + r / 2 * 4096);
+    } else if (HT) {
+      xw[r - FRAGS] = *reinterpret_cast<const uint8_t*>(smem + C::SCALES + kt % NS * 256 + wm * C::WM + 32 * (r - FRAGS) +
+                                                        (lane & 31));
     } else {
       xw[r - FRAGS] = *reinterpret_cast<const int*>(smem + C::SCALES + ((min(kt, kb - 1) >> 2) & 1) * BM * 4 +
                                                     (wm * C::WM + 32 * (r - FRAGS) + (lane & 31)) * 4);
@@ -403,7 +414,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       const int sh = 8 * (kt & 3);
       ws = __builtin_amdgcn_readlane((int)wword, kt >> 2) >> sh;
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) xs[i] = xw[i] >> sh;
+      for (int i = 0; i < C::TM; ++i) xs[i] = HT ? xw[i] : xw[i] >> sh;
     } else {
       landed();  // stage kt + 1, everywhere; stage kt's buffer has been read
     }
@@ -505,57 +516,44 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     // silu, then codes: the block's 128 columns of a row lie in one wave
     // (both lane halves) or in the two of a row of waves
     float* amax = reinterpret_cast<float*>(smem + C::STG);
-    float top[C::TM];
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) top[i] = 0.f;
+    const int np = (p.N + 127) / 128 * 128;
+    const float* bias[C::TN];  // (N is a multiple of 64)
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = col0 + 32 * j + 8 * q + 4 * half;
-        floatx4 b = {0.f, 0.f, 0.f, 0.f};
-        if (p.bias && col < p.N) b = *reinterpret_cast<const floatx4*>(p.bias + (int64_t)expert * p.N + col);
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = silu_value<float>(acc[j][i][4 * q + e] + b[e]);
-            acc[j][i][4 * q + e] = v;
-            top[i] = fmaxf(top[i], __builtin_fabsf(v));
-          }
-      }
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      if (!(top[i] < __builtin_inff())) {  // an infinity does not count (a NaN never did): again, without
-        top[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) top[i] = fmaxf(top[i], fp8_mag(acc[j][i][r]));
-      }
-      top[i] = fmaxf(top[i], __shfl_xor(top[i], 32, 64));
-      if (C::WN < 128 && half == 0) amax[wn * BM + wm * C::WM + 32 * i + lane] = top[i];
-    }
-    if constexpr (C::WN < 128) {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const int r = wm * C::WM + 32 * i + (lane & 31);
-        top[i] = fmaxf(amax[r], amax[BM + r]);
-      }
-    }
-    const int np = (p.N + 127) / 128 * 128, nbp = (np / 128 + 3) / 4 * 4;
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      const int s = fp8_scale_byte(top[i]);
-      const float scale = fp8_scale(s);
-      constexpr int HP = C::WN + 16;
+      bias[j] = col0 + 32 * j < p.N ? p.bias + (int64_t)expert * p.N + col0 + 32 * j : p.zeros;
+    constexpr int HP = C::WN + 16;
+    // (32 rows at a time, with nothing of the next ones moved ahead: 256
+    // accumulators and as many results at once spilled, at 5 us a tile)
+    auto hidden = [&](int i, float v[C::TN * 16]) {
+      float top = 0.f;
 #pragma unroll
       for (int j = 0; j < C::TN; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 4; ++q) {
+          const floatx4 b = *reinterpret_cast<const floatx4*>(bias[j] + 8 * q + 4 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[16 * j + 4 * q + e] = silu_value<float>(acc[j][i][4 * q + e] + b[e]);
+            top = fmaxf(top, __builtin_fabsf(v[16 * j + 4 * q + e]));
+          }
+        }
+      if (__any(!(top < __builtin_inff()))) {  // an infinity does not count (a NaN never did): again, without
+        top = 0.f;
+        for (int r = 0; r < C::TN * 16; ++r) top = fmaxf(top, fp8_mag(v[r]));
+      }
+      return fmaxf(top, __shfl_xor(top, 32, 64));
+    };
+    auto store = [&](int i, const float v[C::TN * 16], float top) {
+      const int s = fp8_scale_byte(top);
+      const float scale = fp8_scale(s);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float* f = v + 16 * j + 4 * q;
           *reinterpret_cast<uint32_t*>(st + (lane & 31) * HP + 32 * j + 8 * q + 4 * half) =
-              fp8_pack4_scaled(acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3], scale);
+              fp8_pack4_scaled(f[0], f[1], f[2], f[3], scale);
+        }
       const int row0 = wm * C::WM + 32 * i;
 #pragma unroll
       for (int it = 0; it < C::WN / 32; ++it) {
@@ -565,7 +563,29 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
               *reinterpret_cast<const u32x4*>(st + r * HP + c);
       }
       if (half == 0 && col0 % 128 == 0 && col0 < np && row0 + lane < rows)
-        p.out_scales[(int64_t)(m0 + row0 + lane) * nbp + col0 / 128] = (uint8_t)s;
+        p.out_scales[col0 / 128 * p.slots + m0 + row0 + lane] = (uint8_t)s;
+    };
+    if constexpr (C::WN == 128) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        float v[C::TN * 16];
+        const float top = hidden(i, v);
+        store(i, v, top);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      float v[C::TM][C::TN * 16], top[C::TM];
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        top[i] = hidden(i, v[i]);
+        if (half == 0) amax[wn * BM + wm * C::WM + 32 * i + lane] = top[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int r = wm * C::WM + 32 * i + (lane & 31);
+        store(i, v[i], fmaxf(amax[r], amax[BM + r]));
+      }
     }
   } else {
     // 32 rows at a time through LDS, so that a store is 16 bytes of a run of
@@ -718,7 +738,9 @@ int fp8_group_rows(int64_t pairs, int experts) {
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
   if (bad_gemm(p) || !p.a || !p.as) return hipErrorInvalidValue;
   if (p.g.tile) {
-    if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll) return hipErrorInvalidValue;
+    if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll || p.slots % 16 || p.slots * (fp8_kp(p.K) / 128) > INT32_MAX)
+      return hipErrorInvalidValue;
+    if (p.epilogue == kFp8HiddenQ && (!p.bias || !p.zeros || p.N % 64)) return hipErrorInvalidValue;
     if (p.epilogue == kFp8HiddenQ)
       return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8HiddenQ, float>(p, s)
                                   : launch_tile<128, 128, 2, false, kFp8HiddenQ, float>(p, s);

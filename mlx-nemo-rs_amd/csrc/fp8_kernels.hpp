@@ -9,7 +9,11 @@
 // two 2^(s - 127), s one byte: for activations 128 inputs of one row, for
 // weights 128 x 128. A matrix [rows, K] is held as codes [rows, Kp], Kp = K
 // rounded up to 128 and the columns past K zero, beside scale bytes
-// [rows or blocks of 128 rows, kbp], kbp = Kp / 128 rounded up to 4.
+// [rows or blocks of 128 rows, kbp], kbp = Kp / 128 rounded up to 4. The
+// experts' hidden rows have their scale bytes by block instead,
+// [Kp / 128, slots]: a tile writes the bytes of its rows for one or two blocks,
+// and single bytes of lines that other tiles write too cost the first product
+// 20 of 440 us (15001 frames to 4 of 64 experts).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -44,7 +48,7 @@ hipError_t fp8_unpad_weight(const uint8_t* codes, const uint8_t* scales, int N, 
 // Where the rows of a product over experts come from (null `tile`: one dense
 // product). tile[t] = {expert, first slot, slots}, t < *n_tiles <= max_tiles;
 // slot s stands for pair[s], which is frame pair[s] / top_k's choice number
-// pair[s] % top_k.
+// pair[s] % top_k. An expert's slots begin at a multiple of 16.
 struct Fp8Groups {
   const int* tile = nullptr;  // [max_tiles, 4]
   const int* n_tiles = nullptr;
@@ -76,6 +80,9 @@ struct Fp8Gemm {
   const uint8_t* w = nullptr;
   const uint8_t* ws = nullptr;
   const float* bias = nullptr;
+  // kFp8HiddenQ needs one (of zeros, if there is none), and 32 zeros for
+  // blocks of columns past N
+  const float* zeros = nullptr;
   int64_t w_stride = 0, ws_stride = 0;  // bytes between experts
   int M = 0, N = 0, K = 0;
   int epilogue = kFp8Out;
@@ -84,6 +91,7 @@ struct Fp8Gemm {
   int64_t ldo = 0;
   uint8_t* out_codes = nullptr;
   uint8_t* out_scales = nullptr;
+  int64_t slots = 0;  // of the hidden rows' scales
   Fp8Groups g;
 };
 // Whether the few-row kernel (activations rounded inside it) takes M rows.
@@ -96,8 +104,12 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s);
 // kernel's groups of 16).
 int fp8_group_rows(int64_t pairs, int experts);
 
-// Experts' bookkeeping: pairs sorted by expert (pair), and the tile list of
-// tile_rows slots. scratch: plan_scratch_ints(pairs, experts) ints.
+// Slots that `pairs` pairs take at most, a multiple of 16.
+inline int64_t expert_slots(int64_t pairs, int experts) {
+  return (pairs + 15 * (pairs < experts ? pairs : experts) + 15) / 16 * 16;
+}
+// Experts' bookkeeping: pairs sorted by expert (pair [expert_slots]), and the
+// tile list of tile_rows slots. scratch: plan_scratch_ints(pairs, experts) ints.
 int64_t plan_scratch_ints(int64_t pairs, int experts);
 hipError_t experts_plan(const int* idx, int pairs, int experts, int tile_rows, int* pair, int* tile, int* n_tiles,
                         int* scratch, hipStream_t s);
