@@ -45,11 +45,10 @@ int32_t on_device(const void* p, bool* yes) {
   return MHSA_OK;
 }
 
-// The bias, or zeros without one, and kBiasTail zeros behind it.
-constexpr int kBiasTail = 32;
+// The bias, or zeros without one, and zeros behind it.
 int32_t load_bias(Fp8Weights& w, int data_dtype, const void* bias) {
   const size_t n = (size_t)w.n * w.N, es = data_dtype == MHSA_F32 ? 4 : 2;
-  std::vector<float> f(n + kBiasTail, 0.f);
+  std::vector<float> f(n + mhsa::kFp8BiasTail, 0.f);
   if (w.use_bias) {
     std::vector<char> raw(n * es);
     HIPCHK(hipMemcpy(raw.data(), bias, raw.size(), hipMemcpyDefault));
@@ -404,7 +403,6 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
     g[i].w_stride = w.stride();
     g[i].ws_stride = w.scale_stride();
     g[i].bias = static_cast<const float*>(w.bias.p);
-    g[i].zeros = g[i].bias + (int64_t)w.n * w.N;
     g[i].N = w.N;
     g[i].K = w.K;
     g[i].M = pairs;

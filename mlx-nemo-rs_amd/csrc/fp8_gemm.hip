@@ -244,7 +244,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
   float v = red[0][row][threadIdx.x & 15];
 #pragma unroll
   for (int i = 1; i < NW; ++i) v += red[i][row][threadIdx.x & 15];
-  if (p.bias) v += p.bias[(int64_t)expert * p.N + n];
+  v += p.bias[(int64_t)expert * p.N + n];
   if (p.epilogue == kFp8HiddenF32) v = silu_value<float>(v);
   store_as(p.epilogue == kFp8Out ? p.out_dt : kF32, p.out, (int64_t)out * p.ldo + n, v);
 }
@@ -265,6 +265,12 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
 // refill its buffer are issued. Row scales come with the stages, 4 stages to a
 // word; the weight's scale is one byte per wave and stage, read from a lane of
 // a register that holds all of them.
+//
+// Workgroups stay and take tile after tile. A large tile has its CU to itself
+// and LDS for staging its results beside the ring, so the next tile's rows are
+// looked up and its first loads issued before the epilogue (3.7 us a tile of
+// waiting on the list, the pairs and the first lines otherwise). Small tiles
+// share a CU, whose other workgroup computes meanwhile.
 // ---------------------------------------------------------------------------
 
 template <int BM, int BN, int NS_>
@@ -273,11 +279,14 @@ struct Fp8Cfg {
   static constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
   static constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
   static constexpr int NA = BM / 32, NB = BN / 32;  // 1 KB loads per wave and stage
-  static constexpr int OP = WN * 4 + 16;            // pitch of a staged output row
-  static constexpr int STG = 4 * 32 * OP, AMAX = 2 * BM * 4;
   static constexpr int SCALES = NS * STAGE;         // two words a row (or 256 bytes a stage) behind the stages
   static constexpr int LOOP = SCALES + 2 * BM * 4;
-  static constexpr int LDS = LOOP > STG + AMAX ? LOOP : STG + AMAX;
+  // results are staged 32 rows of 128 bytes at a time and wave; behind them a
+  // wave keeps its columns' bias and its rows' places
+  static constexpr int OP = 128 + 16, WST = 32 * OP + 4 * (WN + WM), STG = 4 * WST, AMAX = 2 * BM * 4;
+  static constexpr bool AHEAD = BM * BN >= 192 * 256;  // staging beside the ring, else over it
+  static constexpr int OUT = AHEAD ? LOOP : 0;
+  static constexpr int LDS = AHEAD ? LOOP + STG : LOOP > STG + AMAX ? LOOP : STG + AMAX;
   static_assert(LDS <= 160 * 1024, "tile exceeds LDS");
   static_assert(BM <= 256 && (BM < 128 || NS * 256 <= 2 * BM * 4), "scales");
 };
@@ -294,55 +303,67 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   const bool grouped = p.g.tile != nullptr;
   const int tilesM = grouped ? *p.g.n_tiles : (p.M + BM - 1) / BM, tilesN = (p.N + BN - 1) / BN;
   const int nt = tilesM * tilesN, per = (nt + 7) / 8;
-  const int at = (int)(blockIdx.x / 8u), T = (int)(blockIdx.x % 8u) * per + at;
-  if (at >= per || T >= nt) return;
-  constexpr int GM = 8;
-  const int gsz = GM * tilesN, first = T / gsz * GM, gm = min(tilesM - first, GM);
-  const int tm = first + (T % gsz) % gm, n0 = (T % gsz) / gm * BN;
-  int expert = 0, m0 = tm * BM, rows = min(p.M - m0, BM);
-  if (grouped) {
-    expert = p.g.tile[4 * tm];
-    m0 = p.g.tile[4 * tm + 1];
-    rows = p.g.tile[4 * tm + 2];
-  }
-
-  // activations: this tile's rows, or gathered ones (rows past the tile's
-  // repeat its last; their results are not stored)
-  const bool gather = grouped && p.rows == Fp8Gemm::kByFrame;
-  const uint8_t* ab = p.a + (gather ? 0 : (int64_t)m0 * kp);
-  // row scales: a word of 4 blocks to a row, or (HT) by block, bytes of
-  // consecutive slots
-  constexpr bool HT = EPI == kFp8Pair;
-  const uint8_t* sb = HT ? p.as + m0 : p.as + (gather ? 0 : (int64_t)m0 * kbp);
-  const int64_t arows = gather ? p.a_rows : rows;
-  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)ab, (short)0, (int)(uint32_t)(arows * kp), kRawBuffer);
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, (int)(uint32_t)(HT ? kb * p.slots - m0 : arows * kbp), kRawBuffer);
-  auto source = [&](int row) -> uint32_t {
-    row = min(row, rows - 1);
-    return gather ? (uint32_t)(p.g.pair[m0 + row] / p.g.top_k) : (uint32_t)row;
+  const int T0 = (int)(blockIdx.x % 8u) * per, T1 = min(T0 + per, nt);
+  int T = T0 + (int)(blockIdx.x / 8u);
+  if (T >= T1) return;
+  struct Tile {
+    int expert, m0, rows, n0;
   };
-  // load g of wave w fills 8 LDS rows: lane l row l / 8, stored chunk l % 8
-  int aoff[C::NA];
-#pragma unroll
-  for (int g = 0; g < C::NA; ++g) {
-    const int row = (w * C::NA + g) * 8 + (lane >> 3);
-    aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 7) ^ ((row >> 1) & 7)));
-  }
+  auto locate = [&](int t) {
+    constexpr int GM = 8;
+    const int gsz = GM * tilesN, first = t / gsz * GM, gm = min(tilesM - first, GM);
+    const int tm = first + (t % gsz) % gm;
+    Tile r = {0, tm * BM, min(p.M - tm * BM, BM), (t % gsz) / gm * BN};
+    if (grouped) {
+      r.expert = __builtin_amdgcn_readfirstlane(p.g.tile[4 * tm]);
+      r.m0 = __builtin_amdgcn_readfirstlane(p.g.tile[4 * tm + 1]);
+      r.rows = __builtin_amdgcn_readfirstlane(p.g.tile[4 * tm + 2]);
+    }
+    return r;
+  };
+
+  // activations: a tile's rows, or gathered ones (rows past the tile's repeat
+  // its last; their results are not stored). Row scales: a word of 4 blocks
+  // to a row, or (HT) by block, bytes of consecutive slots.
+  constexpr bool HT = EPI == kFp8Pair;
+  const bool gather = grouped && p.rows == Fp8Gemm::kByFrame;
+  __amdgpu_buffer_rsrc_t ra, rs, rb;
+  int aoff[C::NA], boff[C::NB], soff;
+  uint32_t wword;
   const int srow = (w * 64) % BM;
-  const int soff = HT ? 4 * lane : (int)(source(srow + lane) * (uint32_t)kbp);
-  const uint8_t* wb = p.w + expert * p.w_stride + (int64_t)n0 * kp;
-  const __amdgpu_buffer_rsrc_t rb =
-      __builtin_amdgcn_make_buffer_rsrc((void*)wb, (short)0, min(p.N - n0, BN) * kp, kRawBuffer);
-  int boff[C::NB];
 #pragma unroll
-  for (int g = 0; g < C::NB; ++g) {
+  for (int g = 0; g < C::NB; ++g) {  // load g of wave w fills 8 LDS rows: lane l row l / 8, stored chunk l % 8
     const int row = (w * C::NB + g) * 8 + (lane >> 3);
     boff[g] = row * kp + 16 * ((lane & 7) ^ ((row >> 1) & 7));
   }
-  // the weight scales of this wave's 128-column block, a word of 4 to a lane
-  const int wblk = min((n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
-  const uint32_t wword = *reinterpret_cast<const uint32_t*>(p.ws + expert * p.ws_stride + (int64_t)wblk * kbp +
-                                                            4 * min(lane, kbp / 4 - 1));
+  auto rsrc = [](const uint8_t* base, uint32_t n) {
+    // (uniform by its making, which the compiler loses over the tile loop)
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(u), (short)0, __builtin_amdgcn_readfirstlane((int)n),
+                                             kRawBuffer);
+  };
+  auto aim = [&](const Tile& t) {  // the loads below are tile t's
+    const int64_t arows = gather ? p.a_rows : t.rows;
+    ra = rsrc(p.a + (gather ? 0 : (int64_t)t.m0 * kp), (uint32_t)(arows * kp));
+    rs = rsrc(HT ? p.as + t.m0 : p.as + (gather ? 0 : (int64_t)t.m0 * kbp), (uint32_t)(HT ? kb * p.slots - t.m0 : arows * kbp));
+    auto source = [&](int row) -> uint32_t {
+      row = min(row, t.rows - 1);
+      return gather ? (uint32_t)(p.g.pair[t.m0 + row] / p.g.top_k) : (uint32_t)row;
+    };
+#pragma unroll
+    for (int g = 0; g < C::NA; ++g) {
+      const int row = (w * C::NA + g) * 8 + (lane >> 3);
+      aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 7) ^ ((row >> 1) & 7)));
+    }
+    soff = HT ? 4 * lane : (int)(source(srow + lane) * (uint32_t)kbp);
+    rb = rsrc(p.w + t.expert * p.w_stride + (int64_t)t.n0 * kp, (uint32_t)(min(p.N - t.n0, BN) * kp));
+    // the weight scales of this wave's 128-column block, a word of 4 to a lane
+    const int wblk = min((t.n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
+    wword = *reinterpret_cast<const uint32_t*>(p.ws + t.expert * p.ws_stride + (int64_t)wblk * kbp +
+                                               4 * min(lane, kbp / 4 - 1));
+  };
   constexpr int LOADS = C::NA + C::NB + 1, EARLY = (LOADS * 2 + 2) / 3;
   auto issue1 = [&](int g, int kt) {  // load g of stage kt
     char* S = smem + kt % NS * C::STAGE;
@@ -395,10 +416,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     }
   };
   floatx16 acc[C::TN][C::TM], part[EXACT ? C::TN : 1][EXACT ? C::TM : 1];
-#pragma unroll
-  for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
 
   int ws = 0, xs[C::TM];
   // Half h of stage kt, whose fragments are in set h. The reads of the next
@@ -487,154 +504,218 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       }
     }
   };
+  auto prologue = [&]() {
 #pragma unroll
-  for (int st = 0; st < NS; ++st)
+    for (int st = 0; st < NS; ++st)
 #pragma unroll
-    for (int g = 0; g < (st == NS - 1 ? EARLY : LOADS); ++g) issue1(g, st);
-  {
-    constexpr int vm = (NS - 2) * LOADS + EARLY;
-    static_assert(vm < 64, "wait count");
-    __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));
-    asm volatile("s_barrier" ::: "memory");
-  }
-#pragma unroll
-  for (int r = 0; r < FRAGS + C::TM; ++r) rd1(r, 0, 0);
-  for (int kt = 0; kt < kb; ++kt) {
-    step(kt, std::integral_constant<int, 0>{});
-    step(kt, std::integral_constant<int, 1>{});
-  }
-  // the loads past the end still write LDS: all of them are to have landed
-  // before the epilogue reuses it
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
+      for (int g = 0; g < (st == NS - 1 ? EARLY : LOADS); ++g) issue1(g, st);
+  };
 
-  // lane: row 32 i + lane % 32 of the wave's block, columns 32 j + 8 q +
-  // 4 (lane / 32) + [0, 4)
-  const int col0 = n0 + wn * C::WN;
-  char* st = smem + w * 32 * C::OP;
-  if constexpr (EPI == kFp8HiddenQ) {
-    // silu, then codes: the block's 128 columns of a row lie in one wave
-    // (both lane halves) or in the two of a row of waves
-    float* amax = reinterpret_cast<float*>(smem + C::STG);
-    const int np = (p.N + 127) / 128 * 128;
-    const float* bias[C::TN];  // (N is a multiple of 64)
+  Tile now = locate(T);
+  aim(now);
+  prologue();
+  bool waited = false;  // the prologue's loads have landed
+  for (;;) {
+    if (!waited) {  // stage 0 has
+      constexpr int vm = (NS - 2) * LOADS + EARLY;
+      static_assert(vm < 64, "wait count");
+      __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));
+    }
+    asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
-      bias[j] = col0 + 32 * j < p.N ? p.bias + (int64_t)expert * p.N + col0 + 32 * j : p.zeros;
-    constexpr int HP = C::WN + 16;
-    // (32 rows at a time, with nothing of the next ones moved ahead: 256
-    // accumulators and as many results at once spilled, at 5 us a tile)
-    auto hidden = [&](int i, float v[C::TN * 16]) {
-      float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j)
+      for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const floatx4 b = *reinterpret_cast<const floatx4*>(bias[j] + 8 * q + 4 * half);
+    for (int r = 0; r < FRAGS + C::TM; ++r) rd1(r, 0, 0);
+    for (int kt = 0; kt < kb; ++kt) {
+      step(kt, std::integral_constant<int, 0>{});
+      step(kt, std::integral_constant<int, 1>{});
+    }
+    // the loads past the end still write LDS: all of them are to have landed
+    // before the ring is used again
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+
+    const Tile done = now;
+    T += (int)(gridDim.x / 8u);
+    const bool more = T < T1;
+    // What the epilogue loads comes ahead of the next tile's loads, which it
+    // would otherwise wait for. Lane: row 32 i + lane % 32 of the wave's
+    // block, columns 32 j + 8 q + 4 (lane / 32) + [0, 4).
+    const int col0 = done.n0 + wn * C::WN;
+    // (a register each, then LDS: held in registers for all of the lane's
+    // columns and rows, they spilled)
+    constexpr int BL = (C::WN + 63) / 64, PL = EPI == kFp8Pair ? (C::WM + 63) / 64 : 0;
+    float bl[BL];
+    int pl[PL ? PL : 1];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[16 * j + 4 * q + e] = silu_value<float>(acc[j][i][4 * q + e] + b[e]);
-            top = fmaxf(top, __builtin_fabsf(v[16 * j + 4 * q + e]));
+    for (int u = 0; u < BL; ++u) {
+      const int c = col0 + 64 * u + lane;
+      bl[u] = EPI == kFp8HiddenQ && c >= p.N ? 0.f : p.bias[(int64_t)done.expert * p.N + c];
+    }
+#pragma unroll
+    for (int u = 0; u < PL; ++u) pl[u] = p.g.pair[done.m0 + min(wm * C::WM + 64 * u + lane, done.rows - 1)];
+    asm volatile("" ::: "memory");
+    if (C::AHEAD && more) {
+      now = locate(T);
+      aim(now);
+      prologue();
+    }
+    char* st = smem + C::OUT + w * C::WST;
+    float* bias = reinterpret_cast<float*>(st + 32 * C::OP);
+    int* place = reinterpret_cast<int*>(bias + C::WN);
+#pragma unroll
+    for (int u = 0; u < BL; ++u)
+      if (64 * u + lane < C::WN) bias[64 * u + lane] = bl[u];
+#pragma unroll
+    for (int u = 0; u < PL; ++u)
+      if (64 * u + lane < C::WM) place[64 * u + lane] = pl[u];
+    // (keeps the sums of rows 32 i of the block in their accumulators up to
+    // here: read ahead, all of them, they spilled)
+    auto hold = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) asm volatile("" : "+a"(acc[j][i]));
+    };
+    auto bias4 = [&](int j, int q) { return *reinterpret_cast<const floatx4*>(bias + 32 * j + 8 * q + 4 * half); };
+    auto before_stores = [&]() {  // (loads and stores are counted together, in order)
+      if constexpr (C::AHEAD) {
+        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
+        waited = true;
+      }
+    };
+
+    if constexpr (EPI == kFp8HiddenQ) {
+      // silu, then codes: the block's 128 columns of a row lie in one wave
+      // (both lane halves) or in the two of a row of waves
+      float* amax = reinterpret_cast<float*>(smem + C::STG);
+      const int np = (p.N + 127) / 128 * 128;
+      constexpr int HP = C::WN + 16;
+      // (32 rows at a time, with nothing of the next ones moved ahead: 256
+      // accumulators and as many results at once spilled)
+      auto hidden = [&](int i, float v[C::TN * 16]) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const floatx4 b = bias4(j, q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[16 * j + 4 * q + e] = silu_value<float>(acc[j][i][4 * q + e] + b[e]);
+              top = fmaxf(top, __builtin_fabsf(v[16 * j + 4 * q + e]));
+            }
           }
+        if (__any(!(top < __builtin_inff()))) {  // an infinity does not count (a NaN never did): again, without
+          top = 0.f;
+          for (int r = 0; r < C::TN * 16; ++r) top = fmaxf(top, fp8_mag(v[r]));
         }
-      if (__any(!(top < __builtin_inff()))) {  // an infinity does not count (a NaN never did): again, without
-        top = 0.f;
-        for (int r = 0; r < C::TN * 16; ++r) top = fmaxf(top, fp8_mag(v[r]));
-      }
-      return fmaxf(top, __shfl_xor(top, 32, 64));
-    };
-    auto store = [&](int i, const float v[C::TN * 16], float top) {
-      const int s = fp8_scale_byte(top);
-      const float scale = fp8_scale(s);
+        return fmaxf(top, __shfl_xor(top, 32, 64));
+      };
+      auto store = [&](int i, const float v[C::TN * 16], float top) {
+        const int s = fp8_scale_byte(top);
+        const float scale = fp8_scale(s);
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j)
+        for (int j = 0; j < C::TN; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float* f = v + 16 * j + 4 * q;
-          *reinterpret_cast<uint32_t*>(st + (lane & 31) * HP + 32 * j + 8 * q + 4 * half) =
-              fp8_pack4_scaled(f[0], f[1], f[2], f[3], scale);
+          for (int q = 0; q < 4; ++q) {
+            const float* f = v + 16 * j + 4 * q;
+            *reinterpret_cast<uint32_t*>(st + (lane & 31) * HP + 32 * j + 8 * q + 4 * half) =
+                fp8_pack4_scaled(f[0], f[1], f[2], f[3], scale);
+          }
+        const int row0 = wm * C::WM + 32 * i;
+        if (i == 0) before_stores();
+#pragma unroll
+        for (int it = 0; it < C::WN / 32; ++it) {
+          const int id = it * 64 + lane, r = id / (C::WN / 16), c = id % (C::WN / 16) * 16;
+          if (row0 + r < done.rows && col0 + c < np)
+            *reinterpret_cast<u32x4*>(p.out_codes + (int64_t)(done.m0 + row0 + r) * np + col0 + c) =
+                *reinterpret_cast<const u32x4*>(st + r * HP + c);
         }
-      const int row0 = wm * C::WM + 32 * i;
+        if (half == 0 && col0 % 128 == 0 && col0 < np && row0 + lane < done.rows)
+          p.out_scales[col0 / 128 * p.slots + done.m0 + row0 + lane] = (uint8_t)s;
+      };
+      if constexpr (C::WN == 128) {
 #pragma unroll
-      for (int it = 0; it < C::WN / 32; ++it) {
-        const int id = it * 64 + lane, r = id / (C::WN / 16), c = id % (C::WN / 16) * 16;
-        if (row0 + r < rows && col0 + c < np)
-          *reinterpret_cast<u32x4*>(p.out_codes + (int64_t)(m0 + row0 + r) * np + col0 + c) =
-              *reinterpret_cast<const u32x4*>(st + r * HP + c);
-      }
-      if (half == 0 && col0 % 128 == 0 && col0 < np && row0 + lane < rows)
-        p.out_scales[col0 / 128 * p.slots + m0 + row0 + lane] = (uint8_t)s;
-    };
-    if constexpr (C::WN == 128) {
+        for (int i = 0; i < C::TM; ++i) {
+          float v[C::TN * 16];
+          hold(i);
+          const float top = hidden(i, v);
+          store(i, v, top);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        float v[C::TM][C::TN * 16], top[C::TM];
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        float v[C::TN * 16];
-        const float top = hidden(i, v);
-        store(i, v, top);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < C::TM; ++i) {
+          top[i] = hidden(i, v[i]);
+          if (half == 0) amax[wn * BM + wm * C::WM + 32 * i + lane] = top[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+          const int r = wm * C::WM + 32 * i + (lane & 31);
+          store(i, v[i], fmaxf(amax[r], amax[BM + r]));
+        }
       }
     } else {
-      float v[C::TM][C::TN * 16], top[C::TM];
+      // 32 rows of up to 128 bytes at a time through LDS, so that 8 lanes
+      // store a whole line
+      constexpr int V = 16 / sizeof(TOut);               // columns of a lane's store
+      constexpr int JB = C::TN < V / 4 ? C::TN : V / 4;  // blocks of 32 columns staged
+      constexpr int LPR = 32 * JB / V, RPI = 64 / LPR;   // lanes to a row, rows to a store
+      static_assert(C::TN % JB == 0 && (EPI != kFp8Pair || RPI == 8), "blocks");
+      TOut* out = reinterpret_cast<TOut*>(p.out);
+      const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.ldo % V == 0;
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        top[i] = hidden(i, v[i]);
-        if (half == 0) amax[wn * BM + wm * C::WM + 32 * i + lane] = top[i];
-      }
-      __syncthreads();
+      for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const int r = wm * C::WM + 32 * i + (lane & 31);
-        store(i, v[i], fmaxf(amax[r], amax[BM + r]));
-      }
+        for (int j0 = 0; j0 < C::TN; j0 += JB) {
+          if (j0 == 0) hold(i);
+#pragma unroll
+          for (int j = j0; j < j0 + JB; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              TOut* to4 = reinterpret_cast<TOut*>(st + (lane & 31) * C::OP) + 32 * (j - j0) + 8 * q + 4 * half;
+              const floatx4 b = bias4(j, q);
+              TOut v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = (TOut)(acc[j][i][4 * q + e] + b[e]);
+              if constexpr (sizeof(TOut) == 4) *reinterpret_cast<u32x4*>(to4) = *reinterpret_cast<const u32x4*>(v);
+              else *reinterpret_cast<u32x2*>(to4) = *reinterpret_cast<const u32x2*>(v);
+            }
+          if (i == 0 && j0 == 0) before_stores();
+          const int col = col0 + 32 * j0 + lane % LPR * V;
+#pragma unroll
+          for (int it = 0; it < 32 / RPI; ++it) {
+            const int r = RPI * it + lane / LPR, row = wm * C::WM + 32 * i + r;
+            const u32x4 raw = *reinterpret_cast<const u32x4*>(st + r * C::OP + lane % LPR * 16);
+            if (row >= done.rows || col >= p.N) continue;
+            TOut* to16 = out + (EPI == kFp8Pair ? (int64_t)place[32 * i + r] : (int64_t)(done.m0 + row)) * p.ldo + col;
+            if (vec && col + V <= p.N) {
+              *reinterpret_cast<u32x4*>(to16) = raw;
+            } else {
+              const TOut* v = reinterpret_cast<const TOut*>(&raw);
+#pragma unroll
+              for (int e = 0; e < V; ++e)
+                if (col + e < p.N) to16[e] = v[e];
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
     }
-  } else {
-    // 32 rows at a time through LDS, so that a store is 16 bytes of a run of
-    // the row. A lane has the same columns of every row it stores.
-    constexpr int V = 16 / sizeof(TOut), RUNS = C::WN / V, RPI = 64 / RUNS;
-    static_assert(64 % RUNS == 0, "whole rows a store");
-    const int c = lane % RUNS * V, col = col0 + c;
-    TOut* out = reinterpret_cast<TOut*>(p.out);
-    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.ldo % V == 0 && col + V <= p.N;
-    float b[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) b[e] = p.bias && col + e < p.N ? p.bias[(int64_t)expert * p.N + col + e] : 0.f;
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-#pragma unroll
-      for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<floatx4*>(st + (lane & 31) * C::OP + (32 * j + 8 * q + 4 * half) * 4) =
-              floatx4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-#pragma unroll
-      for (int it = 0; it < 32 / RPI; ++it) {
-        const int r = it * RPI + lane / RUNS, row = wm * C::WM + 32 * i + r;
-        float f[V];
-#pragma unroll
-        for (int e = 0; e < V; e += 4) {
-          const floatx4 t = *reinterpret_cast<const floatx4*>(st + r * C::OP + (c + e) * 4);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) f[e + u] = t[u] + b[e + u];
-        }
-        if (row >= rows || col >= p.N) continue;
-        TOut* to = out + (EPI == kFp8Pair ? (int64_t)p.g.pair[m0 + row] : (int64_t)(m0 + row)) * p.ldo + col;
-        if (vec) {
-          TOut v[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[e] = (TOut)f[e];
-          *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (col + e < p.N) to[e] = (TOut)f[e];
-        }
-      }
+    if (!more) break;
+    if constexpr (!C::AHEAD) {
+      __syncthreads();  // the staging lies over the ring
+      now = locate(T);
+      aim(now);
+      prologue();
     }
   }
 }
 
 template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
-__global__ __launch_bounds__(256, 1) void fp8_tile_kernel(Fp8Gemm p) {
+__global__ __launch_bounds__(256, (Fp8Cfg<BM, BN, NS>::AHEAD ? 1 : 2)) void fp8_tile_kernel(Fp8Gemm p) {
   __shared__ __attribute__((aligned(1024))) char smem[Fp8Cfg<BM, BN, NS>::LDS];
   fp8_tile_body<BM, BN, NS, EXACT, EPI, TOut>(p, smem);
 }
@@ -645,12 +726,15 @@ hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
   const int64_t nt = tm * ((p.N + BN - 1) / BN);
   if (p.g.tile && p.g.tile_rows != BM) return hipErrorInvalidValue;
   if (nt > (int64_t)1 << 28) return hipErrorInvalidValue;
-  fp8_tile_kernel<BM, BN, NS, EXACT, EPI, TOut><<<(unsigned)((nt + 7) / 8 * 8), 256, 0, s>>>(p);
+  // as many workgroups as the CUs hold at a time, 8 XCDs alike
+  const int64_t resident = (int64_t)device_cus() * (160 * 1024 / Fp8Cfg<BM, BN, NS>::LDS);
+  const int64_t grid = (std::min(nt, resident) + 7) / 8 * 8;
+  fp8_tile_kernel<BM, BN, NS, EXACT, EPI, TOut><<<(unsigned)grid, 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
 bool bad_gemm(const Fp8Gemm& p) {
-  return p.N <= 0 || p.K <= 0 || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);
+  return p.N <= 0 || p.K <= 0 || !p.bias || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);
 }
 
 }  // namespace
@@ -740,7 +824,7 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
   if (p.g.tile) {
     if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll || p.slots % 16 || p.slots * (fp8_kp(p.K) / 128) > INT32_MAX)
       return hipErrorInvalidValue;
-    if (p.epilogue == kFp8HiddenQ && (!p.bias || !p.zeros || p.N % 64)) return hipErrorInvalidValue;
+    if (p.epilogue == kFp8HiddenQ && p.N % 64) return hipErrorInvalidValue;
     if (p.epilogue == kFp8HiddenQ)
       return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8HiddenQ, float>(p, s)
                                   : launch_tile<128, 128, 2, false, kFp8HiddenQ, float>(p, s);

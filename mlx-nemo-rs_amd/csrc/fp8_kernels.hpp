@@ -27,6 +27,8 @@ constexpr int kFp8Block = 128;
 // A wave holds one row block's weight scales across its lanes, 4 to a word.
 constexpr int kFp8MaxK = 64 * 4 * kFp8Block;
 
+constexpr int kFp8BiasTail = 256;  // tiles read whole blocks of columns of the bias
+
 inline int64_t fp8_kp(int64_t k) { return (k + kFp8Block - 1) / kFp8Block * kFp8Block; }
 inline int64_t fp8_kbp(int64_t k) { return (fp8_kp(k) / kFp8Block + 3) / 4 * 4; }
 
@@ -79,10 +81,9 @@ struct Fp8Gemm {
   int64_t a_rows = 0;  // rows of a (or x) there are
   const uint8_t* w = nullptr;
   const uint8_t* ws = nullptr;
+  // [N] or [experts, N] (zeros, if there is none) with kFp8BiasTail floats
+  // behind it
   const float* bias = nullptr;
-  // kFp8HiddenQ needs one (of zeros, if there is none), and 32 zeros for
-  // blocks of columns past N
-  const float* zeros = nullptr;
   int64_t w_stride = 0, ws_stride = 0;  // bytes between experts
   int M = 0, N = 0, K = 0;
   int epilogue = kFp8Out;
