@@ -161,9 +161,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int* idx
 // the tile list. The order of an expert's pairs among its slots is that of
 // the atomics and may change from call to call: no result depends on it, as a
 // slot's row is computed from that row alone.
-__global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* idx, int pairs, int experts,
-                                                                    int tile_rows, const int* hist, int* pair,
-                                                                    int* tile, int* n_tiles) {
+__global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* idx, int pairs, int top_k,
+                                                                    int experts, int tile_rows, const int* hist,
+                                                                    int* pair, int* frame, int* tile, int* n_tiles) {
   __shared__ int cursor[kPlanExperts], slots[2][kPlanExperts], tiles[2][kPlanExperts];
   const int t = threadIdx.x;
   int mine[kPlanPer];
@@ -206,7 +206,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* i
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i)
-    if (mine[i] >= 0) pair[atomicAdd(&cursor[mine[i]], 1)] = blockIdx.x * kPlanChunk + i * kPlanThreads + t;
+    if (mine[i] >= 0) {
+      const int p = blockIdx.x * kPlanChunk + i * kPlanThreads + t, slot = atomicAdd(&cursor[mine[i]], 1);
+      pair[slot] = p;
+      frame[slot] = p / top_k;
+    }
   if (blockIdx.x == 0) {
     if (t == kPlanThreads - 1) *n_tiles = tiles[cur][t];
     for (int i = 0; i < nt; ++i) {
@@ -286,13 +290,13 @@ hipError_t route(const RouteParams& p, hipStream_t s) {
 
 int64_t plan_scratch_ints(int64_t pairs, int experts) { return (pairs + kPlanChunk - 1) / kPlanChunk * experts; }
 
-hipError_t experts_plan(const int* idx, int pairs, int experts, int tile_rows, int* pair, int* tile, int* n_tiles,
-                        int* scratch, hipStream_t s) {
-  if (pairs <= 0 || experts <= 0 || experts > kPlanExperts || tile_rows <= 0) return hipErrorInvalidValue;
+hipError_t experts_plan(const int* idx, int pairs, int top_k, int experts, int tile_rows, int* pair, int* frame,
+                        int* tile, int* n_tiles, int* scratch, hipStream_t s) {
+  if (pairs <= 0 || top_k <= 0 || experts <= 0 || experts > kPlanExperts || tile_rows <= 0) return hipErrorInvalidValue;
   const int chunks = (pairs + kPlanChunk - 1) / kPlanChunk;
   if (chunks > 1) plan_count_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, experts, scratch);
-  plan_scatter_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, experts, tile_rows, chunks > 1 ? scratch : nullptr,
-                                                      pair, tile, n_tiles);
+  plan_scatter_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, top_k, experts, tile_rows,
+                                                      chunks > 1 ? scratch : nullptr, pair, frame, tile, n_tiles);
   return hipGetLastError();
 }
 

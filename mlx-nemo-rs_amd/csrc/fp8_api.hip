@@ -356,7 +356,7 @@ struct ExpertsPlan {
   int tile_rows = 0;  // 0: no list; 16: few-row kernel; else tiles
   int max_tiles = 0;
   int64_t slots = 0;
-  int *pair = nullptr, *tile = nullptr, *n_tiles = nullptr, *scratch = nullptr;
+  int *pair = nullptr, *frame = nullptr, *tile = nullptr, *n_tiles = nullptr, *scratch = nullptr;
   uint8_t *xc = nullptr, *xs = nullptr, *hc = nullptr, *hsc = nullptr;
   float *h = nullptr, *y = nullptr;
   int64_t bytes = 0;
@@ -370,9 +370,10 @@ ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void*
   const int64_t pairs = p.step * top_k;
   Arena a(ws);
   if (rows * top_k > kFewPairs) {
-    p.tile_rows = mhsa::fp8_group_rows(pairs, e->E);
+    p.tile_rows = mhsa::fp8_group_rows(pairs, e->E, std::min(e->D, e->F));
     p.max_tiles = (int)(pairs / p.tile_rows + std::min<int64_t>(pairs, e->E));
     p.pair = a.take<int>(mhsa::expert_slots(pairs, e->E));
+    p.frame = a.take<int>(mhsa::expert_slots(pairs, e->E));
     p.tile = a.take<int>(4 * (int64_t)p.max_tiles);
     p.n_tiles = a.take<int>(1);
     p.scratch = a.take<int>(mhsa::plan_scratch_ints(pairs, e->E));
@@ -416,6 +417,7 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
       g[i].g.max_tiles = (int)(pairs / plan.tile_rows + std::min(pairs, e->E));
       g[i].g.tile_rows = plan.tile_rows;
       g[i].g.pair = plan.pair;
+      g[i].g.frame = plan.frame;
     } else {
       g[i].g.idx = idx;
     }
@@ -423,7 +425,8 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
   g[1].epilogue = mhsa::kFp8Pair;
   g[1].out = plan.y;
   if (plan.tile_rows)
-    HIPCHK(mhsa::experts_plan(idx, pairs, e->E, plan.tile_rows, plan.pair, plan.tile, plan.n_tiles, plan.scratch, s));
+    HIPCHK(mhsa::experts_plan(idx, pairs, top_k, e->E, plan.tile_rows, plan.pair, plan.frame, plan.tile, plan.n_tiles,
+                              plan.scratch, s));
   if (plan.tile_rows > 16) {
     HIPCHK(mhsa::fp8_quantize_rows(dt, x, e->D, rows, e->D, plan.xc, plan.xs, s));
     g[0].a = plan.xc;

@@ -267,10 +267,11 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
 // a register that holds all of them.
 //
 // Workgroups stay and take tile after tile. A large tile has its CU to itself
-// and LDS for staging its results beside the ring, so the next tile's rows are
-// looked up and its first loads issued before the epilogue (3.7 us a tile of
-// waiting on the list, the pairs and the first lines otherwise). Small tiles
-// share a CU, whose other workgroup computes meanwhile.
+// and LDS for staging its results beside the ring, so the ring runs on from
+// tile to tile: the last stages' loads are the next tile's first, whose place
+// in the list and rows were looked up a tile ahead (waiting for the list, the
+// rows and the first lines took 3.7 us a tile). Small tiles share a CU, whose
+// other workgroup computes meanwhile.
 // ---------------------------------------------------------------------------
 
 template <int BM, int BN, int NS_>
@@ -279,8 +280,8 @@ struct Fp8Cfg {
   static constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
   static constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
   static constexpr int NA = BM / 32, NB = BN / 32;  // 1 KB loads per wave and stage
-  static constexpr int SCALES = NS * STAGE;         // two words a row (or 256 bytes a stage) behind the stages
-  static constexpr int LOOP = SCALES + 2 * BM * 4;
+  static constexpr int SCALES = NS * STAGE;         // a word a row (or 256 bytes) of every stage, behind the stages
+  static constexpr int LOOP = SCALES + NS * BM * 4;
   // results are staged 32 rows of 128 bytes at a time and wave; behind them a
   // wave keeps its columns' bias and its rows' places
   static constexpr int OP = 128 + 16, WST = 32 * OP + 4 * (WN + WM), STG = 4 * WST, AMAX = 2 * BM * 4;
@@ -288,7 +289,7 @@ struct Fp8Cfg {
   static constexpr int OUT = AHEAD ? LOOP : 0;
   static constexpr int LDS = AHEAD ? LOOP + STG : LOOP > STG + AMAX ? LOOP : STG + AMAX;
   static_assert(LDS <= 160 * 1024, "tile exceeds LDS");
-  static_assert(BM <= 256 && (BM < 128 || NS * 256 <= 2 * BM * 4), "scales");
+  static_assert(BM >= 64 && BM <= 256 && (!AHEAD || NS == 2), "scales, stages");
 };
 
 template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
@@ -309,17 +310,24 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   struct Tile {
     int expert, m0, rows, n0;
   };
-  auto locate = [&](int t) {
+  struct Place {  // of a tile: its row tile (of the list, if there is one) and its first column
+    int tm, n0;
+  };
+  auto place_of = [&](int t) -> Place {
     constexpr int GM = 8;
     const int gsz = GM * tilesN, first = t / gsz * GM, gm = min(tilesM - first, GM);
-    const int tm = first + (t % gsz) % gm;
-    Tile r = {0, tm * BM, min(p.M - tm * BM, BM), (t % gsz) / gm * BN};
-    if (grouped) {
-      r.expert = __builtin_amdgcn_readfirstlane(p.g.tile[4 * tm]);
-      r.m0 = __builtin_amdgcn_readfirstlane(p.g.tile[4 * tm + 1]);
-      r.rows = __builtin_amdgcn_readfirstlane(p.g.tile[4 * tm + 2]);
-    }
-    return r;
+    return {first + (t % gsz) % gm, (t % gsz) / gm * BN};
+  };
+  struct Entry {
+    int expert, m0, rows;
+  };
+  auto entry_of = [&](int tm) -> Entry {
+    if (!grouped) return {0, tm * BM, min(p.M - tm * BM, BM)};
+    return {p.g.tile[4 * tm], p.g.tile[4 * tm + 1], p.g.tile[4 * tm + 2]};
+  };
+  auto tile_of = [&](const Entry& e, int n0) -> Tile {
+    return {__builtin_amdgcn_readfirstlane(e.expert), __builtin_amdgcn_readfirstlane(e.m0),
+            __builtin_amdgcn_readfirstlane(e.rows), n0};
   };
 
   // activations: a tile's rows, or gathered ones (rows past the tile's repeat
@@ -329,7 +337,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   const bool gather = grouped && p.rows == Fp8Gemm::kByFrame;
   __amdgpu_buffer_rsrc_t ra, rs, rb;
   int aoff[C::NA], boff[C::NB], soff;
-  uint32_t wword;
+  uint32_t wword = 0;
   const int srow = (w * 64) % BM;
 #pragma unroll
   for (int g = 0; g < C::NB; ++g) {  // load g of wave w fills 8 LDS rows: lane l row l / 8, stored chunk l % 8
@@ -344,46 +352,50 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(u), (short)0, __builtin_amdgcn_readfirstlane((int)n),
                                              kRawBuffer);
   };
-  auto aim = [&](const Tile& t) {  // the loads below are tile t's
+  // source rows of this lane's loads of tile t
+  int src[C::NA + 1];
+  auto look_up = [&](const Tile& t) {
+    auto source = [&](int row) { return gather ? p.g.frame[t.m0 + min(row, t.rows - 1)] : min(row, t.rows - 1); };
+#pragma unroll
+    for (int g = 0; g < C::NA; ++g) src[g] = source((w * C::NA + g) * 8 + (lane >> 3));
+    src[C::NA] = HT ? 0 : source(srow + lane);
+  };
+  auto aim = [&](const Tile& t) {  // the loads below are tile t's, looked up before
     const int64_t arows = gather ? p.a_rows : t.rows;
     ra = rsrc(p.a + (gather ? 0 : (int64_t)t.m0 * kp), (uint32_t)(arows * kp));
     rs = rsrc(HT ? p.as + t.m0 : p.as + (gather ? 0 : (int64_t)t.m0 * kbp), (uint32_t)(HT ? kb * p.slots - t.m0 : arows * kbp));
-    auto source = [&](int row) -> uint32_t {
-      row = min(row, t.rows - 1);
-      return gather ? (uint32_t)(p.g.pair[t.m0 + row] / p.g.top_k) : (uint32_t)row;
-    };
 #pragma unroll
     for (int g = 0; g < C::NA; ++g) {
       const int row = (w * C::NA + g) * 8 + (lane >> 3);
-      aoff[g] = (int)(source(row) * (uint32_t)kp + 16 * ((lane & 7) ^ ((row >> 1) & 7)));
+      aoff[g] = (int)((uint32_t)src[g] * (uint32_t)kp + 16 * ((lane & 7) ^ ((row >> 1) & 7)));
     }
-    soff = HT ? 4 * lane : (int)(source(srow + lane) * (uint32_t)kbp);
+    soff = HT ? 4 * lane : (int)((uint32_t)src[C::NA] * (uint32_t)kbp);
     rb = rsrc(p.w + t.expert * p.w_stride + (int64_t)t.n0 * kp, (uint32_t)(min(p.N - t.n0, BN) * kp));
-    // the weight scales of this wave's 128-column block, a word of 4 to a lane
-    const int wblk = min((t.n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
-    wword = *reinterpret_cast<const uint32_t*>(p.ws + t.expert * p.ws_stride + (int64_t)wblk * kbp +
-                                               4 * min(lane, kbp / 4 - 1));
   };
-  constexpr int LOADS = C::NA + C::NB + 1, EARLY = (LOADS * 2 + 2) / 3;
-  auto issue1 = [&](int g, int kt) {  // load g of stage kt
-    char* S = smem + kt % NS * C::STAGE;
-    const int k = min(kt, kb - 1);  // (past the end: the last stage again, unread)
+  // the weight scales of this wave's 128-column block, a word of 4 to a lane
+  auto weight_scales = [&](const Tile& t) {
+    const int blk = min((t.n0 + wn * C::WN) / 128, (p.N + 127) / 128 - 1);
+    return *reinterpret_cast<const uint32_t*>(p.ws + t.expert * p.ws_stride + (int64_t)blk * kbp + 4 * min(lane, kbp / 4 - 1));
+  };
+  constexpr int LOADS = C::NA + C::NB + 1;
+  auto issue1 = [&](int g, int k, int buf) {  // load g of the aimed tile's stage k
+    char* S = smem + buf * C::STAGE;
     if (g < C::NA)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(S + (w * C::NA + g) * 1024), 16, aoff[g], k * 128, 0, 0);
     else if (g < C::NA + C::NB)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(S + C::ABYTES + (w * C::NB + g - C::NA) * 1024), 16,
                                                boff[g - C::NA], k * 128, 0, 0);
-    else if (HT)  // 256 rows' bytes, by every wave; rows past the slots read as 0
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + kt % NS * 256), 4, soff,
+    else if (HT)  // 256 rows' bytes, the same by every wave; past the slots: 0
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + buf * BM * 4), 4, soff,
                                                (int)(k * p.slots), 0, 0);
-    else  // a word is loaded again by each of its stages, and by two waves of
-          // a tile of under 256 rows: always the same bytes
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + ((k >> 2) & 1) * BM * 4 + srow * 4), 4,
-                                               soff, k & ~3, 0, 0);
+    else  // 64 rows' words, twice the same in a tile of under 256 rows
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(smem + C::SCALES + buf * BM * 4 + srow * 4), 4, soff, k & ~3, 0,
+                                               0);
   };
-  auto landed = [&]() {  // the last NS - 2 stages' loads may still be in flight
-    constexpr int vm = (NS - 2) * LOADS;
-    static_assert(NS >= 2 && vm < 64, "wait count");
+  // everywhere: all but the last `n` memory operations issued are done, LDS reads are
+  auto settled = [&](auto n) {
+    constexpr int vm = decltype(n)::value;
+    static_assert(vm < 64, "wait count");
     __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));  // lgkmcnt(0)
     asm volatile("s_barrier" ::: "memory");
   };
@@ -397,64 +409,56 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     for (int u = 0; u < 2; ++u) off[h][u] = 16 * ((4 * h + 2 * half + u) ^ ((lane >> 1) & 7));
   u32x4 fa[2][C::TM][2], fb[2][C::TN][2];
   int xw[C::TM];
-  // read r of half h of stage kt into set h: its fragments (the weight's
-  // first, then the rows'), then the row scales (past the end: unused)
+  // read r of half h of the stage in buffer buf into set h: its fragments (the
+  // weight's first, then the rows'), then the row scales
   constexpr int FRAGS = 2 * (C::TM + C::TN);
-  auto rd1 = [&](int r, int kt, int h) {
-    const char* S = smem + kt % NS * C::STAGE;
+  auto rd1 = [&](int r, int buf, int h) {
+    const char* S = smem + buf * C::STAGE;
     if (r < 2 * C::TN) {
       fb[h][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + brow + off[h][r % 2] + r / 2 * 4096);
     } else if (r < FRAGS) {
       r -= 2 * C::TN;
       fa[h][r / 2][r % 2] = *reinterpret_cast<const u32x4*>(S + arow + off[h][r % 2] + r / 2 * 4096);
     } else if (HT) {
-      xw[r - FRAGS] = *reinterpret_cast<const uint8_t*>(smem + C::SCALES + kt % NS * 256 + wm * C::WM + 32 * (r - FRAGS) +
+      xw[r - FRAGS] = *reinterpret_cast<const uint8_t*>(smem + C::SCALES + buf * BM * 4 + wm * C::WM + 32 * (r - FRAGS) +
                                                         (lane & 31));
     } else {
-      xw[r - FRAGS] = *reinterpret_cast<const int*>(smem + C::SCALES + ((min(kt, kb - 1) >> 2) & 1) * BM * 4 +
-                                                    (wm * C::WM + 32 * (r - FRAGS) + (lane & 31)) * 4);
+      xw[r - FRAGS] =
+          *reinterpret_cast<const int*>(smem + C::SCALES + buf * BM * 4 + (wm * C::WM + 32 * (r - FRAGS) + (lane & 31)) * 4);
     }
   };
   floatx16 acc[C::TN][C::TM], part[EXACT ? C::TN : 1][EXACT ? C::TM : 1];
 
   int ws = 0, xs[C::TM];
-  // Half h of stage kt, whose fragments are in set h. The reads of the next
-  // half's fragments and the loads that refill the buffer are placed between
-  // the MFMAs (issued ahead of them, the reads filled the wave's queue of 15
-  // and held the first MFMA back). The loads, stage kt + NS's, begin behind the
-  // second half's barrier and end in the next stage's first half: in one half
-  // they came at the rate at which a CU takes lines from its L1, and waves
-  // stood at their issue.
-  auto step = [&](int kt, auto hc) {
+  // Half h of stage kt, whose fragments are in set h and whose buffer is buf.
+  // The reads of the next half's fragments and, behind the second half's
+  // barrier, the loads that refill the buffer (stage `refill` of the aimed
+  // tile) are placed between the MFMAs: issued ahead of
+  // them, the reads filled the wave's queue of 15 and held the first MFMA
+  // back.
+  auto step = [&](int kt, int buf, int refill, auto hc) {
     constexpr int h = decltype(hc)::value;
     if constexpr (h == 0) {
       const int sh = 8 * (kt & 3);
       ws = __builtin_amdgcn_readlane((int)wword, kt >> 2) >> sh;
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) xs[i] = HT ? xw[i] : xw[i] >> sh;
-    } else {
-      landed();  // stage kt + 1, everywhere; stage kt's buffer has been read
     }
+    const int other = buf + 1 == NS ? 0 : buf + 1;
     __builtin_amdgcn_sched_barrier(0);
     constexpr int NMF = EXACT ? 4 * C::TM * C::TN : C::TM * C::TN;
     constexpr int READS = FRAGS + (h == 1 ? C::TM : 0);
     constexpr int SLOTS = (NMF + 1) / 2;  // behind the first MFMAs the reads, behind all the loads
     constexpr int RPM = (READS + SLOTS - 1) / SLOTS;
     auto between = [&](int m) {
-      // load g behind MFMA g NMF / EARLY of the second half, the rest in the
-      // first MFMAs of the next
       if constexpr (h == 1) {
 #pragma unroll
-        for (int g = 0; g < EARLY; ++g)
-          if (g * NMF / EARLY == m) issue1(g, kt + NS);
-      } else {
-#pragma unroll
-        for (int g = EARLY; g < LOADS; ++g)
-          if ((g - EARLY) * SLOTS / (LOADS - EARLY) == m) issue1(g, kt - 1 + NS);
+        for (int g = 0; g < LOADS; ++g)
+          if (g * NMF / LOADS == m) issue1(g, refill, buf);
       }
 #pragma unroll
       for (int r = m * RPM; r < (m + 1) * RPM; ++r)
-        if (r < READS) rd1(r, kt + h, h ^ 1);
+        if (r < READS) rd1(r, h == 0 ? buf : other, h ^ 1);
       __builtin_amdgcn_sched_barrier(0);
     };
     if constexpr (!EXACT) {
@@ -504,64 +508,105 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       }
     }
   };
-  auto prologue = [&]() {
+  constexpr auto H0 = std::integral_constant<int, 0>{};
+  constexpr auto H1 = std::integral_constant<int, 1>{};
+  auto prologue = [&]() {  // the aimed tile's first NS stages
 #pragma unroll
     for (int st = 0; st < NS; ++st)
 #pragma unroll
-      for (int g = 0; g < (st == NS - 1 ? EARLY : LOADS); ++g) issue1(g, st);
+      for (int g = 0; g < LOADS; ++g) issue1(g, min(st, kb - 1), st);
+    settled(std::integral_constant<int, (NS - 1) * LOADS>{});
+  };
+  // The columns' bias and the rows' places that a tile's epilogue needs, a
+  // register each, then LDS (held in registers for all of the lane's columns
+  // and rows, they spilled).
+  constexpr int BL = (C::WN + 63) / 64, PL = EPI == kFp8Pair ? (C::WM + 63) / 64 : 0;
+  float bl[BL];
+  int pl[PL ? PL : 1];
+  auto columns = [&](const Tile& t) {
+#pragma unroll
+    for (int u = 0; u < BL; ++u) {
+      const int c = t.n0 + wn * C::WN + 64 * u + lane;
+      bl[u] = EPI == kFp8HiddenQ && c >= p.N ? 0.f : p.bias[(int64_t)t.expert * p.N + c];
+    }
+#pragma unroll
+    for (int u = 0; u < PL; ++u) pl[u] = p.g.pair[t.m0 + min(wm * C::WM + 64 * u + lane, t.rows - 1)];
   };
 
-  Tile now = locate(T);
+  const int stride = (int)(gridDim.x / 8u);
+  Place where = place_of(T);
+  Tile now = tile_of(entry_of(where.tm), where.n0), next = now;
+  look_up(now);
   aim(now);
-  prologue();
-  bool waited = false;  // the prologue's loads have landed
-  for (;;) {
-    if (!waited) {  // stage 0 has
-      constexpr int vm = (NS - 2) * LOADS + EARLY;
-      static_assert(vm < 64, "wait count");
-      __builtin_amdgcn_s_waitcnt((vm & 15) | ((vm >> 4) << 14) | (7 << 4));
+  wword = weight_scales(now);
+  uint32_t wnext = 0;
+  Entry after = {0, 0, 0};  // the list's entry of the tile after the next
+  int after_n0 = 0, base = 0;
+  // What is looked up ahead of tile T's loop, the ring's loads of which are
+  // on their way: the next tile's rows and scales, the entry of the one after
+  // it, and what this one's epilogue needs.
+  auto look_ahead = [&]() {
+    if (T + stride < T1) {
+      look_up(next);
+      wnext = weight_scales(next);
     }
-    asm volatile("s_barrier" ::: "memory");
+    if (T + 2 * stride < T1) {
+      const Place q = place_of(T + 2 * stride);
+      after = entry_of(q.tm);
+      after_n0 = q.n0;
+    }
+    columns(now);
+  };
+  if constexpr (C::AHEAD) {
+    if (T + stride < T1) {
+      where = place_of(T + stride);
+      next = tile_of(entry_of(where.tm), where.n0);
+    }
+  }
+  prologue();
+  if constexpr (C::AHEAD) look_ahead();
+  bool stored = false;  // the last epilogue's stores, a known number, are behind the ring's loads
+  for (;;) {
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
+    // (a tile's last step read these too, but held over the epilogue they spilled)
 #pragma unroll
-    for (int r = 0; r < FRAGS + C::TM; ++r) rd1(r, 0, 0);
-    for (int kt = 0; kt < kb; ++kt) {
-      step(kt, std::integral_constant<int, 0>{});
-      step(kt, std::integral_constant<int, 1>{});
+    for (int r = 0; r < FRAGS + C::TM; ++r) rd1(r, C::AHEAD ? base & 1 : 0, 0);
+    const bool more = T + stride < T1;
+    constexpr int STORES = C::TM * (C::WN / 32 + 1);
+    if constexpr (C::AHEAD) {
+      auto stage = [&](int kt, int refill) {
+        const int buf = (base + kt) & 1;
+        step(kt, buf, 0, H0);
+        if (EPI == kFp8HiddenQ && kt == 0 && stored) settled(std::integral_constant<int, STORES>{});
+        else settled(H0);
+        step(kt, buf, refill, H1);
+      };
+      int kt = 0;
+      for (; kt < kb - NS; ++kt) stage(kt, kt + NS);
+      if (more) aim(next);
+      for (; kt < kb; ++kt) stage(kt, more ? kt + NS - kb : kb - 1);  // (at the end: unread)
+      base += kb;
+    } else {
+      for (int kt = 0; kt < kb; ++kt) {
+        const int buf = kt % NS;
+        step(kt, buf, 0, H0);
+        settled(std::integral_constant<int, (NS - 2) * LOADS>{});
+        step(kt, buf, min(kt + NS, kb - 1), H1);  // (past the end: the last stage again, unread)
+      }
+      columns(now);
+      // the loads past the end still write LDS: all of them are to have landed
+      // before it is used again
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
     }
-    // the loads past the end still write LDS: all of them are to have landed
-    // before the ring is used again
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
 
     const Tile done = now;
-    T += (int)(gridDim.x / 8u);
-    const bool more = T < T1;
-    // What the epilogue loads comes ahead of the next tile's loads, which it
-    // would otherwise wait for. Lane: row 32 i + lane % 32 of the wave's
-    // block, columns 32 j + 8 q + 4 (lane / 32) + [0, 4).
+    // Lane: row 32 i + lane % 32 of the wave's block, columns 32 j + 8 q +
+    // 4 (lane / 32) + [0, 4).
     const int col0 = done.n0 + wn * C::WN;
-    // (a register each, then LDS: held in registers for all of the lane's
-    // columns and rows, they spilled)
-    constexpr int BL = (C::WN + 63) / 64, PL = EPI == kFp8Pair ? (C::WM + 63) / 64 : 0;
-    float bl[BL];
-    int pl[PL ? PL : 1];
-#pragma unroll
-    for (int u = 0; u < BL; ++u) {
-      const int c = col0 + 64 * u + lane;
-      bl[u] = EPI == kFp8HiddenQ && c >= p.N ? 0.f : p.bias[(int64_t)done.expert * p.N + c];
-    }
-#pragma unroll
-    for (int u = 0; u < PL; ++u) pl[u] = p.g.pair[done.m0 + min(wm * C::WM + 64 * u + lane, done.rows - 1)];
-    asm volatile("" ::: "memory");
-    if (C::AHEAD && more) {
-      now = locate(T);
-      aim(now);
-      prologue();
-    }
     char* st = smem + C::OUT + w * C::WST;
     float* bias = reinterpret_cast<float*>(st + 32 * C::OP);
     int* place = reinterpret_cast<int*>(bias + C::WN);
@@ -578,12 +623,16 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       for (int j = 0; j < C::TN; ++j) asm volatile("" : "+a"(acc[j][i]));
     };
     auto bias4 = [&](int j, int q) { return *reinterpret_cast<const floatx4*>(bias + 32 * j + 8 * q + 4 * half); };
-    auto before_stores = [&]() {  // (loads and stores are counted together, in order)
-      if constexpr (C::AHEAD) {
-        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
-        waited = true;
-      }
-    };
+    T += stride;
+    if (C::AHEAD && more) {
+      // (ahead of the stores, which the ring's next wait leaves behind)
+      now = next;
+      wword = wnext;
+      if (T + stride < T1) next = tile_of(after, after_n0);
+      look_ahead();
+      asm volatile("" ::: "memory");
+      stored = true;
+    }
 
     if constexpr (EPI == kFp8HiddenQ) {
       // silu, then codes: the block's 128 columns of a row lie in one wave
@@ -591,6 +640,9 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       float* amax = reinterpret_cast<float*>(smem + C::STG);
       const int np = (p.N + 127) / 128 * 128;
       constexpr int HP = C::WN + 16;
+      const __amdgpu_buffer_rsrc_t rc = rsrc(p.out_codes + (int64_t)done.m0 * np, (uint32_t)(done.rows * np));
+      const __amdgpu_buffer_rsrc_t rh =
+          rsrc(p.out_scales + min(col0 / 128, np / 128 - 1) * p.slots + done.m0, (uint32_t)done.rows);
       // (32 rows at a time, with nothing of the next ones moved ahead: 256
       // accumulators and as many results at once spilled)
       auto hidden = [&](int i, float v[C::TN * 16]) {
@@ -624,16 +676,16 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
                 fp8_pack4_scaled(f[0], f[1], f[2], f[3], scale);
           }
         const int row0 = wm * C::WM + 32 * i;
-        if (i == 0) before_stores();
+        // (rows and columns that are not the tile's lie past the buffers' ends:
+        // every store is issued, so that their number is known)
 #pragma unroll
         for (int it = 0; it < C::WN / 32; ++it) {
           const int id = it * 64 + lane, r = id / (C::WN / 16), c = id % (C::WN / 16) * 16;
-          if (row0 + r < done.rows && col0 + c < np)
-            *reinterpret_cast<u32x4*>(p.out_codes + (int64_t)(done.m0 + row0 + r) * np + col0 + c) =
-                *reinterpret_cast<const u32x4*>(st + r * HP + c);
+          __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(st + r * HP + c), rc,
+                                                 col0 + c < np ? (row0 + r) * np + col0 + c : -1, 0, 0);
         }
-        if (half == 0 && col0 % 128 == 0 && col0 < np && row0 + lane < done.rows)
-          p.out_scales[col0 / 128 * p.slots + done.m0 + row0 + lane] = (uint8_t)s;
+        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)s, rh, half == 0 && col0 % 128 == 0 && col0 < np ? row0 + lane : -1, 0,
+                                             0);
       };
       if constexpr (C::WN == 128) {
 #pragma unroll
@@ -684,7 +736,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
               if constexpr (sizeof(TOut) == 4) *reinterpret_cast<u32x4*>(to4) = *reinterpret_cast<const u32x4*>(v);
               else *reinterpret_cast<u32x2*>(to4) = *reinterpret_cast<const u32x2*>(v);
             }
-          if (i == 0 && j0 == 0) before_stores();
           const int col = col0 + 32 * j0 + lane % LPR * V;
 #pragma unroll
           for (int it = 0; it < 32 / RPI; ++it) {
@@ -704,11 +755,17 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
           __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if (!more) break;
+    if (!more) {
+      __builtin_amdgcn_s_waitcnt(0);  // nothing is to land in LDS that is no longer this workgroup's
+      break;
+    }
     if constexpr (!C::AHEAD) {
       __syncthreads();  // the staging lies over the ring
-      now = locate(T);
+      where = place_of(T);
+      now = tile_of(entry_of(where.tm), where.n0);
+      look_up(now);
       aim(now);
+      wword = weight_scales(now);
       prologue();
     }
   }
@@ -725,6 +782,7 @@ hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
   const int64_t tm = p.g.tile ? p.g.max_tiles : (p.M + BM - 1) / BM;
   const int64_t nt = tm * ((p.N + BN - 1) / BN);
   if (p.g.tile && p.g.tile_rows != BM) return hipErrorInvalidValue;
+  if (Fp8Cfg<BM, BN, NS>::AHEAD && p.K <= kFp8Block) return hipErrorInvalidValue;
   if (nt > (int64_t)1 << 28) return hipErrorInvalidValue;
   // as many workgroups as the CUs hold at a time, 8 XCDs alike
   const int64_t resident = (int64_t)device_cus() * (160 * 1024 / Fp8Cfg<BM, BN, NS>::LDS);
@@ -814,9 +872,9 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-int fp8_group_rows(int64_t pairs, int experts) {
+int fp8_group_rows(int64_t pairs, int experts, int K) {
   const int64_t mean = pairs / experts;
-  return mean < 24 ? 16 : mean < 192 ? 128 : 256;
+  return mean < 24 ? 16 : mean < 192 || K <= kFp8Block ? 128 : 256;  // (the large tiles' ring takes two stages)
 }
 
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
@@ -839,7 +897,7 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
     return tiles(128, 128) >= 128 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s)
                                   : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
   const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256);
-  if (t256 >= 128) {
+  if (t256 >= 128 && p.K > kFp8Block) {  // (the large tiles' ring takes two stages)
     if ((t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256) return launch_tile<192, 256, 2, false, kFp8Out, bf16>(p, s);
     return launch_tile<256, 256, 2, false, kFp8Out, bf16>(p, s);
   }

@@ -56,6 +56,7 @@ struct Fp8Groups {
   const int* n_tiles = nullptr;
   int max_tiles = 0, tile_rows = 0;
   const int* pair = nullptr;
+  const int* frame = nullptr;  // pair / top_k
   int top_k = 1;
   // few pairs: no tile list; workgroup column y looks at pair y of idx
   const int* idx = nullptr;
@@ -102,18 +103,18 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s);
 // cores (exact products), every other on the fp8 ones.
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s);
 // Rows of a tile for `pairs` pairs over `experts` experts (0: the few-row
-// kernel's groups of 16).
-int fp8_group_rows(int64_t pairs, int experts);
+// kernel's groups of 16); K: the smaller of the two products'.
+int fp8_group_rows(int64_t pairs, int experts, int K);
 
 // Slots that `pairs` pairs take at most, a multiple of 16.
 inline int64_t expert_slots(int64_t pairs, int experts) {
   return (pairs + 15 * (pairs < experts ? pairs : experts) + 15) / 16 * 16;
 }
-// Experts' bookkeeping: pairs sorted by expert (pair [expert_slots]), and the
-// tile list of tile_rows slots. scratch: plan_scratch_ints(pairs, experts) ints.
+// Experts' bookkeeping: pairs sorted by expert and their frames (pair and
+// frame [expert_slots]), and the tile list of tile_rows slots. scratch: plan_scratch_ints(pairs, experts) ints.
 int64_t plan_scratch_ints(int64_t pairs, int experts);
-hipError_t experts_plan(const int* idx, int pairs, int experts, int tile_rows, int* pair, int* tile, int* n_tiles,
-                        int* scratch, hipStream_t s);
+hipError_t experts_plan(const int* idx, int pairs, int top_k, int experts, int tile_rows, int* pair, int* frame,
+                        int* tile, int* n_tiles, int* scratch, hipStream_t s);
 // out = residual + res_scale * sum_j w[r, j] y[r * top_k + j] over the chosen
 // experts in [0, experts); residual may be null or out.
 hipError_t experts_combine(DType dt, const float* y, const int* idx, const float* w, int64_t rows, int top_k,
