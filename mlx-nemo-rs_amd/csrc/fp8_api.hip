@@ -346,7 +346,6 @@ struct mhsa_experts {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTopK = 32;
-constexpr int kFewPairs = 64;  // up to these no list of pairs is built
 constexpr int64_t kMaxPairs = 1 << 18;
 
 // How a call runs, and its pieces of the workspace. Rows go in runs of
@@ -369,8 +368,10 @@ ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void*
   p.step = std::min(rows, most);
   const int64_t pairs = p.step * top_k;
   Arena a(ws);
-  if (rows * top_k > kFewPairs) {
-    p.tile_rows = mhsa::fp8_group_rows(pairs, e->E, std::min(e->D, e->F));
+  // (a list costs a launch; without one every workgroup scans the indices)
+  p.tile_rows = mhsa::fp8_group_rows(pairs, e->E, std::min(e->D, e->F));
+  if (rows * top_k <= 256 || (p.tile_rows == 16 && rows * top_k <= mhsa::fp8_scan_pairs())) p.tile_rows = 0;
+  if (p.tile_rows) {
     p.max_tiles = (int)(pairs / p.tile_rows + std::min<int64_t>(pairs, e->E));
     p.pair = a.take<int>(mhsa::expert_slots(pairs, e->E));
     p.frame = a.take<int>(mhsa::expert_slots(pairs, e->E));
@@ -453,6 +454,12 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
     g[1].x_dt = mhsa::kF32;
     g[1].ldx = e->F;
     g[1].rows = mhsa::Fp8Gemm::kByPair;
+    if (!plan.tile_rows && mhsa::fp8_few_sum_ok(pairs, e->F)) {
+      g[1].out = out;
+      g[1].out_dt = dt;
+      HIPCHK(mhsa::fp8_gemm_few_sum(g[1], weights, residual, res_scale, s));
+      return MHSA_OK;
+    }
     HIPCHK(mhsa::fp8_gemm_few(g[1], s));
   }
   HIPCHK(mhsa::experts_combine(dt, plan.y, idx, weights, rows, top_k, e->E, e->D, residual, res_scale, out, s));

@@ -139,21 +139,14 @@ __global__ __launch_bounds__(256) void unpad_weight_kernel(const uint8_t* codes,
 // ---------------------------------------------------------------------------
 // Few rows
 //
-// Weights are read once and everything else is small: a workgroup computes 16
-// output columns of up to 16 rows, its NW waves take every NW-th block of 128
-// inputs, and their sums are added in wave order at the end. One 16x16x128 MFMA
-// covers a block: lane l holds 32 inputs, 32 (l / 16) on, of weight row l % 16
-// and of activation row l % 16. The activations are rounded to codes in these
-// registers (the block's maximum is one over 4 lanes), so there is no other
-// launch.
+// Weights are read once and everything else is small: a workgroup computes
+// 16 RC output columns of up to 16 rows, its NW waves take every NW-th block
+// of 128 inputs, and their sums are added in wave order at the end. One
+// 16x16x128 MFMA covers a block: lane l holds 32 inputs, 32 (l / 16) on, of
+// weight row l % 16 and of activation row l % 16. The activations are rounded
+// to codes in these registers (the block's maximum is one over 4 lanes), so
+// there is no other launch.
 // ---------------------------------------------------------------------------
-
-// 32 values of row x from column c on, zero past K.
-template <typename T>
-__device__ __forceinline__ void load32(const T* x, int c, int K, bool vec, float v[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) load8(x, c + 8 * i, K, vec, v + 8 * i);
-}
 
 // Stores one value in the output's type.
 __device__ __forceinline__ void store_as(DType dt, void* out, int64_t at, float v) {
@@ -161,92 +154,309 @@ __device__ __forceinline__ void store_as(DType dt, void* out, int64_t at, float 
   else reinterpret_cast<float*>(out)[at] = v;
 }
 
-template <typename TX, int NW, bool EXACT>
-__global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p, bool vec) {
-  __shared__ float red[NW][16][20];
-  __shared__ int dst[16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c4 = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  // row r of this workgroup: its expert, its source row and its output row
-  int expert = 0, src = -1, to = -1;
-  if (p.g.tile) {
-    if ((int)blockIdx.y >= *p.g.n_tiles) return;
-    const int* t = p.g.tile + 4 * blockIdx.y;
-    expert = t[0];
-    if (r < t[2]) to = p.g.pair[t[1] + r];
-  } else if (p.g.idx) {
-    // up to 64 pairs, one to a lane: the pairs of pair y's expert, of which y
-    // is to be the first of a run of 16
-    const int mine = lane < p.g.pairs ? p.g.idx[lane] : -1;
-    expert = __shfl(mine, (int)blockIdx.y, 64);
-    if (expert < 0 || expert >= p.g.experts) return;
-    uint64_t same = __ballot(mine == expert);
-    const int before = __popcll(same & (((uint64_t)1 << blockIdx.y) - 1));
-    if (before % 16) return;
-    for (int i = 0; i < before + r; ++i) same &= same - 1;
-    if (same) to = __builtin_ctzll(same);
-  } else {
-    const int row = blockIdx.y * 16 + r;
-    if (row < p.M) src = to = row;
+// Adds block b's products of RC x 16 weight rows (16 apart, from wrow; this
+// lane's 32 inputs) and the lane's activation row to acc. VEC: rows of whole
+// 16-byte runs of 8 inputs (the code for others is several times as long, and
+// a launch of a few microseconds pays for fetching it).
+template <typename TX, int RC, bool EXACT, bool VEC>
+__device__ __forceinline__ void few_block(const uint8_t* wrow, int64_t wstep, const uint8_t* wsc, int b, const TX* xrow,
+                                          int K, floatx4 acc[RC]) {
+  const int c0 = b * 128 + 32 * ((threadIdx.x & 63) >> 4);
+  u32x4 wf[RC][2];
+#pragma unroll
+  for (int c = 0; c < RC; ++c)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) wf[c][u] = *reinterpret_cast<const u32x4*>(wrow + c * wstep + b * 128 + 16 * u);
+  const int sw = wsc[b];
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (VEC) {
+      TX t[8] = {};
+      if (c0 + 8 * i < K) {
+#pragma unroll
+        for (int u = 0; u < (int)sizeof(TX) / 2; ++u)
+          reinterpret_cast<u32x4*>(t)[u] = reinterpret_cast<const u32x4*>(xrow + c0 + 8 * i)[u];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[8 * i + e] = (float)t[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[8 * i + e] = c0 + 8 * i + e < K ? (float)xrow[c0 + 8 * i + e] : 0.f;
+    }
   }
-  if ((p.g.tile || p.g.idx) && to >= 0) src = p.rows == Fp8Gemm::kByFrame ? to / p.g.top_k : to;
-  if (threadIdx.x < 16) dst[r] = to;
-
-  const int kb = (p.K + 127) / 128, kbp = (kb + 3) / 4 * 4;
-  const uint8_t* wrow = p.w + expert * p.w_stride + (int64_t)min(n0 + r, p.N - 1) * (kb * 128) + 32 * c4;
-  const uint8_t* wsc = p.ws + expert * p.ws_stride + (int64_t)(n0 / 128) * kbp;
-  const TX* xrow = reinterpret_cast<const TX*>(p.x) + (int64_t)max(src, 0) * p.ldx;
-  const int K = src >= 0 ? p.K : 0;
-  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b = w; b < kb; b += NW) {
-    const u32x4 w0 = *reinterpret_cast<const u32x4*>(wrow + b * 128), w1 = *reinterpret_cast<const u32x4*>(wrow + b * 128 + 16);
-    const int sw = wsc[b];
-    float v[32];
-    load32(xrow, b * 128 + 32 * c4, K, vec, v);
-    float m = 0.f;
+  float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m = fmaxf(m, fp8_mag(v[i]));
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    const int s = fp8_scale_byte(m);
-    const float scale = fp8_scale(s);
-    uint32_t q[8];
+  for (int i = 0; i < 32; ++i) m = fmaxf(m, fp8_mag(v[i]));
+  m = fmaxf(m, __shfl_xor(m, 16, 64));
+  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  const int s = fp8_scale_byte(m);
+  const float scale = fp8_scale(s);
+  i32x8 q;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = fp8_pack4_scaled(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
+  for (int i = 0; i < 8; ++i) q[i] = (int)fp8_pack4_scaled(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
+#pragma unroll
+  for (int c = 0; c < RC; ++c) {
     if constexpr (EXACT) {
       // element group j of every lane's 32: the same inputs of both operands
       floatx4 part = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u32x4 wj = j < 2 ? w0 : w1;
+        const u32x4 wj = wf[c][j >> 1];
         part = mma16(fp8_to_bf16(wj[2 * (j & 1)], wj[2 * (j & 1) + 1]), fp8_to_bf16(q[2 * j], q[2 * j + 1]), part);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += __builtin_ldexpf(part[e], s + sw - 254);
+      for (int e = 0; e < 4; ++e) acc[c][e] += __builtin_ldexpf(part[e], s + sw - 254);
     } else {
-      i32x8 a, x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = (int)w0[i];
-        a[i + 4] = (int)w1[i];
-        x[i] = (int)q[i];
-        x[i + 4] = (int)q[i + 4];
-      }
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, acc, 0, 0, 0, sw, 0, s);
+      const i32x8 a = {(int)wf[c][0][0], (int)wf[c][0][1], (int)wf[c][0][2], (int)wf[c][0][3],
+                       (int)wf[c][1][0], (int)wf[c][1][1], (int)wf[c][1][2], (int)wf[c][1][3]};
+      acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc[c], 0, 0, 0, sw, 0, s);
     }
   }
-  // lane: row l % 16, columns 4 (l / 16) + [0, 4)
-  *reinterpret_cast<floatx4*>(&red[w][r][4 * c4]) = acc;
+}
+
+constexpr int kScanPairs = 1024, kScanExperts = 1024;
+
+// The pairs of the `y`-th of the chosen experts, in order, in list; returns
+// their number and the expert (0 if fewer are chosen). All threads call it.
+struct ExpertPairs {
+  int list[kScanPairs], idx[kScanPairs];
+  uint32_t used[kScanExperts / 32];
+  int expert, count;
+};
+__device__ __forceinline__ void find_pairs(const int* idx, int pairs, int experts, int y, ExpertPairs& f) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x < kScanExperts / 32) f.used[threadIdx.x] = 0;
+  if (threadIdx.x == 0) f.count = 0;
   __syncthreads();
-  if (threadIdx.x >= 256) return;
-  const int row = threadIdx.x >> 4, n = n0 + (threadIdx.x & 15), out = dst[row];
-  if (out < 0 || n >= p.N) return;
-  float v = red[0][row][threadIdx.x & 15];
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    const int e = idx[i];
+    f.idx[i] = e;
+    if (e >= 0 && e < experts) atomicOr(&f.used[e >> 5], 1u << (e & 31));
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  // lane's 16 experts; how many are used before them
+  const uint32_t mine = f.used[lane >> 1] >> (16 * (lane & 1)) & 0xFFFFu;
+  int before = 0;
+  for (int o = 1; o < 64; o *= 2) {
+    const int n = __popc(mine) + before, t = __shfl_up(n, o, 64);
+    before += lane >= o ? t : 0;
+  }
+  const int r = y - before;
+  const uint64_t has = __ballot(r >= 0 && r < __popc(mine));
+  int e = -1, n = 0;
+  if (has) {
+    uint32_t m = mine;
+    for (int i = 0; i < min(r, 16); ++i) m &= m - 1;
+    e = __shfl(16 * lane + __builtin_ctz(m | 0x10000u), __builtin_ctzll(has), 64);
+    for (int i = 0; i < pairs; i += 64) {
+      const bool same = i + lane < pairs && f.idx[i + lane] == e;
+      const uint64_t mask = __ballot(same);
+      if (same) f.list[n + __popcll(mask & (((uint64_t)1 << lane) - 1))] = i + lane;
+      n += __popcll(mask);
+    }
+  }
+  if (lane == 0) {
+    f.expert = e;
+    f.count = n;
+  }
+}
+
+// The place of the n-th set bit of m, which has more than n.
+__device__ __forceinline__ int nth_bit(uint64_t m, int n) {
+  for (int i = 0; i < n; ++i) m &= m - 1;
+  return __builtin_ctzll(m);
+}
+
+template <typename TX, int NW, int RC, bool EXACT, bool VEC>
+__global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
+  __shared__ float red[NW][RC][16][20];
+  __shared__ int dst[16];
+  __shared__ ExpertPairs found;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c4 = lane >> 4;
+  const int n0 = blockIdx.x * 16 * RC;
+  int expert = 0, rows = p.M - blockIdx.y * 16;
+  uint64_t same = 0;  // up to 64 pairs, one to a lane: the expert's
+  const bool lanes = !p.g.tile && p.g.idx && p.g.pairs <= 64;
+  if (lanes) {
+    // the y-th of the distinct experts, found by every wave for itself
+    int mine = lane < p.g.pairs ? p.g.idx[lane] : -1;
+    if (mine >= p.g.experts) mine = -1;
+    uint64_t todo = __ballot(mine >= 0);
+    for (int y = blockIdx.y;; --y) {
+      if (!todo) return;
+      expert = __shfl(mine, __builtin_ctzll(todo), 64);
+      same = __ballot(mine == expert);
+      if (y == 0) break;
+      todo &= ~same;
+    }
+    rows = __popcll(same);
+  } else if (p.g.tile) {
+    if ((int)blockIdx.y >= *p.g.n_tiles) return;
+    expert = p.g.tile[4 * blockIdx.y];
+    rows = p.g.tile[4 * blockIdx.y + 2];
+  } else if (p.g.idx) {
+    find_pairs(p.g.idx, p.g.pairs, p.g.experts, blockIdx.y, found);
+    __syncthreads();
+    if (found.count == 0) return;
+    expert = found.expert;
+    rows = found.count;
+  }
+  const int kb = (p.K + 127) / 128, kbp = (kb + 3) / 4 * 4;
+  const int64_t wstep = (int64_t)16 * (kb * 128);
+  // (weight rows past the last repeat rows before them; their columns are not stored)
+  const uint8_t* wrow = p.w + expert * p.w_stride + (int64_t)min(n0 + r, p.N - 1 - 16 * (RC - 1)) * (kb * 128) + 32 * c4;
+  const uint8_t* wsc = p.ws + expert * p.ws_stride + (int64_t)(n0 / 128) * kbp;
+  for (int first = 0; first < rows; first += 16) {  // (one pass but for an expert of many pairs)
+    // row r: its output row and its source row
+    int to = -1;
+    if (first + r < rows) {
+      if (p.g.tile) to = p.g.pair[p.g.tile[4 * blockIdx.y + 1] + r];
+      else if (lanes) to = nth_bit(same, first + r);
+      else if (p.g.idx) to = found.list[first + r];
+      else to = blockIdx.y * 16 + r;
+    }
+    const int src = p.rows == Fp8Gemm::kByFrame ? to / p.g.top_k : to;
+    if (threadIdx.x < 16) dst[r] = to;
+    const TX* xrow = reinterpret_cast<const TX*>(p.x) + (int64_t)(to >= 0 ? src : 0) * p.ldx;
+    const int K = to >= 0 ? p.K : 0;
+    floatx4 acc[RC];
 #pragma unroll
-  for (int i = 1; i < NW; ++i) v += red[i][row][threadIdx.x & 15];
-  v += p.bias[(int64_t)expert * p.N + n];
-  if (p.epilogue == kFp8HiddenF32) v = silu_value<float>(v);
-  store_as(p.epilogue == kFp8Out ? p.out_dt : kF32, p.out, (int64_t)out * p.ldo + n, v);
+    for (int c = 0; c < RC; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int b = w; b < kb; b += NW) few_block<TX, RC, EXACT, VEC>(wrow, wstep, wsc, b, xrow, K, acc);
+    // lane: row l % 16, columns 16 c + 4 (l / 16) + [0, 4)
+#pragma unroll
+    for (int c = 0; c < RC; ++c) *reinterpret_cast<floatx4*>(&red[w][c][r][4 * c4]) = acc[c];
+    __syncthreads();
+    for (int t = threadIdx.x; t < RC * 256; t += NW * 64) {
+      const int c = t >> 8, row = t >> 4 & 15, e = t & 15, n = n0 + 16 * c + e, out = dst[row];
+      if (out < 0 || n >= p.N) continue;
+      float v = red[0][c][row][e];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) v += red[i][c][row][e];
+      v += p.bias[(int64_t)expert * p.N + n];
+      if (p.epilogue == kFp8HiddenF32) v = silu_value<float>(v);
+      store_as(p.epilogue == kFp8Out ? p.out_dt : kF32, p.out, (int64_t)out * p.ldo + n, v);
+    }
+    if (p.g.tile || !p.g.idx) break;
+    __syncthreads();
+  }
+}
+
+// The second product of up to 16 pairs and their weighted sum in one: a
+// workgroup's 16 waves share out the chosen experts and, for each, the blocks
+// of inputs, and 16 columns of every frame are summed at the end, in the order
+// of the choices. A wave's first weights are on their way while the workgroup
+// rounds the hidden rows to codes in LDS.
+constexpr int kSumLds = 64 * 1024;
+template <typename TOut>
+__global__ __launch_bounds__(1024) void fp8_few_sum_kernel(Fp8Gemm p, const float* weights, const TOut* residual,
+                                                           float res_scale) {
+  __shared__ __attribute__((aligned(16))) uint8_t codes[kSumLds];
+  __shared__ uint8_t scales[kSumLds / 128];
+  __shared__ float red[16][16][20];
+  __shared__ int at[16];  // pair: 16 * its expert's place + its place among the expert's pairs, or -1
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c4 = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int kb = (p.K + 127) / 128, kbp = (kb + 3) / 4 * 4, pitch = kb * 128 + 16;
+  // every wave finds the distinct experts by itself: one pair to a lane
+  int mine = lane < p.g.pairs ? p.g.idx[lane] : -1;
+  if (mine >= p.g.experts) mine = -1;
+  const uint64_t valid = __ballot(mine >= 0);
+  int groups = 0, place = -1;
+  for (uint64_t todo = valid; todo; ++groups) {
+    const uint64_t same = __ballot(mine == __shfl(mine, __builtin_ctzll(todo), 64));
+    if (same >> lane & 1) place = 16 * groups + __popcll(same & (((uint64_t)1 << lane) - 1));
+    todo &= ~same;
+  }
+  if (w == 0 && lane < 16) at[lane] = place;
+  int share = 16;  // waves to an expert
+  while (share * groups > 16) share /= 2;
+  const int g = w / share, b0 = w % share;
+  const int expert = g < groups ? __shfl(mine, __builtin_ctzll(__ballot(place == 16 * g)), 64) : 0;
+  const uint8_t* wrow = p.w + expert * p.w_stride + (int64_t)min(n0 + r, p.N - 1) * (kb * 128) + 32 * c4;
+  const uint8_t* wsc = p.ws + expert * p.ws_stride + (int64_t)(n0 / 128) * kbp;
+  constexpr int D = 4;
+  u32x4 wf[D][2];
+  int sw[D];
+  auto fetch = [&](int b, int d) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) wf[d][u] = *reinterpret_cast<const u32x4*>(wrow + b * 128 + 16 * u);
+    sw[d] = wsc[b];
+  };
+  if (g < groups) {
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (b0 + d * share < kb) fetch(b0 + d * share, d);
+  }
+  // 16 lanes round a block of a pair's hidden row
+  for (int i = threadIdx.x >> 4; i < p.g.pairs * kb; i += 64) {
+    const int pr = i / kb, blk = i % kb, c = blk * 128 + 8 * (lane & 15);
+    float v[8] = {};
+    if (c < p.K) {
+      const float* x = reinterpret_cast<const float*>(p.x) + (int64_t)pr * p.ldx + c;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) *reinterpret_cast<floatx4*>(v + 4 * u) = *reinterpret_cast<const floatx4*>(x + 4 * u);
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_mag(v[e]));
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const int s = fp8_scale_byte(m);
+    const float scale = fp8_scale(s);
+    *reinterpret_cast<u32x2*>(codes + pr * pitch + c) =
+        u32x2{fp8_pack4_scaled(v[0], v[1], v[2], v[3], scale), fp8_pack4_scaled(v[4], v[5], v[6], v[7], scale)};
+    if ((lane & 15) == 0) scales[pr * kb + blk] = (uint8_t)s;
+  }
+  __syncthreads();
+  if (g < groups) {
+    // row r: the expert's r-th pair
+    int to = -1;
+    for (int i = 0; i < p.g.pairs; ++i)
+      if (at[i] == 16 * g + r) to = i;
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](int b, int d) {
+      u32x4 x0 = {}, x1 = {};
+      int s = 127;
+      if (to >= 0) {
+        x0 = *reinterpret_cast<const u32x4*>(codes + to * pitch + b * 128 + 32 * c4);
+        x1 = *reinterpret_cast<const u32x4*>(codes + to * pitch + b * 128 + 32 * c4 + 16);
+        s = scales[to * kb + b];
+      }
+      const i32x8 a = {(int)wf[d][0][0], (int)wf[d][0][1], (int)wf[d][0][2], (int)wf[d][0][3],
+                       (int)wf[d][1][0], (int)wf[d][1][1], (int)wf[d][1][2], (int)wf[d][1][3]};
+      const i32x8 q = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, 0, 0, 0, sw[d], 0, s);
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (b0 + d * share < kb) add(b0 + d * share, d);
+#pragma unroll 1
+    for (int b = b0 + D * share; b < kb; b += share) {
+      fetch(b, 0);
+      add(b, 0);
+    }
+    *reinterpret_cast<floatx4*>(&red[w][r][4 * c4]) = acc;
+  }
+  __syncthreads();
+  const int rows = p.g.pairs / p.g.top_k, row = threadIdx.x >> 4, e = threadIdx.x & 15, n = n0 + e;
+  if (row >= rows || n >= p.N) return;
+  float sum = 0.f;
+  for (int j = 0; j < p.g.top_k; ++j) {
+    const int q = row * p.g.top_k + j, a = at[q];
+    if (a < 0) continue;
+    float v = 0.f;
+    for (int i = 0; i < share; ++i) v += red[(a >> 4) * share + i][a & 15][e];
+    v += p.bias[(int64_t)p.g.idx[q] * p.N + n];
+    sum = __builtin_fmaf(weights[q], v, sum);
+  }
+  sum *= res_scale;
+  const int64_t o = (int64_t)row * p.N + n;
+  if (residual) sum += (float)residual[o];
+  reinterpret_cast<TOut*>(p.out)[o] = (TOut)sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -848,27 +1058,52 @@ bool fp8_few_rows(int64_t M, int N, int K) {
   (void)K;
   return M <= 64;
 }
+int fp8_scan_pairs() { return kScanPairs; }
 
 hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
   if (bad_gemm(p) || !p.x) return hipErrorInvalidValue;
-  const int64_t groups = p.g.tile ? p.g.max_tiles : p.g.idx ? p.g.pairs : (p.M + 15) / 16;
-  if (groups <= 0 || groups > 65535 || (p.g.idx && p.g.pairs > 64) || (p.g.tile && p.g.tile_rows != 16)) return hipErrorInvalidValue;
-  const dim3 grid((p.N + 15) / 16, (unsigned)groups);
+  if (p.g.idx && !p.g.tile && (p.g.pairs > kScanPairs || p.g.experts > kScanExperts)) return hipErrorInvalidValue;
+  if (p.g.tile && p.g.tile_rows != 16) return hipErrorInvalidValue;
+  const int64_t groups = p.g.tile ? p.g.max_tiles : p.g.idx ? std::min(p.g.pairs, p.g.experts) : (p.M + 15) / 16;
+  if (groups <= 0 || groups > 65535) return hipErrorInvalidValue;
   const int es = dtype_size(p.x_dt);
-  const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * es % 16 == 0;
+  const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * es % 16 == 0 && p.K % 8 == 0;
   const bool exact = p.epilogue == kFp8Out && p.out_dt == kF32;
-  auto go = [&](auto tx, auto nw) {
+  auto go = [&](auto tx, auto nw, auto rc) {
     using TX = decltype(tx);
-    constexpr int NW = decltype(nw)::value;
-    if (exact) fp8_few_kernel<TX, NW, true><<<grid, NW * 64, 0, s>>>(p, vec);
-    else fp8_few_kernel<TX, NW, false><<<grid, NW * 64, 0, s>>>(p, vec);
+    constexpr int NW = decltype(nw)::value, RC = decltype(rc)::value;
+    const dim3 grid((p.N + 16 * RC - 1) / (16 * RC), (unsigned)groups);
+    if (exact && vec) fp8_few_kernel<TX, NW, RC, true, true><<<grid, NW * 64, 0, s>>>(p);
+    else if (exact) fp8_few_kernel<TX, NW, RC, true, false><<<grid, NW * 64, 0, s>>>(p);
+    else if (vec) fp8_few_kernel<TX, NW, RC, false, true><<<grid, NW * 64, 0, s>>>(p);
+    else fp8_few_kernel<TX, NW, RC, false, false><<<grid, NW * 64, 0, s>>>(p);
   };
-  auto by_type = [&](auto nw) {
-    if (p.x_dt == kBF16) go(bf16{}, nw);
-    else go(float{}, nw);
+  auto by_type = [&](auto nw, auto rc) {
+    if (p.x_dt == kBF16) go(bf16{}, nw, rc);
+    else go(float{}, nw, rc);
   };
-  if (p.K > 2048) by_type(std::integral_constant<int, 16>{});
-  else by_type(std::integral_constant<int, 8>{});
+  using std::integral_constant;
+  // 64 columns where that leaves a workgroup to a CU: the rows are rounded
+  // once for all of them, and a wave has four times the loads in flight
+  const bool wide = p.N % 64 == 0 && p.N / 64 * groups >= device_cus();
+  if (wide && p.K <= 1024) by_type(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  else if (wide) by_type(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  else if (p.K > 2048) by_type(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else by_type(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  return hipGetLastError();
+}
+
+bool fp8_few_sum_ok(int64_t pairs, int K) { return pairs <= 16 && pairs * (fp8_kp(K) + 16) <= kSumLds; }
+
+hipError_t fp8_gemm_few_sum(const Fp8Gemm& p, const float* weights, const void* residual, float res_scale, hipStream_t s) {
+  if (bad_gemm(p) || !p.x || p.x_dt != kF32 || p.ldx % 4 || p.K % 8 || (reinterpret_cast<uintptr_t>(p.x) & 15) || !p.g.idx ||
+      p.g.pairs <= 0 || !fp8_few_sum_ok(p.g.pairs, p.K) || p.g.top_k <= 0 || p.g.pairs % p.g.top_k || p.ldo != p.N)
+    return hipErrorInvalidValue;
+  const unsigned grid = (p.N + 15) / 16;
+  if (p.out_dt == kBF16)
+    fp8_few_sum_kernel<bf16><<<grid, 1024, 0, s>>>(p, weights, static_cast<const bf16*>(residual), res_scale);
+  else
+    fp8_few_sum_kernel<float><<<grid, 1024, 0, s>>>(p, weights, static_cast<const float*>(residual), res_scale);
   return hipGetLastError();
 }
 

@@ -58,7 +58,8 @@ struct Fp8Groups {
   const int* pair = nullptr;
   const int* frame = nullptr;  // pair / top_k
   int top_k = 1;
-  // few pairs: no tile list; workgroup column y looks at pair y of idx
+  // up to fp8_scan_pairs() pairs: no tile list; workgroup column y looks for
+  // the y-th of the experts that idx names
   const int* idx = nullptr;
   int pairs = 0, experts = 0;
 };
@@ -99,6 +100,12 @@ struct Fp8Gemm {
 // Whether the few-row kernel (activations rounded inside it) takes M rows.
 bool fp8_few_rows(int64_t M, int N, int K);
 hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s);
+int fp8_scan_pairs();
+// The second product over few pairs (fp8_few_sum_ok) with the weighted sum:
+// out [pairs / top_k, N] in out_dt = residual (or null, or out) + res_scale *
+// sum_j weights_j (acc + bias); x [pairs, K] f32, by pair.
+bool fp8_few_sum_ok(int64_t pairs, int K);
+hipError_t fp8_gemm_few_sum(const Fp8Gemm& p, const float* weights, const void* residual, float res_scale, hipStream_t s);
 // Tile kernel on codes; a dense product with f32 out sums on the bf16 matrix
 // cores (exact products), every other on the fp8 ones.
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s);

@@ -566,24 +566,38 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
-class _OnDevice:
-    """The GPU of `x` made current for a call, and torch's stream on it."""
+# Calls on single frames take a few microseconds on the GPU, so their checks
+# and look-ups here are kept short: one table of dtypes, torch's own accessors
+# for the current GPU and stream.
+_ACT_CODES: dict = {}
 
-    def __init__(self, x):
-        self._x = x
 
-    def __enter__(self):
+def _act_code(dtype) -> int:
+    """MHSA_F32 or MHSA_BF16 of a torch dtype."""
+    if not _ACT_CODES:
         import torch
-        self._before = torch.cuda.current_device()
-        dev = self._x.get_device()
-        if dev != self._before:
-            torch.cuda.set_device(dev)
-        return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+        _ACT_CODES.update({torch.float32: F32, torch.bfloat16: BF16})
+    code = _ACT_CODES.get(dtype)
+    return _dtype_code(dtype) if code is None else code
 
-    def __exit__(self, *exc):
-        import torch
-        if self._x.get_device() != self._before:
-            torch.cuda.set_device(self._before)
+
+def _U8():
+    import torch
+    return torch.uint8
+
+
+def _launch(x, fn, *args) -> None:
+    """fn(*args, stream) on x's GPU and torch's current stream on it."""
+    import torch
+    dev = x.get_device()
+    before = torch._C._cuda_getDevice()
+    if dev == before:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != MHSA_OK:
+        _check(rc)
 
 
 def _rows_of(x, width: int):
@@ -592,9 +606,9 @@ def _rows_of(x, width: int):
     import torch
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1 or x.shape[-1] != width:
         raise MhsaError(MHSA_EINVAL, f"expected a GPU tensor [..., {width}]")
-    rows = x.numel() // width
     if x.is_contiguous():
-        return rows, width
+        return x.numel() // width, width
+    rows = x.numel() // width
     lead = [(n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
     if rows and (x.stride(-1) == 1 or width == 1):
         if not lead:
@@ -646,23 +660,20 @@ class Fp8Linear:
     def forward(self, x, out_dtype=None, out=None):
         """x [..., in] float32 or bfloat16, rows evenly spaced; the result in
         out_dtype (x's by default), or in `out` [..., out]."""
-        import torch
         rows, ldx = _rows_of(x, self.in_dim)
-        xd = _dtype_code(x.dtype)
+        xd = _act_code(x.dtype)
         if out is None:
-            out = torch.empty((*x.shape[:-1], self.out_dim), device=x.device,
+            out = x.new_empty((*x.shape[:-1], self.out_dim),
                               dtype=x.dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
             ldo = self.out_dim
         else:
             n, ldo = _rows_of(out, self.out_dim)
             if n != rows or out.device != x.device or (out_dtype is not None and _dtype_code(out_dtype) != _dtype_code(out.dtype)):
                 raise MhsaError(MHSA_EINVAL, f"out: expected {rows} rows on {x.device}")
-        with _OnDevice(x) as stream:
-            need = self._lib.mhsa_fp8_linear_workspace(self._h, rows)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
-            _check(self._lib.mhsa_fp8_linear_forward(self._h, x.data_ptr(), xd, rows, ldx, out.data_ptr(),
-                                                     _dtype_code(out.dtype), ldo, ws.data_ptr() if need > 0 else None,
-                                                     max(need, 0), stream))
+        need = self._lib.mhsa_fp8_linear_workspace(self._h, rows)
+        ws = x.new_empty(need, dtype=_U8()) if need > 0 else None
+        _launch(x, self._lib.mhsa_fp8_linear_forward, self._h, x.data_ptr(), xd, rows, ldx, out.data_ptr(),
+                _act_code(out.dtype), ldo, ws.data_ptr() if need > 0 else None, need)
         return out
 
 
@@ -685,12 +696,11 @@ def route(logits, top_k: int, score: str = "softmax", bias=None, n_groups: int =
                              or not bias.is_contiguous()):
         raise MhsaError(MHSA_EINVAL, f"bias: expected a contiguous float32 tensor [{n}] on {logits.device}")
     shape = (*logits.shape[:-1], top_k if top_k > 0 else 0)
-    idx = torch.empty(shape, dtype=torch.int32, device=logits.device)
-    w = torch.empty(shape, dtype=torch.float32, device=logits.device)
-    with _OnDevice(logits) as stream:
-        _check(library().mhsa_route(logits.data_ptr(), _dtype_code(logits.dtype), rows, n, ld, ROUTE_SCORES[score],
-                                    None if bias is None else bias.data_ptr(), n_groups, topk_groups, top_k,
-                                    1 if renormalize else 0, float(scale), idx.data_ptr(), w.data_ptr(), stream))
+    idx = logits.new_empty(shape, dtype=torch.int32)
+    w = logits.new_empty(shape, dtype=torch.float32)
+    _launch(logits, library().mhsa_route, logits.data_ptr(), _act_code(logits.dtype), rows, n, ld, ROUTE_SCORES[score],
+            None if bias is None else bias.data_ptr(), n_groups, topk_groups, top_k, 1 if renormalize else 0, scale,
+            idx.data_ptr(), w.data_ptr())
     return idx, w
 
 
@@ -737,24 +747,25 @@ class ExpertFeedForward:
         import torch
         if not isinstance(x, torch.Tensor) or not x.is_cuda or not x.is_contiguous() or x.dim() < 1 or x.shape[-1] != self.d_model:
             raise MhsaError(MHSA_EINVAL, f"expected a contiguous GPU tensor [..., {self.d_model}]")
-        dtype = _dtype_code(x.dtype)
+        dtype = _act_code(x.dtype)
         top_k = indices.shape[-1] if indices.dim() else 0
+        lead = x.shape[:-1]
         for t, want, name in ((indices, torch.int32, "indices"), (weights, torch.float32, "weights")):
-            if t.dtype != want or t.device != x.device or not t.is_contiguous() or t.shape != (*x.shape[:-1], top_k):
+            if (t.dtype != want or t.get_device() != x.get_device() or not t.is_contiguous() or t.shape[:-1] != lead
+                    or t.shape[-1] != top_k):
                 raise MhsaError(MHSA_EINVAL, f"{name}: expected contiguous {want} [..., top_k] beside x")
         for t in (residual, out):
-            if t is not None and (t.dtype != x.dtype or t.device != x.device or t.shape != x.shape or not t.is_contiguous()):
+            if t is not None and (t.dtype != x.dtype or t.get_device() != x.get_device() or t.shape != x.shape
+                                  or not t.is_contiguous()):
                 raise MhsaError(MHSA_EINVAL, "residual and out are to be like x")
         if out is None:
             out = torch.empty_like(x)
         rows = x.numel() // self.d_model
-        with _OnDevice(x) as stream:
-            need = self._lib.mhsa_experts_workspace(self._h, rows, top_k)
-            ws = torch.empty(max(need, 0), dtype=torch.uint8, device=x.device)
-            _check(self._lib.mhsa_experts_forward(self._h, x.data_ptr(), dtype, rows, indices.data_ptr(),
-                                                  weights.data_ptr(), top_k,
-                                                  None if residual is None else residual.data_ptr(), float(res_scale),
-                                                  out.data_ptr(), ws.data_ptr(), max(need, 0), stream))
+        need = self._lib.mhsa_experts_workspace(self._h, rows, top_k)
+        ws = x.new_empty(max(need, 0), dtype=torch.uint8)
+        _launch(x, self._lib.mhsa_experts_forward, self._h, x.data_ptr(), dtype, rows, indices.data_ptr(), weights.data_ptr(),
+                top_k, None if residual is None else residual.data_ptr(), res_scale, out.data_ptr(), ws.data_ptr(),
+                max(need, 0))
         return out
 
 
