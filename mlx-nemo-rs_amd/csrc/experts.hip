@@ -2,6 +2,7 @@
 // products (fp8_gemm.hip): pairs of frame and expert sorted by expert, and
 // the weighted sum of a frame's experts.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_common.hpp"
 #include "fp8_kernels.hpp"
@@ -17,52 +18,97 @@ namespace {
 // differ by less than f32 resolves, and the choice between them is then not a
 // matter of the order of a sum.
 //
-// One wave per row, expert e in lane e % 64.
+// One wave per row, expert e in lane e % 64. What is bound here is not the
+// logits' bytes but the wave's reductions, so they are DPP moves and lane
+// reads, which the vector unit does itself, and a choice reduces one 32-bit
+// word: a score's f32 rounding, which keeps the order. Only lanes that share
+// the largest word are compared in 64 bits. (With shuffles of 64-bit values,
+// which go through LDS, 30001 rows of 256 experts in 8 groups took 88 us.)
 // ---------------------------------------------------------------------------
 
 constexpr double kNone = -__builtin_inf();
 
-__device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor(v, o, 64); }
-
-// the better of two candidates in (v, i): larger value, then lower index
-__device__ __forceinline__ void better(double& v, int& i, double v2, int i2) {
-  if (v2 > v || (v2 == v && i2 < i)) {
-    v = v2;
-    i = i2;
-  }
+// The value of lane 63 after o(o(...)) over the wave's rows of 16 lanes, then
+// over the rows: `o` combines a lane's value with a neighbour's; lanes without
+// a neighbour keep theirs.
+template <typename T, typename O>
+__device__ __forceinline__ T wave_reduce(T v, O o) {
+  auto move = [](T x, auto ctrl, auto rows) {
+    constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+    if constexpr (sizeof(T) == 4) {
+      const int u = __builtin_bit_cast(int, x);
+      return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(u, u, C, R, 0xF, false));
+    } else {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      i32x2 u = __builtin_bit_cast(i32x2, x);
+      u[0] = __builtin_amdgcn_update_dpp(u[0], u[0], C, R, 0xF, false);
+      u[1] = __builtin_amdgcn_update_dpp(u[1], u[1], C, R, 0xF, false);
+      return __builtin_bit_cast(T, u);
+    }
+  };
+  using std::integral_constant;
+  constexpr auto all = integral_constant<int, 0xF>{};
+  // lanes xor 1, xor 2 (quad permutations), then half rows and rows mirrored:
+  // every lane of a row of 16 has the row's result
+  v = o(v, move(v, integral_constant<int, 0xB1>{}, all));
+  v = o(v, move(v, integral_constant<int, 0x4E>{}, all));
+  v = o(v, move(v, integral_constant<int, 0x141>{}, all));
+  v = o(v, move(v, integral_constant<int, 0x140>{}, all));
+  // four rows: one lane of each
+  auto at = [&](int l) {
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+    } else {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      const i32x2 u = __builtin_bit_cast(i32x2, v);
+      return __builtin_bit_cast(T, i32x2{__builtin_amdgcn_readlane(u[0], l), __builtin_amdgcn_readlane(u[1], l)});
+    }
+  };
+  return o(o(at(0), at(16)), o(at(32), at(48)));
+}
+__device__ __forceinline__ double lane_of(double v, int l) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  const i32x2 u = __builtin_bit_cast(i32x2, v);
+  return __builtin_bit_cast(double, i32x2{__builtin_amdgcn_readlane(u[0], l), __builtin_amdgcn_readlane(u[1], l)});
+}
+// The order of values as unsigned words, 0 for none (-inf itself is 0x7FFFFF,
+// and no value's word is 0).
+__device__ __forceinline__ uint32_t rank_word(double v) {
+  if (!(v > kNone)) return 0;
+  const uint32_t u = __builtin_bit_cast(uint32_t, (float)v);
+  return u >> 31 ? ~u : u | 0x80000000u;
 }
 
 template <typename T, int EPL>
 __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   __shared__ double tab[4][EPL * 64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = (int64_t)blockIdx.x * 4 + wv;
-  const bool live = row < p.rows;
-  const T* x = reinterpret_cast<const T*>(p.logits) + (live ? row : 0) * p.ld;
+  if (row >= p.rows) return;  // (waves do not wait for each other)
+  const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
   double s[EPL], c[EPL];
-  double mx = kNone;
+  float v[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const int e = lane + 64 * i;
-    const double v = e < p.experts ? (double)(float)x[e] : kNone;
-    c[i] = v > kNone ? v : kNone;  // (a NaN is no score)
-    mx = c[i] > mx ? c[i] : mx;
+    const float t = e < p.experts ? (float)x[e] : -__builtin_inff();
+    v[i] = t > -__builtin_inff() ? t : -__builtin_inff();  // (a NaN is no score)
   }
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) s[i] = c[i] > kNone ? 1.0 / (1.0 + exp(-c[i])) : 0.0;
+    for (int i = 0; i < EPL; ++i) s[i] = v[i] > -__builtin_inff() ? 1.0 / (1.0 + exp(-(double)v[i])) : 0.0;
   } else {
-    for (int o = 32; o > 0; o >>= 1) {
-      const double t = shfl_xor_d(mx, o);
-      mx = t > mx ? t : mx;
-    }
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, v[i]);
+    mx = wave_reduce(mx, [](float a, float b) { return fmaxf(a, b); });
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      s[i] = c[i] > kNone ? (c[i] == mx ? 1.0 : exp(c[i] - mx)) : 0.0;
+      s[i] = v[i] > -__builtin_inff() ? (v[i] == mx ? 1.0 : exp((double)v[i] - (double)mx)) : 0.0;
       sum += s[i];
     }
-    for (int o = 32; o > 0; o >>= 1) sum += shfl_xor_d(sum, o);
+    sum = wave_reduce(sum, [](double a, double b) { return a + b; });
     if (sum > 0.0) {
 #pragma unroll
       for (int i = 0; i < EPL; ++i) s[i] /= sum;
@@ -71,32 +117,29 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const int e = lane + 64 * i;
-    const double v = p.bias && e < p.experts ? s[i] + (double)p.bias[e] : s[i];
-    c[i] = c[i] > kNone && v > kNone ? v : kNone;
+    const double t = p.bias && e < p.experts ? s[i] + (double)p.bias[e] : s[i];
+    c[i] = v[i] > -__builtin_inff() && t > kNone ? t : kNone;
   }
   if (p.groups > 1) {
     const int size = p.experts / p.groups;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) tab[wv][lane + 64 * i] = c[i];
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
     double best = kNone;
     if (lane < p.groups) {
       double a = kNone, b = kNone;  // the two largest
+      const double* t = tab[wv] + lane * size;
       for (int e = 0; e < size; ++e) {
-        const double v = tab[wv][lane * size + e];
-        if (v > a) {
-          b = a;
-          a = v;
-        } else if (v > b) {
-          b = v;
-        }
+        const double u = t[e];
+        b = u > a ? a : (u > b ? u : b);
+        a = u > a ? u : a;
       }
       best = b > kNone ? a + b : a;
     }
     int before = 0;  // groups ahead of this lane's
     for (int g = 0; g < p.groups; ++g) {
-      const double v = __shfl(best, g, 64);
-      before += v > best || (v == best && g < lane) ? 1 : 0;
+      const double u = lane_of(best, g);
+      before += u > best || (u == best && g < lane) ? 1 : 0;
     }
     const uint64_t kept = __ballot(lane < p.groups && before < p.topk_groups);
 #pragma unroll
@@ -108,29 +151,47 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   int idx = -1;
   double wj = 0.0, total = 0.0;
   for (int j = 0; j < p.top_k; ++j) {
-    double v = kNone;
-    int at = 1 << 30;
+    // the lane's best (the lower index of equals), then the wave's
+    double top = c[0];
+    int at = 0;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (c[i] > kNone) better(v, at, c[i], lane + 64 * i);
-    for (int o = 32; o > 0; o >>= 1) better(v, at, shfl_xor_d(v, o), __shfl_xor(at, o, 64));
-    if (!(v > kNone)) break;
+    for (int i = 1; i < EPL; ++i) {
+      at = c[i] > top ? i : at;
+      top = c[i] > top ? c[i] : top;
+    }
+    const uint32_t word = rank_word(top);
+    const uint32_t most = wave_reduce(word, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    if (most == 0) break;
+    uint64_t same = __ballot(word == most);
+    int win = __builtin_ctzll(same);
+    if (same & (same - 1)) {  // several f32 equals: the larger in 64 bits, of equals the lower index
+      const int e = lane + 64 * at;
+      double u = lane_of(top, win);
+      int ue = __builtin_amdgcn_readlane(e, win);
+      for (same &= same - 1; same; same &= same - 1) {
+        const int l = __builtin_ctzll(same), le = __builtin_amdgcn_readlane(e, l);
+        const double t = lane_of(top, l);
+        if (t > u || (t == u && le < ue)) {
+          u = t;
+          ue = le;
+          win = l;
+        }
+      }
+    }
     double mine = 0.0;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (lane + 64 * i == at) {
-        mine = s[i];
-        c[i] = kNone;
-      }
-    const double sj = __shfl(mine, at & 63, 64);
-    total += sj;
-    if (lane == j) {
-      idx = at;
-      wj = sj;
+    for (int i = 0; i < EPL; ++i) {
+      mine = i == at ? s[i] : mine;
+      c[i] = lane == win && i == at ? kNone : c[i];
     }
+    const double sj = lane_of(mine, win);
+    const int won = win + 64 * __builtin_amdgcn_readlane(at, win);  // (with all lanes there)
+    total += sj;
+    idx = lane == j ? won : idx;
+    wj = lane == j ? sj : wj;
   }
   if (p.renormalize) wj = total > 0.0 ? wj / total : 0.0;
-  if (live && lane < p.top_k) {
+  if (lane < p.top_k) {
     p.idx[row * p.top_k + lane] = idx;
     p.w[row * p.top_k + lane] = (float)(wj * (double)p.scale);
   }
