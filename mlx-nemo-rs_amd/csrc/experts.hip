@@ -120,77 +120,89 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
     const double t = p.bias && e < p.experts ? s[i] + (double)p.bias[e] : s[i];
     c[i] = v[i] > -__builtin_inff() && t > kNone ? t : kNone;
   }
+  double* t = tab[wv];
   if (p.groups > 1) {
+    // 64 / groups lanes (down to a power of two) to a group find its two best
     const int size = p.experts / p.groups;
+    int lanes = 64;
+    while (lanes * p.groups > 64) lanes /= 2;
+    const int g = lane / lanes;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) tab[wv][lane + 64 * i] = c[i];
+    for (int i = 0; i < EPL; ++i) t[lane + 64 * i] = c[i];
     __builtin_amdgcn_wave_barrier();
-    double best = kNone;
-    if (lane < p.groups) {
-      double a = kNone, b = kNone;  // the two largest
-      const double* t = tab[wv] + lane * size;
-      for (int e = 0; e < size; ++e) {
-        const double u = t[e];
-        b = u > a ? a : (u > b ? u : b);
-        a = u > a ? u : a;
+    double a = kNone, b = kNone;
+    if (g < p.groups)
+      for (int e = lane % lanes; e < size; e += lanes) {
+        const double u = t[g * size + e];
+        b = fmax(b, fmin(a, u));
+        a = fmax(a, u);
       }
-      best = b > kNone ? a + b : a;
+    for (int o = 1; o < lanes; o *= 2) {
+      const double a2 = __shfl_xor(a, o, 64), b2 = __shfl_xor(b, o, 64);
+      b = fmax(fmin(a, a2), fmax(b, b2));
+      a = fmax(a, a2);
     }
+    const double best = b > kNone ? a + b : a;
     int before = 0;  // groups ahead of this lane's
-    for (int g = 0; g < p.groups; ++g) {
-      const double u = lane_of(best, g);
-      before += u > best || (u == best && g < lane) ? 1 : 0;
+    for (int o = 0; o < p.groups; ++o) {
+      const double u = lane_of(best, o * lanes);
+      before += u > best || (u == best && o < g) ? 1 : 0;
     }
-    const uint64_t kept = __ballot(lane < p.groups && before < p.topk_groups);
+    const uint64_t kept = __ballot(g < p.groups && before < p.topk_groups);
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int g = (lane + 64 * i) / size;
-      if (g >= p.groups || !(kept >> g & 1)) c[i] = kNone;
+      const int e = lane + 64 * i;
+      if (e >= p.experts || !(kept >> (e / size * lanes) & 1)) c[i] = kNone;
     }
+    __builtin_amdgcn_wave_barrier();
   }
+  // the scores, for the lanes that will have chosen them
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) t[lane + 64 * i] = s[i];
+  uint32_t word[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) word[i] = rank_word(c[i]);
   int idx = -1;
-  double wj = 0.0, total = 0.0;
   for (int j = 0; j < p.top_k; ++j) {
-    // the lane's best (the lower index of equals), then the wave's
-    double top = c[0];
-    int at = 0;
+    uint32_t most = word[0];
 #pragma unroll
-    for (int i = 1; i < EPL; ++i) {
-      at = c[i] > top ? i : at;
-      top = c[i] > top ? c[i] : top;
-    }
-    const uint32_t word = rank_word(top);
-    const uint32_t most = wave_reduce(word, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    for (int i = 1; i < EPL; ++i) most = max(most, word[i]);
+    most = wave_reduce(most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
     if (most == 0) break;
-    uint64_t same = __ballot(word == most);
-    int win = __builtin_ctzll(same);
-    if (same & (same - 1)) {  // several f32 equals: the larger in 64 bits, of equals the lower index
-      const int e = lane + 64 * at;
-      double u = lane_of(top, win);
-      int ue = __builtin_amdgcn_readlane(e, win);
-      for (same &= same - 1; same; same &= same - 1) {
-        const int l = __builtin_ctzll(same), le = __builtin_amdgcn_readlane(e, l);
-        const double t = lane_of(top, l);
-        if (t > u || (t == u && le < ue)) {
-          u = t;
-          ue = le;
-          win = l;
-        }
-      }
-    }
-    double mine = 0.0;
+    // who has it: one, or several that are alike in f32, of which the larger in
+    // 64 bits, and of equals the lower index
+    int won = -1;
+    double u = kNone;
+    bool alike = false;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      mine = i == at ? s[i] : mine;
-      c[i] = lane == win && i == at ? kNone : c[i];
+      const uint64_t has = __ballot(word[i] == most);
+      alike = alike || (has && (won >= 0 || (has & (has - 1))));
+      if (has && won < 0) won = 64 * i + __builtin_ctzll(has);
     }
-    const double sj = lane_of(mine, win);
-    const int won = win + 64 * __builtin_amdgcn_readlane(at, win);  // (with all lanes there)
-    total += sj;
+    if (alike) {
+      won = -1;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        for (uint64_t has = __ballot(word[i] == most); has; has &= has - 1) {  // (ascending indices)
+          const int l = __builtin_ctzll(has);
+          const double v = lane_of(c[i], l);
+          if (won < 0 || v > u) {
+            u = v;
+            won = 64 * i + l;
+          }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) word[i] = lane + 64 * i == won ? 0 : word[i];
     idx = lane == j ? won : idx;
-    wj = lane == j ? sj : wj;
   }
-  if (p.renormalize) wj = total > 0.0 ? wj / total : 0.0;
+  __builtin_amdgcn_wave_barrier();
+  double wj = idx >= 0 ? t[idx] : 0.0;
+  if (p.renormalize) {
+    const double total = wave_reduce(wj, [](double a, double b) { return a + b; });
+    wj = total > 0.0 ? wj / total : 0.0;
+  }
   if (lane < p.top_k) {
     p.idx[row * p.top_k + lane] = idx;
     p.w[row * p.top_k + lane] = (float)(wj * (double)p.scale);
