@@ -71,6 +71,14 @@ __device__ __forceinline__ double lane_of(double v, int l) {
   const i32x2 u = __builtin_bit_cast(i32x2, v);
   return __builtin_bit_cast(double, i32x2{__builtin_amdgcn_readlane(u[0], l), __builtin_amdgcn_readlane(u[1], l)});
 }
+// 1 / d for d >= 1 to within 2 ulp, 0 for infinity: the hardware's estimate
+// and two Newton steps.
+__device__ __forceinline__ double inverse(double d) {
+  double r = __builtin_amdgcn_rcp(d);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  return d < __builtin_inf() ? r : 0.0;
+}
 // The order of values as unsigned words, 0 for none (-inf itself is 0x7FFFFF,
 // and no value's word is 0).
 __device__ __forceinline__ uint32_t rank_word(double v) {
@@ -96,23 +104,24 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   }
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) s[i] = v[i] > -__builtin_inff() ? 1.0 / (1.0 + exp(-(double)v[i])) : 0.0;
+    for (int i = 0; i < EPL; ++i) s[i] = inverse(1.0 + exp(-(double)v[i]));  // (-inf: e^inf gives 0)
   } else {
     float mx = v[0];
 #pragma unroll
     for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, v[i]);
     mx = wave_reduce(mx, [](float a, float b) { return fmaxf(a, b); });
+    const double top = mx > -__builtin_inff() ? (double)mx : 0.0;
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      s[i] = v[i] > -__builtin_inff() ? (v[i] == mx ? 1.0 : exp((double)v[i] - (double)mx)) : 0.0;
+      const double e = exp((double)v[i] - top);  // (0 for -inf)
+      s[i] = (double)v[i] == top ? 1.0 : e;      // (of infinities too)
       sum += s[i];
     }
     sum = wave_reduce(sum, [](double a, double b) { return a + b; });
-    if (sum > 0.0) {
+    const double inv = sum > 0.0 ? inverse(sum) : 0.0;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) s[i] /= sum;
-    }
+    for (int i = 0; i < EPL; ++i) s[i] *= inv;
   }
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
@@ -124,15 +133,16 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   if (p.groups > 1) {
     // 64 / groups lanes (down to a power of two) to a group find its two best
     const int size = p.experts / p.groups;
-    int lanes = 64;
-    while (lanes * p.groups > 64) lanes /= 2;
-    const int g = lane / lanes;
+    int shift = 6;
+    while (p.groups << shift > 64) --shift;
+    const int lanes = 1 << shift, g = lane >> shift;
+    const float per = 1.f / (float)size;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) t[lane + 64 * i] = c[i];
     __builtin_amdgcn_wave_barrier();
     double a = kNone, b = kNone;
     if (g < p.groups)
-      for (int e = lane % lanes; e < size; e += lanes) {
+      for (int e = lane & (lanes - 1); e < size; e += lanes) {
         const double u = t[g * size + e];
         b = fmax(b, fmin(a, u));
         a = fmax(a, u);
@@ -145,14 +155,15 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
     const double best = b > kNone ? a + b : a;
     int before = 0;  // groups ahead of this lane's
     for (int o = 0; o < p.groups; ++o) {
-      const double u = lane_of(best, o * lanes);
+      const double u = lane_of(best, o << shift);
       before += u > best || (u == best && o < g) ? 1 : 0;
     }
     const uint64_t kept = __ballot(g < p.groups && before < p.topk_groups);
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 64 * i;
-      if (e >= p.experts || !(kept >> (e / size * lanes) & 1)) c[i] = kNone;
+      // (e + 0.5) / size is at least 0.5 / 512 away from a whole number
+      const int e = lane + 64 * i, of = (int)(((float)e + 0.5f) * per);
+      c[i] = e < p.experts && (kept >> (of << shift & 63) & 1) ? c[i] : kNone;
     }
     __builtin_amdgcn_wave_barrier();
   }
