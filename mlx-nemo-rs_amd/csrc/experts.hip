@@ -224,88 +224,116 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
 // Pairs by expert
 // ---------------------------------------------------------------------------
 
-constexpr int kPlanThreads = 1024, kPlanPer = 16, kPlanChunk = kPlanThreads * kPlanPer;
+constexpr int kPlanThreads = 1024, kPlanPer = 8, kPlanChunk = kPlanThreads * kPlanPer;
 constexpr int kPlanExperts = 1024;
 
-// Counts of one chunk of pairs per expert.
-__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const int* idx, int pairs, int experts, int* hist) {
+struct PlanParams {
+  const int* idx = nullptr;
+  int pairs = 0, top_k = 1, experts = 0, tile_rows = 0, chunks = 0;
+  int* hist = nullptr;  // [chunks, experts], with more than one chunk
+  int *pair = nullptr, *frame = nullptr, *tile = nullptr, *n_tiles = nullptr;
+};
+
+// Counts of chunk `chunk` of the pairs per expert.
+__device__ __forceinline__ void plan_count(const PlanParams& p, int chunk) {
   __shared__ int cnt[kPlanExperts];
   cnt[threadIdx.x] = 0;
   __syncthreads();
   for (int i = 0; i < kPlanPer; ++i) {
-    const int p = blockIdx.x * kPlanChunk + i * kPlanThreads + threadIdx.x;
-    const int e = p < pairs ? idx[p] : -1;
-    if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
+    const int q = chunk * kPlanChunk + i * kPlanThreads + threadIdx.x;
+    const int e = q < p.pairs ? p.idx[q] : -1;
+    if (e >= 0 && e < p.experts) atomicAdd(&cnt[e], 1);
   }
   __syncthreads();
-  if ((int)threadIdx.x < experts) hist[blockIdx.x * experts + threadIdx.x] = cnt[threadIdx.x];
+  if ((int)threadIdx.x < p.experts) p.hist[chunk * p.experts + threadIdx.x] = cnt[threadIdx.x];
 }
 
-// Slots of one chunk's pairs (hist null: there is one chunk, counted here) and
-// the tile list. The order of an expert's pairs among its slots is that of
-// the atomics and may change from call to call: no result depends on it, as a
-// slot's row is computed from that row alone.
-__global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(const int* idx, int pairs, int top_k,
-                                                                    int experts, int tile_rows, const int* hist,
-                                                                    int* pair, int* frame, int* tile, int* n_tiles) {
-  __shared__ int cursor[kPlanExperts], slots[2][kPlanExperts], tiles[2][kPlanExperts];
-  const int t = threadIdx.x;
-  int mine[kPlanPer];
+// Slots of chunk `chunk`'s pairs (ONE: there is no other, and they are counted
+// here) and, by chunk 0, the tile list. The order of an expert's pairs among
+// its slots is that of the atomics and may change from call to call: no result
+// depends on it, as a slot's row is computed from that row alone.
+template <bool ONE>
+__device__ __forceinline__ void plan_scatter(const PlanParams& p, int chunk) {
+  __shared__ int cursor[kPlanExperts], part[2][16];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  int mine[kPlanPer], rank[kPlanPer];
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i) {
-    const int p = blockIdx.x * kPlanChunk + i * kPlanThreads + t;
-    mine[i] = p < pairs ? idx[p] : -1;
-    if (mine[i] >= experts) mine[i] = -1;
+    const int q = chunk * kPlanChunk + i * kPlanThreads + t;
+    mine[i] = q < p.pairs ? p.idx[q] : -1;
+    if (mine[i] >= p.experts) mine[i] = -1;
   }
   int total = 0, before = 0;
-  if (hist) {
-    if (t < experts)
-      for (int c = 0; c < (int)gridDim.x; ++c) {
-        const int h = hist[c * experts + t];
-        total += h;
-        before += c < (int)blockIdx.x ? h : 0;
-      }
-  } else {
+  if constexpr (ONE) {
     cursor[t] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i)
-      if (mine[i] >= 0) atomicAdd(&cursor[mine[i]], 1);
+      if (mine[i] >= 0) rank[i] = atomicAdd(&cursor[mine[i]], 1);
     __syncthreads();
     total = cursor[t];
+  } else {
+    if (t < p.experts)
+      for (int c = 0; c < p.chunks; ++c) {
+        const int h = p.hist[c * p.experts + t];
+        total += h;
+        before += c < chunk ? h : 0;
+      }
   }
-  const int nt = (total + tile_rows - 1) / tile_rows;
-  const int mul = (total + 15) / 16 * 16;  // slots taken
-  slots[0][t] = mul;
-  tiles[0][t] = nt;
+  const int nt = (total + p.tile_rows - 1) / p.tile_rows;
+  int slots = (total + 15) / 16 * 16, tiles = nt;  // inclusive sums over the experts: in the wave, then over the waves
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int a = __shfl_up(slots, o, 64), b = __shfl_up(tiles, o, 64);
+    slots += lane >= o ? a : 0;
+    tiles += lane >= o ? b : 0;
+  }
+  if (lane == 63) {
+    part[0][w] = slots;
+    part[1][w] = tiles;
+  }
   __syncthreads();
-  int cur = 0;
-  for (int o = 1; o < kPlanThreads; o *= 2, cur ^= 1) {  // inclusive sums
-    slots[cur ^ 1][t] = slots[cur][t] + (t >= o ? slots[cur][t - o] : 0);
-    tiles[cur ^ 1][t] = tiles[cur][t] + (t >= o ? tiles[cur][t - o] : 0);
-    __syncthreads();
+  for (int i = 0; i < w; ++i) {
+    slots += part[0][i];
+    tiles += part[1][i];
   }
-  const int slot0 = slots[cur][t] - mul, tile0 = tiles[cur][t] - nt;
+  const int slot0 = slots - (total + 15) / 16 * 16, tile0 = tiles - nt;
   cursor[t] = slot0 + before;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i)
     if (mine[i] >= 0) {
-      const int p = blockIdx.x * kPlanChunk + i * kPlanThreads + t, slot = atomicAdd(&cursor[mine[i]], 1);
-      pair[slot] = p;
-      frame[slot] = p / top_k;
+      const int q = chunk * kPlanChunk + i * kPlanThreads + t;
+      const int slot = ONE ? cursor[mine[i]] + rank[i] : atomicAdd(&cursor[mine[i]], 1);
+      p.pair[slot] = q;
+      p.frame[slot] = q / p.top_k;
     }
-  if (blockIdx.x == 0) {
-    if (t == kPlanThreads - 1) *n_tiles = tiles[cur][t];
+  if (chunk == 0) {
+    if (t == kPlanThreads - 1) *p.n_tiles = tiles;
     for (int i = 0; i < nt; ++i) {
-      int* e = tile + 4 * (tile0 + i);
+      int* e = p.tile + 4 * (tile0 + i);
       e[0] = t;
-      e[1] = slot0 + i * tile_rows;
-      e[2] = min(tile_rows, total - i * tile_rows);
+      e[1] = slot0 + i * p.tile_rows;
+      e[2] = min(p.tile_rows, total - i * p.tile_rows);
       e[3] = 0;
     }
   }
 }
+
+// The frames' codes, and beside them, by the first workgroups, the list of
+// pairs (ONE) or the counts for it: neither needs the other, and together they
+// take as long as the longer.
+template <typename T, bool ONE>
+__global__ __launch_bounds__(kPlanThreads) void prepare_kernel(PlanParams p, const T* x, int64_t rows, int K, uint8_t* codes,
+                                                               uint8_t* scales) {
+  if ((int)blockIdx.x < p.chunks) {
+    if constexpr (ONE) plan_scatter<true>(p, 0);
+    else plan_count(p, blockIdx.x);
+  } else {
+    quantize_blocks(x, K, rows, K, true, codes, scales, (int64_t)(blockIdx.x - p.chunks) * 16 + (threadIdx.x >> 6));
+  }
+}
+__global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(PlanParams p) { plan_scatter<false>(p, blockIdx.x); }
 
 // ---------------------------------------------------------------------------
 // The experts' weighted sum, 8 columns to a thread, in the order of the
@@ -374,13 +402,35 @@ hipError_t route(const RouteParams& p, hipStream_t s) {
 
 int64_t plan_scratch_ints(int64_t pairs, int experts) { return (pairs + kPlanChunk - 1) / kPlanChunk * experts; }
 
-hipError_t experts_plan(const int* idx, int pairs, int top_k, int experts, int tile_rows, int* pair, int* frame,
-                        int* tile, int* n_tiles, int* scratch, hipStream_t s) {
-  if (pairs <= 0 || top_k <= 0 || experts <= 0 || experts > kPlanExperts || tile_rows <= 0) return hipErrorInvalidValue;
-  const int chunks = (pairs + kPlanChunk - 1) / kPlanChunk;
-  if (chunks > 1) plan_count_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, experts, scratch);
-  plan_scatter_kernel<<<chunks, kPlanThreads, 0, s>>>(idx, pairs, top_k, experts, tile_rows,
-                                                      chunks > 1 ? scratch : nullptr, pair, frame, tile, n_tiles);
+hipError_t experts_prepare(const int* idx, int pairs, int top_k, int experts, int tile_rows, int* pair, int* frame, int* tile,
+                           int* n_tiles, int* scratch, DType dt, const void* x, int64_t rows, int K, uint8_t* codes,
+                           uint8_t* scales, hipStream_t s) {
+  if (pairs <= 0 || top_k <= 0 || experts <= 0 || experts > kPlanExperts || tile_rows <= 0 || rows < 0 || K <= 0 || K % 8 ||
+      (reinterpret_cast<uintptr_t>(x) & 15))
+    return hipErrorInvalidValue;
+  PlanParams p;
+  p.idx = idx;
+  p.pairs = pairs;
+  p.top_k = top_k;
+  p.experts = experts;
+  p.tile_rows = tile_rows;
+  p.chunks = (pairs + kPlanChunk - 1) / kPlanChunk;
+  p.hist = scratch;
+  p.pair = pair;
+  p.frame = frame;
+  p.tile = tile;
+  p.n_tiles = n_tiles;
+  const int64_t items = codes ? rows * (fp8_kbp(K) / 4) : 0, grid = p.chunks + (items + 15) / 16;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const T* xt = static_cast<const T*>(x);
+    if (p.chunks == 1) prepare_kernel<T, true><<<(unsigned)grid, kPlanThreads, 0, s>>>(p, xt, rows, K, codes, scales);
+    else prepare_kernel<T, false><<<(unsigned)grid, kPlanThreads, 0, s>>>(p, xt, rows, K, codes, scales);
+  };
+  if (dt == kBF16) go(bf16{});
+  else go(float{});
+  if (p.chunks > 1) plan_scatter_kernel<<<p.chunks, kPlanThreads, 0, s>>>(p);
   return hipGetLastError();
 }
 

@@ -426,10 +426,9 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
   g[1].epilogue = mhsa::kFp8Pair;
   g[1].out = plan.y;
   if (plan.tile_rows)
-    HIPCHK(mhsa::experts_plan(idx, pairs, top_k, e->E, plan.tile_rows, plan.pair, plan.frame, plan.tile, plan.n_tiles,
-                              plan.scratch, s));
+    HIPCHK(mhsa::experts_prepare(idx, pairs, top_k, e->E, plan.tile_rows, plan.pair, plan.frame, plan.tile, plan.n_tiles,
+                                 plan.scratch, dt, x, rows, e->D, plan.xc, plan.xs, s));
   if (plan.tile_rows > 16) {
-    HIPCHK(mhsa::fp8_quantize_rows(dt, x, e->D, rows, e->D, plan.xc, plan.xs, s));
     g[0].a = plan.xc;
     g[0].as = plan.xs;
     g[0].a_rows = rows;

@@ -29,44 +29,10 @@ namespace {
 // Rounding to codes
 // ---------------------------------------------------------------------------
 
-// 8 values of row x from column c on, zero past K.
-template <typename T>
-__device__ __forceinline__ void load8(const T* x, int c, int K, bool vec, float v[8]) {
-  if (vec && c + 8 <= K) {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      reinterpret_cast<u32x4*>(t)[i] = reinterpret_cast<const u32x4*>(x + c)[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)x[c + i] : 0.f;
-  }
-}
-
-// A wave rounds 4 blocks of a row, 16 lanes of 8 values to a block.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int64_t rows, int K, bool vec,
                                                             uint8_t* codes, uint8_t* scales) {
-  const int kb = (K + 127) / 128, items = (kb + 3) / 4;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= rows * items) return;
-  const int64_t row = id / items;
-  const int lane = threadIdx.x & 63, blk = (int)(id % items) * 4 + (lane >> 4);
-  float v[8];
-  load8(x + row * ldx, blk * 128 + (lane & 15) * 8, blk < kb ? K : 0, vec, v);
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fp8_mag(v[i]));
-#pragma unroll
-  for (int o = 1; o < 16; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (blk >= kb) return;
-  const int s = fp8_scale_byte(m);
-  const float scale = fp8_scale(s);
-  const u32x2 q = {fp8_pack4_scaled(v[0], v[1], v[2], v[3], scale), fp8_pack4_scaled(v[4], v[5], v[6], v[7], scale)};
-  *reinterpret_cast<u32x2*>(codes + row * ((int64_t)kb * 128) + blk * 128 + (lane & 15) * 8) = q;
-  if ((lane & 15) == 0) scales[row * (items * 4) + blk] = (uint8_t)s;
+  quantize_blocks(x, ldx, rows, K, vec, codes, scales, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6));
 }
 
 // One workgroup per 128 x 128 block of a weight matrix.

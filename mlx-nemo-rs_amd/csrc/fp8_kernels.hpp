@@ -120,8 +120,11 @@ inline int64_t expert_slots(int64_t pairs, int experts) {
 // Experts' bookkeeping: pairs sorted by expert and their frames (pair and
 // frame [expert_slots]), and the tile list of tile_rows slots. scratch: plan_scratch_ints(pairs, experts) ints.
 int64_t plan_scratch_ints(int64_t pairs, int experts);
-hipError_t experts_plan(const int* idx, int pairs, int top_k, int experts, int tile_rows, int* pair, int* frame,
-                        int* tile, int* n_tiles, int* scratch, hipStream_t s);
+// The same launch rounds x [rows, K] (contiguous, 16-byte aligned, K a multiple
+// of 8) to codes, unless `codes` is null.
+hipError_t experts_prepare(const int* idx, int pairs, int top_k, int experts, int tile_rows, int* pair, int* frame, int* tile,
+                           int* n_tiles, int* scratch, DType dt, const void* x, int64_t rows, int K, uint8_t* codes,
+                           uint8_t* scales, hipStream_t s);
 // out = residual + res_scale * sum_j w[r, j] y[r * top_k + j] over the chosen
 // experts in [0, experts); residual may be null or out.
 hipError_t experts_combine(DType dt, const float* y, const int* idx, const float* w, int64_t rows, int top_k,
