@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kPlanThreads) void prepare_kernel(PlanParams p, con
     if constexpr (ONE) plan_scatter<true>(p, 0);
     else plan_count(p, blockIdx.x);
   } else {
-    quantize_blocks(x, K, rows, K, true, codes, scales, (int64_t)(blockIdx.x - p.chunks) * 16 + (threadIdx.x >> 6));
+    quantize_blocks(x, K, rows, K, codes, scales, (int64_t)(blockIdx.x - p.chunks) * 16 + (threadIdx.x >> 6));
   }
 }
 __global__ __launch_bounds__(kPlanThreads) void plan_scatter_kernel(PlanParams p) { plan_scatter<false>(p, blockIdx.x); }

@@ -35,25 +35,30 @@ __device__ __forceinline__ uint32_t fp8_pack4_scaled(float a, float b, float c, 
   r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
   return __builtin_bit_cast(uint32_t, r);
 }
-// Eight codes (two words) as bf16, exactly.
-__device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t lo, uint32_t hi) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+// Eight codes (two words) times a power of two as bf16: exact but for what
+// lies below bf16's smallest subnormal, 2^-133.
+__device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t lo, uint32_t hi, float scale = 1.f) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// 8 values from x on. The loads need no more alignment than an element (the
+// memory unit takes 16 bytes at any address).
+template <typename T>
+__device__ __forceinline__ void load_run(const T* x, float v[8]) {
+  T t[8];
+  __builtin_memcpy(t, x, sizeof t);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+}
 // 8 values of row x from column c on, zero past K.
 template <typename T>
-__device__ __forceinline__ void load8(const T* x, int c, int K, bool vec, float v[8]) {
-  if (vec && c + 8 <= K) {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      reinterpret_cast<u32x4*>(t)[i] = reinterpret_cast<const u32x4*>(x + c)[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+__device__ __forceinline__ void load8(const T* x, int c, int K, float v[8]) {
+  if (c + 8 <= K) {
+    load_run(x + c, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)x[c + i] : 0.f;
@@ -63,14 +68,14 @@ __device__ __forceinline__ void load8(const T* x, int c, int K, bool vec, float 
 // A wave rounds 4 blocks of a row, 16 lanes of 8 values to a block; item `id`
 // of rows * ceil(K / 512).
 template <typename T>
-__device__ __forceinline__ void quantize_blocks(const T* x, int64_t ldx, int64_t rows, int K, bool vec, uint8_t* codes,
-                                                uint8_t* scales, int64_t id) {
+__device__ __forceinline__ void quantize_blocks(const T* x, int64_t ldx, int64_t rows, int K, uint8_t* codes, uint8_t* scales,
+                                                int64_t id) {
   const int kb = (K + 127) / 128, items = (kb + 3) / 4;
   if (id >= rows * items) return;
   const int64_t row = id / items;
   const int lane = threadIdx.x & 63, blk = (int)(id % items) * 4 + (lane >> 4);
   float v[8];
-  load8(x + row * ldx, blk * 128 + (lane & 15) * 8, blk < kb ? K : 0, vec, v);
+  load8(x + row * ldx, blk * 128 + (lane & 15) * 8, blk < kb ? K : 0, v);
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = fmaxf(m, fp8_mag(v[i]));

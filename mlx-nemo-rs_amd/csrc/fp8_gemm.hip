@@ -10,7 +10,8 @@
 // at any K; the running sum keeps its 24 bits). That is far under half a step
 // of a bf16 result (2e-3 in the 2-norm) or of e4m3 codes. An f32 result keeps
 // f32 sums: there the codes go to the bf16 matrix cores, which hold them and
-// their products exactly (1e-7), at half the rate.
+// their products exactly (1e-7; only of blocks under 2^-115 what lies below
+// bf16's smallest number, 2^-133, is lost), at half the rate.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -30,9 +31,9 @@ namespace {
 // ---------------------------------------------------------------------------
 
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int64_t rows, int K, bool vec,
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int64_t rows, int K,
                                                             uint8_t* codes, uint8_t* scales) {
-  quantize_blocks(x, ldx, rows, K, vec, codes, scales, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6));
+  quantize_blocks(x, ldx, rows, K, codes, scales, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6));
 }
 
 // One workgroup per 128 x 128 block of a weight matrix.
@@ -122,8 +123,8 @@ __device__ __forceinline__ void store_as(DType dt, void* out, int64_t at, float 
 
 // Adds block b's products of RC x 16 weight rows (16 apart, from wrow; this
 // lane's 32 inputs) and the lane's activation row to acc. VEC: rows of whole
-// 16-byte runs of 8 inputs (the code for others is several times as long, and
-// a launch of a few microseconds pays for fetching it).
+// runs of 8 inputs (the code for others is several times as long, and a launch
+// of a few microseconds pays for fetching it).
 template <typename TX, int RC, bool EXACT, bool VEC>
 __device__ __forceinline__ void few_block(const uint8_t* wrow, int64_t wstep, const uint8_t* wsc, int b, const TX* xrow,
                                           int K, floatx4 acc[RC]) {
@@ -138,17 +139,11 @@ __device__ __forceinline__ void few_block(const uint8_t* wrow, int64_t wstep, co
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (VEC) {
-      TX t[8] = {};
-      if (c0 + 8 * i < K) {
 #pragma unroll
-        for (int u = 0; u < (int)sizeof(TX) / 2; ++u)
-          reinterpret_cast<u32x4*>(t)[u] = reinterpret_cast<const u32x4*>(xrow + c0 + 8 * i)[u];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 * i + e] = (float)t[e];
+      for (int e = 0; e < 8; ++e) v[8 * i + e] = 0.f;
+      if (c0 + 8 * i < K) load_run(xrow + c0 + 8 * i, v + 8 * i);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 * i + e] = c0 + 8 * i + e < K ? (float)xrow[c0 + 8 * i + e] : 0.f;
+      load8(xrow, c0 + 8 * i, K, v + 8 * i);
     }
   }
   float m = 0.f;
@@ -603,7 +598,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
           *reinterpret_cast<const int*>(smem + C::SCALES + buf * BM * 4 + (wm * C::WM + 32 * (r - FRAGS) + (lane & 31)) * 4);
     }
   };
-  floatx16 acc[C::TN][C::TM], part[EXACT ? C::TN : 1][EXACT ? C::TM : 1];
+  floatx16 acc[C::TN][C::TM];
 
   int ws = 0, xs[C::TM];
   // Half h of stage kt, whose fragments are in set h and whose buffer is buf.
@@ -650,36 +645,23 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
         between(m);
       }
     } else {
-      // exact products and f32 sums: per block on the bf16 cores, then added
-      // with the block's power of two
-      if constexpr (h == 0) {
-#pragma unroll
-        for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-          for (int i = 0; i < C::TM; ++i) part[j][i] = floatx16{};
-      }
+      // Exact products and f32 sums on the bf16 cores. bf16 has f32's range, so
+      // the powers of two go into the conversion of the codes.
+      const float wf = fp8_scale(ws & 255);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         bf16x8 xa[C::TM], xb[C::TN];
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i) xa[i] = fp8_to_bf16(fa[h][i][u >> 1][2 * (u & 1)], fa[h][i][u >> 1][2 * (u & 1) + 1]);
+        for (int i = 0; i < C::TM; ++i)
+          xa[i] = fp8_to_bf16(fa[h][i][u >> 1][2 * (u & 1)], fa[h][i][u >> 1][2 * (u & 1) + 1], fp8_scale(xs[i] & 255));
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) xb[j] = fp8_to_bf16(fb[h][j][u >> 1][2 * (u & 1)], fb[h][j][u >> 1][2 * (u & 1) + 1]);
+        for (int j = 0; j < C::TN; ++j)
+          xb[j] = fp8_to_bf16(fb[h][j][u >> 1][2 * (u & 1)], fb[h][j][u >> 1][2 * (u & 1) + 1], wf);
 #pragma unroll
         for (int m = 0; m < C::TM * C::TN; ++m) {
           const int j = m / C::TM, i = m % C::TM;
-          part[j][i] = mma32(xb[j], xa[i], part[j][i]);
+          acc[j][i] = mma32(xb[j], xa[i], acc[j][i]);
           between(u * C::TM * C::TN + m);
-        }
-      }
-      if constexpr (h == 1) {
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i) {
-          const int e = (xs[i] & 255) + (ws & 255) - 254;
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[j][i][r] += __builtin_ldexpf(part[j][i][r], e);
         }
       }
     }
@@ -894,7 +876,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       constexpr int LPR = 32 * JB / V, RPI = 64 / LPR;   // lanes to a row, rows to a store
       static_assert(C::TN % JB == 0 && (EPI != kFp8Pair || RPI == 8), "blocks");
       TOut* out = reinterpret_cast<TOut*>(p.out);
-      const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.ldo % V == 0;
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -919,8 +900,8 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
             const u32x4 raw = *reinterpret_cast<const u32x4*>(st + r * C::OP + lane % LPR * 16);
             if (row >= done.rows || col >= p.N) continue;
             TOut* to16 = out + (EPI == kFp8Pair ? (int64_t)place[32 * i + r] : (int64_t)(done.m0 + row)) * p.ldo + col;
-            if (vec && col + V <= p.N) {
-              *reinterpret_cast<u32x4*>(to16) = raw;
+            if (col + V <= p.N) {
+              __builtin_memcpy(to16, &raw, 16);  // (at any address)
             } else {
               const TOut* v = reinterpret_cast<const TOut*>(&raw);
 #pragma unroll
@@ -948,7 +929,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
 }
 
 template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
-__global__ __launch_bounds__(256, (Fp8Cfg<BM, BN, NS>::AHEAD ? 1 : 2)) void fp8_tile_kernel(Fp8Gemm p) {
+__global__ __launch_bounds__(256, (2 * Fp8Cfg<BM, BN, NS>::LDS > 160 * 1024 ? 1 : 2)) void fp8_tile_kernel(Fp8Gemm p) {
   __shared__ __attribute__((aligned(1024))) char smem[Fp8Cfg<BM, BN, NS>::LDS];
   fp8_tile_body<BM, BN, NS, EXACT, EPI, TOut>(p, smem);
 }
@@ -978,12 +959,10 @@ hipError_t fp8_quantize_rows(DType dt, const void* x, int64_t ldx, int64_t rows,
   if (rows <= 0 || K <= 0 || K > kFp8MaxK) return hipErrorInvalidValue;
   const int64_t items = rows * (fp8_kbp(K) / 4), grid = (items + 3) / 4;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const int es = dtype_size(dt);
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx * es % 16 == 0;
   if (dt == kBF16)
-    quantize_rows_kernel<bf16><<<(unsigned)grid, 256, 0, s>>>(static_cast<const bf16*>(x), ldx, rows, K, vec, codes, scales);
+    quantize_rows_kernel<bf16><<<(unsigned)grid, 256, 0, s>>>(static_cast<const bf16*>(x), ldx, rows, K, codes, scales);
   else
-    quantize_rows_kernel<float><<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(x), ldx, rows, K, vec, codes, scales);
+    quantize_rows_kernel<float><<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(x), ldx, rows, K, codes, scales);
   return hipGetLastError();
 }
 
@@ -1019,10 +998,14 @@ hipError_t fp8_unpad_weight(const uint8_t* codes, const uint8_t* scales, int N, 
   return hipGetLastError();
 }
 
+// Up to 16 rows read the weights once. More read them once per 16 rows, which
+// saves the second launch and the codes' way through memory while it is not
+// much: with a call from Python at 128 x 1024 -> 4096 8.8 us against 12.6, at
+// 192 rows 11.9 against 12.5, at 256 17.5; 64 x 4096 -> 1024 8.4 against 14.1,
+// 96 rows 14.9 (over K > 2048 16 waves share one row group's inputs).
 bool fp8_few_rows(int64_t M, int N, int K) {
-  (void)N;
-  (void)K;
-  return M <= 64;
+  const int64_t read = (M + 15) / 16 * N * K;
+  return M <= 16 || (M <= 256 && read <= (K <= 2048 ? 40 : 20) << 20);
 }
 int fp8_scan_pairs() { return kScanPairs; }
 
@@ -1032,8 +1015,7 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
   if (p.g.tile && p.g.tile_rows != 16) return hipErrorInvalidValue;
   const int64_t groups = p.g.tile ? p.g.max_tiles : p.g.idx ? std::min(p.g.pairs, p.g.experts) : (p.M + 15) / 16;
   if (groups <= 0 || groups > 65535) return hipErrorInvalidValue;
-  const int es = dtype_size(p.x_dt);
-  const bool vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldx * es % 16 == 0 && p.K % 8 == 0;
+  const bool vec = p.K % 8 == 0;
   const bool exact = p.epilogue == kFp8Out && p.out_dt == kF32;
   auto go = [&](auto tx, auto nw, auto rc) {
     using TX = decltype(tx);
@@ -1100,16 +1082,20 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
   auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  if (p.out_dt == kF32)
-    return tiles(128, 128) >= 128 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s)
-                                  : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
-  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256);
-  if (t256 >= 128 && p.K > kFp8Block) {  // (the large tiles' ring takes two stages)
-    if ((t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256) return launch_tile<192, 256, 2, false, kFp8Out, bf16>(p, s);
-    return launch_tile<256, 256, 2, false, kFp8Out, bf16>(p, s);
+  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256), t128 = tiles(128, 128);
+  const bool large = t256 >= 128 && p.K > kFp8Block;  // (the large tiles' ring takes two stages)
+  const bool fewer = (t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256;  // rows a CU goes through
+  if (p.out_dt == kF32) {
+    if (large && fewer) return launch_tile<192, 256, 2, true, kFp8Out, float>(p, s);
+    if (large) return launch_tile<256, 256, 2, true, kFp8Out, float>(p, s);
+    return t128 >= 128 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s) : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
   }
-  return tiles(128, 128) >= 128 ? launch_tile<128, 128, 2, false, kFp8Out, bf16>(p, s)
-                                : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
+  if (large && fewer) return launch_tile<192, 256, 2, false, kFp8Out, bf16>(p, s);
+  if (large) return launch_tile<256, 256, 2, false, kFp8Out, bf16>(p, s);
+  // a tile alone on its CU keeps four stages, two that share it two each
+  // (3000 x 4096 -> 1024: 36.8 -> 29.7 us with the rows' codes)
+  if (t128 >= 128 && t128 <= device_cus()) return launch_tile<128, 128, 4, false, kFp8Out, bf16>(p, s);
+  return t128 >= 128 ? launch_tile<128, 128, 2, false, kFp8Out, bf16>(p, s) : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
 }
 
 }  // namespace mhsa

@@ -217,14 +217,14 @@ def test_replayed_graphs_and_streams():
 
 def test_workspace_is_checked():
     rng = np.random.default_rng(12)
-    x, codes, scales, bias = make(rng, 200, 256, 96)
+    x, codes, scales, bias = make(rng, 300, 256, 96)  # (up to 256 rows may need none)
     layer, lib = layer_of(256, 96, codes, scales, bias), M.library()
-    t, out = on_gpu(x, "f32"), torch.empty(200, 96, device="cuda")
-    need = lib.mhsa_fp8_linear_workspace(layer._h, 200)
+    t, out = on_gpu(x, "f32"), torch.empty(300, 96, device="cuda")
+    need = lib.mhsa_fp8_linear_workspace(layer._h, 300)
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
 
     def call(ptr, size):
-        return lib.mhsa_fp8_linear_forward(layer._h, t.data_ptr(), M.F32, 200, 256, out.data_ptr(), M.F32, 96, ptr, size, None)
+        return lib.mhsa_fp8_linear_forward(layer._h, t.data_ptr(), M.F32, 300, 256, out.data_ptr(), M.F32, 96, ptr, size, None)
     torch.cuda.synchronize()
     assert call(None, need) == call(ws.data_ptr(), need - 1) == call(ws.data_ptr() + 8, need) == M.MHSA_EINVAL
     assert call(t.data_ptr(), need) == M.MHSA_EINVAL
