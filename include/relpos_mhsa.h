@@ -528,7 +528,7 @@ int32_t mhsa_encoder_step(mhsa_encoder* enc, float* x_inout, const void* pos_emb
  * calls run on the GPU that was current at loading, which is to be current
  * again, and on a stream of it. Loading waits for the GPU; no call that reads
  * the handle may run at the same time. Weight pointers may be host or device
- * memory. */
+ * memory. Calls take up to 2^30 rows, up to 2^30 elements apart. */
 
 /* y = W q(x) + b. */
 typedef struct mhsa_fp8_linear mhsa_fp8_linear;
@@ -553,8 +553,8 @@ int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* linear, int32_t rows);
  * row); x, out and the workspace must not overlap. rows may be 0. Products of
  * an f32 out are exact and summed in f32; for a bf16 out they go through the
  * fp8 matrix unit, whose sums are off by some 1e-5 of the result (at most 9e-4 of
- * their terms' magnitudes). A row's low bits may depend on the number of
- * rows. */
+ * their terms' magnitudes). f32 results of blocks under 2^-115 lose what lies
+ * below 2^-133. A row's low bits may depend on the number of rows. */
 int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* linear, const void* x, int32_t x_dtype, int32_t rows,
                                 int64_t x_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
                                 int64_t workspace_bytes, void* hip_stream);
@@ -572,7 +572,7 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* linear, const void* x, in
  * weights 0 (a frame whose logits are all -inf chooses no expert).
  * indices int32 and weights f32 [rows, top_k], device. n_experts <= 512,
  * n_groups <= 64, top_k <= 32 and at most the experts of topk_groups groups.
- * rows may be 0. */
+ * indices and weights must not overlap another tensor. rows may be 0. */
 #define MHSA_ROUTE_SOFTMAX 0
 #define MHSA_ROUTE_SIGMOID 1
 int32_t mhsa_route(const void* logits, int32_t dtype, int32_t rows, int32_t n_experts, int64_t stride, int32_t score,

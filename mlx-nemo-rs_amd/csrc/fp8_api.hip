@@ -19,6 +19,10 @@ using mhsa::DType;
 
 namespace {
 
+// Bounds under which no size or offset below leaves 63 bits.
+constexpr int32_t kMaxRows = 1 << 30;
+constexpr int64_t kMaxStride = 1 << 30;
+
 // n weight matrices [N, K] in the kernels' format.
 struct Fp8Weights {
   int n = 0, N = 0, K = 0;
@@ -63,7 +67,7 @@ int32_t load_bias(Fp8Weights& w, int data_dtype, const void* bias) {
 // memory. Everything queued on the GPU comes first: a forward may still read
 // the old weights, and device tensors may still be being written.
 int32_t load_weights(Fp8Weights& w, int data_dtype, const void* weight, const uint8_t* codes, const uint8_t* scales,
-                     const void* bias) {
+                     const void* bias) try {
   if (codes ? !scales : !weight) return fail(MHSA_EINVAL, "null weight pointer");
   if (w.use_bias != (bias != nullptr))
     return fail(MHSA_EINVAL, w.use_bias ? "a bias is expected" : "the layer was created without a bias");
@@ -110,6 +114,8 @@ int32_t load_weights(Fp8Weights& w, int data_dtype, const void* weight, const ui
   if (int32_t rc = load_bias(w, codes ? MHSA_F32 : data_dtype, bias)) return rc;
   w.loaded = true;
   return MHSA_OK;
+} catch (const std::bad_alloc&) {
+  return fail(MHSA_ENOMEM, "out of host memory");
 }
 
 // Weights are where they were loaded.
@@ -229,7 +235,7 @@ int32_t mhsa_fp8_linear_read_codes(const mhsa_fp8_linear* h, uint8_t* codes, uin
 }
 
 int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* h, int32_t rows) {
-  if (!h || rows < 0) return -1;
+  if (!h || rows < 0 || rows > kMaxRows) return -1;
   return rows == 0 ? 0 : linear_plan(h->w, rows, nullptr).bytes;
 }
 
@@ -242,6 +248,7 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t
   if (!act_dtype(x_dtype, &xd) || !act_dtype(out_dtype, &od))
     return fail(MHSA_ENOTSUP, "dtypes %d and %d not supported (f32, bf16)", x_dtype, out_dtype);
   if (rows < 0) return fail(MHSA_EINVAL, "rows must not be negative (got %d)", rows);
+  if (rows > kMaxRows) return fail(MHSA_ENOTSUP, "%d rows exceed %d", rows, kMaxRows);
   if (rows == 0) return MHSA_OK;
   if (!x || !out) return fail(MHSA_EINVAL, "null tensor pointer");
   const int xs = mhsa::dtype_size(xd), os = mhsa::dtype_size(od);
@@ -250,7 +257,8 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t
   if (x_stride < w.K || out_stride < w.N)
     return fail(MHSA_EINVAL, "row strides %lld and %lld are shorter than the rows (%d, %d)", (long long)x_stride,
                 (long long)out_stride, w.K, w.N);
-  if (x_stride > (int64_t)1 << 40 || out_stride > (int64_t)1 << 40) return fail(MHSA_EINVAL, "row strides exceed 2^40");
+  if (x_stride > kMaxStride || out_stride > kMaxStride)
+    return fail(MHSA_ENOTSUP, "row strides %lld and %lld exceed 2^30", (long long)x_stride, (long long)out_stride);
   if (!w.loaded) return fail(MHSA_EINVAL, "no weights are loaded");
   const LinearPlan plan = linear_plan(w, rows, workspace);
   if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes))
@@ -316,6 +324,11 @@ extern "C" int32_t mhsa_route(const void* logits, int32_t dtype, int32_t rows, i
   if (reinterpret_cast<uintptr_t>(logits) % mhsa::dtype_size(p.dt) || reinterpret_cast<uintptr_t>(indices) % 4 ||
       reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(bias) % 4)
     return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
+  if (rows > kMaxRows || stride > kMaxStride) return fail(MHSA_ENOTSUP, "%d rows %lld apart exceed 2^30", rows, (long long)stride);
+  const int64_t ln = ((rows - 1) * stride + n_experts) * mhsa::dtype_size(p.dt), kn = (int64_t)rows * top_k * 4;
+  if (overlap(indices, kn, logits, ln) || overlap(weights, kn, logits, ln) || overlap(indices, kn, weights, kn) ||
+      overlap(indices, kn, bias, bias ? n_experts * 4 : 0) || overlap(weights, kn, bias, bias ? n_experts * 4 : 0))
+    return fail(MHSA_EINVAL, "indices and weights must not overlap another tensor");
   p.logits = logits;
   p.ld = stride;
   p.rows = rows;
@@ -519,7 +532,7 @@ int32_t mhsa_experts_load_codes(mhsa_experts* h, const uint8_t* codes1, const ui
 }
 
 int64_t mhsa_experts_workspace(const mhsa_experts* h, int32_t rows, int32_t top_k) {
-  if (!h || rows < 0 || top_k <= 0 || top_k > kMaxTopK) return -1;
+  if (!h || rows < 0 || rows > kMaxRows || top_k <= 0 || top_k > kMaxTopK) return -1;
   return rows == 0 ? 0 : experts_layout(h, rows, top_k, nullptr).bytes;
 }
 
@@ -530,6 +543,7 @@ int32_t mhsa_experts_forward(const mhsa_experts* h, const void* x, int32_t dtype
   DType dt;
   if (!act_dtype(dtype, &dt)) return fail(MHSA_ENOTSUP, "dtype %d not supported (f32, bf16)", dtype);
   if (rows < 0) return fail(MHSA_EINVAL, "rows must not be negative (got %d)", rows);
+  if (rows > kMaxRows) return fail(MHSA_ENOTSUP, "%d rows exceed %d", rows, kMaxRows);
   if (top_k <= 0 || top_k > kMaxTopK) return fail(MHSA_EINVAL, "top_k %d is not in [1, %d]", top_k, kMaxTopK);
   if (rows == 0) return MHSA_OK;
   if (!x || !indices || !weights || !out) return fail(MHSA_EINVAL, "null tensor pointer");

@@ -1081,7 +1081,7 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
     return hipErrorInvalidValue;
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
-  auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  auto tiles = [&](int64_t bm, int64_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };
   const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256), t128 = tiles(128, 128);
   const bool large = t256 >= 128 && p.K > kFp8Block;  // (the large tiles' ring takes two stages)
   const bool fewer = (t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256;  // rows a CU goes through

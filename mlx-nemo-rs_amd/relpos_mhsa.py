@@ -539,10 +539,9 @@ def _load_floats(pairs):
         if b is None:
             ptrs.append(None)
             continue
-        if isinstance(b, np.ndarray):
-            import torch
-            b = torch.from_numpy(np.ascontiguousarray(b))
-        a, ptr, _ = _weight_data(b.to(a.dtype), bshape, bname, "float")
+        a, ptr, code = _weight_data(b, bshape, bname, "float")
+        if code != dtype:
+            raise MhsaError(MHSA_EINVAL, f"{bname}: the bias and the weights are of different dtypes")
         keep.append(a)
         ptrs.append(ptr)
     return keep, ptrs, dtype
@@ -637,7 +636,8 @@ class Fp8Linear:
             self._h = None
 
     def load(self, weight, bias=None) -> None:
-        """weight [out, in] (float32, bfloat16 or float16), rounded to codes."""
+        """weight [out, in] and bias [out] of one dtype (float32, bfloat16 or
+        float16); the weight is rounded to codes."""
         keep, ptrs, dtype = _load_floats([((weight, (self.out_dim, self.in_dim), "weight"),
                                            (bias, (self.out_dim,), "bias"))])
         _check(self._lib.mhsa_fp8_linear_load(self._h, dtype, *ptrs))
@@ -724,7 +724,8 @@ class ExpertFeedForward:
 
     def load(self, weight1, weight2, bias1=None, bias2=None) -> None:
         """weight1 [n_experts, ff_dim, d_model], weight2 [n_experts, d_model,
-        ff_dim] of one float dtype, rounded to codes."""
+        ff_dim], bias1 [n_experts, ff_dim] and bias2 [n_experts, d_model] of one
+        float dtype; the weights are rounded to codes."""
         e, d, f = self.n_experts, self.d_model, self.ff_dim
         keep, ptrs, dtype = _load_floats([((weight1, (e, f, d), "weight1"), (bias1, (e, f), "bias1")),
                                           ((weight2, (e, d, f), "weight2"), (bias2, (e, d), "bias2"))])

@@ -71,6 +71,8 @@ def test_load_refuses():
     assert lib.mhsa_fp8_linear_read_codes(h, w.ctypes.data, w.ctypes.data) == M.MHSA_EINVAL  # nothing loaded
     lib.mhsa_fp8_linear_destroy(h)
     layer = M.Fp8Linear(256, 384, True)
+    with pytest.raises(M.MhsaError):
+        layer.load(w, np.zeros(384, np.float16))  # another dtype than the weight's
     for weight, bias in ((w.T, np.zeros(384, np.float32)), (w.astype(np.float64), np.zeros(384, np.float32)),
                          (w, np.zeros(383, np.float32)), (w, None)):
         with pytest.raises(M.MhsaError):
@@ -85,7 +87,9 @@ def test_linear_forward_refuses():
     lib, h = M.library(), linear()
     f = lib.mhsa_fp8_linear_forward
     assert f(None, SOME, M.F32, 1, 256, SOME, M.F32, 384, None, 0, None) == M.MHSA_EINVAL
-    for args in ((SOME, M.F16, 1, 256, SOME, M.F32, 384), (SOME, M.F32, 1, 256, SOME, M.U32, 384)):
+    for args in ((SOME, M.F16, 1, 256, SOME, M.F32, 384), (SOME, M.F32, 1, 256, SOME, M.U32, 384),
+                 (SOME, M.F32, (1 << 30) + 1, 256, SOME, M.F32, 384), (SOME, M.F32, 2, (1 << 30) + 1, SOME, M.F32, 384),
+                 (SOME, M.F32, 2, 256, SOME, M.F32, (1 << 30) + 1)):
         assert f(h, *args, None, 0, None) == M.MHSA_ENOTSUP
     for args in ((SOME, M.F32, -1, 256, SOME, M.F32, 384), (None, M.F32, 1, 256, SOME, M.F32, 384),
                  (SOME, M.F32, 1, 256, None, M.F32, 384), (SOME, M.F32, 2, 255, SOME, M.F32, 384),
@@ -102,17 +106,19 @@ def test_linear_forward_refuses():
 
 def test_route_refuses():
     f = M.library().mhsa_route
-    good = dict(x=SOME, dt=M.F32, rows=4, e=64, ld=64, score=0, bias=None, g=8, kg=4, k=4, rn=1, s=1.0, i=SOME, w=SOME)
+    good = dict(x=SOME, dt=M.F32, rows=4, e=64, ld=64, score=0, bias=None, g=8, kg=4, k=4, rn=1, s=1.0, i=2 * SOME, w=3 * SOME)
 
     def call(**more):
         a = {**good, **more}
         return f(a["x"], a["dt"], a["rows"], a["e"], a["ld"], a["score"], a["bias"], a["g"], a["kg"], a["k"], a["rn"],
                  a["s"], a["i"], a["w"], None)
-    for more in (dict(dt=M.F16), dict(score=2), dict(e=520, ld=520, g=1, kg=1), dict(e=130, ld=130, g=65), dict(e=512, ld=512, g=1, kg=1, k=33)):
+    for more in (dict(dt=M.F16), dict(score=2), dict(e=520, ld=520, g=1, kg=1), dict(e=130, ld=130, g=65), dict(e=512, ld=512, g=1, kg=1, k=33),
+                 dict(rows=(1 << 30) + 1), dict(ld=(1 << 30) + 1)):
         assert call(**more) == M.MHSA_ENOTSUP, more
     for more in (dict(rows=-1), dict(e=0), dict(g=0), dict(g=7), dict(kg=0), dict(kg=9), dict(k=0), dict(k=33), dict(ld=63),
                  dict(s=float("nan")), dict(s=float("inf")), dict(x=None), dict(i=None), dict(w=None), dict(x=SOME + 2),
-                 dict(i=SOME + 1), dict(bias=SOME + 2)):
+                 dict(i=SOME + 1), dict(bias=SOME + 2), dict(i=SOME + 1020), dict(w=SOME), dict(w=2 * SOME + 60),
+                 dict(bias=2 * SOME - 4), dict(bias=3 * SOME + 60)):
         assert call(**more) == M.MHSA_EINVAL, more
     assert call(rows=0, x=None, i=None, w=None) == M.MHSA_OK
     with pytest.raises(M.MhsaError):
@@ -135,6 +141,8 @@ def test_experts_forward_refuses():
         assert f(h, *args, ws, big, None) == M.MHSA_EINVAL, args
     assert b"no weights" in lib.mhsa_last_error()
     assert f(h, None, M.F32, 0, None, None, 2, None, 1.0, None, None, 0, None) == M.MHSA_OK
+    assert f(h, x, M.F32, (1 << 30) + 1, idx, w, 2, r, 1.0, out, ws, big, None) == M.MHSA_ENOTSUP
+    assert lib.mhsa_experts_workspace(h, (1 << 30) + 1, 2) == -1
     assert lib.mhsa_experts_workspace(h, 5, 0) == -1 and lib.mhsa_experts_workspace(h, -5, 2) == -1
     assert lib.mhsa_experts_workspace(h, 0, 2) == 0 and lib.mhsa_experts_workspace(h, 5, 2) > 0
     # rows run in parts, so the workspace stops growing

@@ -90,6 +90,33 @@ def test_against_oracle(rows, e, d, f, k, dtype):
     assert torch.equal(inplace, got)
 
 
+@pytest.mark.parametrize("rows,e,d,f,k,skew", [(21000, 3, 256, 512, 2, 0.3), (30000, 9, 320, 192, 2, 1.5), (9000, 2, 192, 1088, 3, 0.0)])
+def test_many_large_tiles(rows, e, d, f, k, skew):
+    """Several tiles to a workgroup in both products, experts of very different
+    numbers of frames: sampled frames, and the last ones."""
+    rng = np.random.default_rng(rows)
+    parts = make(rng, e, d, f, bias=True)
+    x = frames(rng, rows, d, "bf16")
+    idx, w = choose(rng, rows, e, k, skew=skew)
+    got = parts[0].forward(x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda())
+    at = np.unique(np.concatenate([rng.integers(0, rows, 500), np.arange(rows - 300, rows)]))
+    check(got[at], x[at], idx[at], w[at], parts)
+    again = parts[0].forward(x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda())
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("rows,e,k", [(700, 150, 4), (3000, 512, 4), (1100, 256, 8), (4000, 70, 3), (129, 1, 2), (40, 1, 5)])
+def test_few_rows_of_many_experts(rows, e, k):
+    """Lists of pairs of several thousands, experts of fewer than 16 frames, of
+    more and of none; one expert of all of them."""
+    rng = np.random.default_rng(rows)
+    parts = make(rng, e, 128, 128, bias=True)
+    x = frames(rng, rows, 128, "bf16")
+    idx, w = choose(rng, rows, e, k, skew=0.2)
+    got = parts[0].forward(x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda())
+    check(got, x, idx, w, parts)
+
+
 @pytest.mark.parametrize("rows", [2, 100, 2000])
 def test_rows_without_experts_are_the_residual(rows):
     rng = np.random.default_rng(1)

@@ -65,6 +65,19 @@ def test_against_oracle(rows, k, n, xd, yd):
     check(got, x, codes, scales, bias, k)
 
 
+@pytest.mark.parametrize("rows,k,n", [(16300, 300, 2040), (9001, 129, 2304), (9001, 520, 2300), (6200, 700, 1800)])
+@pytest.mark.parametrize("yd", ["bf16", "f32"])
+def test_many_large_tiles(rows, k, n, yd):
+    """Several tiles to a workgroup, of 256 and of 192 rows, with two stages and
+    more: sampled rows, and the last ones."""
+    rng = np.random.default_rng(rows + k)
+    x, codes, scales, bias = make(rng, rows, k, n, spread=6)
+    x = on_gpu(x, "bf16")
+    got = layer_of(k, n, codes, scales, bias).forward(x, out_dtype=DTYPES[yd])
+    at = np.unique(np.concatenate([rng.integers(0, rows, 400), np.arange(rows - 300, rows)]))
+    check(got[at], x[at], codes, scales, bias, k)
+
+
 @pytest.mark.parametrize("rows", [5, 200])
 @pytest.mark.parametrize("xd", ["bf16", "f32"])
 def test_activations_round_as_the_format_says(rows, xd):
@@ -90,6 +103,25 @@ def test_activations_round_as_the_format_says(rows, xd):
     # (a bf16 out: the same values, exact in bf16)
     got = layer.forward(x, out_dtype=torch.bfloat16).double().cpu().numpy()
     assert np.array_equal(np.where(np.abs(want) < 2.0 ** -126, 0, got), np.where(np.abs(want) < 2.0 ** -126, 0, want))
+
+
+@pytest.mark.parametrize("rows", [5, 300, 3000])
+@pytest.mark.parametrize("yd", ["bf16", "f32"])
+def test_tiny_rows_and_large_weights(rows, yd):
+    """Rows about 2^-126 on weights about 2^40: an operand may lose what lies
+    below 2^-133, so each product 2^-133 of the other's magnitude."""
+    rng = np.random.default_rng(12)
+    k, n = 520, 300
+    x, codes, scales, _ = make(rng, rows, k, n, bias=False)
+    x, scales = on_gpu(x * 2.0 ** -126, "f32"), scales + 40
+    got = layer_of(k, n, codes, scales, None).forward(x, out_dtype=DTYPES[yd])
+    want, mag = F.linear(x.double().cpu().numpy(), codes, scales)
+    w = np.abs(F.weight_values(codes, scales)).sum(1)
+    tol = (k + 64) * 2.0 ** -24 * mag + 2.0 ** -133 * (w + k * 2.0 ** -100)
+    if yd == "bf16":
+        tol = tol + 7 * 2.0 ** -13 * mag + 2.0 ** -8 * np.abs(want)
+    bad = np.abs(got.double().cpu().numpy() - want) > tol
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist())
 
 
 @pytest.mark.parametrize("rows", [4, 130])
@@ -153,7 +185,7 @@ def test_strided_rows_leave_their_surroundings(rows, yd):
     around[1:-1, 4:4 + n] = 7.0
     assert (around == 7.0).all()
     with pytest.raises(M.MhsaError):
-        layer.forward(wide.T[:k].T.transpose(0, 1))
+        layer.forward(wide.T[:, :1].expand(-1, k))  # rows that do not lie apart
     with pytest.raises(M.MhsaError):
         layer.forward(wide[:, 3:3 + k], out=wide[:, :n])  # overlaps x
 
