@@ -528,7 +528,8 @@ int32_t mhsa_encoder_step(mhsa_encoder* enc, float* x_inout, const void* pos_emb
  * calls run on the GPU that was current at loading, which is to be current
  * again, and on a stream of it. Loading waits for the GPU; no call that reads
  * the handle may run at the same time. Weight pointers may be host or device
- * memory. Calls take up to 2^30 rows, up to 2^30 elements apart. */
+ * memory. Calls take up to 2^25 rows, up to 2^30 elements apart;
+ * weights are loaded again only on the GPU that holds them. */
 
 /* y = W q(x) + b. */
 typedef struct mhsa_fp8_linear mhsa_fp8_linear;

@@ -19,13 +19,15 @@ using mhsa::DType;
 
 namespace {
 
-// Bounds under which no size or offset below leaves 63 bits.
-constexpr int32_t kMaxRows = 1 << 30;
+// Bounds under which no size or offset below leaves 63 bits and no grid has
+// 2^32 threads along one axis.
+constexpr int32_t kMaxRows = 1 << 25, kMaxOut = 1 << 22;
 constexpr int64_t kMaxStride = 1 << 30;
 
 // n weight matrices [N, K] in the kernels' format.
 struct Fp8Weights {
   int n = 0, N = 0, K = 0;
+  int device = -1;  // where the buffers are
   bool use_bias = false, loaded = false;
   DevBuf codes, scales, bias;
   int64_t stride() const { return (int64_t)N * mhsa::fp8_kp(K); }
@@ -77,8 +79,13 @@ int32_t load_weights(Fp8Weights& w, int data_dtype, const void* weight, const ui
   if (codes)
     if (int32_t rc = on_device(scales, &sdev)) return rc;
   if (codes && dev != sdev) return fail(MHSA_EINVAL, "codes and scales are to be both on the host or both on the GPU");
+  int now = 0;
+  HIPCHK(hipGetDevice(&now));
+  if (w.device >= 0 && now != w.device)
+    return fail(MHSA_EINVAL, "the weights are on GPU %d, the current GPU is %d", w.device, now);
   HIPCHK(hipDeviceSynchronize());
   w.loaded = false;
+  w.device = now;
   HIPCHK(w.codes.ensure(w.n * w.stride()));
   HIPCHK(w.scales.ensure(w.n * w.scale_stride()));
   const int64_t es = codes ? 1 : data_dtype == MHSA_F32 ? 4 : 2, mat = (int64_t)w.N * w.K * es;
@@ -90,9 +97,9 @@ int32_t load_weights(Fp8Weights& w, int data_dtype, const void* weight, const ui
     HIPCHK(stage.ensure(mat));
     if (codes) HIPCHK(sstage.ensure(w.scale_in()));
   }
-  // device tensors: as many matrices to a launch as its grid takes; host ones
-  // one by one through the staging buffer
-  const int step = dev ? 1024 : 1;
+  // device tensors: as many matrices to a launch as its grid takes (a matrix
+  // has up to 2 GiB of codes); host ones one by one through the staging buffer
+  const int step = dev ? (int)std::clamp<int64_t>(((int64_t)1 << 32) / w.stride(), 1, 1024) : 1;
   for (int i = 0; i < w.n; i += step) {
     const int m = std::min(step, w.n - i);
     const uint8_t* from = src + i * mat;
@@ -156,7 +163,6 @@ struct Arena {
 
 struct mhsa_fp8_linear {
   Fp8Weights w;
-  int device = -1;
 };
 
 namespace {
@@ -190,6 +196,7 @@ int32_t mhsa_fp8_linear_create(int32_t in_dim, int32_t out_dim, int32_t use_bias
   if (in_dim > mhsa::kFp8MaxK) return fail(MHSA_ENOTSUP, "in_dim %d exceeds %d", in_dim, mhsa::kFp8MaxK);
   if ((int64_t)out_dim * mhsa::fp8_kp(in_dim) > INT32_MAX)
     return fail(MHSA_ENOTSUP, "a weight of %d x %d exceeds 2 GiB", out_dim, in_dim);
+  if (out_dim > kMaxOut) return fail(MHSA_ENOTSUP, "out_dim %d exceeds %d", out_dim, kMaxOut);
   mhsa_fp8_linear* h = new (std::nothrow) mhsa_fp8_linear();
   if (!h) return fail(MHSA_ENOMEM, "out of host memory");
   h->w.n = 1;
@@ -204,24 +211,20 @@ void mhsa_fp8_linear_destroy(mhsa_fp8_linear* h) { delete h; }
 
 int32_t mhsa_fp8_linear_load(mhsa_fp8_linear* h, int32_t data_dtype, const void* weight, const void* bias) {
   if (!h) return fail(MHSA_EINVAL, "null handle");
-  if (int32_t rc = load_weights(h->w, data_dtype, weight, nullptr, nullptr, bias)) return rc;
-  HIPCHK(hipGetDevice(&h->device));
-  return MHSA_OK;
+  return load_weights(h->w, data_dtype, weight, nullptr, nullptr, bias);
 }
 
 int32_t mhsa_fp8_linear_load_codes(mhsa_fp8_linear* h, const uint8_t* codes, const uint8_t* scales, const float* bias) {
   if (!h) return fail(MHSA_EINVAL, "null handle");
   if (!codes) return fail(MHSA_EINVAL, "null weight pointer");
-  if (int32_t rc = load_weights(h->w, MHSA_F32, nullptr, codes, scales, bias)) return rc;
-  HIPCHK(hipGetDevice(&h->device));
-  return MHSA_OK;
+  return load_weights(h->w, MHSA_F32, nullptr, codes, scales, bias);
 }
 
 int32_t mhsa_fp8_linear_read_codes(const mhsa_fp8_linear* h, uint8_t* codes, uint8_t* scales) {
   if (!h) return fail(MHSA_EINVAL, "null handle");
   if (!codes || !scales) return fail(MHSA_EINVAL, "null output pointer");
   if (!h->w.loaded) return fail(MHSA_EINVAL, "no weights are loaded");
-  if (int32_t rc = check_device(h->device)) return rc;
+  if (int32_t rc = check_device(h->w.device)) return rc;
   DevBuf c, s;
   const int64_t n = (int64_t)h->w.N * h->w.K;
   HIPCHK(c.ensure(n));
@@ -266,7 +269,7 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t
   const int64_t xn = ((rows - 1) * x_stride + w.K) * xs, on = ((rows - 1) * out_stride + w.N) * os;
   if (overlap(x, xn, out, on) || overlap(workspace, plan.bytes, x, xn) || overlap(workspace, plan.bytes, out, on))
     return fail(MHSA_EINVAL, "x, out and the workspace must not overlap");
-  if (int32_t rc = check_device(h->device)) return rc;
+  if (int32_t rc = check_device(w.device)) return rc;
   hipStream_t s = static_cast<hipStream_t>(hs);
   mhsa::Fp8Gemm p;
   p.w = static_cast<const uint8_t*>(w.codes.p);
@@ -324,7 +327,7 @@ extern "C" int32_t mhsa_route(const void* logits, int32_t dtype, int32_t rows, i
   if (reinterpret_cast<uintptr_t>(logits) % mhsa::dtype_size(p.dt) || reinterpret_cast<uintptr_t>(indices) % 4 ||
       reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(bias) % 4)
     return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
-  if (rows > kMaxRows || stride > kMaxStride) return fail(MHSA_ENOTSUP, "%d rows %lld apart exceed 2^30", rows, (long long)stride);
+  if (rows > kMaxRows || stride > kMaxStride) return fail(MHSA_ENOTSUP, "%d rows, %lld apart, exceed %d and 2^30", rows, (long long)stride, kMaxRows);
   const int64_t ln = ((rows - 1) * stride + n_experts) * mhsa::dtype_size(p.dt), kn = (int64_t)rows * top_k * 4;
   if (overlap(indices, kn, logits, ln) || overlap(weights, kn, logits, ln) || overlap(indices, kn, weights, kn) ||
       overlap(indices, kn, bias, bias ? n_experts * 4 : 0) || overlap(weights, kn, bias, bias ? n_experts * 4 : 0))
@@ -353,7 +356,6 @@ extern "C" int32_t mhsa_route(const void* logits, int32_t dtype, int32_t rows, i
 struct mhsa_experts {
   Fp8Weights lin[2];  // linear1 [E, F, D], linear2 [E, D, F]
   int E = 0, D = 0, F = 0;
-  int device = -1;
 };
 
 namespace {
@@ -478,8 +480,14 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
   return MHSA_OK;
 }
 
-int32_t experts_loaded(mhsa_experts* h) {
-  HIPCHK(hipGetDevice(&h->device));
+// Both matrices or none: a load that fails halfway leaves no mixture behind.
+int32_t experts_load(mhsa_experts* h, int data_dtype, const void* const weight[2], const uint8_t* const codes[2],
+                     const uint8_t* const scales[2], const void* const bias[2]) {
+  for (int i = 0; i < 2; ++i)
+    if (int32_t rc = load_weights(h->lin[i], data_dtype, weight[i], codes[i], scales[i], bias[i])) {
+      if (i == 1) h->lin[0].loaded = false;
+      return rc;
+    }
   return MHSA_OK;
 }
 
@@ -517,18 +525,18 @@ int32_t mhsa_experts_load(mhsa_experts* h, int32_t data_dtype, const void* weigh
                           const void* weight2, const void* bias2) {
   if (!h) return fail(MHSA_EINVAL, "null handle");
   if (!weight1 || !weight2) return fail(MHSA_EINVAL, "null weight pointer");
-  if (int32_t rc = load_weights(h->lin[0], data_dtype, weight1, nullptr, nullptr, bias1)) return rc;
-  if (int32_t rc = load_weights(h->lin[1], data_dtype, weight2, nullptr, nullptr, bias2)) return rc;
-  return experts_loaded(h);
+  const void *weight[2] = {weight1, weight2}, *bias[2] = {bias1, bias2};
+  const uint8_t* none[2] = {};
+  return experts_load(h, data_dtype, weight, none, none, bias);
 }
 
 int32_t mhsa_experts_load_codes(mhsa_experts* h, const uint8_t* codes1, const uint8_t* scales1, const float* bias1,
                                 const uint8_t* codes2, const uint8_t* scales2, const float* bias2) {
   if (!h) return fail(MHSA_EINVAL, "null handle");
   if (!codes1 || !codes2) return fail(MHSA_EINVAL, "null weight pointer");
-  if (int32_t rc = load_weights(h->lin[0], MHSA_F32, nullptr, codes1, scales1, bias1)) return rc;
-  if (int32_t rc = load_weights(h->lin[1], MHSA_F32, nullptr, codes2, scales2, bias2)) return rc;
-  return experts_loaded(h);
+  const void *none[2] = {}, *bias[2] = {bias1, bias2};
+  const uint8_t *codes[2] = {codes1, codes2}, *scales[2] = {scales1, scales2};
+  return experts_load(h, MHSA_F32, none, codes, scales, bias);
 }
 
 int64_t mhsa_experts_workspace(const mhsa_experts* h, int32_t rows, int32_t top_k) {
@@ -564,7 +572,7 @@ int32_t mhsa_experts_forward(const mhsa_experts* h, const void* x, int32_t dtype
     if (t && overlap(workspace, plan.bytes, t, n)) return fail(MHSA_EINVAL, "the workspace must not overlap a tensor");
   if (overlap(workspace, plan.bytes, indices, np) || overlap(workspace, plan.bytes, weights, np))
     return fail(MHSA_EINVAL, "the workspace must not overlap a tensor");
-  if (int32_t rc = check_device(h->device)) return rc;
+  if (int32_t rc = check_device(h->lin[0].device)) return rc;
   for (int64_t r = 0; r < rows; r += plan.step) {
     const int64_t m = std::min<int64_t>(plan.step, rows - r), at = r * h->D * es;
     const int32_t rc = experts_run(h, plan, static_cast<const char*>(x) + at, dt, m, indices + r * top_k,

@@ -957,12 +957,16 @@ bool bad_gemm(const Fp8Gemm& p) {
 hipError_t fp8_quantize_rows(DType dt, const void* x, int64_t ldx, int64_t rows, int K, uint8_t* codes,
                              uint8_t* scales, hipStream_t s) {
   if (rows <= 0 || K <= 0 || K > kFp8MaxK) return hipErrorInvalidValue;
-  const int64_t items = rows * (fp8_kbp(K) / 4), grid = (items + 3) / 4;
-  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-  if (dt == kBF16)
-    quantize_rows_kernel<bf16><<<(unsigned)grid, 256, 0, s>>>(static_cast<const bf16*>(x), ldx, rows, K, codes, scales);
-  else
-    quantize_rows_kernel<float><<<(unsigned)grid, 256, 0, s>>>(static_cast<const float*>(x), ldx, rows, K, codes, scales);
+  const int64_t per = fp8_kbp(K) / 4, most = ((int64_t)1 << 25) / per;  // (a grid's threads fit 32 bits)
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t m = std::min(most, rows - r);
+    const unsigned grid = (unsigned)((m * per + 3) / 4);
+    uint8_t *c = codes + r * fp8_kp(K), *sc = scales + r * fp8_kbp(K);
+    if (dt == kBF16)
+      quantize_rows_kernel<bf16><<<grid, 256, 0, s>>>(static_cast<const bf16*>(x) + r * ldx, ldx, m, K, c, sc);
+    else
+      quantize_rows_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(x) + r * ldx, ldx, m, K, c, sc);
+  }
   return hipGetLastError();
 }
 

@@ -605,9 +605,11 @@ def _rows_of(x, width: int):
     import torch
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1 or x.shape[-1] != width:
         raise MhsaError(MHSA_EINVAL, f"expected a GPU tensor [..., {width}]")
+    rows = x.numel() // width if width else 0
+    if not width or rows > 0x7FFFFFFF:
+        raise MhsaError(MHSA_ENOTSUP if width else MHSA_EINVAL, f"{rows} rows of {width} elements")
     if x.is_contiguous():
-        return x.numel() // width, width
-    rows = x.numel() // width
+        return rows, width
     lead = [(n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
     if rows and (x.stride(-1) == 1 or width == 1):
         if not lead:
@@ -699,7 +701,7 @@ def route(logits, top_k: int, score: str = "softmax", bias=None, n_groups: int =
     idx = logits.new_empty(shape, dtype=torch.int32)
     w = logits.new_empty(shape, dtype=torch.float32)
     _launch(logits, library().mhsa_route, logits.data_ptr(), _act_code(logits.dtype), rows, n, ld, ROUTE_SCORES[score],
-            None if bias is None else bias.data_ptr(), n_groups, topk_groups, top_k, 1 if renormalize else 0, scale,
+            None if bias is None else bias.data_ptr(), n_groups, topk_groups, top_k, 1 if renormalize else 0, float(scale),
             idx.data_ptr(), w.data_ptr())
     return idx, w
 
@@ -752,7 +754,7 @@ class ExpertFeedForward:
         top_k = indices.shape[-1] if indices.dim() else 0
         lead = x.shape[:-1]
         for t, want, name in ((indices, torch.int32, "indices"), (weights, torch.float32, "weights")):
-            if (t.dtype != want or t.get_device() != x.get_device() or not t.is_contiguous() or t.shape[:-1] != lead
+            if (not t.dim() or t.dtype != want or t.get_device() != x.get_device() or not t.is_contiguous() or t.shape[:-1] != lead
                     or t.shape[-1] != top_k):
                 raise MhsaError(MHSA_EINVAL, f"{name}: expected contiguous {want} [..., top_k] beside x")
         for t in (residual, out):
@@ -762,10 +764,12 @@ class ExpertFeedForward:
         if out is None:
             out = torch.empty_like(x)
         rows = x.numel() // self.d_model
+        if rows > 0x7FFFFFFF:
+            raise MhsaError(MHSA_ENOTSUP, f"{rows} rows")
         need = self._lib.mhsa_experts_workspace(self._h, rows, top_k)
         ws = x.new_empty(max(need, 0), dtype=torch.uint8)
         _launch(x, self._lib.mhsa_experts_forward, self._h, x.data_ptr(), dtype, rows, indices.data_ptr(), weights.data_ptr(),
-                top_k, None if residual is None else residual.data_ptr(), res_scale, out.data_ptr(), ws.data_ptr(),
+                top_k, None if residual is None else residual.data_ptr(), float(res_scale), out.data_ptr(), ws.data_ptr(),
                 max(need, 0))
         return out
 

@@ -50,7 +50,7 @@ def experts(e=4, d=128, f=256, bias=0):
 def test_create_refuses():
     lib, h = M.library(), ctypes.c_void_p()
     for args, code in (((0, 8, 0), M.MHSA_EINVAL), ((8, -1, 0), M.MHSA_EINVAL), ((32769, 8, 0), M.MHSA_ENOTSUP),
-                       ((32768, 1 << 20, 0), M.MHSA_ENOTSUP)):
+                       ((32768, 1 << 20, 0), M.MHSA_ENOTSUP), ((8, (1 << 22) + 1, 0), M.MHSA_ENOTSUP)):
         assert lib.mhsa_fp8_linear_create(*args, ctypes.byref(h)) == code and not h.value
     assert lib.mhsa_fp8_linear_create(8, 8, 0, None) == M.MHSA_EINVAL
     for args, code in (((0, 64, 64, 0), M.MHSA_EINVAL), ((2, 65, 64, 0), M.MHSA_EINVAL), ((2, 64, 0, 0), M.MHSA_EINVAL),
@@ -88,7 +88,7 @@ def test_linear_forward_refuses():
     f = lib.mhsa_fp8_linear_forward
     assert f(None, SOME, M.F32, 1, 256, SOME, M.F32, 384, None, 0, None) == M.MHSA_EINVAL
     for args in ((SOME, M.F16, 1, 256, SOME, M.F32, 384), (SOME, M.F32, 1, 256, SOME, M.U32, 384),
-                 (SOME, M.F32, (1 << 30) + 1, 256, SOME, M.F32, 384), (SOME, M.F32, 2, (1 << 30) + 1, SOME, M.F32, 384),
+                 (SOME, M.F32, (1 << 25) + 1, 256, SOME, M.F32, 384), (SOME, M.F32, 2, (1 << 30) + 1, SOME, M.F32, 384),
                  (SOME, M.F32, 2, 256, SOME, M.F32, (1 << 30) + 1)):
         assert f(h, *args, None, 0, None) == M.MHSA_ENOTSUP
     for args in ((SOME, M.F32, -1, 256, SOME, M.F32, 384), (None, M.F32, 1, 256, SOME, M.F32, 384),
@@ -113,7 +113,7 @@ def test_route_refuses():
         return f(a["x"], a["dt"], a["rows"], a["e"], a["ld"], a["score"], a["bias"], a["g"], a["kg"], a["k"], a["rn"],
                  a["s"], a["i"], a["w"], None)
     for more in (dict(dt=M.F16), dict(score=2), dict(e=520, ld=520, g=1, kg=1), dict(e=130, ld=130, g=65), dict(e=512, ld=512, g=1, kg=1, k=33),
-                 dict(rows=(1 << 30) + 1), dict(ld=(1 << 30) + 1)):
+                 dict(rows=(1 << 25) + 1), dict(ld=(1 << 30) + 1)):
         assert call(**more) == M.MHSA_ENOTSUP, more
     for more in (dict(rows=-1), dict(e=0), dict(g=0), dict(g=7), dict(kg=0), dict(kg=9), dict(k=0), dict(k=33), dict(ld=63),
                  dict(s=float("nan")), dict(s=float("inf")), dict(x=None), dict(i=None), dict(w=None), dict(x=SOME + 2),
@@ -141,8 +141,8 @@ def test_experts_forward_refuses():
         assert f(h, *args, ws, big, None) == M.MHSA_EINVAL, args
     assert b"no weights" in lib.mhsa_last_error()
     assert f(h, None, M.F32, 0, None, None, 2, None, 1.0, None, None, 0, None) == M.MHSA_OK
-    assert f(h, x, M.F32, (1 << 30) + 1, idx, w, 2, r, 1.0, out, ws, big, None) == M.MHSA_ENOTSUP
-    assert lib.mhsa_experts_workspace(h, (1 << 30) + 1, 2) == -1
+    assert f(h, x, M.F32, (1 << 25) + 1, idx, w, 2, r, 1.0, out, ws, big, None) == M.MHSA_ENOTSUP
+    assert lib.mhsa_experts_workspace(h, (1 << 25) + 1, 2) == -1
     assert lib.mhsa_experts_workspace(h, 5, 0) == -1 and lib.mhsa_experts_workspace(h, -5, 2) == -1
     assert lib.mhsa_experts_workspace(h, 0, 2) == 0 and lib.mhsa_experts_workspace(h, 5, 2) > 0
     # rows run in parts, so the workspace stops growing

@@ -199,6 +199,22 @@ def test_empty_shapes_and_refusals():
         layer.forward(x, idx, w, residual=buf[:12], out=buf[6:18])
 
 
+def test_a_load_that_fails_halfway_leaves_no_mixture():
+    rng = np.random.default_rng(11)
+    parts = make(rng, 3, 128, 64, True)
+    layer, x = parts[0], frames(rng, 4, 128, "bf16")
+    idx, w = (torch.from_numpy(a).cuda() for a in choose(rng, 4, 3, 2))
+    w1, w2, b1 = torch.randn(3, 64, 128), torch.randn(3, 128, 64), torch.zeros(3, 64)
+    assert M.library().mhsa_experts_load(layer._h, M.F32, w1.data_ptr(), b1.data_ptr(), w2.data_ptr(), None) == M.MHSA_EINVAL
+    with pytest.raises(M.MhsaError):
+        layer.forward(x, idx, w)
+    layer.load(w1, w2, b1, torch.zeros(3, 128))
+    assert torch.isfinite(layer.forward(x, idx, w)).all()
+    none = torch.zeros((), dtype=torch.int32, device="cuda")
+    with pytest.raises(M.MhsaError):
+        layer.forward(x[0], none, none.float())
+
+
 def test_replayed_graphs_and_streams():
     rng = np.random.default_rng(7)
     parts = make(rng, 4, 128, 256, True)

@@ -87,6 +87,17 @@ def test_strided_rows_shapes_and_no_rows():
         M.route(wide.half(), 3)
 
 
+def test_refusals():
+    x = torch.zeros(3, 8, device="cuda")
+    for bad, kw in ((x[:, :0], {}), (x.double(), {}), (x.cpu(), {}), (x[0, 0], {}), (x, {"score": "tanh"}), (x, {"n_groups": 3}),
+                    (x, {"bias": torch.zeros(7, device="cuda")}), (x, {"bias": torch.zeros(8)}), (x.T, {}), (x, {"scale": float("inf")})):
+        with pytest.raises(M.MhsaError):
+            M.route(bad, 2, **kw)
+    for top_k in (0, -1, 9):
+        with pytest.raises(M.MhsaError):
+            M.route(x, top_k)
+
+
 def test_replayed_graph():
     rng = np.random.default_rng(8)
     x = torch.from_numpy(rng.standard_normal((5, 77, 64)).astype(np.float32)).cuda()
