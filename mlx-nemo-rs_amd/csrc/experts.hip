@@ -18,43 +18,47 @@ namespace {
 // differ by less than f32 resolves, and the choice between them is then not a
 // matter of the order of a sum.
 //
-// One wave per row, expert e in lane e % 64. What is bound here is not the
-// logits' bytes but the wave's reductions, so they are DPP moves and lane
-// reads, which the vector unit does itself, and a choice reduces one 32-bit
-// word: a score's f32 rounding, which keeps the order. Only lanes that share
-// the largest word are compared in 64 bits. (With shuffles of 64-bit values,
-// which go through LDS, 30001 rows of 256 experts in 8 groups took 88 us.)
+// One wave per row, expert e in lane e % 64 (many rows: four to a wave). What
+// is bound here is not the logits' bytes but the wave's instructions, half of
+// them the scores' exponentials in 64 bits and half the reductions. These are
+// DPP moves and lane reads, which the vector unit does itself, and a choice
+// reduces one 32-bit word: a score's f32 rounding, which keeps the order. Only
+// lanes that share the largest word are compared in 64 bits. (With shuffles of
+// 64-bit values, which go through LDS, 30001 rows of 256 experts in 8 groups
+// took 88 us, with these 45, with four rows to a wave 31: 1 TB/s.)
 // ---------------------------------------------------------------------------
 
 constexpr double kNone = -__builtin_inf();
 
-// The value of lane 63 after o(o(...)) over the wave's rows of 16 lanes, then
-// over the rows: `o` combines a lane's value with a neighbour's; lanes without
-// a neighbour keep theirs.
-template <typename T, typename O>
-__device__ __forceinline__ T wave_reduce(T v, O o) {
-  auto move = [](T x, auto ctrl, auto rows) {
-    constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+// Each row of 16 lanes' values under `o`, in all of the row's lanes: the first
+// N steps of: lanes xor 1, xor 2 (quad permutations), half rows and rows
+// mirrored.
+template <int N = 4, typename T, typename O>
+__device__ __forceinline__ T row_reduce(T v, O o) {
+  auto move = [](T x, auto ctrl) {
+    constexpr int C = decltype(ctrl)::value;
     if constexpr (sizeof(T) == 4) {
       const int u = __builtin_bit_cast(int, x);
-      return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(u, u, C, R, 0xF, false));
+      return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(u, u, C, 0xF, 0xF, false));
     } else {
       typedef int i32x2 __attribute__((ext_vector_type(2)));
       i32x2 u = __builtin_bit_cast(i32x2, x);
-      u[0] = __builtin_amdgcn_update_dpp(u[0], u[0], C, R, 0xF, false);
-      u[1] = __builtin_amdgcn_update_dpp(u[1], u[1], C, R, 0xF, false);
+      u[0] = __builtin_amdgcn_update_dpp(u[0], u[0], C, 0xF, 0xF, false);
+      u[1] = __builtin_amdgcn_update_dpp(u[1], u[1], C, 0xF, 0xF, false);
       return __builtin_bit_cast(T, u);
     }
   };
   using std::integral_constant;
-  constexpr auto all = integral_constant<int, 0xF>{};
-  // lanes xor 1, xor 2 (quad permutations), then half rows and rows mirrored:
-  // every lane of a row of 16 has the row's result
-  v = o(v, move(v, integral_constant<int, 0xB1>{}, all));
-  v = o(v, move(v, integral_constant<int, 0x4E>{}, all));
-  v = o(v, move(v, integral_constant<int, 0x141>{}, all));
-  v = o(v, move(v, integral_constant<int, 0x140>{}, all));
-  // four rows: one lane of each
+  if constexpr (N > 0) v = o(v, move(v, integral_constant<int, 0xB1>{}));
+  if constexpr (N > 1) v = o(v, move(v, integral_constant<int, 0x4E>{}));
+  if constexpr (N > 2) v = o(v, move(v, integral_constant<int, 0x141>{}));
+  if constexpr (N > 3) v = o(v, move(v, integral_constant<int, 0x140>{}));
+  return v;
+}
+// The wave's: one lane of each row.
+template <typename T, typename O>
+__device__ __forceinline__ T wave_reduce(T v, O o) {
+  v = row_reduce(v, o);
   auto at = [&](int l) {
     if constexpr (sizeof(T) == 4) {
       return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
@@ -217,6 +221,152 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   if (lane < p.top_k) {
     p.idx[row * p.top_k + lane] = idx;
     p.w[row * p.top_k + lane] = (float)(wj * (double)p.scale);
+  }
+}
+
+// Many rows: four to a wave, 16 lanes each, expert e in lane e / per of them
+// (per = experts / 16, rounded up). A choice's reduction then serves four rows
+// and stays within 16 lanes; the lanes of a group are neighbours, so its two
+// best need no exchange through LDS. For up to 256 experts, 16 choices, and
+// groups that take whole lanes.
+template <typename T, int EPL>
+__global__ __launch_bounds__(256) void route_rows_kernel(RouteParams p) {
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15;
+  const int64_t first = ((int64_t)blockIdx.x * 4 + wv) * 4;
+  if (first >= p.rows) return;  // (waves do not wait for each other)
+  const int64_t row = first + (lane >> 4);
+  const int per = (p.experts + 15) / 16, e0 = l * per;
+  const T* xr = reinterpret_cast<const T*>(p.logits) + (row < p.rows ? row : p.rows - 1) * p.ld;
+  const T* x = xr + e0;
+  const float none = -__builtin_inff();
+  float v[EPL];
+  if (p.experts == 16 * EPL) {
+    T run[EPL];
+    __builtin_memcpy(run, x, sizeof run);  // (rows may lie at any address)
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) v[i] = (float)run[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) v[i] = i < per && e0 + i < p.experts ? (float)x[i] : none;
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) v[i] = v[i] > none ? v[i] : none;  // (a NaN is no score)
+  double c[EPL], top = 0.0, inv = 0.0;
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) c[i] = inverse(1.0 + exp(-(double)v[i]));
+  } else {
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, v[i]);
+    mx = row_reduce(mx, [](float a, float b) { return fmaxf(a, b); });
+    top = mx > none ? (double)mx : 0.0;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const double e = exp((double)v[i] - top);
+      c[i] = (double)v[i] == top ? 1.0 : e;
+      sum += c[i];
+    }
+    sum = row_reduce(sum, [](double a, double b) { return a + b; });
+    inv = sum > 0.0 ? inverse(sum) : 0.0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) c[i] *= inv;
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const double t = p.bias && i < per && e0 + i < p.experts ? c[i] + (double)p.bias[e0 + i] : c[i];
+    c[i] = v[i] > none && t > kNone ? t : kNone;
+  }
+  bool kept = true;
+  if (p.groups > 1) {
+    const int lanes = 16 / p.groups, g = l / lanes;
+    double a = kNone, b = kNone;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      b = fmax(b, fmin(a, c[i]));
+      a = fmax(a, c[i]);
+    }
+    auto join = [&](auto n) {  // with the lane that the n-th step of a reduction takes
+      double a2 = a, b2 = b;
+      constexpr int N = decltype(n)::value;
+      auto move = [](double u) {
+        constexpr int C = N == 0 ? 0xB1 : N == 1 ? 0x4E : 0x141;
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        i32x2 w = __builtin_bit_cast(i32x2, u);
+        w[0] = __builtin_amdgcn_update_dpp(w[0], w[0], C, 0xF, 0xF, false);
+        w[1] = __builtin_amdgcn_update_dpp(w[1], w[1], C, 0xF, 0xF, false);
+        return __builtin_bit_cast(double, w);
+      };
+      a2 = move(a);
+      b2 = move(b);
+      b = fmax(fmin(a, a2), fmax(b, b2));
+      a = fmax(a, a2);
+    };
+    using std::integral_constant;
+    if (lanes > 1) join(integral_constant<int, 0>{});
+    if (lanes > 2) join(integral_constant<int, 1>{});
+    if (lanes > 4) join(integral_constant<int, 2>{});
+    const double best = b > kNone ? a + b : a;
+    int before = 0;  // groups ahead of this lane's
+    for (int o = 0; o < p.groups; ++o) {
+      const double u = __shfl(best, (lane & 48) | o * lanes, 64);
+      before += u > best || (u == best && o < g) ? 1 : 0;
+    }
+    kept = before < p.topk_groups;
+  }
+  uint32_t word[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) word[i] = kept ? rank_word(c[i]) : 0;
+  constexpr uint32_t kNobody = 0xFFFFFFFF;  // (no value's word)
+  uint32_t idx = kNobody;
+  for (int j = 0; j < p.top_k; ++j) {
+    uint32_t most = word[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) most = max(most, word[i]);
+    most = row_reduce(most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    const int rows = __popcll(__ballot(most != 0)) / 16;
+    if (rows == 0) break;
+    most = most ? most : kNobody;
+    // who has it: one of a row, or several that are alike in f32, of which the
+    // larger in 64 bits, and of equals the lower index
+    int hit = -1, hits = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const bool has = word[i] == most;
+      hits += __popcll(__ballot(has));
+      hit = has ? i : hit;
+    }
+    uint32_t won = hit >= 0 ? (uint32_t)(e0 + hit) : kNobody;
+    if (hits > rows) {
+      double u = kNone;
+      hit = -1;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const bool more = word[i] == most && c[i] > u;
+        u = more ? c[i] : u;
+        hit = more ? i : hit;
+      }
+      const double top = row_reduce(u, [](double a, double b) { return fmax(a, b); });
+      won = hit >= 0 && u == top ? (uint32_t)(e0 + hit) : kNobody;
+    }
+    won = row_reduce(won, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+    const int mine = (int)(won - (uint32_t)e0);  // (another lane's: outside 0 .. per - 1)
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) word[i] = mine == i && i < per ? 0 : word[i];
+    idx = l == j ? won : idx;
+  }
+  // the chosen expert's score again, as above: less than to keep all of them
+  const double t = (double)(float)xr[idx != kNobody ? idx : 0];
+  double wj = p.sigmoid ? inverse(1.0 + exp(-t)) : (t == top ? 1.0 : exp(t - top)) * inv;
+  wj = idx != kNobody ? wj : 0.0;
+  if (p.renormalize) {
+    const double total = row_reduce(wj, [](double a, double b) { return a + b; });
+    wj = total > 0.0 ? wj / total : 0.0;
+  }
+  if (l < p.top_k && row < p.rows) {
+    p.idx[row * p.top_k + l] = (int)idx;
+    p.w[row * p.top_k + l] = (float)(wj * (double)p.scale);
   }
 }
 
@@ -388,9 +538,18 @@ hipError_t route(const RouteParams& p, hipStream_t s) {
     return hipErrorInvalidValue;
   const int64_t grid = (p.rows + 3) / 4;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  // Four rows to a wave where there are enough of them: 8000 rows of 256 experts
+  // in 8 groups 15.9 -> 13.6 us, 30001 45.5 -> 31.4; of 64 experts 4.9 -> 4.7 and
+  // 12.2 -> 9.4. At 4000 rows a wave's longer way weighs more (10.3 against
+  // 11.2, 3.6 against 4.2).
+  const bool many = p.rows >= 6144 && p.experts <= 256 && p.top_k <= 16 &&
+                    (p.groups == 1 || (16 % p.groups == 0 && p.experts % 16 == 0));
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (p.experts <= 64) route_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
+    if (many && p.experts <= 64) route_rows_kernel<T, 4><<<(unsigned)((p.rows + 15) / 16), 256, 0, s>>>(p);
+    else if (many && p.experts <= 128) route_rows_kernel<T, 8><<<(unsigned)((p.rows + 15) / 16), 256, 0, s>>>(p);
+    else if (many) route_rows_kernel<T, 16><<<(unsigned)((p.rows + 15) / 16), 256, 0, s>>>(p);
+    else if (p.experts <= 64) route_kernel<T, 1><<<(unsigned)grid, 256, 0, s>>>(p);
     else if (p.experts <= 128) route_kernel<T, 2><<<(unsigned)grid, 256, 0, s>>>(p);
     else if (p.experts <= 256) route_kernel<T, 4><<<(unsigned)grid, 256, 0, s>>>(p);
     else route_kernel<T, 8><<<(unsigned)grid, 256, 0, s>>>(p);

@@ -64,6 +64,61 @@ def test_ties_masks_and_extremes(score, groups, kept):
             assert (idx[1] == -1).all() and (w[1] == 0).all() and (idx[6] == -1).all()
 
 
+ROWS_CASES = [(256, 8, 8, 4), (256, 8, 1, 1), (64, 4, 1, 1), (128, 6, 4, 2), (16, 2, 1, 1), (60, 4, 1, 1), (160, 6, 8, 3),
+              (5, 3, 1, 1), (64, 16, 16, 8), (16, 3, 16, 5), (112, 9, 2, 1), (250, 16, 1, 1), (48, 17, 1, 1), (96, 4, 3, 2)]
+
+
+@pytest.mark.parametrize("experts,top_k,groups,kept", ROWS_CASES)
+@pytest.mark.parametrize("score,dtype", [("softmax", torch.float32), ("sigmoid", torch.bfloat16), ("sigmoid", torch.float32)])
+def test_many_rows(experts, top_k, groups, kept, score, dtype):
+    """6157 rows, at an odd distance: 300 of them and the last ones against the
+    oracle, all against the same rows in smaller calls."""
+    rng = np.random.default_rng(experts + top_k)
+    wide = torch.from_numpy((2 * rng.standard_normal((6157, experts + 3))).astype(np.float32)).to(dtype).cuda()
+    x = wide[:, 1:1 + experts]
+    bias = (0.1 * rng.standard_normal(experts)).astype(np.float32)
+    kw = dict(score=score, n_groups=groups, topk_groups=kept, renormalize=top_k % 2 == 0, scale=1.5)
+    at = np.unique(np.concatenate([rng.integers(0, 6157, 300), np.arange(6130, 6157)]))
+    for b in (None, bias):
+        t = None if b is None else torch.from_numpy(b).cuda()
+        idx, w = M.route(x, top_k, bias=t, **kw)
+        want_i, want_w = F.route(x.float().cpu().numpy()[at], top_k, bias=b, **kw)
+        assert np.array_equal(idx.cpu().numpy()[at], want_i)
+        assert (np.abs(w.double().cpu().numpy()[at] - want_w) <= 2.0 ** -24 * np.abs(want_w) * (1 + 1e-9) + 2.0 ** -149).all()
+        parts = [M.route(x[i:i + 2053], top_k, bias=t, **kw) for i in range(0, 6157, 2053)]
+        assert torch.equal(idx, torch.cat([p[0] for p in parts]))
+        # (sums of 64-bit scores in another order, so an f32 rounding may differ)
+        assert ((w - torch.cat([p[1] for p in parts])).abs() <= 2.0 ** -23 * w.abs()).all()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,kept", [(1, 1), (4, 2), (16, 7)])
+def test_many_rows_with_ties_masks_and_extremes(score, groups, kept):
+    rng = np.random.default_rng(6)
+    x = rng.integers(-2, 3, (48, 64)).astype(np.float32)  # many ties
+    x[1] = -np.inf
+    x[2], x[2, 17] = -np.inf, 3.0
+    x[3, ::2] = -np.inf
+    x[4] = np.finfo(np.float32).min
+    x[5, 10], x[6] = np.nan, np.nan
+    x[7, 20], x[7, 40] = np.inf, np.inf
+    x[8] = 0.0
+    x[9, :32] = -np.inf
+    x[10, 1:] = -1000.0
+    x[11] = 1000.0
+    x[12:16] = np.nextafter(np.float32(0.5), np.float32(1))  # next to 0.5: alike in f32, not in 64 bits
+    x[12:16, 1::3] = 0.5
+    hidden = np.zeros(64, np.float32)
+    hidden[::3], hidden[5], hidden[33], hidden[34] = 0.25, -np.inf, np.nan, np.inf
+    for b in (None, hidden):
+        want_i, want_w = F.route(x, 4, bias=b, score=score, n_groups=groups, topk_groups=kept, renormalize=True)
+        idx, w = M.route(torch.from_numpy(np.tile(x, (130, 1))).cuda(), 4, bias=None if b is None else torch.from_numpy(b).cuda(),
+                         score=score, n_groups=groups, topk_groups=kept, renormalize=True)
+        idx, w = idx.cpu().numpy().reshape(130, 48, 4), w.double().cpu().numpy().reshape(130, 48, 4)
+        assert (idx == want_i).all()
+        assert (np.abs(w - want_w) <= 2.0 ** -24 * np.abs(want_w) * (1 + 1e-9) + 2.0 ** -149).all()
+
+
 def test_near_scores_are_told_apart():
     """Sigmoid scores whose difference f32 rounds away."""
     x = np.full((4, 16), 12.0, np.float32)
