@@ -25,7 +25,8 @@ namespace {
 // reduces one 32-bit word: a score's f32 rounding, which keeps the order. Only
 // lanes that share the largest word are compared in 64 bits. (With shuffles of
 // 64-bit values, which go through LDS, 30001 rows of 256 experts in 8 groups
-// took 88 us, with these 45, with four rows to a wave 31: 1 TB/s.)
+// took 88 us, with these 44, with four rows to a wave 29: 1.1 TB/s, and 423
+// vector instructions a row, which the unit issues in 71% of the time.)
 // ---------------------------------------------------------------------------
 
 constexpr double kNone = -__builtin_inf();
@@ -83,12 +84,36 @@ __device__ __forceinline__ double inverse(double d) {
   r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
   return d < __builtin_inf() ? r : 0.0;
 }
+// e^x for |x| <= 800 to within 2 ulp: e^x = 2^k e^r, |r| <= ln 2 / 2, by the
+// series up to r^12 (the rest is under 2^-52). The range is the callers' to
+// keep, with one instruction, and takes the special cases off the way: beyond
+// it e^x is infinity or 0 in 64 bits.
+__device__ __forceinline__ double exp_within(double x) {
+  const double k = __builtin_rint(x * 1.4426950408889634);
+  // ln 2 in two parts, the first of 32 bits, so that its product with k is exact
+  double r = __builtin_fma(k, -0x1.62e42fefp-1, x);
+  r = __builtin_fma(k, -0x1.473de6af278edp-34, r);
+  double e = 1.0 / 479001600.0;
+  constexpr double c[12] = {1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0,
+                            1.0 / 120.0,      1.0 / 24.0,      1.0 / 6.0,      0.5,           1.0,          1.0};
+#pragma unroll
+  for (int i = 0; i < 12; ++i) e = __builtin_fma(e, r, c[i]);
+  return __builtin_ldexp(e, (int)k);
+}
+__device__ __forceinline__ double sigmoid(float v) {
+  return inverse(1.0 + exp_within(-(double)__builtin_amdgcn_fmed3f(v, -800.f, 800.f)));
+}
+// e^(v - top), 1 also for infinities that are equal
+__device__ __forceinline__ double exp_below(float v, double top) {
+  const double e = exp_within(fmax((double)v - top, -800.0));
+  return (double)v == top ? 1.0 : e;
+}
 // The order of values as unsigned words, 0 for none (-inf itself is 0x7FFFFF,
 // and no value's word is 0).
 __device__ __forceinline__ uint32_t rank_word(double v) {
   if (!(v > kNone)) return 0;
   const uint32_t u = __builtin_bit_cast(uint32_t, (float)v);
-  return u >> 31 ? ~u : u | 0x80000000u;
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 
 template <typename T, int EPL>
@@ -108,7 +133,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   }
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) s[i] = inverse(1.0 + exp(-(double)v[i]));  // (-inf: e^inf gives 0)
+    for (int i = 0; i < EPL; ++i) s[i] = sigmoid(v[i]);
   } else {
     float mx = v[0];
 #pragma unroll
@@ -118,8 +143,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const double e = exp((double)v[i] - top);  // (0 for -inf)
-      s[i] = (double)v[i] == top ? 1.0 : e;      // (of infinities too)
+      s[i] = exp_below(v[i], top);
       sum += s[i];
     }
     sum = wave_reduce(sum, [](double a, double b) { return a + b; });
@@ -254,7 +278,7 @@ __global__ __launch_bounds__(256) void route_rows_kernel(RouteParams p) {
   double c[EPL], top = 0.0, inv = 0.0;
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) c[i] = inverse(1.0 + exp(-(double)v[i]));
+    for (int i = 0; i < EPL; ++i) c[i] = sigmoid(v[i]);
   } else {
     float mx = v[0];
 #pragma unroll
@@ -264,8 +288,7 @@ __global__ __launch_bounds__(256) void route_rows_kernel(RouteParams p) {
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const double e = exp((double)v[i] - top);
-      c[i] = (double)v[i] == top ? 1.0 : e;
+      c[i] = exp_below(v[i], top);
       sum += c[i];
     }
     sum = row_reduce(sum, [](double a, double b) { return a + b; });
@@ -331,11 +354,13 @@ __global__ __launch_bounds__(256) void route_rows_kernel(RouteParams p) {
     // who has it: one of a row, or several that are alike in f32, of which the
     // larger in 64 bits, and of equals the lower index
     int hit = -1, hits = 0;
+    bool has[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const bool has = word[i] == most;
-      hits += __popcll(__ballot(has));
-      hit = has ? i : hit;
+      has[i] = word[i] == most;
+      hits += __popcll(__ballot(has[i]));
+      hit = has[i] ? i : hit;
+      word[i] = has[i] ? 0 : word[i];
     }
     uint32_t won = hit >= 0 ? (uint32_t)(e0 + hit) : kNobody;
     if (hits > rows) {
@@ -343,22 +368,23 @@ __global__ __launch_bounds__(256) void route_rows_kernel(RouteParams p) {
       hit = -1;
 #pragma unroll
       for (int i = 0; i < EPL; ++i) {
-        const bool more = word[i] == most && c[i] > u;
+        const bool more = has[i] && c[i] > u;
         u = more ? c[i] : u;
         hit = more ? i : hit;
       }
-      const double top = row_reduce(u, [](double a, double b) { return fmax(a, b); });
-      won = hit >= 0 && u == top ? (uint32_t)(e0 + hit) : kNobody;
+      const double best = row_reduce(u, [](double a, double b) { return fmax(a, b); });
+      won = hit >= 0 && u == best ? (uint32_t)(e0 + hit) : kNobody;
     }
     won = row_reduce(won, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-    const int mine = (int)(won - (uint32_t)e0);  // (another lane's: outside 0 .. per - 1)
+    if (hits > rows) {  // the others are still to be chosen
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) word[i] = mine == i && i < per ? 0 : word[i];
+      for (int i = 0; i < EPL; ++i) word[i] = has[i] && won != (uint32_t)(e0 + i) ? most : word[i];
+    }
     idx = l == j ? won : idx;
   }
   // the chosen expert's score again, as above: less than to keep all of them
-  const double t = (double)(float)xr[idx != kNobody ? idx : 0];
-  double wj = p.sigmoid ? inverse(1.0 + exp(-t)) : (t == top ? 1.0 : exp(t - top)) * inv;
+  const float t = (float)xr[idx != kNobody ? idx : 0];
+  double wj = p.sigmoid ? sigmoid(t) : exp_below(t, top) * inv;
   wj = idx != kNobody ? wj : 0.0;
   if (p.renormalize) {
     const double total = row_reduce(wj, [](double a, double b) { return a + b; });
@@ -539,9 +565,9 @@ hipError_t route(const RouteParams& p, hipStream_t s) {
   const int64_t grid = (p.rows + 3) / 4;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   // Four rows to a wave where there are enough of them: 8000 rows of 256 experts
-  // in 8 groups 15.9 -> 13.6 us, 30001 45.5 -> 31.4; of 64 experts 4.9 -> 4.7 and
-  // 12.2 -> 9.4. At 4000 rows a wave's longer way weighs more (10.3 against
-  // 11.2, 3.6 against 4.2).
+  // in 8 groups 15.4 -> 12.3 us, 30001 44.4 -> 29.4; of 64 experts 4.8 -> 4.4 and
+  // 12.3 -> 9.1. Of fewer rows a wave's longer way weighs more (3000: 8.9 against
+  // 10.0 and 3.2 against 3.9).
   const bool many = p.rows >= 6144 && p.experts <= 256 && p.top_k <= 16 &&
                     (p.groups == 1 || (16 % p.groups == 0 && p.experts % 16 == 0));
   auto go = [&](auto t) {
