@@ -117,6 +117,34 @@ def test_few_rows_of_many_experts(rows, e, k):
     check(got, x, idx, w, parts)
 
 
+@pytest.mark.parametrize("rows,e", [(1, 2), (14, 2), (60, 2), (250, 1), (900, 64)])
+def test_few_rows_round_hidden_values_from_f32_sums(rows, e):
+    """A second matrix of the identity returns the hidden values' codes: those
+    of a value that is off by at most (K + 64) steps of 2^-24 of its sum's
+    magnitudes (silu's slope is at most 1.1) and 8 of its own."""
+    rng = np.random.default_rng(rows + e)
+    d = 512
+    lin1 = [F.quantize_weight(rng.standard_normal((d, d)) / np.sqrt(d)) for _ in range(e)]
+    one = np.zeros((d, d), np.uint8)
+    one[np.arange(d), np.arange(d)] = 0x38
+    layer = M.ExpertFeedForward(e, d, d, False)
+    layer.load_codes(np.stack([m[0] for m in lin1]), np.stack([m[1] for m in lin1]), np.stack([one] * e),
+                     np.full((e, 4, 4), 127, np.uint8))
+    x, idx = frames(rng, rows, d, "f32"), rng.integers(0, e, (rows, 1)).astype(np.int32)
+    got = host(layer.forward(x, torch.from_numpy(idx).cuda(), torch.ones(rows, 1, device="cuda")))
+    for k in range(e):
+        at = idx[:, 0] == k
+        h, mag = F.linear(host(x)[at], *lin1[k])
+        v = h / (1 + np.exp(-h))
+        err = 1.1 * (d + 64) * 2.0 ** -24 * mag + 8 * 2.0 ** -24 * np.abs(v)
+        for c in range(0, d, 128):
+            b, eb, y = v[:, c:c + 128], err[:, c:c + 128], got[at, c:c + 128]
+            s = [F.scale_byte((np.abs(b) + i * eb).max(1, initial=0))[:, None] - 127 for i in (-1, 1)]
+            same = (s[0] == s[1])[:, 0]  # (a largest value next to a power's edge may take either)
+            lo, hi = (np.ldexp(F.VALUES[F.encode(np.clip(np.ldexp(b + i * eb, -s[0]), -448, 448))], s[0]) for i in (-1, 1))
+            assert ((lo <= y) & (y <= hi))[same].all()
+
+
 @pytest.mark.parametrize("rows", [2, 100, 2000])
 def test_rows_without_experts_are_the_residual(rows):
     rng = np.random.default_rng(1)
