@@ -121,19 +121,19 @@ __device__ __forceinline__ void store_as(DType dt, void* out, int64_t at, float 
   else reinterpret_cast<float*>(out)[at] = v;
 }
 
-// Adds block b's products of RC x 16 weight rows (16 apart, from wrow; this
-// lane's 32 inputs) and the lane's activation row to acc. VEC: rows of whole
+// Adds block b's products of RC x 16 weight rows (at wrow + off; this lane's 32
+// inputs) and the lane's activation row to acc. VEC: rows of whole
 // runs of 8 inputs (the code for others is several times as long, and a launch
 // of a few microseconds pays for fetching it).
 template <typename TX, int RC, bool EXACT, bool VEC>
-__device__ __forceinline__ void few_block(const uint8_t* wrow, int64_t wstep, const uint8_t* wsc, int b, const TX* xrow,
+__device__ __forceinline__ void few_block(const uint8_t* wrow, const int off[RC], const uint8_t* wsc, int b, const TX* xrow,
                                           int K, floatx4 acc[RC]) {
   const int c0 = b * 128 + 32 * ((threadIdx.x & 63) >> 4);
   u32x4 wf[RC][2];
 #pragma unroll
   for (int c = 0; c < RC; ++c)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) wf[c][u] = *reinterpret_cast<const u32x4*>(wrow + c * wstep + b * 128 + 16 * u);
+    for (int u = 0; u < 2; ++u) wf[c][u] = *reinterpret_cast<const u32x4*>(wrow + off[c] + b * 128 + 16 * u);
   const int sw = wsc[b];
   float v[32];
 #pragma unroll
@@ -265,9 +265,10 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
     rows = found.count;
   }
   const int kb = (p.K + 127) / 128, kbp = (kb + 3) / 4 * 4;
-  const int64_t wstep = (int64_t)16 * (kb * 128);
-  // (weight rows past the last repeat rows before them; their columns are not stored)
-  const uint8_t* wrow = p.w + expert * p.w_stride + (int64_t)min(n0 + r, p.N - 1 - 16 * (RC - 1)) * (kb * 128) + 32 * c4;
+  const uint8_t* wrow = p.w + expert * p.w_stride + 32 * c4;
+  int off[RC];  // (a matrix's codes are under 2 GiB; rows past the last repeat it, and their columns are not stored)
+#pragma unroll
+  for (int c = 0; c < RC; ++c) off[c] = min(n0 + 16 * c + r, p.N - 1) * (kb * 128);
   const uint8_t* wsc = p.ws + expert * p.ws_stride + (int64_t)(n0 / 128) * kbp;
   for (int first = 0; first < rows; first += 16) {  // (one pass but for an expert of many pairs)
     // row r: its output row and its source row
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
 #pragma unroll
     for (int c = 0; c < RC; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int b = w; b < kb; b += NW) few_block<TX, RC, EXACT, VEC>(wrow, wstep, wsc, b, xrow, K, acc);
+    for (int b = w; b < kb; b += NW) few_block<TX, RC, EXACT, VEC>(wrow, off, wsc, b, xrow, K, acc);
     // lane: row l % 16, columns 16 c + 4 (l / 16) + [0, 4)
 #pragma unroll
     for (int c = 0; c < RC; ++c) *reinterpret_cast<floatx4*>(&red[w][c][r][4 * c4]) = acc[c];
@@ -1038,9 +1039,11 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
     else go(float{}, nw, rc);
   };
   using std::integral_constant;
-  // 64 columns where that leaves a workgroup to a CU: the rows are rounded
-  // once for all of them, and a wave has four times the loads in flight
-  const bool wide = p.N % 64 == 0 && p.N / 64 * groups >= device_cus();
+  // 64 columns where that leaves a workgroup to two CUs: the rows are rounded
+  // once for all of them, and a wave has four times the loads in flight (112 f32
+  // rows x 512 -> 2048 8.1 -> 5.6 us, 96 x 384 -> 1536 5.8 -> 4.5; 32 x 1024 ->
+  // 4096 6.0 -> 6.5)
+  const bool wide = (p.N + 63) / 64 * groups >= device_cus() / 2;
   if (wide && p.K <= 1024) by_type(integral_constant<int, 4>{}, integral_constant<int, 4>{});
   else if (wide) by_type(integral_constant<int, 8>{}, integral_constant<int, 4>{});
   else if (p.K > 2048) by_type(integral_constant<int, 16>{}, integral_constant<int, 1>{});
