@@ -1,6 +1,8 @@
 // Device helpers of the e4m3 block format.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace mhsa {
@@ -63,6 +65,47 @@ __device__ __forceinline__ void load8(const T* x, int c, int K, float v[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)x[c + i] : 0.f;
   }
+}
+
+// Each row of 16 lanes' values under `o`, in all of the row's lanes: the first
+// N steps of: lanes xor 1, xor 2 (quad permutations), half rows and rows
+// mirrored.
+template <int N = 4, typename T, typename O>
+__device__ __forceinline__ T row_reduce(T v, O o) {
+  auto move = [](T x, auto ctrl) {
+    constexpr int C = decltype(ctrl)::value;
+    if constexpr (sizeof(T) == 4) {
+      const int u = __builtin_bit_cast(int, x);
+      return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(u, u, C, 0xF, 0xF, false));
+    } else {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      i32x2 u = __builtin_bit_cast(i32x2, x);
+      u[0] = __builtin_amdgcn_update_dpp(u[0], u[0], C, 0xF, 0xF, false);
+      u[1] = __builtin_amdgcn_update_dpp(u[1], u[1], C, 0xF, 0xF, false);
+      return __builtin_bit_cast(T, u);
+    }
+  };
+  using std::integral_constant;
+  if constexpr (N > 0) v = o(v, move(v, integral_constant<int, 0xB1>{}));
+  if constexpr (N > 1) v = o(v, move(v, integral_constant<int, 0x4E>{}));
+  if constexpr (N > 2) v = o(v, move(v, integral_constant<int, 0x141>{}));
+  if constexpr (N > 3) v = o(v, move(v, integral_constant<int, 0x140>{}));
+  return v;
+}
+// The wave's: one lane of each row.
+template <typename T, typename O>
+__device__ __forceinline__ T wave_reduce(T v, O o) {
+  v = row_reduce(v, o);
+  auto at = [&](int l) {
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+    } else {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      const i32x2 u = __builtin_bit_cast(i32x2, v);
+      return __builtin_bit_cast(T, i32x2{__builtin_amdgcn_readlane(u[0], l), __builtin_amdgcn_readlane(u[1], l)});
+    }
+  };
+  return o(o(at(0), at(16)), o(at(32), at(48)));
 }
 
 // A wave rounds 4 blocks of a row, 16 lanes of 8 values to a block; item `id`

@@ -226,8 +226,14 @@ __device__ __forceinline__ void find_pairs(const int* idx, int pairs, int expert
 
 // The place of the n-th set bit of m, which has more than n.
 __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
-  for (int i = 0; i < n; ++i) m &= m - 1;
-  return __builtin_ctzll(m);
+  int at = 0;
+#pragma unroll
+  for (int w = 32; w; w /= 2) {
+    const int c = __popcll(m >> at & (((uint64_t)1 << w) - 1));
+    at += n >= c ? w : 0;
+    n -= n >= c ? c : 0;
+  }
+  return at;
 }
 
 template <typename TX, int NW, int RC, bool EXACT, bool VEC>
@@ -238,21 +244,47 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c4 = lane >> 4;
   const int n0 = blockIdx.x * 16 * RC;
   int expert = 0, rows = p.M - blockIdx.y * 16;
-  uint64_t same = 0;  // up to 64 pairs, one to a lane: the expert's
-  const bool lanes = !p.g.tile && p.g.idx && p.g.pairs <= 64;
-  if (lanes) {
-    // the y-th of the distinct experts, found by every wave for itself
+  // Up to 256 pairs of up to 64 experts, four to a lane: those of the expert that
+  // is the y-th of the chosen ones, found by every wave for itself. (Through LDS,
+  // with two barriers and one wave's work between, the scan of 224 pairs took 3.8
+  // of 18.8 us.) The experts of up to 16 pairs, or of 64 where there are more
+  // experts, are gone through one by one (a frame's two: 7.0 us instead of 7.6).
+  constexpr int Q = 4;
+  uint64_t same[Q] = {};
+  const bool masks = p.g.pairs > 16 && p.g.pairs <= 64 * Q && p.g.experts <= 64;
+  const bool lanes = !p.g.tile && p.g.idx && (masks || p.g.pairs <= 64);
+  if (lanes && !masks) {
     int mine = lane < p.g.pairs ? p.g.idx[lane] : -1;
     if (mine >= p.g.experts) mine = -1;
     uint64_t todo = __ballot(mine >= 0);
     for (int y = blockIdx.y;; --y) {
       if (!todo) return;
       expert = __shfl(mine, __builtin_ctzll(todo), 64);
-      same = __ballot(mine == expert);
+      same[0] = __ballot(mine == expert);
       if (y == 0) break;
-      todo &= ~same;
+      todo &= ~same[0];
     }
-    rows = __popcll(same);
+    rows = __popcll(same[0]);
+  } else if (lanes) {
+    int mine[Q];
+    uint32_t used[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      mine[i] = 64 * i + lane < p.g.pairs ? p.g.idx[64 * i + lane] : -1;
+      const bool one = mine[i] >= 0 && mine[i] < p.g.experts;
+      used[0] |= one && mine[i] < 32 ? 1u << mine[i] : 0;
+      used[1] |= one && mine[i] >= 32 ? 1u << (mine[i] - 32) : 0;
+    }
+    auto either = [](uint32_t a, uint32_t b) { return a | b; };
+    const uint64_t all = (uint64_t)wave_reduce(used[1], either) << 32 | wave_reduce(used[0], either);
+    if ((int)blockIdx.y >= __popcll(all)) return;
+    expert = nth_bit(all, blockIdx.y);
+    rows = 0;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      same[i] = __ballot(mine[i] == expert);
+      rows += __popcll(same[i]);
+    }
   } else if (p.g.tile) {
     if ((int)blockIdx.y >= *p.g.n_tiles) return;
     expert = p.g.tile[4 * blockIdx.y];
@@ -275,7 +307,20 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
     int to = -1;
     if (first + r < rows) {
       if (p.g.tile) to = p.g.pair[p.g.tile[4 * blockIdx.y + 1] + r];
-      else if (lanes) to = nth_bit(same, first + r);
+      else if (lanes) {
+        int n = first + r, base = 0;
+        uint64_t in = same[0];
+#pragma unroll
+        for (int i = 1; i < Q; ++i) {
+          const int c = __popcll(in);
+          if (base == 64 * (i - 1) && n >= c) {
+            n -= c;
+            base = 64 * i;
+            in = same[i];
+          }
+        }
+        to = base + nth_bit(in, n);
+      }
       else if (p.g.idx) to = found.list[first + r];
       else to = blockIdx.y * 16 + r;
     }
@@ -1039,11 +1084,12 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
     else go(float{}, nw, rc);
   };
   using std::integral_constant;
-  // 64 columns where that leaves a workgroup to two CUs: the rows are rounded
-  // once for all of them, and a wave has four times the loads in flight (112 f32
-  // rows x 512 -> 2048 8.1 -> 5.6 us, 96 x 384 -> 1536 5.8 -> 4.5; 32 x 1024 ->
-  // 4096 6.0 -> 6.5)
-  const bool wide = (p.N + 63) / 64 * groups >= device_cus() / 2;
+  // 64 columns where that leaves a workgroup to somewhat more than half of the
+  // CUs: the rows are rounded once for all of them, and a wave has four times the
+  // loads in flight (96 f32 rows x 512 -> 2048, 192 workgroups, 7.2 -> 5.6 us; 96
+  // x 384 -> 1536, 144, 5.8 -> 4.5; with 128 of them 32 x 1024 -> 4096 took 6.5
+  // instead of 6.0 and a frame's two experts of 1024 -> 4096 10.9 instead of 7.0)
+  const bool wide = (p.N + 63) / 64 * groups >= device_cus() * 9 / 16;
   if (wide && p.K <= 1024) by_type(integral_constant<int, 4>{}, integral_constant<int, 4>{});
   else if (wide) by_type(integral_constant<int, 8>{}, integral_constant<int, 4>{});
   else if (p.K > 2048) by_type(integral_constant<int, 16>{}, integral_constant<int, 1>{});

@@ -105,7 +105,8 @@ def test_many_large_tiles(rows, e, d, f, k, skew):
     assert torch.equal(got, again)
 
 
-@pytest.mark.parametrize("rows,e,k", [(700, 150, 4), (3000, 512, 4), (1100, 256, 8), (4000, 70, 3), (129, 1, 2), (40, 1, 5)])
+@pytest.mark.parametrize("rows,e,k", [(700, 150, 4), (3000, 512, 4), (1100, 256, 8), (4000, 70, 3), (129, 1, 2), (40, 1, 5),
+                                      (1, 256, 8), (8, 100, 8), (9, 100, 8), (16, 64, 16), (63, 64, 4), (32, 33, 8)])
 def test_few_rows_of_many_experts(rows, e, k):
     """Lists of pairs of several thousands, experts of fewer than 16 frames, of
     more and of none; one expert of all of them."""
