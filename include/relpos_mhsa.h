@@ -528,12 +528,12 @@ int32_t mhsa_encoder_step(mhsa_encoder* enc, float* x_inout, const void* pos_emb
  * calls run on the GPU that was current at loading, which is to be current
  * again, and on a stream of it. Loading waits for the GPU; no call that reads
  * the handle may run at the same time. Weight pointers may be host or device
- * memory. Calls take up to 2^25 rows, up to 2^30 elements apart;
- * weights are loaded again only on the GPU that holds them. */
+ * memory; weights are loaded again only on the GPU that holds them. Calls take
+ * up to 2^25 rows, up to 2^30 elements apart. */
 
 /* y = W q(x) + b. */
 typedef struct mhsa_fp8_linear mhsa_fp8_linear;
-/* Any in_dim up to 32768 and any out_dim, up to 2 GiB of weights. */
+/* Any in_dim up to 32768 and out_dim up to 2^22, up to 2 GiB of weights. */
 int32_t mhsa_fp8_linear_create(int32_t in_dim, int32_t out_dim, int32_t use_bias, mhsa_fp8_linear** out);
 void mhsa_fp8_linear_destroy(mhsa_fp8_linear* linear);
 /* weight [out_dim, in_dim] and bias [out_dim] (NULL without one) in data_dtype

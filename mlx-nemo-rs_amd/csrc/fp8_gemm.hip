@@ -1050,12 +1050,13 @@ hipError_t fp8_unpad_weight(const uint8_t* codes, const uint8_t* scales, int N, 
 
 // Up to 16 rows read the weights once. More read them once per 16 rows, which
 // saves the second launch and the codes' way through memory while it is not
-// much: with a call from Python at 128 x 1024 -> 4096 8.8 us against 12.6, at
-// 192 rows 11.9 against 12.5, at 256 17.5; 64 x 4096 -> 1024 8.4 against 14.1,
-// 96 rows 14.9 (over K > 2048 16 waves share one row group's inputs).
+// much: with a call from Python at 128 x 1024 -> 4096 9.7 us against 12.5 and at
+// 224 rows 16.9 against 13.1, at 128 x 2048 -> 2048 9.4 against 12.6 and at 160
+// rows 16.8 against 12.1; 64 x 4096 -> 1024 9.0 against 14.1, 96 rows 16.0
+// against 14.3 (over K > 2048 16 waves share one row group's inputs).
 bool fp8_few_rows(int64_t M, int N, int K) {
   const int64_t read = (M + 15) / 16 * N * K;
-  return M <= 16 || (M <= 256 && read <= (K <= 2048 ? 40 : 20) << 20);
+  return M <= 16 || (M <= 256 && read < (K <= 2048 ? 40 : 20) << 20);
 }
 int fp8_scan_pairs() { return kScanPairs; }
 
