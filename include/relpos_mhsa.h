@@ -601,8 +601,13 @@ int64_t mhsa_experts_workspace(const mhsa_experts* experts, int32_t rows, int32_
 /* x, residual (or NULL) and out [rows, d_model] in dtype (MHSA_F32 or
  * MHSA_BF16), indices int32 and weights f32 [rows, top_k], all device. out may
  * be the residual (the block's half step), and must not overlap anything else.
- * top_k <= 32; rows may be 0. Sums go through the fp8 matrix unit in either
- * dtype. */
+ * top_k <= 32; rows may be 0. F32 calls multiply exactly and sum in f32. Of
+ * bf16 calls the second product, and over more than 256 pairs with a mean of 24
+ * or more to an expert the first, go through the fp8 matrix unit
+ * (mhsa_fp8_linear_forward has its bound), so that a hidden value at the edge of
+ * its code may take the code beside it. A row's low bits may depend on the
+ * number of rows, and bf16 rows through such codes by about 1e-3 in the 2-norm,
+ * half of their own rounding. */
 int32_t mhsa_experts_forward(const mhsa_experts* experts, const void* x, int32_t dtype, int32_t rows,
                              const int32_t* indices, const float* weights, int32_t top_k, const void* residual,
                              float res_scale, void* out, void* workspace, int64_t workspace_bytes, void* hip_stream);

@@ -424,6 +424,7 @@ int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* 
     g[i].K = w.K;
     g[i].M = pairs;
     g[i].ldo = w.N;
+    g[i].exact = dt == mhsa::kF32;
     g[i].g.top_k = top_k;
     g[i].g.experts = e->E;
     g[i].g.pairs = pairs;

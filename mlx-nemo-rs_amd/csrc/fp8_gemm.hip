@@ -8,10 +8,11 @@
 // terms' magnitudes (measured: 1.4e-5 of the result in the 2-norm for normally
 // distributed values, 5.5e-5 for codes spread over the whole exponent range,
 // at any K; the running sum keeps its 24 bits). That is far under half a step
-// of a bf16 result (2e-3 in the 2-norm) or of e4m3 codes. An f32 result keeps
-// f32 sums: there the codes go to the bf16 matrix cores, which hold them and
-// their products exactly (1e-7; only of blocks under 2^-115 what lies below
-// bf16's smallest number, 2^-133, is lost), at half the rate.
+// of a bf16 result (2e-3 in the 2-norm) or of e4m3 codes. An f32 result, and
+// the hidden values on the way to one, keep f32 sums: there the codes go to the
+// bf16 matrix cores, which hold them and their products exactly (1e-7; only of
+// blocks under 2^-115 what lies below bf16's smallest number, 2^-133, is lost),
+// at half the rate.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
 // of the choices. A wave's first weights are on their way while the workgroup
 // rounds the hidden rows to codes in LDS.
 constexpr int kSumLds = 64 * 1024;
-template <typename TOut>
+template <typename TOut, bool EXACT>
 __global__ __launch_bounds__(1024) void fp8_few_sum_kernel(Fp8Gemm p, const float* weights, const TOut* residual,
                                                            float res_scale) {
   __shared__ __attribute__((aligned(16))) uint8_t codes[kSumLds];
@@ -433,10 +434,22 @@ __global__ __launch_bounds__(1024) void fp8_few_sum_kernel(Fp8Gemm p, const floa
         x1 = *reinterpret_cast<const u32x4*>(codes + to * pitch + b * 128 + 32 * c4 + 16);
         s = scales[to * kb + b];
       }
-      const i32x8 a = {(int)wf[d][0][0], (int)wf[d][0][1], (int)wf[d][0][2], (int)wf[d][0][3],
-                       (int)wf[d][1][0], (int)wf[d][1][1], (int)wf[d][1][2], (int)wf[d][1][3]};
-      const i32x8 q = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, 0, 0, 0, sw[d], 0, s);
+      if constexpr (EXACT) {
+        floatx4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 wj = wf[d][j >> 1], xj = j < 2 ? x0 : x1;
+          part = mma16(fp8_to_bf16(wj[2 * (j & 1)], wj[2 * (j & 1) + 1]), fp8_to_bf16(xj[2 * (j & 1)], xj[2 * (j & 1) + 1]),
+                       part);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __builtin_ldexpf(part[e], s + sw[d] - 254);
+      } else {
+        const i32x8 a = {(int)wf[d][0][0], (int)wf[d][0][1], (int)wf[d][0][2], (int)wf[d][0][3],
+                         (int)wf[d][1][0], (int)wf[d][1][1], (int)wf[d][1][2], (int)wf[d][1][3]};
+        const i32x8 q = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, acc, 0, 0, 0, sw[d], 0, s);
+      }
     };
 #pragma unroll
     for (int d = 0; d < D; ++d)
@@ -994,6 +1007,26 @@ hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
   return hipGetLastError();
 }
 
+// A product over experts. f32 calls are EXACT: 3000 frames to 2 of 16 experts
+// of 1024 -> 4096 take 151 us so, 15001 to 4 of 64 1060. A bf16 call is not
+// (100 and 720): through the fp8 unit's sums 8% of its results are a bf16 step
+// off, and their error in the 2-norm goes from 1.58e-3 to 1.61e-3.
+template <bool EXACT>
+hipError_t launch_experts(const Fp8Gemm& p, hipStream_t s) {
+  if (p.epilogue == kFp8HiddenQ)
+    return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, EXACT, kFp8HiddenQ, float>(p, s)
+                                : launch_tile<128, 128, 2, EXACT, kFp8HiddenQ, float>(p, s);
+  if (p.epilogue != kFp8Pair) return hipErrorInvalidValue;
+  // too few tiles of 256 columns to fill the CUs (the experts' last tiles
+  // are half full on average): 128 columns, 3000 frames to 2 of 16 experts
+  // 55 -> 46 us
+  const int64_t tiles = (p.M / 256 + p.g.experts / 2) * ((p.N + 255) / 256);
+  if (p.g.tile_rows == 256 && tiles <= device_cus() / 2 + device_cus() / 4)
+    return launch_tile<256, 128, 2, EXACT, kFp8Pair, float>(p, s);
+  return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, EXACT, kFp8Pair, float>(p, s)
+                              : launch_tile<128, 128, 2, EXACT, kFp8Pair, float>(p, s);
+}
+
 bool bad_gemm(const Fp8Gemm& p) {
   return p.N <= 0 || p.K <= 0 || !p.bias || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);
 }
@@ -1070,7 +1103,7 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
   // (hidden values are rounded to codes next: a sum at a code's edge that is off
   // by 1e-5 gives the code beside it, and one such code of a frame's 8192 can be
   // off by as much as the frame's bf16 result is rounded)
-  const bool exact = p.epilogue == kFp8HiddenF32 || (p.epilogue == kFp8Out && p.out_dt == kF32);
+  const bool exact = p.exact || p.epilogue == kFp8HiddenF32 || (p.epilogue == kFp8Out && p.out_dt == kF32);
   auto go = [&](auto tx, auto nw, auto rc) {
     using TX = decltype(tx);
     constexpr int NW = decltype(nw)::value, RC = decltype(rc)::value;
@@ -1105,10 +1138,11 @@ hipError_t fp8_gemm_few_sum(const Fp8Gemm& p, const float* weights, const void* 
       p.g.pairs <= 0 || !fp8_few_sum_ok(p.g.pairs, p.K) || p.g.top_k <= 0 || p.g.pairs % p.g.top_k || p.ldo != p.N)
     return hipErrorInvalidValue;
   const unsigned grid = (p.N + 15) / 16;
+  if (p.exact != (p.out_dt == kF32)) return hipErrorInvalidValue;
   if (p.out_dt == kBF16)
-    fp8_few_sum_kernel<bf16><<<grid, 1024, 0, s>>>(p, weights, static_cast<const bf16*>(residual), res_scale);
+    fp8_few_sum_kernel<bf16, false><<<grid, 1024, 0, s>>>(p, weights, static_cast<const bf16*>(residual), res_scale);
   else
-    fp8_few_sum_kernel<float><<<grid, 1024, 0, s>>>(p, weights, static_cast<const float*>(residual), res_scale);
+    fp8_few_sum_kernel<float, true><<<grid, 1024, 0, s>>>(p, weights, static_cast<const float*>(residual), res_scale);
   return hipGetLastError();
 }
 
@@ -1123,19 +1157,7 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
     if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll || p.slots % 16 || p.slots * (fp8_kp(p.K) / 128) > INT32_MAX)
       return hipErrorInvalidValue;
     if (p.epilogue == kFp8HiddenQ && p.N % 64) return hipErrorInvalidValue;
-    if (p.epilogue == kFp8HiddenQ)
-      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8HiddenQ, float>(p, s)
-                                  : launch_tile<128, 128, 2, false, kFp8HiddenQ, float>(p, s);
-    // too few tiles of 256 columns to fill the CUs (the experts' last tiles
-    // are half full on average): 128 columns, 3000 frames to 2 of 16 experts
-    // 55 -> 46 us
-    const int64_t tiles = (p.M / 256 + p.g.experts / 2) * ((p.N + 255) / 256);
-    if (p.epilogue == kFp8Pair && p.g.tile_rows == 256 && tiles <= device_cus() / 2 + device_cus() / 4)
-      return launch_tile<256, 128, 2, false, kFp8Pair, float>(p, s);
-    if (p.epilogue == kFp8Pair)
-      return p.g.tile_rows == 256 ? launch_tile<256, 256, 2, false, kFp8Pair, float>(p, s)
-                                  : launch_tile<128, 128, 2, false, kFp8Pair, float>(p, s);
-    return hipErrorInvalidValue;
+    return p.exact ? launch_experts<true>(p, s) : launch_experts<false>(p, s);
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
   auto tiles = [&](int64_t bm, int64_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };

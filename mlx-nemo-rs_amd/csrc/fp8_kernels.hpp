@@ -89,6 +89,9 @@ struct Fp8Gemm {
   int64_t w_stride = 0, ws_stride = 0;  // bytes between experts
   int M = 0, N = 0, K = 0;
   int epilogue = kFp8Out;
+  // products over experts: exact products and f32 sums, as a dense product with
+  // f32 out always has
+  bool exact = false;
   void* out = nullptr;
   DType out_dt = kF32;
   int64_t ldo = 0;
@@ -106,8 +109,9 @@ int fp8_scan_pairs();
 // sum_j weights_j (acc + bias); x [pairs, K] f32, by pair.
 bool fp8_few_sum_ok(int64_t pairs, int K);
 hipError_t fp8_gemm_few_sum(const Fp8Gemm& p, const float* weights, const void* residual, float res_scale, hipStream_t s);
-// Tile kernel on codes; a dense product with f32 out sums on the bf16 matrix
-// cores (exact products), every other on the fp8 ones.
+// Tile kernel on codes; a dense product with f32 out and an `exact` one over
+// experts sum on the bf16 matrix cores (exact products), every other on the fp8
+// ones.
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s);
 // Rows of a tile for `pairs` pairs over `experts` experts (0: the few-row
 // kernel's groups of 16); K: the smaller of the two products'.
