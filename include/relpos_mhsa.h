@@ -554,8 +554,10 @@ int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* linear, int32_t rows);
  * row); x, out and the workspace must not overlap. rows may be 0. Products of
  * an f32 out are exact and summed in f32; for a bf16 out they go through the
  * fp8 matrix unit, whose sums are off by some 1e-5 of the result (at most 9e-4 of
- * their terms' magnitudes). f32 results of blocks under 2^-115 lose what lies
- * below 2^-133. A row's low bits may depend on the number of rows. */
+ * their terms' magnitudes). f32 results lose, of activations' blocks under
+ * 2^-115, what lies below 2^-133; an activation that rounds to 2^128 (from
+ * 0.97 of the largest float on) may count as an infinity. A row's low bits may
+ * depend on the number of rows. */
 int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* linear, const void* x, int32_t x_dtype, int32_t rows,
                                 int64_t x_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
                                 int64_t workspace_bytes, void* hip_stream);

@@ -11,8 +11,8 @@
 // of a bf16 result (2e-3 in the 2-norm) or of e4m3 codes. An f32 result, and
 // the hidden values on the way to one, keep f32 sums: there the codes go to the
 // bf16 matrix cores, which hold them and their products exactly (1e-7; only of
-// blocks under 2^-115 what lies below bf16's smallest number, 2^-133, is lost),
-// at half the rate.
+// activations' blocks under 2^-115 what lies below bf16's smallest number,
+// 2^-133, is lost), at half the rate.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -673,6 +673,17 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       ws = __builtin_amdgcn_readlane((int)wword, kt >> 2) >> sh;
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) xs[i] = HT ? xw[i] : xw[i] >> sh;
+      if constexpr (EXACT) {
+        // Codes times powers of two that bf16 holds: of the weight's power what
+        // lies past 2^-100 and 2^100 goes over to the rows' (from 2^120 on the
+        // largest codes would pass bf16's range). What the rows then lose or
+        // pass belongs to products that f32 does not hold either; below
+        // infinity, so that with codes of zero these stay zero.
+        const int wb = ws & 255, in = min(max(wb, 27), 227), more = wb - in;
+        ws = in;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) xs[i] = min(max((xs[i] & 255) + more, 0), more > 0 ? 246 : 255);
+      }
     }
     const int other = buf + 1 == NS ? 0 : buf + 1;
     __builtin_amdgcn_sched_barrier(0);
@@ -706,13 +717,13 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     } else {
       // Exact products and f32 sums on the bf16 cores. bf16 has f32's range, so
       // the powers of two go into the conversion of the codes.
-      const float wf = fp8_scale(ws & 255);
+      const float wf = fp8_scale(ws);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         bf16x8 xa[C::TM], xb[C::TN];
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
-          xa[i] = fp8_to_bf16(fa[h][i][u >> 1][2 * (u & 1)], fa[h][i][u >> 1][2 * (u & 1) + 1], fp8_scale(xs[i] & 255));
+          xa[i] = fp8_to_bf16(fa[h][i][u >> 1][2 * (u & 1)], fa[h][i][u >> 1][2 * (u & 1) + 1], fp8_scale(xs[i]));
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
           xb[j] = fp8_to_bf16(fb[h][j][u >> 1][2 * (u & 1)], fb[h][j][u >> 1][2 * (u & 1) + 1], wf);
