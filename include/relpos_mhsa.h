@@ -546,8 +546,8 @@ int32_t mhsa_fp8_linear_load_codes(mhsa_fp8_linear* linear, const uint8_t* codes
 /* The weight as held, in load_codes' layout (host or device memory). Waits for
  * the GPU. */
 int32_t mhsa_fp8_linear_read_codes(const mhsa_fp8_linear* linear, uint8_t* codes, uint8_t* scales);
-/* Workspace bytes of a forward of `rows` rows (0 for few rows, -1 for bad
- * arguments). */
+/* Workspace bytes of a forward of `rows` rows or fewer (0 for few rows, -1 for
+ * bad arguments). */
 int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* linear, int32_t rows);
 /* x [rows, in_dim] in x_dtype and out [rows, out_dim] in out_dtype (MHSA_F32 or
  * MHSA_BF16 each), device, rows x_stride and out_stride elements apart (>= the
@@ -597,8 +597,8 @@ int32_t mhsa_experts_load(mhsa_experts* experts, int32_t data_dtype, const void*
                           const void* weight2, const void* bias2);
 int32_t mhsa_experts_load_codes(mhsa_experts* experts, const uint8_t* codes1, const uint8_t* scales1,
                                 const float* bias1, const uint8_t* codes2, const uint8_t* scales2, const float* bias2);
-/* Workspace bytes of a forward (-1 for bad arguments). Rows run in parts of
- * up to 2^18 frame and expert pairs, which bounds it. */
+/* Workspace bytes of a forward of `rows` rows or fewer (-1 for bad arguments).
+ * Rows run in parts of up to 2^18 frame and expert pairs, which bounds it. */
 int64_t mhsa_experts_workspace(const mhsa_experts* experts, int32_t rows, int32_t top_k);
 /* x, residual (or NULL) and out [rows, d_model] in dtype (MHSA_F32 or
  * MHSA_BF16), indices int32 and weights f32 [rows, top_k], all device. out may

@@ -361,7 +361,7 @@ struct mhsa_experts {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTopK = 32;
-constexpr int64_t kMaxPairs = 1 << 18;
+constexpr int64_t kMaxPairs = 1 << 18, kListPairs = 256;
 
 // How a call runs, and its pieces of the workspace. Rows go in runs of
 // `step`, each through the same buffers, which bounds them.
@@ -385,7 +385,7 @@ ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void*
   Arena a(ws);
   // (a list costs a launch; without one every workgroup scans the indices)
   p.tile_rows = mhsa::fp8_group_rows(pairs, e->E, std::min(e->D, e->F));
-  if (rows * top_k <= 256 || (p.tile_rows == 16 && rows * top_k <= mhsa::fp8_scan_pairs())) p.tile_rows = 0;
+  if (rows * top_k <= kListPairs || (p.tile_rows == 16 && rows * top_k <= mhsa::fp8_scan_pairs())) p.tile_rows = 0;
   if (p.tile_rows) {
     p.max_tiles = (int)(pairs / p.tile_rows + std::min<int64_t>(pairs, e->E));
     p.pair = a.take<int>(mhsa::expert_slots(pairs, e->E));
@@ -406,6 +406,18 @@ ExpertsPlan experts_layout(const mhsa_experts* e, int64_t rows, int top_k, void*
   p.y = a.take<float>(pairs * e->D);
   p.bytes = a.used;
   return p;
+}
+
+// Bytes of a workspace that serves `rows` rows and any fewer: a call's kernels
+// change with its number of pairs, and those of fewer keep hidden rows in f32,
+// which takes more than the next ones' codes. Within a range the bytes grow with
+// the rows, so the most are those of `rows` or of the end of a range before it.
+int64_t experts_bytes(const mhsa_experts* e, int64_t rows, int top_k) {
+  int64_t most = experts_layout(e, rows, top_k, nullptr).bytes;
+  for (const int64_t pairs : {kListPairs, (int64_t)mhsa::fp8_scan_pairs(), (int64_t)mhsa::kFp8TileMean * e->E - 1,
+                              (int64_t)mhsa::kFp8LargeMean * e->E - 1})
+    if (const int64_t r = pairs / top_k; r > 0 && r < rows) most = std::max(most, experts_layout(e, r, top_k, nullptr).bytes);
+  return most;
 }
 
 int32_t experts_run(const mhsa_experts* e, const ExpertsPlan& plan, const void* x, DType dt, int64_t rows,
@@ -542,7 +554,7 @@ int32_t mhsa_experts_load_codes(mhsa_experts* h, const uint8_t* codes1, const ui
 
 int64_t mhsa_experts_workspace(const mhsa_experts* h, int32_t rows, int32_t top_k) {
   if (!h || rows < 0 || rows > kMaxRows || top_k <= 0 || top_k > kMaxTopK) return -1;
-  return rows == 0 ? 0 : experts_layout(h, rows, top_k, nullptr).bytes;
+  return rows == 0 ? 0 : experts_bytes(h, rows, top_k);
 }
 
 int32_t mhsa_experts_forward(const mhsa_experts* h, const void* x, int32_t dtype, int32_t rows, const int32_t* indices,
@@ -562,9 +574,10 @@ int32_t mhsa_experts_forward(const mhsa_experts* h, const void* x, int32_t dtype
     return fail(MHSA_EINVAL, "indices and weights must be aligned to their elements");
   if (!h->lin[0].loaded || !h->lin[1].loaded) return fail(MHSA_EINVAL, "no weights are loaded");
   const ExpertsPlan plan = experts_layout(h, rows, top_k, workspace);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes)
+  const int64_t need = experts_bytes(h, rows, top_k);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
     return fail(MHSA_EINVAL, "%d rows of %d experts need a 16-byte aligned workspace of %lld bytes", rows, top_k,
-                (long long)plan.bytes);
+                (long long)need);
   const int64_t es = mhsa::dtype_size(dt), n = (int64_t)rows * h->D * es, np = (int64_t)rows * top_k * 4;
   if (overlap(x, n, out, n) || (residual && residual != out && overlap(residual, n, out, n)) ||
       overlap(indices, np, out, n) || overlap(weights, np, out, n))

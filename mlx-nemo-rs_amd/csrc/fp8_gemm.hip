@@ -1159,7 +1159,7 @@ hipError_t fp8_gemm_few_sum(const Fp8Gemm& p, const float* weights, const void* 
 
 int fp8_group_rows(int64_t pairs, int experts, int K) {
   const int64_t mean = pairs / experts;
-  return mean < 24 ? 16 : mean < 192 || K <= kFp8Block ? 128 : 256;  // (the large tiles' ring takes two stages)
+  return mean < kFp8TileMean ? 16 : mean < kFp8LargeMean || K <= kFp8Block ? 128 : 256;  // (the large tiles' ring takes two stages)
 }
 
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {

@@ -113,8 +113,10 @@ hipError_t fp8_gemm_few_sum(const Fp8Gemm& p, const float* weights, const void* 
 // experts sum on the bf16 matrix cores (exact products), every other on the fp8
 // ones.
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s);
-// Rows of a tile for `pairs` pairs over `experts` experts (0: the few-row
-// kernel's groups of 16); K: the smaller of the two products'.
+// Rows of a tile for `pairs` pairs over `experts` experts (16: the few-row
+// kernel's groups), by the pairs an expert has in the mean; K: the smaller of the
+// two products'.
+constexpr int kFp8TileMean = 24, kFp8LargeMean = 192;
 int fp8_group_rows(int64_t pairs, int experts, int K);
 
 // Slots that `pairs` pairs take at most, a multiple of 16.
