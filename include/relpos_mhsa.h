@@ -551,7 +551,8 @@ int32_t mhsa_fp8_linear_read_codes(const mhsa_fp8_linear* linear, uint8_t* codes
 int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* linear, int32_t rows);
 /* x [rows, in_dim] in x_dtype and out [rows, out_dim] in out_dtype (MHSA_F32 or
  * MHSA_BF16 each), device, rows x_stride and out_stride elements apart (>= the
- * row); x, out and the workspace must not overlap. rows may be 0. Products of
+ * row); x, out and the workspace must not overlap (x's and out's rows may lie in
+ * one buffer side by side, as many bytes apart). rows may be 0. Products of
  * an f32 out are exact and summed in f32; for a bf16 out they go through the
  * fp8 matrix unit, whose sums are off by some 1e-5 of the result (at most 9e-4 of
  * their terms' magnitudes). f32 results lose, of activations' blocks under

@@ -143,6 +143,18 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
+// Whether rows of na bytes from a on, pa bytes apart, and rows of nb bytes from
+// b on share bytes. Rows of two tensors in one buffer side by side (the same
+// distance, none within the other's) do not; of two that are interleaved in any
+// other way it is taken that they do.
+bool rows_overlap(const void* a, int64_t na, int64_t pa, const void* b, int64_t nb, int64_t pb, int64_t rows) {
+  if (!overlap(a, (rows - 1) * pa + na, b, (rows - 1) * pb + nb)) return false;
+  if (pa != pb) return true;
+  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+  const int64_t at = (off % pa + pa) % pa;  // of b's rows within a's distance
+  return at < na || at + nb > pa;
+}
+
 // Hands out 256-byte aligned pieces of a workspace (or only adds them up).
 struct Arena {
   char* base;
@@ -267,7 +279,7 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t
   if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes))
     return fail(MHSA_EINVAL, "%d rows need a 16-byte aligned workspace of %lld bytes", rows, (long long)plan.bytes);
   const int64_t xn = ((rows - 1) * x_stride + w.K) * xs, on = ((rows - 1) * out_stride + w.N) * os;
-  if (overlap(x, xn, out, on) || overlap(workspace, plan.bytes, x, xn) || overlap(workspace, plan.bytes, out, on))
+  if (rows_overlap(x, w.K * xs, x_stride * xs, out, w.N * os, out_stride * os, rows) || overlap(workspace, plan.bytes, x, xn) || overlap(workspace, plan.bytes, out, on))
     return fail(MHSA_EINVAL, "x, out and the workspace must not overlap");
   if (int32_t rc = check_device(w.device)) return rc;
   hipStream_t s = static_cast<hipStream_t>(hs);
