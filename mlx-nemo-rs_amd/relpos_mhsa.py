@@ -694,8 +694,8 @@ def route(logits, top_k: int, score: str = "softmax", bias=None, n_groups: int =
         raise MhsaError(MHSA_EINVAL, "expected a GPU tensor [..., n_experts]")
     n = logits.shape[-1]
     rows, ld = _rows_of(logits, n)
-    if bias is not None and (bias.device != logits.device or bias.dtype != torch.float32 or tuple(bias.shape) != (n,)
-                             or not bias.is_contiguous()):
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.device != logits.device or bias.dtype != torch.float32
+                             or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
         raise MhsaError(MHSA_EINVAL, f"bias: expected a contiguous float32 tensor [{n}] on {logits.device}")
     shape = (*logits.shape[:-1], top_k if top_k > 0 else 0)
     idx = logits.new_empty(shape, dtype=torch.int32)
@@ -751,15 +751,15 @@ class ExpertFeedForward:
         if not isinstance(x, torch.Tensor) or not x.is_cuda or not x.is_contiguous() or x.dim() < 1 or x.shape[-1] != self.d_model:
             raise MhsaError(MHSA_EINVAL, f"expected a contiguous GPU tensor [..., {self.d_model}]")
         dtype = _act_code(x.dtype)
-        top_k = indices.shape[-1] if indices.dim() else 0
+        top_k = indices.shape[-1] if isinstance(indices, torch.Tensor) and indices.dim() else 0
         lead = x.shape[:-1]
         for t, want, name in ((indices, torch.int32, "indices"), (weights, torch.float32, "weights")):
-            if (not t.dim() or t.dtype != want or t.get_device() != x.get_device() or not t.is_contiguous() or t.shape[:-1] != lead
-                    or t.shape[-1] != top_k):
+            if (not isinstance(t, torch.Tensor) or not t.dim() or t.dtype != want or t.get_device() != x.get_device()
+                    or not t.is_contiguous() or t.shape[:-1] != lead or t.shape[-1] != top_k):
                 raise MhsaError(MHSA_EINVAL, f"{name}: expected contiguous {want} [..., top_k] beside x")
         for t in (residual, out):
-            if t is not None and (t.dtype != x.dtype or t.get_device() != x.get_device() or t.shape != x.shape
-                                  or not t.is_contiguous()):
+            if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != x.dtype or t.get_device() != x.get_device()
+                                  or t.shape != x.shape or not t.is_contiguous()):
                 raise MhsaError(MHSA_EINVAL, "residual and out are to be like x")
         if out is None:
             out = torch.empty_like(x)
