@@ -1172,20 +1172,27 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
   auto tiles = [&](int64_t bm, int64_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };
-  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256), t128 = tiles(128, 128);
-  const bool large = t256 >= 128 && p.K > kFp8Block;  // (the large tiles' ring takes two stages)
-  const bool fewer = (t192 + 255) / 256 * 192 < (t256 + 255) / 256 * 256;  // rows a CU goes through
+  // Large tiles from half of the CUs on, and tiles of 128 rows likewise. About
+  // there either side wins, by K (us, the larger tiles against the smaller):
+  // 128 large tiles of 2048 x 1024 -> 4096 23.2 and 20.1, of 2048 x 4096 -> 4096
+  // 48 and 48, 188 of 3000 x 1024 -> 4096 24.8 and 27.1; 128 tiles of 128 rows of
+  // 1024 x 1024 -> 2048 12.1 and 10.5, of 1000 x 4096 -> 2048 25.0 and 26.8. 192
+  // rows where a CU then goes through fewer (3000 x 1024 -> 4096 24.8 against
+  // 27.6, 8200 x 1024 -> 2048 37.8 against 43.8).
+  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256), t128 = tiles(128, 128), cus = device_cus();
+  const bool large = t256 >= cus / 2 && p.K > kFp8Block;  // (the large tiles' ring takes two stages)
+  const bool fewer = (t192 + cus - 1) / cus * 192 < (t256 + cus - 1) / cus * 256;  // rows a CU goes through
   if (p.out_dt == kF32) {
     if (large && fewer) return launch_tile<192, 256, 2, true, kFp8Out, float>(p, s);
     if (large) return launch_tile<256, 256, 2, true, kFp8Out, float>(p, s);
-    return t128 >= 128 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s) : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
+    return t128 >= cus / 2 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s) : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
   }
   if (large && fewer) return launch_tile<192, 256, 2, false, kFp8Out, bf16>(p, s);
   if (large) return launch_tile<256, 256, 2, false, kFp8Out, bf16>(p, s);
   // a tile alone on its CU keeps four stages, two that share it two each
   // (3000 x 4096 -> 1024: 36.8 -> 29.7 us with the rows' codes)
-  if (t128 >= 128 && t128 <= device_cus()) return launch_tile<128, 128, 4, false, kFp8Out, bf16>(p, s);
-  return t128 >= 128 ? launch_tile<128, 128, 2, false, kFp8Out, bf16>(p, s) : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
+  if (t128 >= cus / 2 && t128 <= cus) return launch_tile<128, 128, 4, false, kFp8Out, bf16>(p, s);
+  return t128 >= cus / 2 ? launch_tile<128, 128, 2, false, kFp8Out, bf16>(p, s) : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
 }
 
 }  // namespace mhsa
