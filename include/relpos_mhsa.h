@@ -518,7 +518,8 @@ int32_t mhsa_encoder_step(mhsa_encoder* enc, float* x_inout, const void* pos_emb
  * in the call, one s for each row's 128 inputs. s is the smallest s >= 0 with
  * max |v| <= 448 * 2^(s - 127) over the block's finite values (127 for a block
  * of zeros), codes are rounded to nearest even, and an infinity or a NaN
- * becomes a NaN.
+ * becomes a NaN. Scales are powers of two only: weights that have f32 scales
+ * come in as floats, and are rounded again.
  *
  * Weight handles are written by the load calls alone. Forward calls are const:
  * their scratch memory is the caller's workspace (device, 16-byte aligned,

@@ -25,8 +25,9 @@ namespace {
 // reduces one 32-bit word: a score's f32 rounding, which keeps the order. Only
 // lanes that share the largest word are compared in 64 bits. (With shuffles of
 // 64-bit values, which go through LDS, 30001 rows of 256 experts in 8 groups
-// took 88 us, with these 44, with four rows to a wave 29: 1.1 TB/s, and 423
-// vector instructions a row, which the unit issues in 71% of the time.)
+// took 88 us, with these 44, with four rows to a wave 29.8, calls one after the
+// other in a graph: 1.1 TB/s, and 423 vector instructions a row, which the unit
+// issues in 70% of the time. Alone, under a profiler, a call takes 32.6.)
 // ---------------------------------------------------------------------------
 
 constexpr double kNone = -__builtin_inf();
@@ -44,10 +45,10 @@ __device__ __forceinline__ double inverse(double d) {
   r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
   return d < __builtin_inf() ? r : 0.0;
 }
-// e^x for |x| <= 800 to within 2 ulp: e^x = 2^k e^r, |r| <= ln 2 / 2, by the
-// series up to r^12 (the rest is under 2^-52). The range is the callers' to
-// keep, with one instruction, and takes the special cases off the way: beyond
-// it e^x is infinity or 0 in 64 bits.
+// e^x for |x| <= 800 to within 2.5 ulp: e^x = 2^k e^r, |r| <= ln 2 / 2, by the
+// series up to r^12 (the rest is up to 1.5 ulp; over 10^8 values the most was
+// 2.32). The range is the callers' to keep, with one instruction, and takes the
+// special cases off the way: beyond it e^x is infinity or 0 in 64 bits.
 __device__ __forceinline__ double exp_within(double x) {
   const double k = __builtin_rint(x * 1.4426950408889634);
   // ln 2 in two parts, the first of 32 bits, so that its product with k is exact
@@ -525,9 +526,9 @@ hipError_t route(const RouteParams& p, hipStream_t s) {
   const int64_t grid = (p.rows + 3) / 4;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   // Four rows to a wave where there are enough of them: 8000 rows of 256 experts
-  // in 8 groups 15.4 -> 12.3 us, 30001 44.4 -> 29.4; of 64 experts 4.8 -> 4.4 and
-  // 12.3 -> 9.1. Of fewer rows a wave's longer way weighs more (3000: 8.9 against
-  // 10.0 and 3.2 against 3.9).
+  // in 8 groups 15.3 -> 12.3 us, 30001 44.4 -> 29.8; of 64 experts 4.8 -> 4.4 and
+  // 12.6 -> 9.2 (in a graph, as all of these). Of fewer rows a wave's longer way
+  // weighs more (3000: 9.0 against 10.0 and 3.2 against 3.9).
   const bool many = p.rows >= 6144 && p.experts <= 256 && p.top_k <= 16 &&
                     (p.groups == 1 || (16 % p.groups == 0 && p.experts % 16 == 0));
   auto go = [&](auto t) {

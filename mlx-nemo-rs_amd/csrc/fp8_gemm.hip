@@ -1019,9 +1019,10 @@ hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
 }
 
 // A product over experts. f32 calls are EXACT: 3000 frames to 2 of 16 experts
-// of 1024 -> 4096 take 151 us so, 15001 to 4 of 64 1060. A bf16 call is not
-// (100 and 720): through the fp8 unit's sums 8% of its results are a bf16 step
-// off, and their error in the 2-norm goes from 1.58e-3 to 1.61e-3.
+// of 1024 -> 4096 take 155 us so, 15001 to 4 of 64 1070. A bf16 call is not (101
+// and 740): with the fp8 unit's sums 8% of its results are a bf16 step or so off,
+// and their error in the 2-norm goes from 1.58e-3 to 1.61e-3. (The first product
+// alone EXACT would add 30 and 180 us.)
 template <bool EXACT>
 hipError_t launch_experts(const Fp8Gemm& p, hipStream_t s) {
   if (p.epilogue == kFp8HiddenQ)

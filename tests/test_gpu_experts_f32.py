@@ -126,3 +126,18 @@ def test_against_oracle(rows, e, d, f, k):
     tol = bound + 64 * 2.0 ** -24 * (np.abs(want) + bound / step)
     bad = np.abs(got - want) > tol + 1e-30
     assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist())
+
+
+@pytest.mark.parametrize("rows", [5, 300, 3000])
+def test_infinities_and_nans_stay_in_their_rows(rows):
+    rng = np.random.default_rng(rows)
+    lin = [[F.quantize_weight(rng.standard_normal(s) / 12) for _ in range(2)] for s in ((192, 256), (256, 192))]
+    layer = load(*(np.stack([m[i] for m in part]) for part in lin for i in (0, 1)))
+    x = torch.from_numpy(rng.standard_normal((rows, 256)).astype(np.float32)).cuda()
+    idx = torch.from_numpy(rng.integers(0, 2, (rows, 1)).astype(np.int32)).cuda()
+    w = torch.ones(rows, 1, device="cuda")
+    clean = layer.forward(x, idx, w)
+    x[1, 200], x[3, 5] = float("nan"), float("inf")
+    got = layer.forward(x, idx, w)
+    keep = [r for r in range(rows) if r not in (1, 3)]
+    assert torch.isnan(got[[1, 3]]).all() and torch.equal(got[keep], clean[keep])
