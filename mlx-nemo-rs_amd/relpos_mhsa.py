@@ -697,7 +697,9 @@ def route(logits, top_k: int, score: str = "softmax", bias=None, n_groups: int =
     if bias is not None and (not isinstance(bias, torch.Tensor) or bias.device != logits.device or bias.dtype != torch.float32
                              or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
         raise MhsaError(MHSA_EINVAL, f"bias: expected a contiguous float32 tensor [{n}] on {logits.device}")
-    shape = (*logits.shape[:-1], top_k if top_k > 0 else 0)
+    if top_k <= 0 or top_k > n:  # (before there is memory for them)
+        raise MhsaError(MHSA_EINVAL, f"top_k {top_k} is not in [1, {n}]")
+    shape = (*logits.shape[:-1], top_k)
     idx = logits.new_empty(shape, dtype=torch.int32)
     w = logits.new_empty(shape, dtype=torch.float32)
     _launch(logits, library().mhsa_route, logits.data_ptr(), _act_code(logits.dtype), rows, n, ld, ROUTE_SCORES[score],

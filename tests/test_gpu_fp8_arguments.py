@@ -1,4 +1,5 @@
-"""Arguments that are not tensors are refused as any other wrong argument."""
+"""Arguments that are not tensors, and numbers of choices that no row has, are
+refused as any other wrong argument."""
 import numpy as np
 import pytest
 import torch
@@ -12,6 +13,13 @@ pytestmark = pytest.mark.gpu
 def test_route_bias(bad):
     with pytest.raises(M.MhsaError):
         M.route(torch.zeros(3, 8, device="cuda"), 2, bias=bad)
+
+
+@pytest.mark.parametrize("top_k", [-1, 0, 9, 1 << 31, 1 << 40])
+def test_route_choices(top_k):
+    """Refused before memory is taken for the results."""
+    with pytest.raises(M.MhsaError):
+        M.route(torch.zeros(30000, 8, device="cuda"), top_k)
 
 
 @pytest.mark.parametrize("bad", [None, 3, [[0], [1]], np.zeros((2, 1), np.int32)])
