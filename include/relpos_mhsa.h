@@ -616,6 +616,54 @@ int32_t mhsa_experts_forward(const mhsa_experts* experts, const void* x, int32_t
                              const int32_t* indices, const float* weights, int32_t top_k, const void* residual,
                              float res_scale, void* out, void* workspace, int64_t workspace_bytes, void* hip_stream);
 
+/* ---- operators on rows -------------------------------------------------------- */
+
+/* No counterpart in the reference. Neither call has a handle, waits, or keeps
+ * anything; both may be captured, and run at once with others on other streams.
+ * They run on the current GPU, on a stream of it. */
+
+/* A residual's addition with the norm behind it, over rows of dim values
+ * (dim <= 32768):
+ *   v = x + delta_scale * delta (delta NULL: v = x); sum = v
+ *   MHSA_NORM_RMS:   y = v / sqrt(mean(v^2) + eps) * weight + bias
+ *   MHSA_NORM_LAYER: y = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias
+ * x, delta and sum in dtype, y in out (NULL without) in out_dtype (MHSA_F32 or
+ * MHSA_BF16 each), rows a stride apart; weight and bias [dim] device f32 (NULL:
+ * ones, zeros). y is taken from v before sum's rounding, all in f32, whose
+ * squares are to have a sum below 2^127.
+ * codes and scales (NULL without): y as mhsa_fp8_linear_forward would round it,
+ * for mhsa_fp8_linear_forward_rounded: codes [rows, ceil(dim/128) * 128], zeros
+ * past dim, scales [rows, ceil(dim/128) rounded up to 4], 127 past the last
+ * block; 16-byte aligned.
+ * sum may be NULL. sum and out may each be x or delta (the same rows, in place);
+ * otherwise results overlap nothing. rows may be 0. */
+#define MHSA_NORM_RMS 0
+#define MHSA_NORM_LAYER 1
+int32_t mhsa_add_norm(const void* x, int32_t dtype, int32_t rows, int32_t dim, int64_t x_stride, const void* delta,
+                      int64_t delta_stride, float delta_scale, void* sum, int64_t sum_stride, int32_t kind,
+                      const float* weight, const float* bias, float eps, void* out, int32_t out_dtype, int64_t out_stride,
+                      uint8_t* codes, uint8_t* scales, void* hip_stream);
+
+/* Of rows of logits [rows, vocab] (MHSA_F32 or MHSA_BF16, device, rows `stride`
+ * elements apart), p = softmax(logits / temperature), temperature in [0.01, 100]:
+ *   log_probs [rows, n_tokens] f32: log p of tokens [rows, n_tokens] int32; of
+ *     a token outside [0, vocab) 0 (padding).
+ *   entropy [rows] f32 (NULL without): -sum p log p.
+ *   top_indices int32 and top_log_probs f32 [rows, top_k]: the top_k largest
+ *     logits, largest first, ties to the lower index, and their log p. Logits of
+ *     -inf and NaN are not among them: where fewer are left, -1 and -inf.
+ * A row whose logits are all -inf has log_probs -inf and entropy 0; a row that
+ * holds a NaN or +inf has NaN for both and for its alternatives' log p. All in f32.
+ * vocab <= 2^24, top_k <= 32, n_tokens <= 1024, both may be 0, as may rows.
+ * Results and the workspace overlap nothing. */
+int32_t mhsa_token_log_probs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t stride,
+                             float temperature, const int32_t* tokens, int32_t n_tokens, float* log_probs, float* entropy,
+                             int32_t top_k, int32_t* top_indices, float* top_log_probs, void* workspace,
+                             int64_t workspace_bytes, void* hip_stream);
+/* Workspace bytes of a call of `rows` rows or fewer (0: none; -1 for bad
+ * arguments). */
+int64_t mhsa_token_log_probs_workspace(int32_t rows, int32_t vocab, int32_t top_k);
+
 /* ---- encoder-level streaming ---------------------------------------------- */
 
 /* The per-chunk layer loop of ConformerEncoder::forward_streaming

@@ -11,18 +11,10 @@
 #include <new>
 #include <vector>
 
+#include "api_common.hpp"
 #include "fp8_kernels.hpp"
-#include "host_common.hpp"
-#include "kernels.hpp"
-
-using mhsa::DType;
 
 namespace {
-
-// Bounds under which no size or offset below leaves 63 bits and no grid has
-// 2^32 threads along one axis.
-constexpr int32_t kMaxRows = 1 << 25, kMaxOut = 1 << 22;
-constexpr int64_t kMaxStride = 1 << 30;
 
 // n weight matrices [N, K] in the kernels' format.
 struct Fp8Weights {
@@ -34,22 +26,6 @@ struct Fp8Weights {
   int64_t scale_stride() const { return (int64_t)((N + 127) / 128) * mhsa::fp8_kbp(K); }
   int64_t scale_in() const { return (int64_t)((N + 127) / 128) * ((K + 127) / 128); }
 };
-
-// Whether p is memory of the current GPU (true) or host memory (false).
-int32_t on_device(const void* p, bool* yes) {
-  hipPointerAttribute_t a{};
-  *yes = false;
-  if (hipPointerGetAttributes(&a, p) != hipSuccess) {
-    (void)hipGetLastError();  // memory that HIP does not know: the host's
-    return MHSA_OK;
-  }
-  if (a.type != hipMemoryTypeDevice) return MHSA_OK;
-  int dev = 0;
-  HIPCHK(hipGetDevice(&dev));
-  if (a.device != dev) return fail(MHSA_EINVAL, "the tensor is on GPU %d, the current GPU is %d", a.device, dev);
-  *yes = true;
-  return MHSA_OK;
-}
 
 // The bias, or zeros without one, and zeros behind it.
 int32_t load_bias(Fp8Weights& w, int data_dtype, const void* bias) {
@@ -124,48 +100,6 @@ int32_t load_weights(Fp8Weights& w, int data_dtype, const void* weight, const ui
 } catch (const std::bad_alloc&) {
   return fail(MHSA_ENOMEM, "out of host memory");
 }
-
-// Weights are where they were loaded.
-int32_t check_device(int device) {
-  int dev = 0;
-  HIPCHK(hipGetDevice(&dev));
-  if (dev != device) return fail(MHSA_EINVAL, "the weights are on GPU %d, the current GPU is %d", device, dev);
-  return MHSA_OK;
-}
-
-bool act_dtype(int32_t d, DType* out) {
-  *out = d == MHSA_BF16 ? mhsa::kBF16 : mhsa::kF32;
-  return d == MHSA_F32 || d == MHSA_BF16;
-}
-
-bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
-}
-
-// Whether rows of na bytes from a on, pa bytes apart, and rows of nb bytes from
-// b on share bytes. Rows of two tensors in one buffer side by side (the same
-// distance, none within the other's) do not; of two that are interleaved in any
-// other way it is taken that they do.
-bool rows_overlap(const void* a, int64_t na, int64_t pa, const void* b, int64_t nb, int64_t pb, int64_t rows) {
-  if (!overlap(a, (rows - 1) * pa + na, b, (rows - 1) * pb + nb)) return false;
-  if (pa != pb) return true;
-  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
-  const int64_t at = (off % pa + pa) % pa;  // of b's rows within a's distance
-  return at < na || at + nb > pa;
-}
-
-// Hands out 256-byte aligned pieces of a workspace (or only adds them up).
-struct Arena {
-  char* base;
-  int64_t used = 0;
-  explicit Arena(void* p) : base(static_cast<char*>(p)) {}
-  template <typename T> T* take(int64_t n) {
-    T* p = reinterpret_cast<T*>(base + used);
-    used = align_up(used + n * (int64_t)sizeof(T), 256);
-    return p;
-  }
-};
 
 }  // namespace
 

@@ -1,0 +1,169 @@
+// A residual's addition with its norm, as floats or as 8-bit codes.
+//
+//   v = x + a d                                   (f32; sum: v rounded once)
+//   rms:   y = v / sqrt(mean(v^2) + eps) * w + b
+//   layer: y = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * w + b
+//
+// A row lies in the registers of its W waves, 8 columns to a lane and chunk, so
+// that x and d are read once whatever the norm needs, the variance is taken
+// around the mean itself, and results may lie over their inputs. 16 lanes hold a
+// block of 128 columns: its largest magnitude is four DPP steps, and a wave's
+// four blocks of a chunk are one word of scale bytes. Bound: HBM, one pass.
+#include <algorithm>
+
+#include "fp8_common.hpp"
+#include "fp8_kernels.hpp"
+#include "row_kernels.hpp"
+
+namespace mhsa {
+namespace {
+
+// 8 values to columns [c, c + 8) of a row of D.
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int c, int D, const float v[8]) {
+  T t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
+  if (c + 8 <= D) {
+    __builtin_memcpy(row + c, t, sizeof t);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < D) row[c + e] = t[e];
+  }
+}
+
+template <typename T, int CH, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormParams p) {
+  constexpr int RPB = W == 1 ? 4 : 1;  // rows of a workgroup at a time
+  __shared__ float red[4][W];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wr = W == 1 ? 0 : wv;
+  const int kb = (p.D + 127) / 128, kbp = (kb + 3) / 4 * 4;
+  auto col = [&](int i) { return 8 * (64 * (wr + W * i) + lane); };
+  float w[CH][8], b[CH][8];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[i][e] = 1.f, b[i][e] = 0.f;
+    if (p.w) load8(p.w, col(i), p.D, w[i]);
+    if (p.b) load8(p.b, col(i), p.D, b[i]);
+  }
+  const float n = 1.f / (float)p.D;
+  int turn = 0;  // (a row's sums lie where no wave still reads the last row's)
+  auto total = [&](float v, int which) {
+    v = wave_reduce(v, [](float a, float c) { return a + c; });
+    if constexpr (W > 1) {
+      float* r = red[2 * turn + which];
+      if (lane == 0) r[wr] = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v += r[i];
+    }
+    return v;
+  };
+  for (int64_t row = (int64_t)blockIdx.x * RPB + (W == 1 ? wv : 0); row < p.rows; row += (int64_t)gridDim.x * RPB) {
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    float v[CH][8];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) load8(x, col(i), p.D, v[i]);
+    if (p.delta) {
+      const T* d = static_cast<const T*>(p.delta) + row * p.ldd;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        float t[8];
+        load8(d, col(i), p.D, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(p.scale, t[e], v[i][e]);
+      }
+    }
+    if (p.sum) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) store8(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
+    }
+    if (p.layer) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[i][e];
+      const float mean = total(s, 0) * n;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = col(i) + e < p.D ? v[i][e] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q = __builtin_fmaf(v[i][e], v[i][e], q);
+    const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(total(q, 1), n, p.eps));
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(v[i][e] * r, w[i][e], b[i][e]);
+    if (p.out) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        if (p.out_dt == kBF16) store8(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+        else store8(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+      }
+    }
+    if (p.codes) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int word = wr + W * i;  // of the row's scale bytes
+        if (4 * word >= kb) continue;
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (col(i) + e >= p.D) v[i][e] = 0.f;  // (b and NaN sums reach there too)
+          m = fmaxf(m, fp8_mag(v[i][e]));
+        }
+        m = row_reduce(m, [](float a, float c) { return fmaxf(a, c); });
+        const int s = fp8_scale_byte(m);
+        const float scale = fp8_scale(s);
+        if (col(i) < kb * 128)
+          *reinterpret_cast<u32x2*>(p.codes + row * ((int64_t)kb * 128) + col(i)) =
+              u32x2{fp8_pack4_scaled(v[i][0], v[i][1], v[i][2], v[i][3], scale),
+                    fp8_pack4_scaled(v[i][4], v[i][5], v[i][6], v[i][7], scale)};
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          bytes |= (uint32_t)(4 * word + j < kb ? __builtin_amdgcn_readlane(s, 16 * j) : 127) << 8 * j;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + row * kbp + 4 * word) = bytes;
+      }
+    }
+  }
+}
+
+template <typename T, int CH, int W>
+hipError_t launch(const NormParams& p, hipStream_t s) {
+  if ((int64_t)512 * CH * W < p.D) return hipErrorInvalidValue;
+  const int64_t groups = W == 1 ? (p.rows + 3) / 4 : p.rows;
+  const unsigned grid = (unsigned)std::min<int64_t>(groups, 1 << 16);
+  add_norm_kernel<T, CH, W><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t by_width(const NormParams& p, hipStream_t s) {
+  if (p.D <= 512) return launch<T, 1, 1>(p, s);
+  if (p.D <= 1024) return launch<T, 2, 1>(p, s);
+  if (p.D <= 2048) return launch<T, 1, 4>(p, s);
+  if (p.D <= 4096) return launch<T, 2, 4>(p, s);
+  if (p.D <= 8192) return launch<T, 4, 4>(p, s);
+  return p.D <= 16384 ? launch<T, 2, 16>(p, s) : launch<T, 4, 16>(p, s);
+}
+
+}  // namespace
+
+hipError_t add_norm(const NormParams& p, hipStream_t s) {
+  if (p.rows <= 0 || p.D <= 0 || p.D > kNormMaxD || !p.x || (p.codes != nullptr) != (p.scales != nullptr))
+    return hipErrorInvalidValue;
+  return p.dt == kBF16 ? by_width<bf16>(p, s) : by_width<float>(p, s);
+}
+
+}  // namespace mhsa

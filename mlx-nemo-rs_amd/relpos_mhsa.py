@@ -17,7 +17,7 @@ from __future__ import annotations
 import ctypes
 import os
 from dataclasses import dataclass
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Dict, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -61,6 +61,7 @@ EXPORTS = (
     "mhsa_fp8_linear_read_codes", "mhsa_fp8_linear_workspace", "mhsa_fp8_linear_forward", "mhsa_route",
     "mhsa_experts_create", "mhsa_experts_destroy", "mhsa_experts_load", "mhsa_experts_load_codes",
     "mhsa_experts_workspace", "mhsa_experts_forward",
+    "mhsa_add_norm", "mhsa_token_log_probs", "mhsa_token_log_probs_workspace",
 )
 
 
@@ -221,6 +222,9 @@ def library(path: str = LIB_PATH) -> ctypes.CDLL:
         "mhsa_experts_load_codes": (I, [VP, VP, VP, VP, VP, VP, VP]),
         "mhsa_experts_workspace": (L, [VP, I, I]),
         "mhsa_experts_forward": (I, [VP, VP, I, I, VP, VP, I, VP, F, VP, VP, L, VP]),
+        "mhsa_add_norm": (I, [VP, I, I, I, L, VP, L, F, VP, L, I, VP, VP, F, VP, I, L, VP, VP, VP]),
+        "mhsa_token_log_probs": (I, [VP, I, I, I, L, F, VP, I, VP, VP, I, VP, VP, VP, L, VP]),
+        "mhsa_token_log_probs_workspace": (L, [I, I, I]),
     })
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -774,6 +778,131 @@ class ExpertFeedForward:
                 top_k, None if residual is None else residual.data_ptr(), float(res_scale), out.data_ptr(), ws.data_ptr(),
                 max(need, 0))
         return out
+
+
+# ---------------------------------------------------------------------------
+# Operators on rows
+# ---------------------------------------------------------------------------
+
+class Fp8Rows:
+    """Rows [..., width] rounded to e4m3 codes with a power of two for each
+    row's 128 values, as Fp8Linear rounds its activations: codes uint8 [rows,
+    ceil(width / 128) * 128], scales uint8 [rows, ceil(width / 128) rounded up
+    to 4] (value = code * 2^(scale - 127))."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+
+
+class Normed(NamedTuple):
+    out: object    # [..., dim] or None
+    codes: object  # Fp8Rows or None
+    sum: object    # [..., dim] or None
+
+
+NORM_KINDS = {"rms": 0, "layer": 1}
+
+
+def _beside(t, x, name):
+    """Checks that t is a GPU tensor of x's shape on its GPU, rows evenly
+    spaced; returns its row stride."""
+    if not hasattr(t, "get_device") or t.get_device() != x.get_device() or t.shape != x.shape:
+        raise MhsaError(MHSA_EINVAL, f"{name}: expected {tuple(x.shape)} on {x.device}")
+    return _rows_of(t, x.shape[-1])[1]
+
+
+def add_norm(x, delta=None, weight=None, bias=None, kind: str = "rms", eps: float = 1e-5, scale: float = 1.0,
+             want: str = "out", out_dtype=None, out=None, sum_out=None) -> Normed:
+    """v = x + scale * delta and its norm ("rms" or "layer") times weight plus
+    bias (mhsa_add_norm); x and delta [..., dim] float32 or bfloat16, rows evenly
+    spaced, weight and bias [dim] float32. want: "out" (in out_dtype, x's by
+    default, or in `out`), "codes" (Fp8Rows for Fp8Linear) or "both". With a
+    delta, v also comes as `sum`, in `sum_out` if given (x or delta: in place);
+    sum_out alone copies x."""
+    import torch
+    if kind not in NORM_KINDS:
+        raise MhsaError(MHSA_ENOTSUP, f"norm `{kind}` (only rms and layer are supported)")
+    if want not in ("out", "codes", "both"):
+        raise MhsaError(MHSA_EINVAL, f"want `{want}` (out, codes or both)")
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise MhsaError(MHSA_EINVAL, "expected a GPU tensor [..., dim]")
+    d = x.shape[-1]
+    rows, ldx = _rows_of(x, d)
+    code = _act_code(x.dtype)
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != x.get_device() or t.dtype != torch.float32
+                              or tuple(t.shape) != (d,) or not t.is_contiguous()):
+            raise MhsaError(MHSA_EINVAL, f"{name}: expected a contiguous float32 tensor [{d}] on {x.device}")
+    ldd = lds = ldo = 0
+    for t, name in ((delta, "delta"), (sum_out, "sum_out")):
+        if t is not None and getattr(t, "dtype", None) != x.dtype:
+            raise MhsaError(MHSA_EINVAL, f"{name}: expected {x.dtype}")
+    if delta is not None:
+        ldd = _beside(delta, x, "delta")
+        if sum_out is None:
+            sum_out = x.new_empty(x.shape)
+    if sum_out is not None:
+        lds = _beside(sum_out, x, "sum_out")
+    rounded = None
+    if want == "codes":
+        if out is not None or out_dtype is not None:
+            raise MhsaError(MHSA_EINVAL, "out and out_dtype are for float results")
+    else:
+        if out is None:
+            out = x.new_empty(x.shape, dtype=x.dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
+        elif out_dtype is not None and _dtype_code(out_dtype) != _dtype_code(out.dtype):
+            raise MhsaError(MHSA_EINVAL, f"out is not {out_dtype}")
+        ldo = _beside(out, x, "out")
+    if want != "out":
+        kb = (d + 127) // 128
+        rounded = Fp8Rows(x.new_empty((rows, kb * 128), dtype=torch.uint8),
+                          x.new_empty((rows, (kb + 3) // 4 * 4), dtype=torch.uint8), x.shape)
+    _launch(x, library().mhsa_add_norm, x.data_ptr(), code, rows, d, ldx, None if delta is None else delta.data_ptr(), ldd,
+            float(scale), None if sum_out is None else sum_out.data_ptr(), lds, NORM_KINDS[kind],
+            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), float(eps),
+            None if out is None else out.data_ptr(), code if out is None else _act_code(out.dtype), ldo,
+            None if rounded is None else rounded.codes.data_ptr(), None if rounded is None else rounded.scales.data_ptr())
+    return Normed(out, rounded, sum_out)
+
+
+class TokenScores(NamedTuple):
+    log_probs: object      # like tokens, float32, or None
+    entropy: object        # [...] float32
+    top_indices: object    # [..., top_k] int32, or None
+    top_log_probs: object  # [..., top_k] float32, or None
+
+
+def token_log_probs(logits, tokens=None, top_k: int = 0, temperature: float = 1.0) -> TokenScores:
+    """Log probabilities of tokens int32 [...] or [..., n] (outside the
+    vocabulary: 0), entropy, and the top_k likeliest tokens of logits [...,
+    vocab] float32 or bfloat16, rows evenly spaced (mhsa_token_log_probs)."""
+    import torch
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
+        raise MhsaError(MHSA_EINVAL, "expected a GPU tensor [..., vocab]")
+    v = logits.shape[-1]
+    rows, ld = _rows_of(logits, v)
+    lead, n = logits.shape[:-1], 0
+    if tokens is not None:
+        if (not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int32 or tokens.get_device() != logits.get_device()
+                or not tokens.is_contiguous() or (tokens.shape != lead and tokens.shape[:-1] != lead)):
+            raise MhsaError(MHSA_EINVAL, f"tokens: expected contiguous int32 {tuple(lead)} or {(*lead, 'n')} on {logits.device}")
+        n = 1 if tokens.shape == lead else tokens.shape[-1]
+    if top_k < 0 or top_k > v:  # (before there is memory for them)
+        raise MhsaError(MHSA_EINVAL, f"top_k {top_k} is not in [0, {v}]")
+    lp = None if tokens is None else logits.new_empty(tokens.shape, dtype=torch.float32)
+    h = logits.new_empty(lead, dtype=torch.float32)
+    idx = logits.new_empty((*lead, top_k), dtype=torch.int32) if top_k else None
+    top = logits.new_empty((*lead, top_k), dtype=torch.float32) if top_k else None
+    lib = library()
+    need = lib.mhsa_token_log_probs_workspace(rows, v, top_k)
+    ws = logits.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    _launch(logits, lib.mhsa_token_log_probs, logits.data_ptr(), _act_code(logits.dtype), rows, v, ld, float(temperature),
+            tokens.data_ptr() if n else None, n, lp.data_ptr() if n else None, h.data_ptr(), top_k,
+            idx.data_ptr() if top_k else None, top.data_ptr() if top_k else None, ws.data_ptr() if need > 0 else None,
+            max(need, 0))
+    return TokenScores(lp, h, idx, top)
 
 
 CONV_BATCH_NORM, CONV_LAYER_NORM = 0, 1
