@@ -564,6 +564,44 @@ int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* linear, const void* x, in
                                 int64_t x_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
                                 int64_t workspace_bytes, void* hip_stream);
 
+/* The same from rows that are codes already, as mhsa_add_norm writes them: codes
+ * [rows, ceil(in_dim/128) * 128], zeros past in_dim, and scales [rows,
+ * ceil(in_dim/128) rounded up to 4], 16-byte aligned. The result is that of
+ * mhsa_fp8_linear_forward on rows whose rounding gives these codes. adapters
+ * (NULL without) as below, on the values that the codes stand for; a workspace
+ * only with them. */
+typedef struct mhsa_adapters mhsa_adapters;
+int32_t mhsa_fp8_linear_forward_rounded(const mhsa_fp8_linear* linear, const uint8_t* codes, const uint8_t* scales,
+                                        int32_t rows, const mhsa_adapters* adapters, const int32_t* which, void* out,
+                                        int32_t out_dtype, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                        void* hip_stream);
+
+/* Low-rank adapters of many requests beside a projection:
+ *   y_r = W q(x_r) + b + s_a B_a (A_a x_r), a = which[r],
+ * A_a [rank, in_dim], B_a [out_dim, rank] held in bf16, which [rows] device
+ * int32; a row whose a is outside [0, n_adapters) has none. x enters A_a x
+ * unrounded. The inner sums are f32, and are rounded to bf16 for a bf16 y. Up to
+ * 4096 adapters of up to max_rank <= 128 each, side by side in memory that the
+ * first load takes: n_adapters * (in_dim + out_dim) * 2 bytes * (max_rank rounded
+ * up to 16, 32, 64 or 128). */
+int32_t mhsa_adapters_create(int32_t in_dim, int32_t out_dim, int32_t n_adapters, int32_t max_rank, mhsa_adapters** out);
+void mhsa_adapters_destroy(mhsa_adapters* adapters);
+/* Adapter `slot`: a [rank, in_dim], b [out_dim, rank] in data_dtype (MHSA_F32 /
+ * MHSA_BF16 / MHSA_F16; host or device memory), finite after their rounding to
+ * bf16; rank 0 (a and b NULL) empties the slot, as all are before their first
+ * load. Waits for the GPU; no call that reads the adapters may run at the same
+ * time, other slots' either. A refused load leaves the slot as it was. */
+int32_t mhsa_adapters_load(mhsa_adapters* adapters, int32_t slot, int32_t rank, int32_t data_dtype, const void* a,
+                           const void* b, float scale);
+/* Workspace bytes of a call with adapters of `rows` rows or fewer, on floats or
+ * on codes (-1 for bad arguments). */
+int64_t mhsa_fp8_linear_adapted_workspace(const mhsa_fp8_linear* linear, const mhsa_adapters* adapters, int32_t rows);
+/* mhsa_fp8_linear_forward with adapters (NULL: without). */
+int32_t mhsa_fp8_linear_forward_adapted(const mhsa_fp8_linear* linear, const void* x, int32_t x_dtype, int32_t rows,
+                                        int64_t x_stride, const mhsa_adapters* adapters, const int32_t* which, void* out,
+                                        int32_t out_dtype, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                        void* hip_stream);
+
 /* Routing of frames to experts from the gate's logits [rows, n_experts]
  * (MHSA_F32 or MHSA_BF16, device, rows `stride` elements apart):
  *   s = softmax(logits) or sigmoid(logits); c = s + bias (bias [n_experts]

@@ -1,5 +1,5 @@
-// C ABI of the 8-bit block-scaled projection, the routing of frames to
-// experts and the experts' FeedForward. The handles hold weights alone, laid
+// C ABI of the 8-bit block-scaled projection and the low-rank adapters beside
+// it, the routing of frames to experts and the experts' FeedForward. The handles hold weights alone, laid
 // out once at loading; a forward call takes its scratch memory from the
 // caller, so calls on one handle may run at once on different streams, and
 // captured graphs share nothing.
@@ -26,6 +26,8 @@ struct Fp8Weights {
   int64_t scale_stride() const { return (int64_t)((N + 127) / 128) * mhsa::fp8_kbp(K); }
   int64_t scale_in() const { return (int64_t)((N + 127) / 128) * ((K + 127) / 128); }
 };
+
+constexpr int32_t kMaxAdapters = 4096, kMaxRank = 128;
 
 // The bias, or zeros without one, and zeros behind it.
 int32_t load_bias(Fp8Weights& w, int data_dtype, const void* bias) {
@@ -111,24 +113,123 @@ struct mhsa_fp8_linear {
   Fp8Weights w;
 };
 
+// Adapters [n]: A [rank, Kp] and B [N, rank] bf16 each, zeros past an adapter's
+// own rank (and for one that is not loaded), and its scale.
+struct mhsa_adapters {
+  int n = 0, K = 0, N = 0, rank = 0;  // rank: 16, 32, 64 or 128
+  int max_rank = 0, device = -1;
+  bool loaded = false;
+  DevBuf a, b, scale;
+  int64_t a_stride() const { return (int64_t)rank * mhsa::fp8_kp(K); }
+  int64_t b_stride() const { return (int64_t)N * rank; }
+};
+
 namespace {
+
+// What a projection reads: floats, or rows that are codes already.
+struct LinearInput {
+  const void* x = nullptr;
+  DType dt = mhsa::kF32;
+  int64_t ld = 0;
+  const uint8_t* codes = nullptr;
+  const uint8_t* scales = nullptr;
+};
 
 struct LinearPlan {
   bool few = false;
-  uint8_t* codes = nullptr;
+  uint8_t* codes = nullptr;  // of floats, for the tiles
   uint8_t* scales = nullptr;
+  uint16_t* t = nullptr;
   int64_t bytes = 0;
 };
 
-LinearPlan linear_plan(const Fp8Weights& w, int64_t rows, void* ws) {
+// rank 0: no adapters. A row of t takes as much whatever the result's dtype, so
+// that a workspace serves both.
+LinearPlan linear_plan(const Fp8Weights& w, int64_t rows, void* ws, int rank = 0, bool coded = false) {
   LinearPlan p;
   p.few = mhsa::fp8_few_rows(rows, w.N, w.K);
-  if (p.few) return p;
   Arena a(ws);
-  p.codes = a.take<uint8_t>(rows * mhsa::fp8_kp(w.K));
-  p.scales = a.take<uint8_t>(rows * mhsa::fp8_kbp(w.K));
+  if (!p.few && !coded) {
+    p.codes = a.take<uint8_t>(rows * mhsa::fp8_kp(w.K));
+    p.scales = a.take<uint8_t>(rows * mhsa::fp8_kbp(w.K));
+  }
+  if (rank) p.t = a.take<uint16_t>(rows * 3 * rank);
   p.bytes = a.used;
   return p;
+}
+
+// Checks of a projection's call, all but those of its input; the workspace is
+// `plan`'s.
+int32_t linear_check(const Fp8Weights& w, int32_t rows, const void* out, int32_t out_dtype, int64_t out_stride, DType* od) {
+  if (!act_dtype(out_dtype, od)) return fail(MHSA_ENOTSUP, "dtype %d not supported (f32, bf16)", out_dtype);
+  if (rows < 0) return fail(MHSA_EINVAL, "rows must not be negative (got %d)", rows);
+  if (rows > kMaxRows) return fail(MHSA_ENOTSUP, "%d rows exceed %d", rows, kMaxRows);
+  if (rows == 0) return MHSA_OK;
+  if (!out) return fail(MHSA_EINVAL, "null tensor pointer");
+  if (reinterpret_cast<uintptr_t>(out) % mhsa::dtype_size(*od))
+    return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
+  if (out_stride < w.N) return fail(MHSA_EINVAL, "row stride %lld is shorter than the row (%d)", (long long)out_stride, w.N);
+  if (out_stride > kMaxStride) return fail(MHSA_ENOTSUP, "row stride %lld exceeds 2^30", (long long)out_stride);
+  return MHSA_OK;
+}
+
+int32_t linear_run(const Fp8Weights& w, const LinearInput& in, int32_t rows, const mhsa_adapters* ad, const int32_t* which,
+                   void* out, DType od, int64_t out_stride, const LinearPlan& plan, hipStream_t s) {
+  mhsa::Fp8Gemm p;
+  p.w = static_cast<const uint8_t*>(w.codes.p);
+  p.ws = static_cast<const uint8_t*>(w.scales.p);
+  p.bias = static_cast<const float*>(w.bias.p);
+  p.M = rows;
+  p.N = w.N;
+  p.K = w.K;
+  p.out = out;
+  p.out_dt = od;
+  p.ldo = out_stride;
+  p.a = in.codes ? in.codes : plan.codes;
+  p.as = in.codes ? in.scales : plan.scales;
+  p.a_rows = rows;
+  if (ad) {
+    mhsa::AdapterRows r;
+    r.x = in.x;
+    r.x_dt = in.dt;
+    r.ldx = in.ld;
+    r.rows = rows;
+    r.K = w.K;
+    r.codes = in.codes;
+    r.scales = in.scales;
+    r.which = p.ad.which = which;
+    r.n = p.ad.n = ad->n;
+    r.rank = p.ad.rank = ad->rank;
+    r.parts = p.ad.parts = od == mhsa::kBF16 ? 1 : 3;
+    r.a = static_cast<const uint16_t*>(ad->a.p);
+    r.scale = static_cast<const float*>(ad->scale.p);
+    r.t = plan.t;
+    r.q_codes = plan.codes;
+    r.q_scales = plan.scales;
+    p.ad.t = plan.t;
+    p.ad.b = static_cast<const uint16_t*>(ad->b.p);
+    HIPCHK(mhsa::adapter_rows(r, s));
+  }
+  if (plan.few) {
+    p.x = in.x;
+    p.x_dt = in.dt;
+    p.ldx = in.ld;
+    HIPCHK(mhsa::fp8_gemm_few(p, s));
+    return MHSA_OK;
+  }
+  if (!in.codes && !ad) HIPCHK(mhsa::fp8_quantize_rows(in.dt, in.x, in.ld, rows, w.K, plan.codes, plan.scales, s));
+  HIPCHK(mhsa::fp8_gemm_tile(p, s));
+  return MHSA_OK;
+}
+
+// Adapters that fit a projection and are where it is.
+int32_t adapters_check(const mhsa_adapters* ad, const Fp8Weights& w, const int32_t* which) {
+  if (ad->K != w.K || ad->N != w.N)
+    return fail(MHSA_EINVAL, "adapters of %d -> %d beside a projection of %d -> %d", ad->K, ad->N, w.K, w.N);
+  if (!ad->loaded) return fail(MHSA_EINVAL, "no adapter is loaded");
+  if (!which) return fail(MHSA_EINVAL, "null tensor pointer");
+  if (reinterpret_cast<uintptr_t>(which) % 4) return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
+  return check_device(ad->device);
 }
 
 }  // namespace
@@ -191,54 +292,162 @@ int64_t mhsa_fp8_linear_workspace(const mhsa_fp8_linear* h, int32_t rows) {
 int32_t mhsa_fp8_linear_forward(const mhsa_fp8_linear* h, const void* x, int32_t x_dtype, int32_t rows,
                                 int64_t x_stride, void* out, int32_t out_dtype, int64_t out_stride, void* workspace,
                                 int64_t workspace_bytes, void* hs) {
+  return mhsa_fp8_linear_forward_adapted(h, x, x_dtype, rows, x_stride, nullptr, nullptr, out, out_dtype, out_stride, workspace,
+                                         workspace_bytes, hs);
+}
+
+int32_t mhsa_fp8_linear_forward_adapted(const mhsa_fp8_linear* h, const void* x, int32_t x_dtype, int32_t rows, int64_t x_stride,
+                                        const mhsa_adapters* adapters, const int32_t* which, void* out, int32_t out_dtype,
+                                        int64_t out_stride, void* workspace, int64_t workspace_bytes, void* hs) {
   if (!h) return fail(MHSA_EINVAL, "null handle");
   const Fp8Weights& w = h->w;
-  DType xd, od;
-  if (!act_dtype(x_dtype, &xd) || !act_dtype(out_dtype, &od))
-    return fail(MHSA_ENOTSUP, "dtypes %d and %d not supported (f32, bf16)", x_dtype, out_dtype);
-  if (rows < 0) return fail(MHSA_EINVAL, "rows must not be negative (got %d)", rows);
-  if (rows > kMaxRows) return fail(MHSA_ENOTSUP, "%d rows exceed %d", rows, kMaxRows);
+  LinearInput in;
+  DType od;
+  if (!act_dtype(x_dtype, &in.dt)) return fail(MHSA_ENOTSUP, "dtype %d not supported (f32, bf16)", x_dtype);
+  if (int32_t rc = linear_check(w, rows, out, out_dtype, out_stride, &od)) return rc;
   if (rows == 0) return MHSA_OK;
-  if (!x || !out) return fail(MHSA_EINVAL, "null tensor pointer");
-  const int xs = mhsa::dtype_size(xd), os = mhsa::dtype_size(od);
-  if (reinterpret_cast<uintptr_t>(x) % xs || reinterpret_cast<uintptr_t>(out) % os)
-    return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
-  if (x_stride < w.K || out_stride < w.N)
-    return fail(MHSA_EINVAL, "row strides %lld and %lld are shorter than the rows (%d, %d)", (long long)x_stride,
-                (long long)out_stride, w.K, w.N);
-  if (x_stride > kMaxStride || out_stride > kMaxStride)
-    return fail(MHSA_ENOTSUP, "row strides %lld and %lld exceed 2^30", (long long)x_stride, (long long)out_stride);
+  if (!x) return fail(MHSA_EINVAL, "null tensor pointer");
+  const int xs = mhsa::dtype_size(in.dt), os = mhsa::dtype_size(od);
+  if (reinterpret_cast<uintptr_t>(x) % xs) return fail(MHSA_EINVAL, "device tensors must be aligned to their elements");
+  if (x_stride < w.K) return fail(MHSA_EINVAL, "row stride %lld is shorter than the row (%d)", (long long)x_stride, w.K);
+  if (x_stride > kMaxStride) return fail(MHSA_ENOTSUP, "row stride %lld exceeds 2^30", (long long)x_stride);
   if (!w.loaded) return fail(MHSA_EINVAL, "no weights are loaded");
-  const LinearPlan plan = linear_plan(w, rows, workspace);
+  const LinearPlan plan = linear_plan(w, rows, workspace, adapters ? adapters->rank : 0);
   if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes))
     return fail(MHSA_EINVAL, "%d rows need a 16-byte aligned workspace of %lld bytes", rows, (long long)plan.bytes);
   const int64_t xn = ((rows - 1) * x_stride + w.K) * xs, on = ((rows - 1) * out_stride + w.N) * os;
-  if (rows_overlap(x, w.K * xs, x_stride * xs, out, w.N * os, out_stride * os, rows) || overlap(workspace, plan.bytes, x, xn) || overlap(workspace, plan.bytes, out, on))
+  const int64_t wn = adapters ? (int64_t)rows * 4 : 0;
+  if (rows_overlap(x, w.K * xs, x_stride * xs, out, w.N * os, out_stride * os, rows) || overlap(workspace, plan.bytes, x, xn) ||
+      overlap(workspace, plan.bytes, out, on) || overlap(which, wn, out, on) || overlap(which, wn, workspace, plan.bytes))
     return fail(MHSA_EINVAL, "x, out and the workspace must not overlap");
   if (int32_t rc = check_device(w.device)) return rc;
-  hipStream_t s = static_cast<hipStream_t>(hs);
-  mhsa::Fp8Gemm p;
-  p.w = static_cast<const uint8_t*>(w.codes.p);
-  p.ws = static_cast<const uint8_t*>(w.scales.p);
-  p.bias = static_cast<const float*>(w.bias.p);
-  p.M = rows;
-  p.N = w.N;
-  p.K = w.K;
-  p.out = out;
-  p.out_dt = od;
-  p.ldo = out_stride;
-  if (plan.few) {
-    p.x = x;
-    p.x_dt = xd;
-    p.ldx = x_stride;
-    HIPCHK(mhsa::fp8_gemm_few(p, s));
-    return MHSA_OK;
+  if (adapters)
+    if (int32_t rc = adapters_check(adapters, w, which)) return rc;
+  in.x = x;
+  in.ld = x_stride;
+  return linear_run(w, in, rows, adapters, which, out, od, out_stride, plan, static_cast<hipStream_t>(hs));
+}
+
+int32_t mhsa_fp8_linear_forward_rounded(const mhsa_fp8_linear* h, const uint8_t* codes, const uint8_t* scales, int32_t rows,
+                                        const mhsa_adapters* adapters, const int32_t* which, void* out, int32_t out_dtype,
+                                        int64_t out_stride, void* workspace, int64_t workspace_bytes, void* hs) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  const Fp8Weights& w = h->w;
+  DType od;
+  if (int32_t rc = linear_check(w, rows, out, out_dtype, out_stride, &od)) return rc;
+  if (rows == 0) return MHSA_OK;
+  if (!codes || !scales) return fail(MHSA_EINVAL, "null tensor pointer");
+  if (!aligned16(codes) || !aligned16(scales)) return fail(MHSA_EINVAL, "codes and scales must be 16-byte aligned");
+  if (!w.loaded) return fail(MHSA_EINVAL, "no weights are loaded");
+  const LinearPlan plan = linear_plan(w, rows, workspace, adapters ? adapters->rank : 0, true);
+  if (plan.bytes > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes))
+    return fail(MHSA_EINVAL, "%d rows need a 16-byte aligned workspace of %lld bytes", rows, (long long)plan.bytes);
+  const int64_t cn = rows * mhsa::fp8_kp(w.K), sn = rows * mhsa::fp8_kbp(w.K);
+  const int64_t on = ((rows - 1) * out_stride + w.N) * mhsa::dtype_size(od), wn = adapters ? (int64_t)rows * 4 : 0;
+  if (overlap(codes, cn, out, on) || overlap(scales, sn, out, on) || overlap(workspace, plan.bytes, codes, cn) ||
+      overlap(workspace, plan.bytes, scales, sn) || overlap(workspace, plan.bytes, out, on) || overlap(which, wn, out, on) ||
+      overlap(which, wn, workspace, plan.bytes))
+    return fail(MHSA_EINVAL, "the rows, out and the workspace must not overlap");
+  if (int32_t rc = check_device(w.device)) return rc;
+  if (adapters)
+    if (int32_t rc = adapters_check(adapters, w, which)) return rc;
+  LinearInput in;
+  in.codes = codes;
+  in.scales = scales;
+  return linear_run(w, in, rows, adapters, which, out, od, out_stride, plan, static_cast<hipStream_t>(hs));
+}
+
+int64_t mhsa_fp8_linear_adapted_workspace(const mhsa_fp8_linear* h, const mhsa_adapters* adapters, int32_t rows) {
+  if (!h || !adapters || rows < 0 || rows > kMaxRows) return -1;
+  return rows == 0 ? 0 : linear_plan(h->w, rows, nullptr, adapters->rank).bytes;
+}
+
+int32_t mhsa_adapters_create(int32_t in_dim, int32_t out_dim, int32_t n_adapters, int32_t max_rank, mhsa_adapters** out) {
+  if (!out) return fail(MHSA_EINVAL, "null output pointer");
+  *out = nullptr;
+  if (in_dim <= 0 || out_dim <= 0 || n_adapters <= 0 || max_rank <= 0)
+    return fail(MHSA_EINVAL, "in_dim %d, out_dim %d, n_adapters %d and max_rank %d must be positive", in_dim, out_dim, n_adapters,
+                max_rank);
+  if (in_dim > mhsa::kFp8MaxK || out_dim > kMaxOut || n_adapters > kMaxAdapters || max_rank > kMaxRank)
+    return fail(MHSA_ENOTSUP, "in_dim %d, out_dim %d, n_adapters %d, max_rank %d exceed %d, %d, %d, %d", in_dim, out_dim, n_adapters,
+                max_rank, mhsa::kFp8MaxK, kMaxOut, kMaxAdapters, kMaxRank);
+  mhsa_adapters* h = new (std::nothrow) mhsa_adapters();
+  if (!h) return fail(MHSA_ENOMEM, "out of host memory");
+  h->K = in_dim;
+  h->N = out_dim;
+  h->n = n_adapters;
+  h->max_rank = max_rank;
+  h->rank = 16;
+  while (h->rank < max_rank) h->rank *= 2;
+  *out = h;
+  return MHSA_OK;
+}
+
+void mhsa_adapters_destroy(mhsa_adapters* h) { delete h; }
+
+// Everything queued on the GPU comes first, as at the loading of weights. The
+// tensors are looked over before anything of the slot is written.
+int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t data_dtype, const void* a, const void* b,
+                           float scale) {
+  if (!h) return fail(MHSA_EINVAL, "null handle");
+  if (slot < 0 || slot >= h->n) return fail(MHSA_EINVAL, "slot %d is not in [0, %d)", slot, h->n);
+  if (rank < 0 || rank > h->max_rank) return fail(MHSA_EINVAL, "rank %d is not in [0, %d]", rank, h->max_rank);
+  if (rank && (!a || !b)) return fail(MHSA_EINVAL, "null weight pointer");
+  if (rank && !float_dtype(data_dtype)) return fail(MHSA_ENOTSUP, "weight dtype %d not supported (f32, bf16, f16)", data_dtype);
+  if (!std::isfinite(scale)) return fail(MHSA_EINVAL, "scale must be finite");
+  bool dev[2] = {};
+  if (rank) {
+    if (int32_t rc = on_device(a, &dev[0])) return rc;
+    if (int32_t rc = on_device(b, &dev[1])) return rc;
   }
-  HIPCHK(mhsa::fp8_quantize_rows(xd, x, x_stride, rows, w.K, plan.codes, plan.scales, s));
-  p.a = plan.codes;
-  p.as = plan.scales;
-  p.a_rows = rows;
-  HIPCHK(mhsa::fp8_gemm_tile(p, s));
+  int now = 0;
+  HIPCHK(hipGetDevice(&now));
+  if (h->device >= 0 && now != h->device)
+    return fail(MHSA_EINVAL, "the adapters are on GPU %d, the current GPU is %d", h->device, now);
+  HIPCHK(hipDeviceSynchronize());
+  const int kp = (int)mhsa::fp8_kp(h->K);
+  const int64_t es = data_dtype == MHSA_F32 ? 4 : 2;
+  DevBuf stage[2], bad;
+  const void* src[2] = {a, b};
+  if (rank) {
+    for (int i = 0; i < 2; ++i) {
+      const int64_t bytes = (int64_t)rank * (i == 0 ? h->K : h->N) * es;
+      if (dev[i]) continue;
+      HIPCHK(stage[i].ensure(bytes));
+      HIPCHK(hipMemcpy(stage[i].p, src[i], bytes, hipMemcpyHostToDevice));
+      src[i] = stage[i].p;
+    }
+    int found = 0;
+    HIPCHK(bad.ensure(sizeof found));
+    int* flag = static_cast<int*>(bad.p);
+    HIPCHK(hipMemcpy(flag, &found, sizeof found, hipMemcpyHostToDevice));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, nullptr, rank, h->K, flag, nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, nullptr, h->N, rank, flag, nullptr));
+    HIPCHK(hipMemcpy(&found, flag, sizeof found, hipMemcpyDeviceToHost));
+    if (found) return fail(MHSA_EINVAL, "an adapter's weights must be finite in bf16");
+  }
+  if (!h->loaded) {
+    const int64_t na = h->n * h->a_stride() * 2, nb = h->n * h->b_stride() * 2;
+    HIPCHK(h->a.ensure(na));
+    HIPCHK(h->b.ensure(nb));
+    HIPCHK(h->scale.ensure((size_t)h->n * 4));
+    HIPCHK(hipMemset(h->a.p, 0, na));
+    HIPCHK(hipMemset(h->b.p, 0, nb));
+    HIPCHK(hipMemset(h->scale.p, 0, (size_t)h->n * 4));
+    h->device = now;
+    h->loaded = true;
+  }
+  uint16_t* ta = static_cast<uint16_t*>(h->a.p) + slot * h->a_stride();
+  uint16_t* tb = static_cast<uint16_t*>(h->b.p) + slot * h->b_stride();
+  if (rank) {
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, ta, h->rank, kp, static_cast<int*>(bad.p), nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, tb, h->N, h->rank, static_cast<int*>(bad.p), nullptr));
+  } else {
+    HIPCHK(hipMemset(ta, 0, h->a_stride() * 2));
+    HIPCHK(hipMemset(tb, 0, h->b_stride() * 2));
+  }
+  HIPCHK(hipMemcpy(static_cast<float*>(h->scale.p) + slot, &scale, 4, hipMemcpyHostToDevice));
+  HIPCHK(hipDeviceSynchronize());
   return MHSA_OK;
 }
 

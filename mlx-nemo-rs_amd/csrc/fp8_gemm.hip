@@ -128,7 +128,7 @@ __device__ __forceinline__ void store_as(DType dt, void* out, int64_t at, float 
 // of a few microseconds pays for fetching it).
 template <typename TX, int RC, bool EXACT, bool VEC>
 __device__ __forceinline__ void few_block(const uint8_t* wrow, const int off[RC], const uint8_t* wsc, int b, const TX* xrow,
-                                          int K, floatx4 acc[RC]) {
+                                          const uint8_t* xsc, int K, floatx4 acc[RC]) {
   const int c0 = b * 128 + 32 * ((threadIdx.x & 63) >> 4);
   u32x4 wf[RC][2];
 #pragma unroll
@@ -136,6 +136,14 @@ __device__ __forceinline__ void few_block(const uint8_t* wrow, const int off[RC]
 #pragma unroll
     for (int u = 0; u < 2; ++u) wf[c][u] = *reinterpret_cast<const u32x4*>(wrow + off[c] + b * 128 + 16 * u);
   const int sw = wsc[b];
+  i32x8 q = {};
+  int s = 127;
+  if constexpr (std::is_same_v<TX, uint8_t>) {  // (zeros past K)
+    if (K > 0) {
+      __builtin_memcpy(&q, xrow + c0, sizeof q);
+      s = xsc[b];
+    }
+  } else {
   float v[32];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -152,11 +160,11 @@ __device__ __forceinline__ void few_block(const uint8_t* wrow, const int off[RC]
   for (int i = 0; i < 32; ++i) m = fmaxf(m, fp8_mag(v[i]));
   m = fmaxf(m, __shfl_xor(m, 16, 64));
   m = fmaxf(m, __shfl_xor(m, 32, 64));
-  const int s = fp8_scale_byte(m);
+  s = fp8_scale_byte(m);
   const float scale = fp8_scale(s);
-  i32x8 q;
 #pragma unroll
   for (int i = 0; i < 8; ++i) q[i] = (int)fp8_pack4_scaled(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
+  }
 #pragma unroll
   for (int c = 0; c < RC; ++c) {
     if constexpr (EXACT) {
@@ -237,7 +245,33 @@ __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
   return at;
 }
 
-template <typename TX, int NW, int RC, bool EXACT, bool VEC>
+// Adds the adapters' products of this lane's row `to` (-1: none) and 16 RC
+// columns from n0 on to acc, as few_block its block's. The distinct adapters of
+// the 16 rows, 32 ranks at a time, are shared out to the waves; a row of another
+// adapter counts as zero.
+template <int NW, int RC>
+__device__ __forceinline__ void few_adapters(const Fp8Gemm& p, int w, int to, int n0, floatx4 acc[RC]) {
+  const int lane = threadIdx.x & 63, r = lane & 15, c4 = lane >> 4, ext = p.ad.parts * p.ad.rank;
+  int mine = to >= 0 ? p.ad.which[to] : -1;
+  if (mine >= p.ad.n) mine = -1;
+  int item = 0;
+  for (uint64_t todo = __ballot(mine >= 0); todo;) {
+    const int d = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    todo &= ~__ballot(mine == d);
+    for (int k0 = 0; k0 < ext; k0 += 32, ++item) {
+      if (item % NW != w) continue;
+      const int k = k0 + 8 * c4;
+      const bf16x8 t = load16<bf16x8>(p.ad.t + (int64_t)(to >= 0 ? to : 0) * ext + k, mine == d && k < ext);
+#pragma unroll
+      for (int c = 0; c < RC; ++c) {
+        const int64_t row = (int64_t)d * p.N + min(n0 + 16 * c + r, p.N - 1);
+        acc[c] = mma16(load16<bf16x8>(p.ad.b + row * p.ad.rank + (k & (p.ad.rank - 1)), k < ext), t, acc[c]);
+      }
+    }
+  }
+}
+
+template <typename TX, int NW, int RC, bool EXACT, bool VEC, bool ADD>
 __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
   __shared__ float red[NW][RC][16][20];
   __shared__ int dst[16];
@@ -327,13 +361,17 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
     }
     const int src = p.rows == Fp8Gemm::kByFrame ? to / p.g.top_k : to;
     if (threadIdx.x < 16) dst[r] = to;
-    const TX* xrow = reinterpret_cast<const TX*>(p.x) + (int64_t)(to >= 0 ? src : 0) * p.ldx;
+    constexpr bool CODES = std::is_same_v<TX, uint8_t>;
+    const TX* xrow = CODES ? reinterpret_cast<const TX*>(p.a) + (int64_t)(to >= 0 ? to : 0) * (kb * 128)
+                           : reinterpret_cast<const TX*>(p.x) + (int64_t)(to >= 0 ? src : 0) * p.ldx;
+    const uint8_t* xsc = CODES ? p.as + (int64_t)(to >= 0 ? to : 0) * kbp : nullptr;
     const int K = to >= 0 ? p.K : 0;
     floatx4 acc[RC];
 #pragma unroll
     for (int c = 0; c < RC; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int b = w; b < kb; b += NW) few_block<TX, RC, EXACT, VEC>(wrow, off, wsc, b, xrow, K, acc);
+    for (int b = w; b < kb; b += NW) few_block<TX, RC, EXACT, VEC>(wrow, off, wsc, b, xrow, xsc, K, acc);
+    if constexpr (ADD) few_adapters<NW, RC>(p, w, to, n0, acc);
     // lane: row l % 16, columns 16 c + 4 (l / 16) + [0, 4)
 #pragma unroll
     for (int c = 0; c < RC; ++c) *reinterpret_cast<floatx4*>(&red[w][c][r][4 * c4]) = acc[c];
@@ -522,7 +560,7 @@ struct Fp8Cfg {
   static_assert(BM >= 64 && BM <= 256 && (!AHEAD || NS == 2), "scales, stages");
 };
 
-template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
+template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut, bool ADD>
 __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   using C = Fp8Cfg<BM, BN, NS>;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
@@ -761,6 +799,56 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     for (int u = 0; u < PL; ++u) pl[u] = p.g.pair[t.m0 + min(wm * C::WM + 64 * u + lane, t.rows - 1)];
   };
 
+  // The sums of tile t begin with the adapters' products: the distinct adapters
+  // of the wave's rows one by one, 16 ranks at a time; a row of another adapter
+  // counts as zero.
+  auto adapters = [&](const Tile& t) {
+    const int ext = p.ad.parts * p.ad.rank;
+    int64_t row[C::TM];
+    int mine[C::TM];
+    uint64_t left[C::TM];
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const int r = wm * C::WM + 32 * i + (lane & 31);
+      row[i] = t.m0 + min(r, t.rows - 1);
+      mine[i] = r < t.rows ? p.ad.which[row[i]] : -1;
+      if (mine[i] >= p.ad.n) mine[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) left[i] = __ballot(mine[i] >= 0);
+    for (;;) {
+      int d = -1;
+#pragma unroll
+      for (int i = C::TM - 1; i >= 0; --i)
+        if (left[i]) d = __builtin_amdgcn_readlane(mine[i], __builtin_ctzll(left[i]));
+      if (d < 0) break;
+      bool some[C::TM];
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const uint64_t same = __ballot(mine[i] == d);
+        some[i] = same != 0;
+        left[i] &= ~same;
+      }
+#pragma unroll 1
+      for (int k0 = 0; k0 < ext; k0 += 16) {
+        const int k = k0 + 8 * half;
+        bf16x8 fb16[C::TN];
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
+          const int64_t col = (int64_t)d * p.N + min(t.n0 + wn * C::WN + 32 * j + (lane & 31), p.N - 1);
+          fb16[j] = *reinterpret_cast<const bf16x8*>(p.ad.b + col * p.ad.rank + (k & (p.ad.rank - 1)));
+        }
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) {
+          if (!some[i]) continue;
+          const bf16x8 ft = load16<bf16x8>(p.ad.t + row[i] * ext + k, mine[i] == d);
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) acc[j][i] = mma32(fb16[j], ft, acc[j][i]);
+        }
+      }
+    }
+  };
+
   const int stride = (int)(gridDim.x / 8u);
   Place where = place_of(T);
   Tile now = tile_of(entry_of(where.tm), where.n0), next = now;
@@ -799,6 +887,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     for (int j = 0; j < C::TN; ++j)
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) acc[j][i] = floatx16{};
+    if constexpr (ADD) adapters(now);
     // (a tile's last step read these too, but held over the epilogue they spilled)
 #pragma unroll
     for (int r = 0; r < FRAGS + C::TM; ++r) rd1(r, C::AHEAD ? base & 1 : 0, 0);
@@ -998,13 +1087,13 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   }
 }
 
-template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
+template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut, bool ADD>
 __global__ __launch_bounds__(256, (2 * Fp8Cfg<BM, BN, NS>::LDS > 160 * 1024 ? 1 : 2)) void fp8_tile_kernel(Fp8Gemm p) {
   __shared__ __attribute__((aligned(1024))) char smem[Fp8Cfg<BM, BN, NS>::LDS];
-  fp8_tile_body<BM, BN, NS, EXACT, EPI, TOut>(p, smem);
+  fp8_tile_body<BM, BN, NS, EXACT, EPI, TOut, ADD>(p, smem);
 }
 
-template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut>
+template <int BM, int BN, int NS, bool EXACT, int EPI, typename TOut, bool ADD = false>
 hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
   const int64_t tm = p.g.tile ? p.g.max_tiles : (p.M + BM - 1) / BM;
   const int64_t nt = tm * ((p.N + BN - 1) / BN);
@@ -1014,7 +1103,7 @@ hipError_t launch_tile(const Fp8Gemm& p, hipStream_t s) {
   // as many workgroups as the CUs hold at a time, 8 XCDs alike
   const int64_t resident = (int64_t)device_cus() * (160 * 1024 / Fp8Cfg<BM, BN, NS>::LDS);
   const int64_t grid = (std::min(nt, resident) + 7) / 8 * 8;
-  fp8_tile_kernel<BM, BN, NS, EXACT, EPI, TOut><<<(unsigned)grid, 256, 0, s>>>(p);
+  fp8_tile_kernel<BM, BN, NS, EXACT, EPI, TOut, ADD><<<(unsigned)grid, 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
@@ -1039,7 +1128,38 @@ hipError_t launch_experts(const Fp8Gemm& p, hipStream_t s) {
                               : launch_tile<128, 128, 2, EXACT, kFp8Pair, float>(p, s);
 }
 
+// A dense product.
+template <bool ADD>
+hipError_t launch_dense(const Fp8Gemm& p, hipStream_t s) {
+  auto tiles = [&](int64_t bm, int64_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };
+  // Large tiles from half of the CUs on, and tiles of 128 rows likewise. About
+  // there either side wins, by K (us, the larger tiles against the smaller):
+  // 128 large tiles of 2048 x 1024 -> 4096 23.2 and 20.1, of 2048 x 4096 -> 4096
+  // 48 and 48, 188 of 3000 x 1024 -> 4096 24.8 and 27.1; 128 tiles of 128 rows of
+  // 1024 x 1024 -> 2048 12.1 and 10.5, of 1000 x 4096 -> 2048 25.0 and 26.8. 192
+  // rows where a CU then goes through fewer (3000 x 1024 -> 4096 24.8 against
+  // 27.6, 8200 x 1024 -> 2048 37.8 against 43.8).
+  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256), t128 = tiles(128, 128), cus = device_cus();
+  const bool large = t256 >= cus / 2 && p.K > kFp8Block;  // (the large tiles' ring takes two stages)
+  const bool fewer = (t192 + cus - 1) / cus * 192 < (t256 + cus - 1) / cus * 256;  // rows a CU goes through
+  if (p.out_dt == kF32) {
+    if (large && fewer) return launch_tile<192, 256, 2, true, kFp8Out, float, ADD>(p, s);
+    if (large) return launch_tile<256, 256, 2, true, kFp8Out, float, ADD>(p, s);
+    return t128 >= cus / 2 ? launch_tile<128, 128, 2, true, kFp8Out, float, ADD>(p, s) : launch_tile<64, 64, 4, true, kFp8Out, float, ADD>(p, s);
+  }
+  if (large && fewer) return launch_tile<192, 256, 2, false, kFp8Out, bf16, ADD>(p, s);
+  if (large) return launch_tile<256, 256, 2, false, kFp8Out, bf16, ADD>(p, s);
+  // a tile alone on its CU keeps four stages, two that share it two each
+  // (3000 x 4096 -> 1024: 36.8 -> 29.7 us with the rows' codes)
+  if (t128 >= cus / 2 && t128 <= cus) return launch_tile<128, 128, 4, false, kFp8Out, bf16, ADD>(p, s);
+  return t128 >= cus / 2 ? launch_tile<128, 128, 2, false, kFp8Out, bf16, ADD>(p, s) : launch_tile<64, 64, 4, false, kFp8Out, bf16, ADD>(p, s);
+}
+
 bool bad_gemm(const Fp8Gemm& p) {
+  const Fp8Adapted& a = p.ad;
+  if (a.which && (!a.t || !a.b || a.n <= 0 || (a.parts != 1 && a.parts != 3) || p.g.tile || p.g.idx || p.epilogue != kFp8Out ||
+                  (a.rank != 16 && a.rank != 32 && a.rank != 64 && a.rank != 128)))
+    return true;
   return p.N <= 0 || p.K <= 0 || !p.bias || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);
 }
 
@@ -1106,7 +1226,7 @@ bool fp8_few_rows(int64_t M, int N, int K) {
 int fp8_scan_pairs() { return kScanPairs; }
 
 hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
-  if (bad_gemm(p) || !p.x) return hipErrorInvalidValue;
+  if (bad_gemm(p) || (!p.x && (!p.a || !p.as || p.epilogue != kFp8Out || p.g.tile || p.g.idx))) return hipErrorInvalidValue;
   if (p.g.idx && !p.g.tile && (p.g.pairs > kScanPairs || p.g.experts > kScanExperts)) return hipErrorInvalidValue;
   if (p.g.tile && p.g.tile_rows != 16) return hipErrorInvalidValue;
   const int64_t groups = p.g.tile ? p.g.max_tiles : p.g.idx ? std::min(p.g.pairs, p.g.experts) : (p.M + 15) / 16;
@@ -1120,13 +1240,28 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
     using TX = decltype(tx);
     constexpr int NW = decltype(nw)::value, RC = decltype(rc)::value;
     const dim3 grid((p.N + 16 * RC - 1) / (16 * RC), (unsigned)groups);
-    if (exact && vec) fp8_few_kernel<TX, NW, RC, true, true><<<grid, NW * 64, 0, s>>>(p);
-    else if (exact) fp8_few_kernel<TX, NW, RC, true, false><<<grid, NW * 64, 0, s>>>(p);
-    else if (vec) fp8_few_kernel<TX, NW, RC, false, true><<<grid, NW * 64, 0, s>>>(p);
-    else fp8_few_kernel<TX, NW, RC, false, false><<<grid, NW * 64, 0, s>>>(p);
+    auto run = [&](auto ex, auto ve, auto ad) {
+      fp8_few_kernel<TX, NW, RC, decltype(ex)::value, decltype(ve)::value, decltype(ad)::value><<<grid, NW * 64, 0, s>>>(p);
+    };
+    auto by_form = [&](auto ad) {
+      constexpr std::true_type yes;
+      constexpr std::false_type no;
+      if constexpr (std::is_same_v<TX, uint8_t>) {  // (codes come in whole blocks)
+        if (exact) run(yes, yes, ad);
+        else run(no, yes, ad);
+      } else {
+        if (exact && vec) run(yes, yes, ad);
+        else if (exact) run(yes, no, ad);
+        else if (vec) run(no, yes, ad);
+        else run(no, no, ad);
+      }
+    };
+    if (p.ad.which) by_form(std::true_type());
+    else by_form(std::false_type());
   };
   auto by_type = [&](auto nw, auto rc) {
-    if (p.x_dt == kBF16) go(bf16{}, nw, rc);
+    if (!p.x) go(uint8_t{}, nw, rc);
+    else if (p.x_dt == kBF16) go(bf16{}, nw, rc);
     else go(float{}, nw, rc);
   };
   using std::integral_constant;
@@ -1172,28 +1307,7 @@ hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
     return p.exact ? launch_experts<true>(p, s) : launch_experts<false>(p, s);
   }
   if (p.M <= 0 || p.epilogue != kFp8Out) return hipErrorInvalidValue;
-  auto tiles = [&](int64_t bm, int64_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };
-  // Large tiles from half of the CUs on, and tiles of 128 rows likewise. About
-  // there either side wins, by K (us, the larger tiles against the smaller):
-  // 128 large tiles of 2048 x 1024 -> 4096 23.2 and 20.1, of 2048 x 4096 -> 4096
-  // 48 and 48, 188 of 3000 x 1024 -> 4096 24.8 and 27.1; 128 tiles of 128 rows of
-  // 1024 x 1024 -> 2048 12.1 and 10.5, of 1000 x 4096 -> 2048 25.0 and 26.8. 192
-  // rows where a CU then goes through fewer (3000 x 1024 -> 4096 24.8 against
-  // 27.6, 8200 x 1024 -> 2048 37.8 against 43.8).
-  const int64_t t256 = tiles(256, 256), t192 = tiles(192, 256), t128 = tiles(128, 128), cus = device_cus();
-  const bool large = t256 >= cus / 2 && p.K > kFp8Block;  // (the large tiles' ring takes two stages)
-  const bool fewer = (t192 + cus - 1) / cus * 192 < (t256 + cus - 1) / cus * 256;  // rows a CU goes through
-  if (p.out_dt == kF32) {
-    if (large && fewer) return launch_tile<192, 256, 2, true, kFp8Out, float>(p, s);
-    if (large) return launch_tile<256, 256, 2, true, kFp8Out, float>(p, s);
-    return t128 >= cus / 2 ? launch_tile<128, 128, 2, true, kFp8Out, float>(p, s) : launch_tile<64, 64, 4, true, kFp8Out, float>(p, s);
-  }
-  if (large && fewer) return launch_tile<192, 256, 2, false, kFp8Out, bf16>(p, s);
-  if (large) return launch_tile<256, 256, 2, false, kFp8Out, bf16>(p, s);
-  // a tile alone on its CU keeps four stages, two that share it two each
-  // (3000 x 4096 -> 1024: 36.8 -> 29.7 us with the rows' codes)
-  if (t128 >= cus / 2 && t128 <= cus) return launch_tile<128, 128, 4, false, kFp8Out, bf16>(p, s);
-  return t128 >= cus / 2 ? launch_tile<128, 128, 2, false, kFp8Out, bf16>(p, s) : launch_tile<64, 64, 4, false, kFp8Out, bf16>(p, s);
+  return p.ad.which ? launch_dense<true>(p, s) : launch_dense<false>(p, s);
 }
 
 }  // namespace mhsa

@@ -64,6 +64,18 @@ struct Fp8Groups {
   int pairs = 0, experts = 0;
 };
 
+// Low-rank adapters beside a dense product (null `which`: none): out row r gets
+// B_a t_r, a = which[r], nothing for a outside [0, n). t_r = s_a A_a x_r comes
+// as `parts` bf16 numbers that add up to it, [rows, parts * rank], from
+// adapter_rows: one part, rounded, for a bf16 result, whose own rounding
+// is as coarse, and three, which hold f32, for an f32 one. B_a [N, rank] bf16.
+struct Fp8Adapted {
+  const int* which = nullptr;
+  int n = 0, rank = 0, parts = 1;  // rank 16, 32, 64 or 128
+  const uint16_t* t = nullptr;
+  const uint16_t* b = nullptr;  // [n, N, rank]
+};
+
 enum Fp8Epilogue {
   kFp8Out = 0,     // out [M, N] = acc + bias, in out_dt
   kFp8HiddenQ,     // silu(acc + bias) as codes [slots, Np] and scales
@@ -72,7 +84,8 @@ enum Fp8Epilogue {
 };
 
 struct Fp8Gemm {
-  // activations: codes and scales (a, as), or, for the few-row kernel, x
+  // activations: codes and scales (a, as), or, for the few-row kernel, x (of
+  // dense products also codes, x null)
   const uint8_t* a = nullptr;
   const uint8_t* as = nullptr;
   const void* x = nullptr;
@@ -99,6 +112,7 @@ struct Fp8Gemm {
   uint8_t* out_scales = nullptr;
   int64_t slots = 0;  // of the hidden rows' scales
   Fp8Groups g;
+  Fp8Adapted ad;
 };
 // Whether the few-row kernel (activations rounded inside it) takes M rows.
 bool fp8_few_rows(int64_t M, int N, int K);
@@ -135,6 +149,30 @@ hipError_t experts_prepare(const int* idx, int pairs, int top_k, int experts, in
 // experts in [0, experts); residual may be null or out.
 hipError_t experts_combine(DType dt, const float* y, const int* idx, const float* w, int64_t rows, int top_k,
                            int experts, int D, const void* residual, float res_scale, void* out, hipStream_t s);
+
+// t of Fp8Adapted for x [rows, K] (f32, bf16 or, x null, codes and scales): a
+// [n, rank, Kp] bf16, zeros past K, scale [n] f32. With q_codes, the rows' codes
+// and scales are written there in the same launch (x given).
+struct AdapterRows {
+  const void* x = nullptr;
+  DType x_dt = kF32;
+  int64_t ldx = 0, rows = 0;
+  int K = 0;
+  const uint8_t* codes = nullptr;
+  const uint8_t* scales = nullptr;
+  const int* which = nullptr;
+  int n = 0, rank = 0, parts = 1;
+  const uint16_t* a = nullptr;
+  const float* scale = nullptr;
+  uint16_t* t = nullptr;
+  uint8_t* q_codes = nullptr;
+  uint8_t* q_scales = nullptr;
+};
+hipError_t adapter_rows(const AdapterRows& p, hipStream_t s);
+// [rows, cols] floats (host dtype codes) to bf16 [rows_to, cols_to], zeros
+// behind; *bad is set to 1 if one is not finite as bf16 (to null: only that).
+hipError_t adapter_weights(int data_dtype, const void* from, int rows, int cols, uint16_t* to, int rows_to, int cols_to,
+                           int* bad, hipStream_t s);
 
 struct RouteParams {
   const void* logits = nullptr;

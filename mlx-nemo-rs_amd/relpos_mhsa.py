@@ -61,6 +61,8 @@ EXPORTS = (
     "mhsa_fp8_linear_read_codes", "mhsa_fp8_linear_workspace", "mhsa_fp8_linear_forward", "mhsa_route",
     "mhsa_experts_create", "mhsa_experts_destroy", "mhsa_experts_load", "mhsa_experts_load_codes",
     "mhsa_experts_workspace", "mhsa_experts_forward",
+    "mhsa_fp8_linear_forward_rounded", "mhsa_fp8_linear_forward_adapted", "mhsa_fp8_linear_adapted_workspace",
+    "mhsa_adapters_create", "mhsa_adapters_destroy", "mhsa_adapters_load",
     "mhsa_add_norm", "mhsa_token_log_probs", "mhsa_token_log_probs_workspace",
 )
 
@@ -222,6 +224,12 @@ def library(path: str = LIB_PATH) -> ctypes.CDLL:
         "mhsa_experts_load_codes": (I, [VP, VP, VP, VP, VP, VP, VP]),
         "mhsa_experts_workspace": (L, [VP, I, I]),
         "mhsa_experts_forward": (I, [VP, VP, I, I, VP, VP, I, VP, F, VP, VP, L, VP]),
+        "mhsa_fp8_linear_forward_rounded": (I, [VP, VP, VP, I, VP, VP, VP, I, L, VP, L, VP]),
+        "mhsa_fp8_linear_forward_adapted": (I, [VP, VP, I, I, L, VP, VP, VP, I, L, VP, L, VP]),
+        "mhsa_fp8_linear_adapted_workspace": (L, [VP, VP, I]),
+        "mhsa_adapters_create": (I, [I, I, I, I, P(VP)]),
+        "mhsa_adapters_destroy": (None, [VP]),
+        "mhsa_adapters_load": (I, [VP, I, I, I, VP, VP, F]),
         "mhsa_add_norm": (I, [VP, I, I, I, L, VP, L, F, VP, L, I, VP, VP, F, VP, I, L, VP, VP, VP]),
         "mhsa_token_log_probs": (I, [VP, I, I, I, L, F, VP, I, VP, VP, I, VP, VP, VP, L, VP]),
         "mhsa_token_log_probs_workspace": (L, [I, I, I]),
@@ -589,6 +597,11 @@ def _U8():
     return torch.uint8
 
 
+def _is_int32(t) -> bool:
+    import torch
+    return isinstance(t, torch.Tensor) and t.dtype == torch.int32
+
+
 def _launch(x, fn, *args) -> None:
     """fn(*args, stream) on x's GPU and torch's current stream on it."""
     import torch
@@ -663,24 +676,86 @@ class Fp8Linear:
         _check(self._lib.mhsa_fp8_linear_read_codes(self._h, codes.ctypes.data, scales.ctypes.data))
         return codes, scales
 
-    def forward(self, x, out_dtype=None, out=None):
-        """x [..., in] float32 or bfloat16, rows evenly spaced; the result in
-        out_dtype (x's by default), or in `out` [..., out]."""
-        rows, ldx = _rows_of(x, self.in_dim)
-        xd = _act_code(x.dtype)
+    def forward(self, x, out_dtype=None, out=None, adapters=None, which=None):
+        """x [..., in] float32 or bfloat16, rows evenly spaced, or Fp8Rows; the
+        result in out_dtype (x's by default, bfloat16 of Fp8Rows), or in `out`
+        [..., out]. With adapters, row r gets adapter which[r]'s product (which
+        [...] int32; none where it is outside [0, n_adapters))."""
+        coded = isinstance(x, Fp8Rows)
+        if coded:
+            if x.shape[-1] != self.in_dim:
+                raise MhsaError(MHSA_EINVAL, f"expected rows [..., {self.in_dim}]")
+            lead, x, rounded = x.shape[:-1], x.codes, x
+            rows, dtype = x.shape[0], _torch_dtype(BF16)
+        else:
+            rows, ldx = _rows_of(x, self.in_dim)
+            lead, dtype, xd = x.shape[:-1], x.dtype, _act_code(x.dtype)
         if out is None:
-            out = x.new_empty((*x.shape[:-1], self.out_dim),
-                              dtype=x.dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
+            out = x.new_empty((*lead, self.out_dim), dtype=dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
             ldo = self.out_dim
         else:
             n, ldo = _rows_of(out, self.out_dim)
             if n != rows or out.device != x.device or (out_dtype is not None and _dtype_code(out_dtype) != _dtype_code(out.dtype)):
                 raise MhsaError(MHSA_EINVAL, f"out: expected {rows} rows on {x.device}")
-        need = self._lib.mhsa_fp8_linear_workspace(self._h, rows)
+        od = _act_code(out.dtype)
+        if adapters is None:
+            if which is not None:
+                raise MhsaError(MHSA_EINVAL, "which without adapters")
+            need = 0 if coded else self._lib.mhsa_fp8_linear_workspace(self._h, rows)
+            handle = ids = None
+        else:
+            if not isinstance(adapters, LowRankAdapters):
+                raise MhsaError(MHSA_EINVAL, "adapters: expected LowRankAdapters")
+            if (not _is_int32(which) or which.get_device() != x.get_device() or which.shape != lead
+                    or not which.is_contiguous()):
+                raise MhsaError(MHSA_EINVAL, f"which: expected contiguous int32 {tuple(lead)} on {x.device}")
+            need = self._lib.mhsa_fp8_linear_adapted_workspace(self._h, adapters._h, rows)
+            handle, ids = adapters._h, which.data_ptr()
         ws = x.new_empty(need, dtype=_U8()) if need > 0 else None
-        _launch(x, self._lib.mhsa_fp8_linear_forward, self._h, x.data_ptr(), xd, rows, ldx, out.data_ptr(),
-                _act_code(out.dtype), ldo, ws.data_ptr() if need > 0 else None, need)
+        wp = ws.data_ptr() if need > 0 else None
+        if coded:
+            _launch(x, self._lib.mhsa_fp8_linear_forward_rounded, self._h, x.data_ptr(), rounded.scales.data_ptr(), rows, handle,
+                    ids, out.data_ptr(), od, ldo, wp, need)
+        elif handle is None:
+            _launch(x, self._lib.mhsa_fp8_linear_forward, self._h, x.data_ptr(), xd, rows, ldx, out.data_ptr(), od, ldo, wp, need)
+        else:
+            _launch(x, self._lib.mhsa_fp8_linear_forward_adapted, self._h, x.data_ptr(), xd, rows, ldx, handle, ids,
+                    out.data_ptr(), od, ldo, wp, need)
         return out
+
+
+class LowRankAdapters:
+    """Low-rank adapters of many requests beside an Fp8Linear of the same sizes
+    (mhsa_adapters_*): scale * B (A x), A [rank, in], B [out, rank] held in
+    bfloat16, a slot for each adapter."""
+
+    def __init__(self, in_dim: int, out_dim: int, n_adapters: int, max_rank: int):
+        lib = library()
+        h = ctypes.c_void_p()
+        _check(lib.mhsa_adapters_create(in_dim, out_dim, n_adapters, max_rank, ctypes.byref(h)))
+        self._h, self._lib = h, lib
+        self.in_dim, self.out_dim, self.n_adapters, self.max_rank = in_dim, out_dim, n_adapters, max_rank
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            self._lib.mhsa_adapters_destroy(h)
+            self._h = None
+
+    def load(self, slot: int, a, b, scale: float = 1.0) -> None:
+        """a [rank, in] and b [out, rank] of one dtype (float32, bfloat16 or
+        float16), finite; rank <= max_rank."""
+        rank = a.shape[0] if getattr(a, "ndim", 0) == 2 else 0
+        if rank == 0:
+            raise MhsaError(MHSA_EINVAL, f"a: expected [rank, {self.in_dim}]")
+        keep, ptrs, dtype = _load_floats([((a, (rank, self.in_dim), "a"), (b, (self.out_dim, rank), "b"))])
+        if ptrs[1] is None:
+            raise MhsaError(MHSA_EINVAL, f"b: expected [{self.out_dim}, {rank}]")
+        _check(self._lib.mhsa_adapters_load(self._h, slot, rank, dtype, *ptrs, float(scale)))
+
+    def clear(self, slot: int) -> None:
+        """Empties a slot: its rows get the projection alone."""
+        _check(self._lib.mhsa_adapters_load(self._h, slot, 0, F32, None, None, 0.0))
 
 
 ROUTE_SCORES = {"softmax": 0, "sigmoid": 1}

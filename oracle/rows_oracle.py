@@ -22,6 +22,27 @@ def norm(x, delta=None, scale=1.0, weight=None, bias=None, kind="rms", eps=1e-5)
         return y, v, np.abs(b) + np.abs(w) * r * (np.abs(u) + spread) + 0.0 * y
 
 
+def adapted(x, which, adapters):
+    """The adapters' part of a projection and the sums of its products'
+    magnitudes: adapters [(a [rank, in], b [out, rank], scale)] as held (bf16
+    values); rows of no adapter 0. The third result: the magnitudes that enter
+    through the inner sums' size alone, sum |b| |t|."""
+    x = np.asarray(x, np.float64)
+    n = adapters[0][1].shape[0]
+    y, mag, inner = np.zeros((len(x), n)), np.zeros((len(x), n)), np.zeros((len(x), n))
+    for d, (a, b, s) in enumerate(adapters):
+        at = np.nonzero(which == d)[0]
+        if not len(at):
+            continue
+        s = np.float64(np.float32(s))
+        with np.errstate(invalid="ignore"):
+            t = s * (x[at] @ a.T)
+            y[at] = t @ b.T
+            mag[at] = (abs(s) * (np.abs(x[at]) @ np.abs(a).T)) @ np.abs(b).T
+            inner[at] = np.abs(t) @ np.abs(b).T
+    return y, mag, inner
+
+
 def scores(logits, tokens, top_k, temperature=1.0):
     """Per row: log p of tokens [rows, n], entropy, the top_k tokens and their
     log p, and what the errors of f32 sums are relative to: (|z - M|'s mean
