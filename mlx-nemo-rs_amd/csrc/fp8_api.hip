@@ -421,8 +421,8 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
     HIPCHK(bad.ensure(sizeof found));
     int* flag = static_cast<int*>(bad.p);
     HIPCHK(hipMemcpy(flag, &found, sizeof found, hipMemcpyHostToDevice));
-    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, nullptr, rank, h->K, flag, nullptr));
-    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, nullptr, h->N, rank, flag, nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, nullptr, rank, h->K, false, flag, nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, nullptr, h->N, rank, false, flag, nullptr));
     HIPCHK(hipMemcpy(&found, flag, sizeof found, hipMemcpyDeviceToHost));
     if (found) return fail(MHSA_EINVAL, "an adapter's weights must be finite in bf16");
   }
@@ -440,8 +440,8 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
   uint16_t* ta = static_cast<uint16_t*>(h->a.p) + slot * h->a_stride();
   uint16_t* tb = static_cast<uint16_t*>(h->b.p) + slot * h->b_stride();
   if (rank) {
-    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, ta, h->rank, kp, static_cast<int*>(bad.p), nullptr));
-    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, tb, h->N, h->rank, static_cast<int*>(bad.p), nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, ta, h->rank, kp, true, static_cast<int*>(bad.p), nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, tb, h->N, h->rank, false, static_cast<int*>(bad.p), nullptr));
   } else {
     HIPCHK(hipMemset(ta, 0, h->a_stride() * 2));
     HIPCHK(hipMemset(tb, 0, h->b_stride() * 2));

@@ -67,6 +67,56 @@ __device__ __forceinline__ void load8(const T* x, int c, int K, float v[8]) {
   }
 }
 
+// 8 values of a row of K from column c on as they lie in memory, in one load, so
+// that many are on their way at a time (load8's branches wait for each). Where
+// the row ends before them the row's last 8 are loaded; trim, where something
+// waits for them anyway, puts them in their places and zeros behind them. VEC:
+// K and c are multiples of 8.
+template <typename T, bool VEC> struct Run {
+  static constexpr int N = 2 * (int)sizeof(T);
+  uint32_t u[N];
+  __device__ __forceinline__ float operator[](int e) const {
+    T t[8];
+    __builtin_memcpy(t, u, sizeof t);
+    return (float)t[e];
+  }
+  __device__ __forceinline__ void load(const T* row, int c, int K) {
+    if (VEC || K >= 8) {
+      __builtin_memcpy(u, row + min(c, K - 8), sizeof u);
+    } else {
+      T t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = row[min(e, K - 1)];
+      __builtin_memcpy(u, t, sizeof u);
+    }
+  }
+  __device__ __forceinline__ void trim(int c, int K) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) u[e] = c < K ? u[e] : 0;
+      return;
+    }
+    // elements too many (of a row of under 8, whose only run begins with it: past its end)
+    int s = min(max(c + 8 - K, 0), 8) * (int)sizeof(T) / 2;  // in half words
+    if (K >= 8) {
+#pragma unroll
+      for (int step = N; step; step /= 2)  // words: N, N / 2, ..., 1
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (s & 2 * step) u[e] = e + step < N ? u[e + step] : 0;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (s & 1) u[e] = u[e] >> 16 | (e + 1 < N ? u[e + 1] << 16 : 0);
+      }
+    } else {
+      s = 2 * N - s;  // half words left
+#pragma unroll
+      for (int e = 0; e < N; ++e) u[e] = 2 * e + 2 <= s ? u[e] : 2 * e < s ? u[e] & 0xFFFF : 0;
+    }
+  }
+};
+
 // Each row of 16 lanes' values under `o`, in all of the row's lanes: the first
 // N steps of: lanes xor 1, xor 2 (quad permutations), half rows and rows
 // mirrored.

@@ -800,52 +800,61 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   };
 
   // The sums of tile t begin with the adapters' products: the distinct adapters
-  // of the wave's rows one by one, 16 ranks at a time; a row of another adapter
-  // counts as zero.
+  // of the wave's rows one by one, 16 ranks at a time, the next ones' operands on
+  // their way meanwhile. A row of another adapter counts as zero (its offset
+  // lies past the buffer's end; branches around the MFMAs would have the sums
+  // copied from register to register).
   auto adapters = [&](const Tile& t) {
     const int ext = p.ad.parts * p.ad.rank;
-    int64_t row[C::TM];
-    int mine[C::TM];
+    const auto rt = rsrc(reinterpret_cast<const uint8_t*>(p.ad.t + (int64_t)t.m0 * ext), (uint32_t)(t.rows * ext * 2));
+    int mine[C::TM], toff[C::TM], coff[C::TN];
     uint64_t left[C::TM];
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
       const int r = wm * C::WM + 32 * i + (lane & 31);
-      row[i] = t.m0 + min(r, t.rows - 1);
-      mine[i] = r < t.rows ? p.ad.which[row[i]] : -1;
+      mine[i] = r < t.rows ? p.ad.which[t.m0 + r] : -1;
       if (mine[i] >= p.ad.n) mine[i] = -1;
+      toff[i] = (r * ext + 8 * half) * 2;
+      left[i] = __ballot(mine[i] >= 0);
     }
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) left[i] = __ballot(mine[i] >= 0);
-    for (;;) {
-      int d = -1;
+    for (int j = 0; j < C::TN; ++j)
+      coff[j] = min(t.n0 + wn * C::WN + 32 * j + (lane & 31), p.N - 1) * p.ad.rank * 2 + 16 * half;
+    struct Operands {
+      u32x4 b[C::TN], t[C::TM];
+    } now, next;
+    int d = -1, k0 = 0;
+    auto advance = [&]() {  // to the next 16 ranks; whether there are any
+      k0 += 16;
+      if (d >= 0 && k0 < ext) return true;
+      k0 = 0;
+      d = -1;
 #pragma unroll
       for (int i = C::TM - 1; i >= 0; --i)
         if (left[i]) d = __builtin_amdgcn_readlane(mine[i], __builtin_ctzll(left[i]));
-      if (d < 0) break;
-      bool some[C::TM];
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const uint64_t same = __ballot(mine[i] == d);
-        some[i] = same != 0;
-        left[i] &= ~same;
-      }
-#pragma unroll 1
-      for (int k0 = 0; k0 < ext; k0 += 16) {
-        const int k = k0 + 8 * half;
-        bf16x8 fb16[C::TN];
+      for (int i = 0; i < C::TM; ++i) left[i] &= ~__ballot(mine[i] == d);
+      return d >= 0;
+    };
+    auto fetch = [&](Operands& o) {
+      const auto rb16 = rsrc(reinterpret_cast<const uint8_t*>(p.ad.b + (int64_t)d * p.N * p.ad.rank), (uint32_t)(p.N * p.ad.rank * 2));
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) {
-          const int64_t col = (int64_t)d * p.N + min(t.n0 + wn * C::WN + 32 * j + (lane & 31), p.N - 1);
-          fb16[j] = *reinterpret_cast<const bf16x8*>(p.ad.b + col * p.ad.rank + (k & (p.ad.rank - 1)));
-        }
+      for (int j = 0; j < C::TN; ++j)
+        o.b[j] = __builtin_amdgcn_raw_buffer_load_b128(rb16, coff[j], (k0 & (p.ad.rank - 1)) * 2, 0);
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i) {
-          if (!some[i]) continue;
-          const bf16x8 ft = load16<bf16x8>(p.ad.t + row[i] * ext + k, mine[i] == d);
+      for (int i = 0; i < C::TM; ++i) o.t[i] = __builtin_amdgcn_raw_buffer_load_b128(rt, mine[i] == d ? toff[i] : -1, k0 * 2, 0);
+    };
+    bool more = advance();
+    if (more) fetch(next);
+    while (more) {
+      now = next;
+      more = advance();
+      if (more) fetch(next);
 #pragma unroll
-          for (int j = 0; j < C::TN; ++j) acc[j][i] = mma32(fb16[j], ft, acc[j][i]);
-        }
-      }
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+          acc[j][i] = mma32(__builtin_bit_cast(bf16x8, now.b[j]), __builtin_bit_cast(bf16x8, now.t[i]), acc[j][i]);
     }
   };
 

@@ -151,7 +151,8 @@ hipError_t experts_combine(DType dt, const float* y, const int* idx, const float
                            int experts, int D, const void* residual, float res_scale, void* out, hipStream_t s);
 
 // t of Fp8Adapted for x [rows, K] (f32, bf16 or, x null, codes and scales): a
-// [n, rank, Kp] bf16, zeros past K, scale [n] f32. With q_codes, the rows' codes
+// [n, rank, Kp] bf16, each adapter's as adapter_weights leaves it in fragments,
+// scale [n] f32. With q_codes, the rows' codes
 // and scales are written there in the same launch (x given).
 struct AdapterRows {
   const void* x = nullptr;
@@ -170,9 +171,10 @@ struct AdapterRows {
 };
 hipError_t adapter_rows(const AdapterRows& p, hipStream_t s);
 // [rows, cols] floats (host dtype codes) to bf16 [rows_to, cols_to], zeros
-// behind; *bad is set to 1 if one is not finite as bf16 (to null: only that).
+// behind, in rows or in the fragments that adapter_rows reads; *bad is set to 1
+// if one is not finite as bf16 (to null: only that).
 hipError_t adapter_weights(int data_dtype, const void* from, int rows, int cols, uint16_t* to, int rows_to, int cols_to,
-                           int* bad, hipStream_t s);
+                           bool fragments, int* bad, hipStream_t s);
 
 struct RouteParams {
   const void* logits = nullptr;

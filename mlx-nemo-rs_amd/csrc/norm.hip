@@ -19,34 +19,51 @@ namespace mhsa {
 namespace {
 
 // 8 values to columns [c, c + 8) of a row of D.
-template <typename T>
+template <bool VEC, typename T>
 __device__ __forceinline__ void store8(T* row, int c, int D, const float v[8]) {
   T t[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
   if (c + 8 <= D) {
     __builtin_memcpy(row + c, t, sizeof t);
-  } else {
+  } else if constexpr (!VEC) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (c + e < D) row[c + e] = t[e];
   }
 }
 
-template <typename T, int CH, int W>
+// VEC: rows of whole runs of 8 columns.
+template <typename T, int CH, int W, bool VEC>
 __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormParams p) {
   constexpr int RPB = W == 1 ? 4 : 1;  // rows of a workgroup at a time
   __shared__ float red[4][W];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wr = W == 1 ? 0 : wv;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = W == 1 ? 0 : wv;
   const int kb = (p.D + 127) / 128, kbp = (kb + 3) / 4 * 4;
   auto col = [&](int i) { return 8 * (64 * (wr + W * i) + lane); };
-  float w[CH][8], b[CH][8];
+  auto in = [&](int i, int e) { return VEC ? col(i) < p.D : col(i) + e < p.D; };
+  // weight and bias stay in registers from row to row where there are enough
+  constexpr bool HOLD = CH <= 2;
+  Run<float, VEC> w[CH], b[CH];
+  auto weights = [&](int i) {
+    if (p.w) {
+      w[i].load(p.w, col(i), p.D);
+      w[i].trim(col(i), p.D);
+    } else {
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
+      for (int e = 0; e < 8; ++e) w[i].u[e] = 0x3F800000u;
+    }
+    if (p.b) {
+      b[i].load(p.b, col(i), p.D);
+      b[i].trim(col(i), p.D);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[i][e] = 1.f, b[i][e] = 0.f;
-    if (p.w) load8(p.w, col(i), p.D, w[i]);
-    if (p.b) load8(p.b, col(i), p.D, b[i]);
+      for (int e = 0; e < 8; ++e) b[i].u[e] = 0;
+    }
+  };
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) weights(i);
   }
   const float n = 1.f / (float)p.D;
   int turn = 0;  // (a row's sums lie where no wave still reads the last row's)
@@ -64,22 +81,30 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
   };
   for (int64_t row = (int64_t)blockIdx.x * RPB + (W == 1 ? wv : 0); row < p.rows; row += (int64_t)gridDim.x * RPB) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* d = static_cast<const T*>(p.delta) + row * p.ldd;
+    Run<T, VEC> tx[CH], td[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) tx[i].load(x, col(i), p.D);
+    if (p.delta) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) td[i].load(d, col(i), p.D);
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < Run<T, VEC>::N; ++e) td[i].u[e] = 0;
+    }
     float v[CH][8];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) load8(x, col(i), p.D, v[i]);
-    if (p.delta) {
-      const T* d = static_cast<const T*>(p.delta) + row * p.ldd;
+    for (int i = 0; i < CH; ++i) {
+      tx[i].trim(col(i), p.D);
+      td[i].trim(col(i), p.D);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        float t[8];
-        load8(d, col(i), p.D, t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(p.scale, t[e], v[i][e]);
-      }
+      for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(p.scale, td[i][e], tx[i][e]);
     }
     if (p.sum) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) store8(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
+      for (int i = 0; i < CH; ++i) store8<VEC>(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
     }
     if (p.layer) {
       float s = 0.f;
@@ -91,7 +116,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
 #pragma unroll
       for (int i = 0; i < CH; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = col(i) + e < p.D ? v[i][e] - mean : 0.f;
+        for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] - mean : 0.f;
     }
     float q = 0.f;
 #pragma unroll
@@ -101,14 +126,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
     const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(total(q, 1), n, p.eps));
     turn ^= 1;
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i) {
+      if constexpr (!HOLD) weights(i);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(v[i][e] * r, w[i][e], b[i][e]);
+      if constexpr (!HOLD) __builtin_amdgcn_sched_barrier(0);
+    }
     if (p.out) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        if (p.out_dt == kBF16) store8(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
-        else store8(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+        if (p.out_dt == kBF16) store8<VEC>(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+        else store8<VEC>(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
       }
     }
     if (p.codes) {
@@ -119,7 +147,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
         float m = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (col(i) + e >= p.D) v[i][e] = 0.f;  // (b and NaN sums reach there too)
+          v[i][e] = in(i, e) ? v[i][e] : 0.f;  // (a NaN of the sums reaches there too)
           m = fmaxf(m, fp8_mag(v[i][e]));
         }
         m = row_reduce(m, [](float a, float c) { return fmaxf(a, c); });
@@ -144,7 +172,8 @@ hipError_t launch(const NormParams& p, hipStream_t s) {
   if ((int64_t)512 * CH * W < p.D) return hipErrorInvalidValue;
   const int64_t groups = W == 1 ? (p.rows + 3) / 4 : p.rows;
   const unsigned grid = (unsigned)std::min<int64_t>(groups, 1 << 16);
-  add_norm_kernel<T, CH, W><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(p);
+  if (p.D % 8 == 0) add_norm_kernel<T, CH, W, true><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(p);
+  else add_norm_kernel<T, CH, W, false><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(p);
   return hipGetLastError();
 }
 
