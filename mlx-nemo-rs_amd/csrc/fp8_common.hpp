@@ -158,6 +158,68 @@ __device__ __forceinline__ T wave_reduce(T v, O o) {
   return o(o(at(0), at(16)), o(at(32), at(48)));
 }
 
+// The largest finite magnitude of a block, 16 lanes' runs of 8 values. An
+// infinity or a NaN in one of the wave's blocks costs a second look.
+__device__ __forceinline__ float block_max(const float v[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, __builtin_fabsf(v[e]));  // (a NaN does not count)
+  auto larger = [](float a, float b) { return fmaxf(a, b); };
+  m = row_reduce(m, larger);
+  if (__any(!(m < __builtin_inff()))) {
+    m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_mag(v[e]));
+    m = row_reduce(m, larger);
+  }
+  return m;
+}
+template <bool VEC>
+__device__ __forceinline__ float block_max(const Run<float, VEC>& x) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = x[e];
+  return block_max(v);
+}
+// bf16 magnitudes have the order of their bits.
+template <bool VEC>
+__device__ __forceinline__ float block_max(const Run<bf16, VEC>& x) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x.u[e] & 0x7FFF7FFFu));
+  auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
+  uint32_t t = row_reduce((uint32_t)max(m[0], m[1]), larger);
+  if (__any(t >= 0x7F80u)) {
+    t = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t a = x.u[e / 2] >> 16 * (e % 2) & 0x7FFFu;
+      t = max(t, a < 0x7F80u ? a : 0);
+    }
+    t = row_reduce(t, larger);
+  }
+  return __builtin_bit_cast(float, t << 16);
+}
+// Its codes.
+template <bool VEC>
+__device__ __forceinline__ u32x2 fp8_pack8_scaled(const Run<float, VEC>& x, float scale) {
+  return u32x2{fp8_pack4_scaled(x[0], x[1], x[2], x[3], scale), fp8_pack4_scaled(x[4], x[5], x[6], x[7], scale)};
+}
+template <bool VEC>
+__device__ __forceinline__ u32x2 fp8_pack8_scaled(const Run<bf16, VEC>& x, float scale) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  u32x2 q;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    s16x2 r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, x.u[2 * e]), scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, x.u[2 * e + 1]), scale, true);
+    q[e] = __builtin_bit_cast(uint32_t, r);
+  }
+  return q;
+}
+
 // A wave rounds 4 blocks of a row, 16 lanes of 8 values to a block; item `id`
 // of rows * ceil(K / 512).
 template <typename T>

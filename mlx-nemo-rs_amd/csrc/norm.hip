@@ -85,7 +85,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
     Run<T, VEC> tx[CH], td[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) tx[i].load(x, col(i), p.D);
-    if (p.delta) {
+    if (HOLD && p.delta) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) td[i].load(d, col(i), p.D);
     } else {
@@ -97,10 +97,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
     float v[CH][8];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
+      if (!HOLD && p.delta) td[i].load(d, col(i), p.D);
       tx[i].trim(col(i), p.D);
       td[i].trim(col(i), p.D);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(p.scale, td[i][e], tx[i][e]);
+      if constexpr (!HOLD) __builtin_amdgcn_sched_barrier(0);
     }
     if (p.sum) {
 #pragma unroll
@@ -144,14 +146,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
       for (int i = 0; i < CH; ++i) {
         const int word = wr + W * i;  // of the row's scale bytes
         if (4 * word >= kb) continue;
-        float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[i][e] = in(i, e) ? v[i][e] : 0.f;  // (a NaN of the sums reaches there too)
-          m = fmaxf(m, fp8_mag(v[i][e]));
-        }
-        m = row_reduce(m, [](float a, float c) { return fmaxf(a, c); });
-        const int s = fp8_scale_byte(m);
+        for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] : 0.f;  // (a NaN of the sums reaches there too)
+        const int s = fp8_scale_byte(block_max(v[i]));
         const float scale = fp8_scale(s);
         if (col(i) < kb * 128)
           *reinterpret_cast<u32x2*>(p.codes + row * ((int64_t)kb * 128) + col(i)) =
@@ -183,7 +180,7 @@ hipError_t by_width(const NormParams& p, hipStream_t s) {
   if (p.D <= 1024) return launch<T, 2, 1>(p, s);
   if (p.D <= 2048) return launch<T, 1, 4>(p, s);
   if (p.D <= 4096) return launch<T, 2, 4>(p, s);
-  if (p.D <= 8192) return launch<T, 4, 4>(p, s);
+  if (p.D <= 8192) return launch<T, 2, 8>(p, s);
   return p.D <= 16384 ? launch<T, 2, 16>(p, s) : launch<T, 4, 16>(p, s);
 }
 
