@@ -10,13 +10,18 @@
 // logits of the type's lowest value do not overflow, and d is held at -200 where
 // it is multiplied by 2^d = 0 (a masked logit of -inf).
 //
-// The k best: a wave keeps a list of candidates in LDS and a border that k of
-// them reach; a chunk whose maximum does not reach it (nearly every one, after
-// the first) costs one comparison. The border starts from the lanes' maxima of
-// the first chunk. Keys are 64 bits, the value's bits in their order above the
-// complement of the index, so that no two are alike and ties go to the lower
-// index; candidates of all waves that reach the highest border are ranked by
-// counting the larger ones.
+// The k best. Keys are 64 bits, a value's bits in their order above the
+// complement of its index, so that no two are alike and ties go to the lower
+// index. Each of NW waves keeps a list of candidates in LDS, and in LDS for all to
+// see a key that q = ceil(k / NW) of its values reach; k of the row then reach the
+// ceil(k / q)-th largest of these keys, and a value below it is none of the k
+// best. A chunk whose maximum is below costs one comparison. The keys start from
+// the lanes' maxima of the first chunk (some 50 candidates of 16384 for 20 best;
+// with a border of each wave's own it was 140, and ranking them took longer than
+// reading the row) and rise with the lists; they are read without a barrier, for
+// an old one is only lower. At the end the candidates that reach the border, and
+// then those of a long row's parts, are ranked by counting the larger ones. Rows
+// of up to 8 loads to a lane stay in one wave's registers as a single chunk.
 #include <algorithm>
 
 #include "fp8_common.hpp"
@@ -29,8 +34,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kLoads = 4;  // of 16 bytes, of a lane and chunk
 
-template <typename T> constexpr int kPer = 16 / (int)sizeof(T);            // values of a load
-template <typename T> constexpr int kChunk = 64 * kLoads * kPer<T>;       // values of a wave's chunk
+template <typename T> constexpr int kPer = 16 / (int)sizeof(T);      // values of a load
+template <typename T> constexpr int kChunk = 64 * kLoads * kPer<T>;  // values of a wave's chunk
 
 // The order of floats as that of unsigned integers; -0 counts as 0.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -65,30 +70,40 @@ __device__ __forceinline__ Stats wave_stats(Stats a, float c) {
 }
 
 // The largest number with the low `skip` bits clear that k of the wave's 64 R
-// numbers reach (0 if fewer than k are not 0).
+// numbers reach (0 if fewer than k are not 0), two bits at a time.
 template <int R>
 __device__ __forceinline__ uint32_t kth(const uint32_t o[R], int k, int skip) {
   uint32_t t = 0;
-  for (int bit = 31; bit >= skip; --bit) {
-    const uint32_t at = t | 1u << bit;
-    int n = 0;
+  for (int bit = 30; bit >= skip; bit -= 2) {
+    int n[3] = {0, 0, 0};
 #pragma unroll
-    for (int r = 0; r < R; ++r) n += __popcll(__ballot(o[r] >= at));
-    if (n >= k) t = at;
+    for (uint32_t q = 1; q < 4; ++q)
+#pragma unroll
+      for (int r = 0; r < R; ++r) n[q - 1] += __popcll(__ballot(o[r] >= (t | q << bit)));
+    t |= (uint32_t)((n[0] >= k) + (n[1] >= k) + (n[2] >= k)) << bit;
   }
   return t;
 }
 
 constexpr int kList = 128;  // up to 64 candidates, and 64 more
 
-// A wave's candidates and border: values above `low`, or equal to it and of an
-// index below `before`.
+// A wave's candidates, and its border: keys below it are not looked at. A border
+// of no index (kAnyIndex) takes all values that are equal to its own.
+constexpr uint32_t kAnyIndex = 0x80000000u;
 struct Best {
   uint64_t* list;
-  int n, k;
-  float low;
-  int before;
-  __device__ __forceinline__ bool in(float v, int i) const { return v > low || (v == low && i < before); }
+  int k = 0, end = 0, n = 0;  // k best of the values up to `end`
+  float low = -__builtin_inff();  // values above it, or equal and of an index under `before`
+  int before = 0;
+  uint64_t key = 0;
+  __device__ __forceinline__ void raise(uint64_t to) {
+    if (to <= key) return;
+    key = to;
+    const uint32_t hi = (uint32_t)(to >> 32), lo = (uint32_t)to;
+    if (hi <= ordered(-__builtin_inff())) return;  // (logits of -inf are none)
+    low = value_of(hi);
+    before = lo == kAnyIndex ? 0x7FFFFFFF : (int)~lo + 1;
+  }
 };
 
 // The k best of the list's n > k candidates stay.
@@ -109,30 +124,75 @@ __device__ __forceinline__ void shrink(Best& b) {
     lo[r] = hi[r] == t ? (uint32_t)key[r] : 0;
   }
   const uint32_t l = kth<2>(lo, b.k - above, 0);  // (complements of indices are not 0)
+  const uint64_t least = (uint64_t)t << 32 | l;
   int n = 0;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const bool keep = hi[r] > t || (hi[r] == t && lo[r] >= l);
+    const bool keep = key[r] >= least;
     const uint64_t mask = __ballot(keep);
     if (keep) b.list[n + __popcll(mask & (((uint64_t)1 << lane) - 1))] = key[r];
     n += __popcll(mask);
   }
   b.n = n;
-  b.low = value_of(t);
-  b.before = (int)~l;
+  b.raise(least);
 }
 
-// Ranks n keys in LDS and gives the best min(n, k) to `put(rank, key)`; `put`
-// gets key 0 for ranks past n. All of `threads` threads take part.
-template <typename F>
-__device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int k, int at, int threads, F put) {
-  for (int i = at; i < n; i += threads) {
-    const uint64_t key = list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += list[j] > key;
-    if (rank < k) put(rank, key);
+// A key that `nth` of the list's up to 64 candidates reach, 0 if there are not so
+// many: 16 bits of a value are enough, and the last index of that very value.
+__device__ __forceinline__ uint64_t reached(const Best& b, int nth) {
+  const int lane = threadIdx.x & 63;
+  if (b.n < nth) return 0;
+  const uint64_t key = lane < b.n ? b.list[lane] : 0;
+  const uint32_t hi[1] = {(uint32_t)(key >> 32)};
+  const uint32_t t = kth<1>(hi, nth, 16);
+  const uint32_t lo = wave_reduce(hi[0] == t ? (uint32_t)key : ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
+  return (uint64_t)t << 32 | lo;
+}
+
+// Value i of the words that a lane has loaded.
+template <typename T>
+__device__ __forceinline__ float unpack(const uint32_t* raw, int i) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, raw[i]);
+  else return __builtin_bit_cast(float, i % 2 ? raw[i / 2] & 0xFFFF0000u : raw[i / 2] << 16);
+}
+// The place-th largest (from 1) of the keys of lanes 0 to N - 1, of which equal
+// ones count as one behind the other.
+template <int N>
+__device__ __forceinline__ uint64_t nth_largest(uint64_t key, int place) {
+  const int lane = threadIdx.x & 63, lo = (int)(uint32_t)key, hi = (int)(key >> 32);
+  int rank = 1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, j);
+    rank += other > key || (other == key && j < lane);
   }
-  for (int i = n + at; i < k; i += threads) put(i, (uint64_t)0);
+  const int at = __builtin_ctzll(__ballot(lane < N && rank == place));
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, at) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, at);
+}
+
+// Ranks the n keys in LDS and gives the best min(n, k) to `put(rank, key)`, and
+// key 0 for the ranks past n. One wave.
+template <typename F>
+__device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int k, F put) {
+  const int lane = threadIdx.x & 63;
+  if (n <= 64) {
+    const uint64_t key = lane < n ? list[lane] : 0;
+    const int lo = (int)(uint32_t)key, hi = (int)(key >> 32);
+    int rank = 0;
+    for (int j = 0; j < n; ++j) {
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, j);
+      rank += other > key;
+    }
+    if (lane < n && rank < k) put(rank, key);
+  } else {
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t key = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += list[j] > key;
+      if (rank < k) put(rank, key);
+    }
+  }
+  if (n + lane < k) put(n + lane, (uint64_t)0);
 }
 
 template <typename T>
@@ -175,205 +235,305 @@ struct Partial {
 };
 __device__ __host__ inline int64_t partial_bytes(int k) { return (int64_t)sizeof(Partial) + 8 * (int64_t)k; }
 
-// NW waves to a row, or to each of its `parts` parts; one wave: four rows to a
-// workgroup.
-template <typename T, int NW>
-__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void scores_kernel(ScoresParams p, int parts, int per) {
-  constexpr int WAVES = NW == 1 ? 4 : NW, E = kPer<T>, G = kLoads * E;
-  __shared__ uint64_t lists[WAVES][kList];
-  __shared__ uint64_t all[NW == 1 ? 1 : NW * 64];
-  __shared__ float stats[WAVES][3];
-  __shared__ uint32_t border[WAVES];
-  __shared__ int total;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wr = NW == 1 ? 0 : w;
-  const float c = kLog2e * p.inv_t;
-  const int64_t items = p.rows * parts;
-  for (int64_t item = NW == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x; item < items;
-       item += (int64_t)gridDim.x * (NW == 1 ? 4 : 1)) {
-    const int64_t row = item / parts;
-    const int part = (int)(item % parts), v0 = part * per, v1 = min(p.V, v0 + per);
-    const T* x = static_cast<const T*>(p.x) + row * p.ld;
-    Stats a;
-    Best b{lists[w], 0, p.k, -__builtin_inff(), 0};
-    bool first = true;
-#pragma unroll 1
-    for (int base = v0 + wr * kChunk<T>; base < v1; base += NW * kChunk<T>) {
-      float v[G];
-      if (base + kChunk<T> <= v1) {
+// L loads of a lane from x + base on (values up to v1, the first FULL loads of all
+// lanes below it) as they lie in memory, into the statistics; the largest value.
+template <typename T, int L, int FULL>
+__device__ __forceinline__ float load_chunk(const T* x, int base, int v1, float c, uint32_t raw[4 * L], Stats& a) {
+  constexpr int E = kPer<T>;
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-          T t[E];
-          __builtin_memcpy(t, x + base + (u * 64 + lane) * E, sizeof t);
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[u * E + e] = (float)t[e];
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-          const int at = base + (u * 64 + lane) * E;
-          if (at + E <= v1) {
-            T t[E];
-            __builtin_memcpy(t, x + at, sizeof t);
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[u * E + e] = (float)t[e];
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[u * E + e] = at + e < v1 ? (float)x[at + e] : -__builtin_inff();
-          }
-        }
-      }
-      float top = v[0];
-#pragma unroll
-      for (int i = 1; i < G; ++i) top = fmaxf(top, v[i]);
-      a.to(fmaxf(a.m, top), c);
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const float d = (v[i] - a.m) * c, e = __builtin_amdgcn_exp2f(d);
-        a.s += e;
-        a.u = __builtin_fmaf(e, fmaxf(d, -200.f), a.u);
-      }
-      if (p.k == 0) continue;
-      if (!(top > -__builtin_inff())) top = -__builtin_inff();  // (all of them NaN)
-      if (first) {
-        // 16 bits are enough of a border, and any lower one is right
-        const uint32_t o[1] = {ordered(top)};
-        const float t = value_of(kth<1>(o, p.k, 16));
-        if (t > -__builtin_inff()) b.low = t, b.before = 0x7FFFFFFF;
-        first = false;
-      }
-      if (__ballot(b.in(top, base + lane * E)) == 0) continue;
-      uint32_t bits = 0;
-#pragma unroll
-      for (int i = 0; i < G; ++i)
-        bits |= b.in(v[i], base + (i / E * 64 + lane) * E + i % E) ? 1u << i : 0;
-      while (__ballot(bits != 0)) {
-        const int i = __builtin_ctz(bits | 1u << 31), at = base + (i / E * 64 + lane) * E + i % E;
-        // (read again: registers have no index)
-        const float vi = bits ? value_at(x, at) : -__builtin_inff();
-        const bool in = bits && b.in(vi, at);
-        const uint64_t mask = __ballot(in);
-        if (in) b.list[b.n + __popcll(mask & (((uint64_t)1 << lane) - 1))] = key_of(vi, at);
-        b.n += __popcll(mask);
-        bits &= bits - 1;
-        if (b.n > 64) shrink(b);
-      }
-    }
-    a = wave_stats(a, c);
-    if constexpr (NW == 1) {
-      write_row<T>(p, row, a, lane, 64);
-      if (p.k) {
-        const RowOut o(a, p.inv_t);
-        rank_keys(b.list, b.n, p.k, lane, 64, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
-      }
+  for (int u = 0; u < L; ++u) {
+    const int at = base + (u * 64 + lane) * E;
+    if (u < FULL || base + (u + 1) * 64 * E <= v1) {
+      __builtin_memcpy(raw + 4 * u, x + at, 16);
     } else {
-      if (p.k) {
-        const uint64_t mine = lane < b.n ? b.list[lane] : 0;
-        const uint32_t o[1] = {(uint32_t)(mine >> 32)};
-        const uint32_t t = kth<1>(o, p.k, 16);
-        if (lane == 0) border[w] = t;
-      }
-      if (lane == 0) stats[w][0] = a.m, stats[w][1] = a.s, stats[w][2] = a.u;
-      if (threadIdx.x == 0) total = 0;
-      __syncthreads();
-      Stats r;
-      if (lane < NW) r.m = stats[lane][0], r.s = stats[lane][1], r.u = stats[lane][2];
-      r = wave_stats(r, c);
-      if (p.k) {
-        uint32_t t = 0;
+      T t[E];
 #pragma unroll
-        for (int i = 0; i < NW; ++i) t = max(t, border[i]);
-        const uint64_t mine = lane < b.n ? b.list[lane] : 0;
-        const bool in = mine != 0 && (uint32_t)(mine >> 32) >= t;
-        const uint64_t mask = __ballot(in);
-        int at = 0;
-        if (lane == 0 && mask) at = atomicAdd(&total, __popcll(mask));
-        at = __builtin_amdgcn_readfirstlane(at);
-        if (in) all[at + __popcll(mask & (((uint64_t)1 << lane) - 1))] = mine;
-        __syncthreads();
-      }
-      if (parts == 1) {
-        write_row<T>(p, row, r, threadIdx.x, NW * 64);
-        if (p.k) {
-          const RowOut o(r, p.inv_t);
-          rank_keys(all, total, p.k, threadIdx.x, NW * 64, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
-        }
-      } else {
-        char* to = static_cast<char*>(p.ws) + item * partial_bytes(p.k);
-        if (threadIdx.x == 0) *reinterpret_cast<Partial*>(to) = Partial{r.m, r.s, r.u, 0.f};
-        uint64_t* keys = reinterpret_cast<uint64_t*>(to + sizeof(Partial));
-        if (p.k) rank_keys(all, total, p.k, threadIdx.x, NW * 64, [&](int rank, uint64_t key) { keys[rank] = key; });
-      }
-      __syncthreads();
+      for (int e = 0; e < E; ++e) t[e] = x[min(at + e, v1 - 1)];
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at + e >= v1) t[e] = (T)-__builtin_inff();
+      __builtin_memcpy(raw + 4 * u, t, 16);
     }
+  }
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < L * E; ++i) top = fmaxf(top, unpack<T>(raw, i));  // (a NaN does not count)
+  a.to(fmaxf(a.m, top), c);
+#pragma unroll
+  for (int i = 0; i < L * E; ++i) {
+    const float d = (unpack<T>(raw, i) - a.m) * c, e = __builtin_amdgcn_exp2f(d);
+    a.s += e;
+    a.u = __builtin_fmaf(e, fmaxf(d, -200.f), a.u);
+  }
+  return top;
+}
+
+// Whether a chunk may have candidates.
+template <typename T>
+__device__ __forceinline__ bool any_candidate(const Best& b, int base, float top) {
+  return __ballot(top > b.low || (top == b.low && base + (int)(threadIdx.x & 63) * kPer<T> < b.before)) != 0;
+}
+
+// Those that the border lets through join the list, element by element of all
+// lanes; so many at a time that they may not find room, one of each lane at a
+// time, read again (registers have no index).
+template <typename T, int L>
+__device__ __forceinline__ void collect(Best& b, const T* x, int base, const uint32_t raw[4 * L]) {
+  constexpr int E = kPer<T>, G = L * E;
+  const int lane = threadIdx.x & 63, at0 = base + lane * E;
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  const float low = fmaxf(b.low, kLowest);  // (-inf is never one)
+  const int before = b.low < kLowest ? 0x7FFFFFFF : b.before;
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < G; ++i) total += __popcll(__ballot(unpack<T>(raw, i) >= low));
+  if (b.n + total <= kList) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float v = unpack<T>(raw, i);
+      const int at = at0 + i / E * 64 * E + i % E;
+      const bool in = v >= low && (v > low || at < before);
+      const uint64_t mask = __ballot(in);
+      if (mask) {
+        if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, at);
+        b.n += __popcll(mask);
+      }
+    }
+    if (b.n > 64) shrink(b);
+    return;
+  }
+#pragma unroll 1
+  for (int i = 0; i < G; ++i) {
+    const int at = at0 + i / E * 64 * E + i % E;
+    const float v = (float)x[min(at, b.end - 1)];
+    const bool in = at < b.end && (v > b.low || (v == b.low && at < b.before));
+    const uint64_t mask = __ballot(in);
+    if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, at);
+    b.n += __popcll(mask);
+    if (b.n > 64) shrink(b);
+  }
+}
+
+// The border that k values of the wave's lanes' largest ones reach.
+__device__ __forceinline__ uint64_t lanes_border(float top, int k) {
+  const uint32_t o[1] = {ordered(top)};
+  const uint32_t t = kth<1>(o, k, 16);  // (16 bits are enough, and any lower one is right)
+  return t > ordered(-__builtin_inff()) ? (uint64_t)t << 32 | kAnyIndex : 0;
+}
+
+// Rows of L loads to a lane, a wave to each.
+template <typename T, int L>
+__global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
+  __shared__ uint64_t lists[4][kList];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float c = kLog2e * p.inv_t;
+  const int64_t row = (int64_t)blockIdx.x * 4 + w;
+  if (row >= p.rows) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.ld;
+  Stats a;
+  uint32_t raw[4 * L];
+  const float top = load_chunk<T, L, L - 1>(x, 0, p.V, c, raw, a);
+  a = wave_stats(a, c);
+  write_row<T>(p, row, a, lane, 64);
+  if (p.k == 0) return;
+  Best b{lists[w]};
+  b.k = p.k;
+  b.end = p.V;
+  b.raise(lanes_border(top, p.k));
+  if (any_candidate<T>(b, 0, top)) collect<T, L>(b, x, 0, raw);
+  const RowOut o(a, p.inv_t);
+  rank_keys(b.list, b.n, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
+}
+
+// NW waves to a row, or to each of its `parts` parts of `per` values.
+template <typename T, int NW>
+__global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int parts, int per) {
+  constexpr int E = kPer<T>, L = kLoads, CHUNK = 64 * L * E;
+  __shared__ uint64_t lists[NW][kList];
+  __shared__ uint64_t all[NW * 64];
+  __shared__ float stats[NW][3];
+  __shared__ uint64_t border[NW];  // of each wave
+  __shared__ int total;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float c = kLog2e * p.inv_t;
+  const int nth = (p.k + NW - 1) / NW, place = p.k ? (p.k + nth - 1) / nth : 0;
+  const int64_t item = blockIdx.x;
+  const int64_t row = item / parts;
+  const int part = (int)(item % parts), v0 = part * per, v1 = min(p.V, v0 + per);
+  const T* x = static_cast<const T*>(p.x) + row * p.ld;
+  Stats a;
+  Best b{lists[w]};
+  b.k = p.k;
+  b.end = v1;
+  auto common = [&]() {
+    const uint64_t mine =
+        lane < NW ? __hip_atomic_load(&border[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : (uint64_t)0;
+    return nth_largest<NW>(mine, place);
+  };
+  auto publish = [&]() {
+    const uint64_t key = reached(b, nth);
+    if (lane == 0 && key > border[w]) __hip_atomic_store(&border[w], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  int base = v0 + w * CHUNK, known = 0;  // candidates when the wave's border was last made
+  {
+    uint32_t raw[4 * L];
+    float top = -__builtin_inff();
+    if (base < v1) top = load_chunk<T, L, 0>(x, base, v1, c, raw, a);
+    if (p.k) {
+      const uint64_t mine = lanes_border(top, nth);
+      if (lane == 0) border[w] = mine;
+      __syncthreads();
+      uint64_t key = common();
+      if (key == 0) key = lanes_border(top, p.k);  // (too few waves have values)
+      b.raise(key);
+      if (base < v1 && any_candidate<T>(b, base, top)) {
+        collect<T, L>(b, x, base, raw);
+        if (base + NW * CHUNK < v1) {
+          publish();
+          known = b.n;
+        }
+      }
+    }
+    base += NW * CHUNK;
+  }
+  // whole chunks, then single loads
+  auto follow = [&](auto loads) {
+    constexpr int M = decltype(loads)::value;
+    uint32_t raw[4 * M];
+    const float top = load_chunk<T, M, M == L ? L : 0>(x, base, v1, c, raw, a);
+    if (p.k == 0 || !any_candidate<T>(b, base, top)) return;
+    b.raise(common());
+    if (!any_candidate<T>(b, base, top)) return;
+    collect<T, M>(b, x, base, raw);
+    if (b.n < known || 2 * b.n >= 3 * known + 2) {  // (a new border costs more than a candidate)
+      publish();
+      known = b.n;
+    }
+  };
+#pragma unroll 1
+  for (; base + CHUNK <= v1; base += NW * CHUNK) follow(std::integral_constant<int, L>());
+#pragma unroll 1
+  for (; base < v1; base += 64 * E) follow(std::integral_constant<int, 1>());
+
+  a = wave_stats(a, c);
+  if (p.k) publish();
+  if (lane == 0) stats[w][0] = a.m, stats[w][1] = a.s, stats[w][2] = a.u;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  Stats r;
+  if (lane < NW) r.m = stats[lane][0], r.s = stats[lane][1], r.u = stats[lane][2];
+  r = wave_stats(r, c);
+  if (p.k) {
+    const uint64_t least = common(), mine = lane < b.n ? b.list[lane] : 0;
+    const bool in = mine != 0 && ((uint32_t)least == kAnyIndex ? mine >> 32 >= least >> 32 : mine >= least);
+    const uint64_t mask = __ballot(in);
+    int at = 0;
+    if (lane == 0 && mask) at = atomicAdd(&total, __popcll(mask));
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (in) all[at + __popcll(mask & (((uint64_t)1 << lane) - 1))] = mine;
+    __syncthreads();
+  }
+  if (parts == 1) {
+    if (w == NW - 1) write_row<T>(p, row, r, lane, 64);
+    if (p.k && w == 0) {
+      const RowOut o(r, p.inv_t);
+      rank_keys(all, total, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
+    }
+  } else {
+    char* to = static_cast<char*>(p.ws) + item * partial_bytes(p.k);
+    if (threadIdx.x == 0) *reinterpret_cast<Partial*>(to) = Partial{r.m, r.s, r.u, 0.f};
+    uint64_t* keys = reinterpret_cast<uint64_t*>(to + sizeof(Partial));
+    if (p.k && w == 0) rank_keys(all, total, p.k, [&](int rank, uint64_t key) { keys[rank] = key; });
   }
 }
 
 constexpr int kMaxParts = 16;
 
-// The parts of long rows joined, a wave to a row.
+// The parts of long rows joined, a wave to a row; everything is read at once.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(ScoresParams p, int parts) {
-  __shared__ uint64_t lists[4][kMaxParts * kScoresMaxK];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const float c = kLog2e * p.inv_t;
-  for (int64_t row = (int64_t)blockIdx.x * 4 + w; row < p.rows; row += (int64_t)gridDim.x * 4) {
-    const int64_t pb = partial_bytes(p.k);
-    const char* from = static_cast<const char*>(p.ws) + row * parts * pb;
-    Stats a;
-    if (lane < parts) {
-      const Partial q = *reinterpret_cast<const Partial*>(from + lane * pb);
-      a.m = q.m, a.s = q.s, a.u = q.u;
-    }
-    a = wave_stats(a, c);
-    write_row<T>(p, row, a, lane, 64);
-    if (p.k) {
-      auto key = [&](int part, int i) { return reinterpret_cast<const uint64_t*>(from + part * pb + sizeof(Partial))[i]; };
-      // the highest of the parts' k-th best
-      uint32_t t = lane < parts ? (uint32_t)(key(lane, p.k - 1) >> 32) : 0;
-      t = wave_reduce(t, [](uint32_t x, uint32_t y) { return max(x, y); });
-      int n = 0;
-      for (int i = lane; i < (parts * p.k + 63) / 64 * 64; i += 64) {
-        const uint64_t mine = i < parts * p.k ? key(i / p.k, i % p.k) : 0;
-        const bool in = mine != 0 && (uint32_t)(mine >> 32) >= t;
-        const uint64_t mask = __ballot(in);
-        if (in) lists[w][n + __popcll(mask & (((uint64_t)1 << lane) - 1))] = mine;
-        n += __popcll(mask);
-      }
-      const RowOut o(a, p.inv_t);
-      rank_keys(lists[w], n, p.k, lane, 64, [&](int rank, uint64_t k) { write_top(p, row, o, rank, k); });
-    }
+__global__ __launch_bounds__(64) void join_kernel(ScoresParams p, int parts) {
+  constexpr int PER = kMaxParts * kScoresMaxK / 64;
+  __shared__ uint64_t list[kMaxParts * kScoresMaxK];
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x, pb = partial_bytes(p.k);
+  const char* from = static_cast<const char*>(p.ws) + row * parts * pb;
+  Stats a;
+  uint64_t key[PER];
+  if (lane < parts) {
+    const Partial q = *reinterpret_cast<const Partial*>(from + lane * pb);
+    a.m = q.m, a.s = q.s, a.u = q.u;
   }
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int i = 64 * u + lane;
+    key[u] = 0;
+    if (64 * u < parts * p.k && i < parts * p.k)
+      key[u] = reinterpret_cast<const uint64_t*>(from + i / p.k * pb + sizeof(Partial))[i % p.k];
+  }
+  a = wave_stats(a, kLog2e * p.inv_t);
+  write_row<T>(p, row, a, lane, 64);
+  if (p.k == 0) return;
+  // (a part's keys are in order)
+  const int nth = (p.k + parts - 1) / parts, place = (p.k + nth - 1) / nth;
+  uint64_t best = lane < parts ? reinterpret_cast<const uint64_t*>(from + lane * pb + sizeof(Partial))[nth - 1] : 0;
+  const uint64_t least = nth_largest<kMaxParts>(best, place);
+  int n = 0;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const bool in = key[u] != 0 && key[u] >= least;
+    const uint64_t mask = __ballot(in);
+    if (in) list[n + __popcll(mask & (((uint64_t)1 << lane) - 1))] = key[u];
+    n += __popcll(mask);
+  }
+  const RowOut o(a, p.inv_t);
+  rank_keys(list, n, p.k, [&](int rank, uint64_t k) { write_top(p, row, o, rank, k); });
 }
 
-struct Plan {
-  int waves = 1, parts = 1, per = 0;
-};
+int64_t max_parts(int V) { return std::clamp<int64_t>(V / 8192, 1, kMaxParts); }
 
-int64_t max_parts(int V) { return std::clamp<int64_t>(V / 16384, 1, kMaxParts); }
-
-Plan plan_of(int64_t rows, int V) {
-  Plan q;
-  q.per = V;
-  if (V <= 4096) return q;
-  q.waves = 8;
-  // parts of 16384 values or more while there are fewer of them than 2 to a CU
-  const int64_t most = max_parts(V);
-  while (q.parts < most && rows * q.parts < 2 * device_cus()) ++q.parts;
-  q.per = ((V + q.parts - 1) / q.parts + 63) / 64 * 64;
-  return q;
+// parts of 8192 values or more while there are fewer of them than 2 to a CU
+int64_t parts_of(int64_t rows, int V) {
+  return std::clamp<int64_t>((2 * device_cus() + rows - 1) / rows, 1, max_parts(V));
 }
 
 template <typename T>
 hipError_t go(const ScoresParams& p, hipStream_t s) {
-  const Plan q = plan_of(p.rows, p.V);
-  if (q.parts > 1 && !p.ws) return hipErrorInvalidValue;
-  if (q.waves == 1) {
-    const unsigned grid = (unsigned)std::min<int64_t>((p.rows + 3) / 4, 1 << 20);
-    scores_kernel<T, 1><<<grid, 256, 0, s>>>(p, 1, p.V);
-  } else {
-    const unsigned grid = (unsigned)std::min<int64_t>(p.rows * q.parts, 1 << 20);
-    scores_kernel<T, 8><<<grid, 512, 0, s>>>(p, q.parts, q.per);
-    if (q.parts > 1) join_kernel<T><<<(unsigned)((p.rows + 3) / 4), 256, 0, s>>>(p, q.parts);
+  const int loads = (p.V + 64 * kPer<T> - 1) / (64 * kPer<T>);
+  if (loads <= 8) {
+    const unsigned grid = (unsigned)((p.rows + 3) / 4);
+    auto run = [&](auto l) { scores_small_kernel<T, decltype(l)::value><<<grid, 256, 0, s>>>(p); };
+    using std::integral_constant;
+    switch (loads) {
+      case 1: run(integral_constant<int, 1>()); break;
+      case 2: run(integral_constant<int, 2>()); break;
+      case 3: run(integral_constant<int, 3>()); break;
+      case 4: run(integral_constant<int, 4>()); break;
+      case 5: run(integral_constant<int, 5>()); break;
+      case 6: run(integral_constant<int, 6>()); break;
+      case 7: run(integral_constant<int, 7>()); break;
+      default: run(integral_constant<int, 8>()); break;
+    }
+    return hipGetLastError();
+  }
+  const int parts = (int)parts_of(p.rows, p.V), per = ((p.V + parts - 1) / parts + 63) / 64 * 64;
+  if (parts > 1) {
+    if (!p.ws) return hipErrorInvalidValue;
+    scores_kernel<T, 8><<<(unsigned)(p.rows * parts), 512, 0, s>>>(p, parts, per);
+    join_kernel<T><<<(unsigned)p.rows, 64, 0, s>>>(p, parts);
+    return hipGetLastError();
+  }
+  constexpr int64_t most = 1 << 22;  // rows of a launch: a grid's threads fit 32 bits
+  for (int64_t r = 0; r < p.rows; r += most) {
+    ScoresParams q = p;
+    q.rows = std::min(most, p.rows - r);
+    q.x = static_cast<const T*>(p.x) + r * p.ld;
+    q.tokens = p.tokens ? p.tokens + r * p.nt : nullptr;
+    q.log_probs = p.log_probs ? p.log_probs + r * p.nt : nullptr;
+    q.entropy = p.entropy ? p.entropy + r : nullptr;
+    q.top = p.top ? p.top + r * p.k : nullptr;
+    q.top_lp = p.top_lp ? p.top_lp + r * p.k : nullptr;
+    scores_kernel<T, 8><<<(unsigned)q.rows, 512, 0, s>>>(q, 1, per);
   }
   return hipGetLastError();
 }

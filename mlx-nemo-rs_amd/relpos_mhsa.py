@@ -592,19 +592,30 @@ def _act_code(dtype) -> int:
     return _dtype_code(dtype) if code is None else code
 
 
+_TORCH = None
+
+
+def _torch():
+    """The torch module, without the import statement's look-up in each call."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
+
+
 def _U8():
-    import torch
-    return torch.uint8
+    return _torch().uint8
 
 
 def _is_int32(t) -> bool:
-    import torch
+    torch = _torch()
     return isinstance(t, torch.Tensor) and t.dtype == torch.int32
 
 
 def _launch(x, fn, *args) -> None:
     """fn(*args, stream) on x's GPU and torch's current stream on it."""
-    import torch
+    torch = _torch()
     dev = x.get_device()
     before = torch._C._cuda_getDevice()
     if dev == before:
@@ -619,8 +630,7 @@ def _launch(x, fn, *args) -> None:
 def _rows_of(x, width: int):
     """(rows, row stride) of x [..., width] whose rows are evenly spaced with
     contiguous elements; raises for others."""
-    import torch
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1 or x.shape[-1] != width:
+    if not isinstance(x, _torch().Tensor) or not x.is_cuda or x.dim() < 1 or x.shape[-1] != width:
         raise MhsaError(MHSA_EINVAL, f"expected a GPU tensor [..., {width}]")
     rows = x.numel() // width if width else 0
     if not width or rows > 0x7FFFFFFF:
@@ -683,21 +693,24 @@ class Fp8Linear:
         [...] int32; none where it is outside [0, n_adapters))."""
         coded = isinstance(x, Fp8Rows)
         if coded:
+            x.check()
             if x.shape[-1] != self.in_dim:
                 raise MhsaError(MHSA_EINVAL, f"expected rows [..., {self.in_dim}]")
             lead, x, rounded = x.shape[:-1], x.codes, x
             rows, dtype = x.shape[0], _torch_dtype(BF16)
         else:
             rows, ldx = _rows_of(x, self.in_dim)
-            lead, dtype, xd = x.shape[:-1], x.dtype, _act_code(x.dtype)
+            lead, dtype = x.shape[:-1], x.dtype
+            xd = _act_code(dtype)
         if out is None:
-            out = x.new_empty((*lead, self.out_dim), dtype=dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
-            ldo = self.out_dim
+            want = dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype))
+            out = x.new_empty((*lead, self.out_dim), dtype=want)
+            ldo, od = self.out_dim, _act_code(want)
         else:
             n, ldo = _rows_of(out, self.out_dim)
             if n != rows or out.device != x.device or (out_dtype is not None and _dtype_code(out_dtype) != _dtype_code(out.dtype)):
                 raise MhsaError(MHSA_EINVAL, f"out: expected {rows} rows on {x.device}")
-        od = _act_code(out.dtype)
+            od = _act_code(out.dtype)
         if adapters is None:
             if which is not None:
                 raise MhsaError(MHSA_EINVAL, "which without adapters")
@@ -870,6 +883,16 @@ class Fp8Rows:
     def __init__(self, codes, scales, shape):
         self.codes, self.scales, self.shape = codes, scales, tuple(shape)
 
+    def check(self) -> None:
+        """Raises unless codes and scales are as said (those that a caller has
+        put together)."""
+        torch = _torch()
+        rows, kb = int(np.prod(self.shape[:-1], dtype=np.int64)), _blocks(self.shape[-1])
+        for t, n, name in ((self.codes, kb * 128, "codes"), (self.scales, (kb + 3) // 4 * 4, "scales")):
+            if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous()
+                    or tuple(t.shape) != (rows, n) or t.get_device() != self.codes.get_device()):
+                raise MhsaError(MHSA_EINVAL, f"{name}: expected contiguous uint8 ({rows}, {n}) on one GPU")
+
 
 class Normed(NamedTuple):
     out: object    # [..., dim] or None
@@ -880,12 +903,26 @@ class Normed(NamedTuple):
 NORM_KINDS = {"rms": 0, "layer": 1}
 
 
-def _beside(t, x, name):
-    """Checks that t is a GPU tensor of x's shape on its GPU, rows evenly
-    spaced; returns its row stride."""
-    if not hasattr(t, "get_device") or t.get_device() != x.get_device() or t.shape != x.shape:
-        raise MhsaError(MHSA_EINVAL, f"{name}: expected {tuple(x.shape)} on {x.device}")
-    return _rows_of(t, x.shape[-1])[1]
+def _beside(t, x, dtype, name) -> int:
+    """The row stride of t, which is to be a GPU tensor like x, its rows evenly
+    spaced, in dtype (None: any)."""
+    if not isinstance(t, _torch().Tensor) or (dtype is not None and t.dtype != dtype):
+        raise MhsaError(MHSA_EINVAL, f"{name}: expected {dtype} on {x.device}")
+    shape = x.shape
+    if t.get_device() != x.get_device() or t.shape != shape:
+        raise MhsaError(MHSA_EINVAL, f"{name}: expected {tuple(shape)} on {x.device}")
+    return shape[-1] if t.is_contiguous() else _rows_of(t, shape[-1])[1]
+
+
+def _vector(t, x, d, name):
+    """The address of a contiguous float32 vector [d] beside x, or None."""
+    if t is None:
+        return None
+    torch = _torch()
+    if (not isinstance(t, torch.Tensor) or t.get_device() != x.get_device() or t.dtype != torch.float32 or t.dim() != 1
+            or t.numel() != d or not t.is_contiguous()):
+        raise MhsaError(MHSA_EINVAL, f"{name}: expected a contiguous float32 tensor [{d}] on {x.device}")
+    return t.data_ptr()
 
 
 def add_norm(x, delta=None, weight=None, bias=None, kind: str = "rms", eps: float = 1e-5, scale: float = 1.0,
@@ -896,49 +933,47 @@ def add_norm(x, delta=None, weight=None, bias=None, kind: str = "rms", eps: floa
     default, or in `out`), "codes" (Fp8Rows for Fp8Linear) or "both". With a
     delta, v also comes as `sum`, in `sum_out` if given (x or delta: in place);
     sum_out alone copies x."""
-    import torch
-    if kind not in NORM_KINDS:
+    norm = NORM_KINDS.get(kind)
+    if norm is None:
         raise MhsaError(MHSA_ENOTSUP, f"norm `{kind}` (only rms and layer are supported)")
     if want not in ("out", "codes", "both"):
         raise MhsaError(MHSA_EINVAL, f"want `{want}` (out, codes or both)")
+    torch = _torch()
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise MhsaError(MHSA_EINVAL, "expected a GPU tensor [..., dim]")
-    d = x.shape[-1]
+    shape, dtype = x.shape, x.dtype
+    d = shape[-1]
     rows, ldx = _rows_of(x, d)
-    code = _act_code(x.dtype)
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != x.get_device() or t.dtype != torch.float32
-                              or tuple(t.shape) != (d,) or not t.is_contiguous()):
-            raise MhsaError(MHSA_EINVAL, f"{name}: expected a contiguous float32 tensor [{d}] on {x.device}")
+    code = od = _act_code(dtype)
+    wp, bp = _vector(weight, x, d, "weight"), _vector(bias, x, d, "bias")
+    dp = sp = op = cp = kp = None
     ldd = lds = ldo = 0
-    for t, name in ((delta, "delta"), (sum_out, "sum_out")):
-        if t is not None and getattr(t, "dtype", None) != x.dtype:
-            raise MhsaError(MHSA_EINVAL, f"{name}: expected {x.dtype}")
     if delta is not None:
-        ldd = _beside(delta, x, "delta")
+        ldd, dp = _beside(delta, x, dtype, "delta"), delta.data_ptr()
         if sum_out is None:
-            sum_out = x.new_empty(x.shape)
-    if sum_out is not None:
-        lds = _beside(sum_out, x, "sum_out")
+            sum_out = x.new_empty(shape)
+            lds, sp = d, sum_out.data_ptr()
+    if sum_out is not None and sp is None:
+        lds, sp = _beside(sum_out, x, dtype, "sum_out"), sum_out.data_ptr()
     rounded = None
     if want == "codes":
         if out is not None or out_dtype is not None:
             raise MhsaError(MHSA_EINVAL, "out and out_dtype are for float results")
+    elif out is None:
+        out = x.new_empty(shape) if out_dtype is None else x.new_empty(shape, dtype=_torch_dtype(_dtype_code(out_dtype)))
+        ldo, op, od = d, out.data_ptr(), _act_code(out.dtype)
     else:
-        if out is None:
-            out = x.new_empty(x.shape, dtype=x.dtype if out_dtype is None else _torch_dtype(_dtype_code(out_dtype)))
-        elif out_dtype is not None and _dtype_code(out_dtype) != _dtype_code(out.dtype):
+        ldo, op, od = _beside(out, x, None, "out"), out.data_ptr(), _act_code(out.dtype)
+        if out_dtype is not None and _dtype_code(out_dtype) != od:
             raise MhsaError(MHSA_EINVAL, f"out is not {out_dtype}")
-        ldo = _beside(out, x, "out")
     if want != "out":
         kb = (d + 127) // 128
-        rounded = Fp8Rows(x.new_empty((rows, kb * 128), dtype=torch.uint8),
-                          x.new_empty((rows, (kb + 3) // 4 * 4), dtype=torch.uint8), x.shape)
-    _launch(x, library().mhsa_add_norm, x.data_ptr(), code, rows, d, ldx, None if delta is None else delta.data_ptr(), ldd,
-            float(scale), None if sum_out is None else sum_out.data_ptr(), lds, NORM_KINDS[kind],
-            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), float(eps),
-            None if out is None else out.data_ptr(), code if out is None else _act_code(out.dtype), ldo,
-            None if rounded is None else rounded.codes.data_ptr(), None if rounded is None else rounded.scales.data_ptr())
+        codes = x.new_empty((rows, kb * 128), dtype=torch.uint8)
+        scales = x.new_empty((rows, (kb + 3) // 4 * 4), dtype=torch.uint8)
+        rounded = Fp8Rows(codes, scales, shape)
+        cp, kp = codes.data_ptr(), scales.data_ptr()
+    _launch(x, library().mhsa_add_norm, x.data_ptr(), code, rows, d, ldx, dp, ldd, float(scale), sp, lds, norm, wp, bp, float(eps), op,
+            od, ldo, cp, kp)
     return Normed(out, rounded, sum_out)
 
 
@@ -953,30 +988,39 @@ def token_log_probs(logits, tokens=None, top_k: int = 0, temperature: float = 1.
     """Log probabilities of tokens int32 [...] or [..., n] (outside the
     vocabulary: 0), entropy, and the top_k likeliest tokens of logits [...,
     vocab] float32 or bfloat16, rows evenly spaced (mhsa_token_log_probs)."""
-    import torch
+    torch = _torch()
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
         raise MhsaError(MHSA_EINVAL, "expected a GPU tensor [..., vocab]")
-    v = logits.shape[-1]
+    shape = logits.shape
+    v, lead = shape[-1], shape[:-1]
     rows, ld = _rows_of(logits, v)
-    lead, n = logits.shape[:-1], 0
+    lp = idx = top = tp = lpp = ip = pp = None
+    n = 0
     if tokens is not None:
-        if (not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int32 or tokens.get_device() != logits.get_device()
-                or not tokens.is_contiguous() or (tokens.shape != lead and tokens.shape[:-1] != lead)):
-            raise MhsaError(MHSA_EINVAL, f"tokens: expected contiguous int32 {tuple(lead)} or {(*lead, 'n')} on {logits.device}")
-        n = 1 if tokens.shape == lead else tokens.shape[-1]
+        if not _is_int32(tokens) or tokens.get_device() != logits.get_device() or not tokens.is_contiguous():
+            raise MhsaError(MHSA_EINVAL, f"tokens: expected a contiguous int32 tensor on {logits.device}")
+        of = tokens.shape
+        if of == lead:
+            n = 1
+        elif of[:-1] == lead and len(of):
+            n = of[-1]
+        else:
+            raise MhsaError(MHSA_EINVAL, f"tokens: expected {tuple(lead)} or {(*lead, 'n')}, got {tuple(of)}")
+        lp = logits.new_empty(of, dtype=torch.float32)
+        if n:
+            tp, lpp = tokens.data_ptr(), lp.data_ptr()
     if top_k < 0 or top_k > v:  # (before there is memory for them)
         raise MhsaError(MHSA_EINVAL, f"top_k {top_k} is not in [0, {v}]")
-    lp = None if tokens is None else logits.new_empty(tokens.shape, dtype=torch.float32)
     h = logits.new_empty(lead, dtype=torch.float32)
-    idx = logits.new_empty((*lead, top_k), dtype=torch.int32) if top_k else None
-    top = logits.new_empty((*lead, top_k), dtype=torch.float32) if top_k else None
+    if top_k:
+        idx = logits.new_empty((*lead, top_k), dtype=torch.int32)
+        top = logits.new_empty((*lead, top_k), dtype=torch.float32)
+        ip, pp = idx.data_ptr(), top.data_ptr()
     lib = library()
     need = lib.mhsa_token_log_probs_workspace(rows, v, top_k)
     ws = logits.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    _launch(logits, lib.mhsa_token_log_probs, logits.data_ptr(), _act_code(logits.dtype), rows, v, ld, float(temperature),
-            tokens.data_ptr() if n else None, n, lp.data_ptr() if n else None, h.data_ptr(), top_k,
-            idx.data_ptr() if top_k else None, top.data_ptr() if top_k else None, ws.data_ptr() if need > 0 else None,
-            max(need, 0))
+    _launch(logits, lib.mhsa_token_log_probs, logits.data_ptr(), _act_code(logits.dtype), rows, v, ld, float(temperature), tp, n,
+            lpp, h.data_ptr(), top_k, ip, pp, ws.data_ptr() if need > 0 else None, max(need, 0))
     return TokenScores(lp, h, idx, top)
 
 
