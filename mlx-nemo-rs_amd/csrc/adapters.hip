@@ -29,10 +29,6 @@
 namespace mhsa {
 namespace {
 
-// A is held in fragments: step k / 32, block of 16 ranks, lane, 8 values; lane l
-// has rank l % 16 and inputs 32 step + 8 (l / 16) on.
-__device__ __host__ inline int64_t fragment(int step, int block, int rank) { return ((int64_t)step * (rank / 16) + block) * 512; }
-
 // VEC: rows of whole runs of 8 inputs.
 template <typename TX, int RT, bool VEC>
 __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
@@ -113,7 +109,7 @@ __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
       bf16x8 fa[AHEAD][RT];
       auto fetch_a = [&](int st) {
 #pragma unroll
-        for (int j = 0; j < RT; ++j) fa[st % AHEAD][j] = *reinterpret_cast<const bf16x8*>(a + fragment(4 * b + st, j, 16 * RT));
+        for (int j = 0; j < RT; ++j) fa[st % AHEAD][j] = *reinterpret_cast<const bf16x8*>(a + adapter_fragment(4 * b + st, j, 16 * RT));
       };
       fetch_a(0);
 #pragma unroll
@@ -185,7 +181,7 @@ __global__ __launch_bounds__(256) void adapter_weights_kernel(const T* from, int
   const bf16 v = row < rows && col < cols ? (bf16)(float)from[(int64_t)row * cols + col] : (bf16)0.f;
   if (!(__builtin_fabsf((float)v) < __builtin_inff())) *bad = 1;
   if (!to) return;
-  const int64_t f = fragment(col / 32, row / 16, rows_to) + (row % 16 + col % 32 / 8 * 16) * 8 + col % 8;
+  const int64_t f = adapter_fragment(col / 32, row / 16, rows_to) + (row % 16 + col % 32 / 8 * 16) * 8 + col % 8;
   to[FRAGMENTS ? f : at] = __builtin_bit_cast(uint16_t, v);
 }
 

@@ -119,7 +119,7 @@ struct mhsa_adapters {
   int n = 0, K = 0, N = 0, rank = 0;  // rank: 16, 32, 64 or 128
   int max_rank = 0, device = -1;
   bool loaded = false;
-  DevBuf a, b, scale;
+  DevBuf a, b, scale, flag;
   int64_t a_stride() const { return (int64_t)rank * mhsa::fp8_kp(K); }
   int64_t b_stride() const { return (int64_t)N * rank; }
 };
@@ -153,7 +153,7 @@ LinearPlan linear_plan(const Fp8Weights& w, int64_t rows, void* ws, int rank = 0
     p.codes = a.take<uint8_t>(rows * mhsa::fp8_kp(w.K));
     p.scales = a.take<uint8_t>(rows * mhsa::fp8_kbp(w.K));
   }
-  if (rank) p.t = a.take<uint16_t>(rows * 3 * rank);
+  if (rank && !mhsa::fp8_few_inner(rows, w.K, rank)) p.t = a.take<uint16_t>(rows * 3 * rank);
   p.bytes = a.used;
   return p;
 }
@@ -189,6 +189,16 @@ int32_t linear_run(const Fp8Weights& w, const LinearInput& in, int32_t rows, con
   p.as = in.codes ? in.scales : plan.scales;
   p.a_rows = rows;
   if (ad) {
+    p.ad.which = which;
+    p.ad.n = ad->n;
+    p.ad.rank = ad->rank;
+    p.ad.parts = od == mhsa::kBF16 ? 1 : 3;
+    p.ad.a = static_cast<const uint16_t*>(ad->a.p);
+    p.ad.scale = static_cast<const float*>(ad->scale.p);
+    p.ad.b = static_cast<const uint16_t*>(ad->b.p);
+  }
+  if (ad && !mhsa::fp8_few_inner(rows, w.K, ad->rank)) {
+    p.ad.t = plan.t;
     mhsa::AdapterRows r;
     r.x = in.x;
     r.x_dt = in.dt;
@@ -197,17 +207,15 @@ int32_t linear_run(const Fp8Weights& w, const LinearInput& in, int32_t rows, con
     r.K = w.K;
     r.codes = in.codes;
     r.scales = in.scales;
-    r.which = p.ad.which = which;
-    r.n = p.ad.n = ad->n;
-    r.rank = p.ad.rank = ad->rank;
-    r.parts = p.ad.parts = od == mhsa::kBF16 ? 1 : 3;
-    r.a = static_cast<const uint16_t*>(ad->a.p);
-    r.scale = static_cast<const float*>(ad->scale.p);
+    r.which = which;
+    r.n = p.ad.n;
+    r.rank = p.ad.rank;
+    r.parts = p.ad.parts;
+    r.a = p.ad.a;
+    r.scale = p.ad.scale;
     r.t = plan.t;
     r.q_codes = plan.codes;
     r.q_scales = plan.scales;
-    p.ad.t = plan.t;
-    p.ad.b = static_cast<const uint16_t*>(ad->b.p);
     HIPCHK(mhsa::adapter_rows(r, s));
   }
   if (plan.few) {
@@ -407,7 +415,7 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
   HIPCHK(hipDeviceSynchronize());
   const int kp = (int)mhsa::fp8_kp(h->K);
   const int64_t es = data_dtype == MHSA_F32 ? 4 : 2;
-  DevBuf stage[2], bad;
+  DevBuf stage[2];
   const void* src[2] = {a, b};
   if (rank) {
     for (int i = 0; i < 2; ++i) {
@@ -418,8 +426,8 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
       src[i] = stage[i].p;
     }
     int found = 0;
-    HIPCHK(bad.ensure(sizeof found));
-    int* flag = static_cast<int*>(bad.p);
+    HIPCHK(h->flag.ensure(sizeof found));
+    int* flag = static_cast<int*>(h->flag.p);
     HIPCHK(hipMemcpy(flag, &found, sizeof found, hipMemcpyHostToDevice));
     HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, nullptr, rank, h->K, false, flag, nullptr));
     HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, nullptr, h->N, rank, false, flag, nullptr));
@@ -440,8 +448,8 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
   uint16_t* ta = static_cast<uint16_t*>(h->a.p) + slot * h->a_stride();
   uint16_t* tb = static_cast<uint16_t*>(h->b.p) + slot * h->b_stride();
   if (rank) {
-    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, ta, h->rank, kp, true, static_cast<int*>(bad.p), nullptr));
-    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, tb, h->N, h->rank, false, static_cast<int*>(bad.p), nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[0], rank, h->K, ta, h->rank, kp, true, static_cast<int*>(h->flag.p), nullptr));
+    HIPCHK(mhsa::adapter_weights(data_dtype, src[1], h->N, rank, tb, h->N, h->rank, false, static_cast<int*>(h->flag.p), nullptr));
   } else {
     HIPCHK(hipMemset(ta, 0, h->a_stride() * 2));
     HIPCHK(hipMemset(tb, 0, h->b_stride() * 2));

@@ -245,37 +245,129 @@ __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
   return at;
 }
 
-// Adds the adapters' products of this lane's row `to` (-1: none) and 16 RC
+// The distinct adapters of a wave's 16 rows, `mine` of its lane's row (-1: none).
+template <typename F>
+__device__ __forceinline__ void each_adapter(int mine, F f) {
+  for (uint64_t todo = __ballot(mine >= 0); todo;) {
+    const int d = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    todo &= ~__ballot(mine == d);
+    f(d);
+  }
+}
+
+// t of up to kInnerRows rows (this lane's is `to`, -1: none) into LDS, 16 ranks
+// at a time: every wave takes every NW-th block of 128 inputs, and their sums are
+// added in wave order. A is in the L2 (a workgroup's part of it goes with the
+// rows, which are few), and the launch that adapter_rows would take is saved: one
+// row of 1024 -> 4096 with an adapter of rank 16 13.0 -> 8.4 us with its call from
+// Python.
+constexpr int kInnerRows = 4;
+template <typename TX, int NW>
+__device__ __forceinline__ void few_inner(const Fp8Gemm& p, int w, int to, int mine, float* red, uint16_t* t) {
+  constexpr bool CODES = std::is_same_v<TX, uint8_t>, F32 = std::is_same_v<TX, float>;
+  const int lane = threadIdx.x & 63, r = lane & 15, c4 = lane >> 4;
+  const int kb = (p.K + 127) / 128, kbp = (kb + 3) / 4 * 4, ext = p.ad.parts * p.ad.rank;
+  const int64_t row = to >= 0 ? to : 0;
+  for (int j = 0; j < p.ad.rank / 16; ++j) {
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int b = w; b < kb; b += NW) {
+      u32x4 x[4][F32 ? 3 : 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = b * 128 + 32 * i + 8 * c4;
+        if constexpr (CODES) {
+          u32x2 q;
+          __builtin_memcpy(&q, p.a + row * (kb * 128) + c, 8);
+          x[i][0] = __builtin_bit_cast(u32x4, fp8_to_bf16(q[0], q[1], fp8_scale(p.as[row * kbp + b])));
+        } else {
+          float v[8];
+          load8(reinterpret_cast<const TX*>(p.x) + row * p.ldx, c, p.K, v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (F32) {
+              uint32_t h, m, l;
+              split_pair(v[2 * e], v[2 * e + 1], h, m, l);
+              x[i][0][e] = h;
+              x[i][1][e] = m;
+              x[i][2][e] = l;
+            } else {
+              x[i][0][e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+            }
+          }
+        }
+      }
+      each_adapter(mine, [&](int d) {
+        const uint16_t* a = p.ad.a + (int64_t)d * p.ad.rank * (kb * 128) + 8 * lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bf16x8 fa = *reinterpret_cast<const bf16x8*>(a + adapter_fragment(4 * b + i, j, p.ad.rank));
+#pragma unroll
+          for (int q = 0; q < (F32 ? 3 : 1); ++q) {
+            u32x4 f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = mine == d ? x[i][q][e] : 0;
+            acc = mma16(fa, __builtin_bit_cast(bf16x8, f), acc);
+          }
+        }
+      });
+    }
+    floatx4* part = reinterpret_cast<floatx4*>(red);
+    part[w * 64 + lane] = acc;
+    __syncthreads();
+    // lane: row r, ranks 16 j + 4 c4 + [0, 4)
+    if (w == 0 && r < kInnerRows && to >= 0) {
+      floatx4 v = part[lane];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) v += part[i * 64 + lane];
+      const float s = mine >= 0 ? p.ad.scale[mine] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= s;
+      uint32_t* out = reinterpret_cast<uint32_t*>(t + r * ext + 16 * j + 4 * c4);
+      if (p.ad.parts == 1) {
+        out[0] = pack_bf16(v[0], v[1]);
+        out[1] = pack_bf16(v[2], v[3]);
+      } else {
+        const int next = p.ad.rank / 2;
+        split_pair(v[0], v[1], out[0], out[next], out[2 * next]);
+        split_pair(v[2], v[3], out[1], out[next + 1], out[2 * next + 1]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Adds the adapters' products of this lane's row, of which t is given, and 16 RC
 // columns from n0 on to acc, as few_block its block's. The distinct adapters of
 // the 16 rows, 32 ranks at a time, are shared out to the waves; a row of another
 // adapter counts as zero.
 template <int NW, int RC>
-__device__ __forceinline__ void few_adapters(const Fp8Gemm& p, int w, int to, int n0, floatx4 acc[RC]) {
+__device__ __forceinline__ void few_adapters(const Fp8Gemm& p, int w, int mine, const uint16_t* t, int n0, floatx4 acc[RC]) {
   const int lane = threadIdx.x & 63, r = lane & 15, c4 = lane >> 4, ext = p.ad.parts * p.ad.rank;
-  int mine = to >= 0 ? p.ad.which[to] : -1;
-  if (mine >= p.ad.n) mine = -1;
   int item = 0;
-  for (uint64_t todo = __ballot(mine >= 0); todo;) {
-    const int d = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-    todo &= ~__ballot(mine == d);
+  each_adapter(mine, [&](int d) {
     for (int k0 = 0; k0 < ext; k0 += 32, ++item) {
       if (item % NW != w) continue;
       const int k = k0 + 8 * c4;
-      const bf16x8 t = load16<bf16x8>(p.ad.t + (int64_t)(to >= 0 ? to : 0) * ext + k, mine == d && k < ext);
+      const bf16x8 ft = load16<bf16x8>(t + k, mine == d && k < ext);
 #pragma unroll
       for (int c = 0; c < RC; ++c) {
         const int64_t row = (int64_t)d * p.N + min(n0 + 16 * c + r, p.N - 1);
-        acc[c] = mma16(load16<bf16x8>(p.ad.b + row * p.ad.rank + (k & (p.ad.rank - 1)), k < ext), t, acc[c]);
+        acc[c] = mma16(load16<bf16x8>(p.ad.b + row * p.ad.rank + (k & (p.ad.rank - 1)), k < ext), ft, acc[c]);
       }
     }
-  }
+  });
 }
 
-template <typename TX, int NW, int RC, bool EXACT, bool VEC, bool ADD>
+// The adapters of a projection: none, with t from memory, with t formed here.
+enum FewAdd { kFewPlain = 0, kFewAdd, kFewInner };
+
+template <typename TX, int NW, int RC, bool EXACT, bool VEC, int ADD>
 __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
-  __shared__ float red[NW][RC][16][20];
+  __shared__ __attribute__((aligned(16))) float red[NW][RC][16][20];
   __shared__ int dst[16];
   __shared__ ExpertPairs found;
+  __shared__ __attribute__((aligned(16))) uint16_t inner[ADD == kFewInner ? kInnerRows * 3 * 128 : 8];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, c4 = lane >> 4;
   const int n0 = blockIdx.x * 16 * RC;
   int expert = 0, rows = p.M - blockIdx.y * 16;
@@ -366,12 +458,20 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
                            : reinterpret_cast<const TX*>(p.x) + (int64_t)(to >= 0 ? src : 0) * p.ldx;
     const uint8_t* xsc = CODES ? p.as + (int64_t)(to >= 0 ? to : 0) * kbp : nullptr;
     const int K = to >= 0 ? p.K : 0;
+    int mine = -1;  // the row's adapter
+    if constexpr (ADD != kFewPlain) {
+      mine = to >= 0 ? p.ad.which[to] : -1;
+      if (mine >= p.ad.n) mine = -1;
+    }
+    if constexpr (ADD == kFewInner) few_inner<TX, NW>(p, w, to, mine, &red[0][0][0][0], inner);
     floatx4 acc[RC];
 #pragma unroll
     for (int c = 0; c < RC; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int b = w; b < kb; b += NW) few_block<TX, RC, EXACT, VEC>(wrow, off, wsc, b, xrow, xsc, K, acc);
-    if constexpr (ADD) few_adapters<NW, RC>(p, w, to, n0, acc);
+    if constexpr (ADD == kFewAdd)
+      few_adapters<NW, RC>(p, w, mine, p.ad.t + (int64_t)(to >= 0 ? to : 0) * (p.ad.parts * p.ad.rank), n0, acc);
+    if constexpr (ADD == kFewInner) few_adapters<NW, RC>(p, w, mine, inner + min(r, kInnerRows - 1) * (p.ad.parts * p.ad.rank), n0, acc);
     // lane: row l % 16, columns 16 c + 4 (l / 16) + [0, 4)
 #pragma unroll
     for (int c = 0; c < RC; ++c) *reinterpret_cast<floatx4*>(&red[w][c][r][4 * c4]) = acc[c];
@@ -804,16 +904,23 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   // their way meanwhile. A row of another adapter counts as zero (its offset
   // lies past the buffer's end; branches around the MFMAs would have the sums
   // copied from register to register).
+  int mine[ADD ? C::TM : 1], mine_next[ADD ? C::TM : 1];  // the adapters of this lane's rows, and of the next tile's
+  auto look_up_adapters = [&](const Tile& t, int* m) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const int r = wm * C::WM + 32 * i + (lane & 31);
+      m[i] = p.ad.which[t.m0 + min(r, t.rows - 1)];
+    }
+  };
   auto adapters = [&](const Tile& t) {
     const int ext = p.ad.parts * p.ad.rank;
     const auto rt = rsrc(reinterpret_cast<const uint8_t*>(p.ad.t + (int64_t)t.m0 * ext), (uint32_t)(t.rows * ext * 2));
-    int mine[C::TM], toff[C::TM], coff[C::TN];
+    int toff[C::TM], coff[C::TN];
     uint64_t left[C::TM];
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
       const int r = wm * C::WM + 32 * i + (lane & 31);
-      mine[i] = r < t.rows ? p.ad.which[t.m0 + r] : -1;
-      if (mine[i] >= p.ad.n) mine[i] = -1;
+      if (r >= t.rows || mine[i] >= p.ad.n) mine[i] = -1;
       toff[i] = (r * ext + 8 * half) * 2;
       left[i] = __ballot(mine[i] >= 0);
     }
@@ -874,6 +981,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     if (T + stride < T1) {
       look_up(next);
       wnext = weight_scales(next);
+      if constexpr (ADD) look_up_adapters(next, mine_next);
     }
     if (T + 2 * stride < T1) {
       const Place q = place_of(T + 2 * stride);
@@ -888,6 +996,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       next = tile_of(entry_of(where.tm), where.n0);
     }
   }
+  if constexpr (ADD) look_up_adapters(now, mine);
   prologue();
   if constexpr (C::AHEAD) look_ahead();
   bool stored = false;  // the last epilogue's stores, a known number, are behind the ring's loads
@@ -954,6 +1063,10 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       // (ahead of the stores, which the ring's next wait leaves behind)
       now = next;
       wword = wnext;
+      if constexpr (ADD) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) mine[i] = mine_next[i];
+      }
       if (T + stride < T1) next = tile_of(after, after_n0);
       look_ahead();
       asm volatile("" ::: "memory");
@@ -1091,6 +1204,7 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       look_up(now);
       aim(now);
       wword = weight_scales(now);
+      if constexpr (ADD) look_up_adapters(now, mine);
       prologue();
     }
   }
@@ -1166,7 +1280,7 @@ hipError_t launch_dense(const Fp8Gemm& p, hipStream_t s) {
 
 bool bad_gemm(const Fp8Gemm& p) {
   const Fp8Adapted& a = p.ad;
-  if (a.which && (!a.t || !a.b || a.n <= 0 || (a.parts != 1 && a.parts != 3) || p.g.tile || p.g.idx || p.epilogue != kFp8Out ||
+  if (a.which && ((!a.t && (!a.a || !a.scale)) || !a.b || a.n <= 0 || (a.parts != 1 && a.parts != 3) || p.g.tile || p.g.idx || p.epilogue != kFp8Out ||
                   (a.rank != 16 && a.rank != 32 && a.rank != 64 && a.rank != 128)))
     return true;
   return p.N <= 0 || p.K <= 0 || !p.bias || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);
@@ -1233,8 +1347,11 @@ bool fp8_few_rows(int64_t M, int N, int K) {
   return M <= 16 || (M <= 256 && read < (K <= 2048 ? 40 : 20) << 20);
 }
 int fp8_scan_pairs() { return kScanPairs; }
+// Every workgroup reads A of each of its rows: up to 128 KB.
+bool fp8_few_inner(int64_t M, int K, int rank) { return M <= kInnerRows && M * rank * fp8_kp(K) <= 64 * 1024; }
 
 hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
+  if (p.ad.which && !p.ad.t && !fp8_few_inner(p.M, p.K, p.ad.rank)) return hipErrorInvalidValue;
   if (bad_gemm(p) || (!p.x && (!p.a || !p.as || p.epilogue != kFp8Out || p.g.tile || p.g.idx))) return hipErrorInvalidValue;
   if (p.g.idx && !p.g.tile && (p.g.pairs > kScanPairs || p.g.experts > kScanExperts)) return hipErrorInvalidValue;
   if (p.g.tile && p.g.tile_rows != 16) return hipErrorInvalidValue;
@@ -1265,8 +1382,9 @@ hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s) {
         else run(no, no, ad);
       }
     };
-    if (p.ad.which) by_form(std::true_type());
-    else by_form(std::false_type());
+    if (!p.ad.which) by_form(std::integral_constant<int, kFewPlain>());
+    else if (p.ad.t) by_form(std::integral_constant<int, kFewAdd>());
+    else by_form(std::integral_constant<int, kFewInner>());
   };
   auto by_type = [&](auto nw, auto rc) {
     if (!p.x) go(uint8_t{}, nw, rc);
@@ -1308,7 +1426,7 @@ int fp8_group_rows(int64_t pairs, int experts, int K) {
 }
 
 hipError_t fp8_gemm_tile(const Fp8Gemm& p, hipStream_t s) {
-  if (bad_gemm(p) || !p.a || !p.as) return hipErrorInvalidValue;
+  if (bad_gemm(p) || !p.a || !p.as || (p.ad.which && !p.ad.t)) return hipErrorInvalidValue;
   if (p.g.tile) {
     if (p.a_rows * fp8_kp(p.K) > 0xFFFFFFFFll || p.slots % 16 || p.slots * (fp8_kp(p.K) / 128) > INT32_MAX)
       return hipErrorInvalidValue;

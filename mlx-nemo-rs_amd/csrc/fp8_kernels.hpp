@@ -72,7 +72,9 @@ struct Fp8Groups {
 struct Fp8Adapted {
   const int* which = nullptr;
   int n = 0, rank = 0, parts = 1;  // rank 16, 32, 64 or 128
-  const uint16_t* t = nullptr;
+  const uint16_t* t = nullptr;  // null: formed in the few-row kernel (fp8_few_inner) from
+  const uint16_t* a = nullptr;  // A and the scales, as AdapterRows has them
+  const float* scale = nullptr;
   const uint16_t* b = nullptr;  // [n, N, rank]
 };
 
@@ -116,6 +118,8 @@ struct Fp8Gemm {
 };
 // Whether the few-row kernel (activations rounded inside it) takes M rows.
 bool fp8_few_rows(int64_t M, int N, int K);
+// Whether it forms the adapters' inner products as well.
+bool fp8_few_inner(int64_t M, int K, int rank);
 hipError_t fp8_gemm_few(const Fp8Gemm& p, hipStream_t s);
 int fp8_scan_pairs();
 // The second product over few pairs (fp8_few_sum_ok) with the weighted sum:
@@ -170,6 +174,11 @@ struct AdapterRows {
   uint8_t* q_scales = nullptr;
 };
 hipError_t adapter_rows(const AdapterRows& p, hipStream_t s);
+// A is held in fragments: step of 32 inputs, block of 16 ranks, lane, 8 values;
+// lane l has rank l % 16 and inputs 32 step + 8 (l / 16) on.
+__device__ __host__ inline int64_t adapter_fragment(int step, int block, int rank) {
+  return ((int64_t)step * (rank / 16) + block) * 512;
+}
 // [rows, cols] floats (host dtype codes) to bf16 [rows_to, cols_to], zeros
 // behind, in rows or in the fragments that adapter_rows reads; *bad is set to 1
 // if one is not finite as bf16 (to null: only that).
