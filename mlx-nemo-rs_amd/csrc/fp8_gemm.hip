@@ -903,24 +903,19 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   // of the wave's rows one by one, 16 ranks at a time, the next ones' operands on
   // their way meanwhile. A row of another adapter counts as zero (its offset
   // lies past the buffer's end; branches around the MFMAs would have the sums
-  // copied from register to register).
-  int mine[ADD ? C::TM : 1], mine_next[ADD ? C::TM : 1];  // the adapters of this lane's rows, and of the next tile's
-  auto look_up_adapters = [&](const Tile& t, int* m) {
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      const int r = wm * C::WM + 32 * i + (lane & 31);
-      m[i] = p.ad.which[t.m0 + min(r, t.rows - 1)];
-    }
-  };
+  // copied from register to register: 15001 x 4096 -> 1024 with rank 64 124 us,
+  // 67 so, and 60 without adapters). Rows' adapters looked up a tile ahead, or two
+  // steps ahead of the ring's loads, gained nothing.
   auto adapters = [&](const Tile& t) {
     const int ext = p.ad.parts * p.ad.rank;
     const auto rt = rsrc(reinterpret_cast<const uint8_t*>(p.ad.t + (int64_t)t.m0 * ext), (uint32_t)(t.rows * ext * 2));
-    int toff[C::TM], coff[C::TN];
+    int mine[C::TM], toff[C::TM], coff[C::TN];
     uint64_t left[C::TM];
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
       const int r = wm * C::WM + 32 * i + (lane & 31);
-      if (r >= t.rows || mine[i] >= p.ad.n) mine[i] = -1;
+      mine[i] = r < t.rows ? p.ad.which[t.m0 + r] : -1;
+      if (mine[i] >= p.ad.n) mine[i] = -1;
       toff[i] = (r * ext + 8 * half) * 2;
       left[i] = __ballot(mine[i] >= 0);
     }
@@ -981,7 +976,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
     if (T + stride < T1) {
       look_up(next);
       wnext = weight_scales(next);
-      if constexpr (ADD) look_up_adapters(next, mine_next);
     }
     if (T + 2 * stride < T1) {
       const Place q = place_of(T + 2 * stride);
@@ -996,7 +990,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       next = tile_of(entry_of(where.tm), where.n0);
     }
   }
-  if constexpr (ADD) look_up_adapters(now, mine);
   prologue();
   if constexpr (C::AHEAD) look_ahead();
   bool stored = false;  // the last epilogue's stores, a known number, are behind the ring's loads
@@ -1063,10 +1056,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       // (ahead of the stores, which the ring's next wait leaves behind)
       now = next;
       wword = wnext;
-      if constexpr (ADD) {
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i) mine[i] = mine_next[i];
-      }
       if (T + stride < T1) next = tile_of(after, after_n0);
       look_ahead();
       asm volatile("" ::: "memory");
@@ -1204,7 +1193,6 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
       look_up(now);
       aim(now);
       wword = weight_scales(now);
-      if constexpr (ADD) look_up_adapters(now, mine);
       prologue();
     }
   }

@@ -977,6 +977,9 @@ def add_norm(x, delta=None, weight=None, bias=None, kind: str = "rms", eps: floa
     return Normed(out, rounded, sum_out)
 
 
+TOP_TOKENS = 32  # the most alternatives of a row
+
+
 class TokenScores(NamedTuple):
     log_probs: object      # like tokens, float32, or None
     entropy: object        # [...] float32
@@ -1009,8 +1012,8 @@ def token_log_probs(logits, tokens=None, top_k: int = 0, temperature: float = 1.
         lp = logits.new_empty(of, dtype=torch.float32)
         if n:
             tp, lpp = tokens.data_ptr(), lp.data_ptr()
-    if top_k < 0 or top_k > v:  # (before there is memory for them)
-        raise MhsaError(MHSA_EINVAL, f"top_k {top_k} is not in [0, {v}]")
+    if top_k < 0 or top_k > v or top_k > TOP_TOKENS:  # (before there is memory for them)
+        raise MhsaError(MHSA_ENOTSUP if 0 < top_k <= v else MHSA_EINVAL, f"top_k {top_k} is not in [0, {min(v, TOP_TOKENS)}]")
     h = logits.new_empty(lead, dtype=torch.float32)
     if top_k:
         idx = logits.new_empty((*lead, top_k), dtype=torch.int32)
