@@ -92,7 +92,7 @@ constexpr int kList = 128;  // up to 64 candidates, and 64 more
 constexpr uint32_t kAnyIndex = 0x80000000u;
 struct Best {
   uint64_t* list;
-  int k = 0, end = 0, n = 0;  // k best of the values up to `end`
+  int k = 0, n = 0;
   float low = -__builtin_inff();  // values above it, or equal and of an index under `before`
   int before = 0;
   uint64_t key = 0;
@@ -275,42 +275,29 @@ __device__ __forceinline__ bool any_candidate(const Best& b, int base, float top
   return __ballot(top > b.low || (top == b.low && base + (int)(threadIdx.x & 63) * kPer<T> < b.before)) != 0;
 }
 
-// Those that the border lets through join the list, element by element of all
-// lanes; so many at a time that they may not find room, one of each lane at a
-// time, read again (registers have no index).
+// Those that the border lets through join the list, one of each lane at a time;
+// `stash` (LDS of the wave) takes the chunk, for registers have no index.
 template <typename T, int L>
-__device__ __forceinline__ void collect(Best& b, const T* x, int base, const uint32_t raw[4 * L]) {
+__device__ __forceinline__ void collect(Best& b, int base, const uint32_t raw[4 * L], T* stash) {
   constexpr int E = kPer<T>, G = L * E;
-  const int lane = threadIdx.x & 63, at0 = base + lane * E;
+  const int lane = threadIdx.x & 63;
   const uint64_t below = ((uint64_t)1 << lane) - 1;
   const float low = fmaxf(b.low, kLowest);  // (-inf is never one)
-  const int before = b.low < kLowest ? 0x7FFFFFFF : b.before;
-  int total = 0;
+  typedef std::conditional_t<(G > 32), uint64_t, uint32_t> Bits;
+  Bits bits = 0;
 #pragma unroll
-  for (int i = 0; i < G; ++i) total += __popcll(__ballot(unpack<T>(raw, i) >= low));
-  if (b.n + total <= kList) {
+  for (int i = G - 1; i >= 0; --i) bits = bits + bits + (unpack<T>(raw, i) >= low);
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const float v = unpack<T>(raw, i);
-      const int at = at0 + i / E * 64 * E + i % E;
-      const bool in = v >= low && (v > low || at < before);
-      const uint64_t mask = __ballot(in);
-      if (mask) {
-        if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, at);
-        b.n += __popcll(mask);
-      }
-    }
-    if (b.n > 64) shrink(b);
-    return;
-  }
-#pragma unroll 1
-  for (int i = 0; i < G; ++i) {
-    const int at = at0 + i / E * 64 * E + i % E;
-    const float v = (float)x[min(at, b.end - 1)];
-    const bool in = at < b.end && (v > b.low || (v == b.low && at < b.before));
+  for (int u = 0; u < L; ++u)
+    *reinterpret_cast<u32x4*>(stash + (u * 64 + lane) * E) = u32x4{raw[4 * u], raw[4 * u + 1], raw[4 * u + 2], raw[4 * u + 3]};
+  while (__ballot(bits != 0)) {
+    const int i = bits ? __builtin_ctzll((uint64_t)bits) : 0, at = (i / E * 64 + lane) * E + i % E;
+    const float v = (float)stash[at];
+    const bool in = bits && (v > b.low || (v == b.low && base + at < b.before));
     const uint64_t mask = __ballot(in);
-    if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, at);
+    if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, base + at);
     b.n += __popcll(mask);
+    bits &= bits - 1;
     if (b.n > 64) shrink(b);
   }
 }
@@ -326,6 +313,7 @@ __device__ __forceinline__ uint64_t lanes_border(float top, int k) {
 template <typename T, int L>
 __global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
   __shared__ uint64_t lists[4][kList];
+  __shared__ __attribute__((aligned(16))) T stash[4][64 * L * kPer<T>];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float c = kLog2e * p.inv_t;
   const int64_t row = (int64_t)blockIdx.x * 4 + w;
@@ -339,9 +327,8 @@ __global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
   if (p.k == 0) return;
   Best b{lists[w]};
   b.k = p.k;
-  b.end = p.V;
   b.raise(lanes_border(top, p.k));
-  if (any_candidate<T>(b, 0, top)) collect<T, L>(b, x, 0, raw);
+  if (any_candidate<T>(b, 0, top)) collect<T, L>(b, 0, raw, stash[w]);
   const RowOut o(a, p.inv_t);
   rank_keys(b.list, b.n, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
 }
@@ -352,7 +339,9 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
   constexpr int E = kPer<T>, L = kLoads, CHUNK = 64 * L * E;
   __shared__ uint64_t lists[NW][kList];
   __shared__ uint64_t all[NW * 64];
+  __shared__ __attribute__((aligned(16))) T stash[NW][CHUNK];
   __shared__ float stats[NW][3];
+  __shared__ int found[NW];
   __shared__ uint64_t border[NW];  // of each wave
   __shared__ int total;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -365,7 +354,6 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
   Stats a;
   Best b{lists[w]};
   b.k = p.k;
-  b.end = v1;
   auto common = [&]() {
     const uint64_t mine =
         lane < NW ? __hip_atomic_load(&border[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : (uint64_t)0;
@@ -388,7 +376,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
       if (key == 0) key = lanes_border(top, p.k);  // (too few waves have values)
       b.raise(key);
       if (base < v1 && any_candidate<T>(b, base, top)) {
-        collect<T, L>(b, x, base, raw);
+        collect<T, L>(b, base, raw, stash[w]);
         if (base + NW * CHUNK < v1) {
           publish();
           known = b.n;
@@ -405,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
     if (p.k == 0 || !any_candidate<T>(b, base, top)) return;
     b.raise(common());
     if (!any_candidate<T>(b, base, top)) return;
-    collect<T, M>(b, x, base, raw);
+    collect<T, M>(b, base, raw, stash[w]);
     if (b.n < known || 2 * b.n >= 3 * known + 2) {  // (a new border costs more than a candidate)
       publish();
       known = b.n;
@@ -417,34 +405,48 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
   for (; base < v1; base += 64 * E) follow(std::integral_constant<int, 1>());
 
   a = wave_stats(a, c);
-  if (p.k) publish();
-  if (lane == 0) stats[w][0] = a.m, stats[w][1] = a.s, stats[w][2] = a.u;
+  if (lane == 0) stats[w][0] = a.m, stats[w][1] = a.s, stats[w][2] = a.u, found[w] = b.n;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
   Stats r;
   if (lane < NW) r.m = stats[lane][0], r.s = stats[lane][1], r.u = stats[lane][2];
   r = wave_stats(r, c);
+  int n = 0;
   if (p.k) {
-    const uint64_t least = common(), mine = lane < b.n ? b.list[lane] : 0;
-    const bool in = mine != 0 && ((uint32_t)least == kAnyIndex ? mine >> 32 >= least >> 32 : mine >= least);
-    const uint64_t mask = __ballot(in);
-    int at = 0;
-    if (lane == 0 && mask) at = atomicAdd(&total, __popcll(mask));
-    at = __builtin_amdgcn_readfirstlane(at);
-    if (in) all[at + __popcll(mask & (((uint64_t)1 << lane) - 1))] = mine;
+    const uint64_t mine = lane < b.n ? b.list[lane] : 0;
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      before += i < w ? found[i] : 0;
+      n += found[i];
+    }
+    if (n <= 64) {
+      if (mine) all[before + lane] = mine;
+    } else {  // more than a wave ranks at once: those that reach the border
+      publish();
+      __syncthreads();
+      const uint64_t least = common();
+      const bool in = mine != 0 && ((uint32_t)least == kAnyIndex ? mine >> 32 >= least >> 32 : mine >= least);
+      const uint64_t mask = __ballot(in);
+      int at = 0;
+      if (lane == 0 && mask) at = atomicAdd(&total, __popcll(mask));
+      at = __builtin_amdgcn_readfirstlane(at);
+      if (in) all[at + __popcll(mask & (((uint64_t)1 << lane) - 1))] = mine;
+    }
     __syncthreads();
+    if (n > 64) n = total;
   }
   if (parts == 1) {
     if (w == NW - 1) write_row<T>(p, row, r, lane, 64);
     if (p.k && w == 0) {
       const RowOut o(r, p.inv_t);
-      rank_keys(all, total, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
+      rank_keys(all, n, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
     }
   } else {
     char* to = static_cast<char*>(p.ws) + item * partial_bytes(p.k);
     if (threadIdx.x == 0) *reinterpret_cast<Partial*>(to) = Partial{r.m, r.s, r.u, 0.f};
     uint64_t* keys = reinterpret_cast<uint64_t*>(to + sizeof(Partial));
-    if (p.k && w == 0) rank_keys(all, total, p.k, [&](int rank, uint64_t key) { keys[rank] = key; });
+    if (p.k && w == 0) rank_keys(all, n, p.k, [&](int rank, uint64_t key) { keys[rank] = key; });
   }
 }
 
