@@ -98,6 +98,7 @@ template <typename T, bool VEC> struct Run {
     }
     // elements too many (of a row of under 8, whose only run begins with it: past its end)
     int s = min(max(c + 8 - K, 0), 8) * (int)sizeof(T) / 2;  // in half words
+    if (__ballot(s != 0) == 0) return;
     if (K >= 8) {
 #pragma unroll
       for (int step = N; step; step /= 2)  // words: N, N / 2, ..., 1

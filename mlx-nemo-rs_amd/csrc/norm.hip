@@ -8,7 +8,11 @@
 // that x and d are read once whatever the norm needs, the variance is taken
 // around the mean itself, and results may lie over their inputs. 16 lanes hold a
 // block of 128 columns: its largest magnitude is four DPP steps, and a wave's
-// four blocks of a chunk are one word of scale bytes. Bound: HBM, one pass.
+// four blocks of a chunk are one word of scale bytes. Bound: HBM, one pass: x, delta
+// and sum of 15001 x 4096 bf16 with codes, 431 MB, take 76 us (5.7 TB/s); one row of
+// 1024 takes 2.5, a launch and one chain of loads and sums.
+// Rows that are no whole runs of 8 pay for unaligned accesses and for putting the
+// row's end in place (2^25 bf16 in rows of 2047: 84 us, of 2048: 39).
 #include <algorithm>
 
 #include "fp8_common.hpp"
@@ -36,14 +40,14 @@ __device__ __forceinline__ void store8(T* row, int c, int D, const float v[8]) {
 // VEC: rows of whole runs of 8 columns.
 template <typename T, int CH, int W, bool VEC>
 __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormParams p) {
-  constexpr int RPB = W == 1 ? 4 : 1;  // rows of a workgroup at a time
-  __shared__ float red[4][W];
+  __shared__ float red[2][W];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = W == 1 ? 0 : wv;
+  const int64_t row = (int64_t)blockIdx.x * (W == 1 ? 4 : 1) + (W == 1 ? wv : 0);
+  if (row >= p.rows) return;
   const int kb = (p.D + 127) / 128, kbp = (kb + 3) / 4 * 4;
   auto col = [&](int i) { return 8 * (64 * (wr + W * i) + lane); };
   auto in = [&](int i, int e) { return VEC ? col(i) < p.D : col(i) + e < p.D; };
-  // weight and bias stay in registers from row to row where there are enough
-  constexpr bool HOLD = CH <= 2;
+  constexpr bool HOLD = CH <= 2;  // registers for all that is read, at once
   Run<float, VEC> w[CH], b[CH];
   auto weights = [&](int i) {
     if (p.w) {
@@ -66,11 +70,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
     for (int i = 0; i < CH; ++i) weights(i);
   }
   const float n = 1.f / (float)p.D;
-  int turn = 0;  // (a row's sums lie where no wave still reads the last row's)
   auto total = [&](float v, int which) {
     v = wave_reduce(v, [](float a, float c) { return a + c; });
     if constexpr (W > 1) {
-      float* r = red[2 * turn + which];
+      float* r = red[which];
       if (lane == 0) r[wr] = v;
       __syncthreads();
       v = 0.f;
@@ -79,87 +82,84 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
     }
     return v;
   };
-  for (int64_t row = (int64_t)blockIdx.x * RPB + (W == 1 ? wv : 0); row < p.rows; row += (int64_t)gridDim.x * RPB) {
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* d = static_cast<const T*>(p.delta) + row * p.ldd;
-    Run<T, VEC> tx[CH], td[CH];
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* d = static_cast<const T*>(p.delta) + row * p.ldd;
+  Run<T, VEC> tx[CH], td[CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) tx[i].load(x, col(i), p.D);
-    if (HOLD && p.delta) {
+  for (int i = 0; i < CH; ++i) tx[i].load(x, col(i), p.D);
+  if (HOLD && p.delta) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) td[i].load(d, col(i), p.D);
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int e = 0; e < Run<T, VEC>::N; ++e) td[i].u[e] = 0;
-    }
-    float v[CH][8];
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      if (!HOLD && p.delta) td[i].load(d, col(i), p.D);
-      tx[i].trim(col(i), p.D);
-      td[i].trim(col(i), p.D);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(p.scale, td[i][e], tx[i][e]);
-      if constexpr (!HOLD) __builtin_amdgcn_sched_barrier(0);
-    }
-    if (p.sum) {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) store8<VEC>(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
-    }
-    if (p.layer) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[i][e];
-      const float mean = total(s, 0) * n;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] - mean : 0.f;
-    }
-    float q = 0.f;
+    for (int i = 0; i < CH; ++i) td[i].load(d, col(i), p.D);
+  } else {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q = __builtin_fmaf(v[i][e], v[i][e], q);
-    const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(total(q, 1), n, p.eps));
-    turn ^= 1;
+      for (int e = 0; e < Run<T, VEC>::N; ++e) td[i].u[e] = 0;
+  }
+  float v[CH][8];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if (!HOLD && p.delta) td[i].load(d, col(i), p.D);
+    tx[i].trim(col(i), p.D);
+    td[i].trim(col(i), p.D);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(p.scale, td[i][e], tx[i][e]);
+    if constexpr (!HOLD) __builtin_amdgcn_sched_barrier(0);
+  }
+  if (p.sum) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) store8<VEC>(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
+  }
+  if (p.layer) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[i][e];
+    const float mean = total(s, 0) * n;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] - mean : 0.f;
+  }
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q = __builtin_fmaf(v[i][e], v[i][e], q);
+  const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(total(q, 1), n, p.eps));
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    if constexpr (!HOLD) weights(i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(v[i][e] * r, w[i][e], b[i][e]);
+    if constexpr (!HOLD) __builtin_amdgcn_sched_barrier(0);
+  }
+  if (p.out) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if constexpr (!HOLD) weights(i);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = __builtin_fmaf(v[i][e] * r, w[i][e], b[i][e]);
-      if constexpr (!HOLD) __builtin_amdgcn_sched_barrier(0);
+      if (p.out_dt == kBF16) store8<VEC>(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+      else store8<VEC>(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
     }
-    if (p.out) {
+  }
+  if (p.codes) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (p.out_dt == kBF16) store8<VEC>(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
-        else store8<VEC>(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
-      }
-    }
-    if (p.codes) {
+    for (int i = 0; i < CH; ++i) {
+      const int word = wr + W * i;  // of the row's scale bytes
+      if (4 * word >= kb) continue;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int word = wr + W * i;  // of the row's scale bytes
-        if (4 * word >= kb) continue;
+      for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] : 0.f;  // (a NaN of the sums reaches there too)
+      const int s = fp8_scale_byte(block_max(v[i]));
+      const float scale = fp8_scale(s);
+      if (col(i) < kb * 128)
+        *reinterpret_cast<u32x2*>(p.codes + row * ((int64_t)kb * 128) + col(i)) =
+            u32x2{fp8_pack4_scaled(v[i][0], v[i][1], v[i][2], v[i][3], scale),
+                  fp8_pack4_scaled(v[i][4], v[i][5], v[i][6], v[i][7], scale)};
+      uint32_t bytes = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] : 0.f;  // (a NaN of the sums reaches there too)
-        const int s = fp8_scale_byte(block_max(v[i]));
-        const float scale = fp8_scale(s);
-        if (col(i) < kb * 128)
-          *reinterpret_cast<u32x2*>(p.codes + row * ((int64_t)kb * 128) + col(i)) =
-              u32x2{fp8_pack4_scaled(v[i][0], v[i][1], v[i][2], v[i][3], scale),
-                    fp8_pack4_scaled(v[i][4], v[i][5], v[i][6], v[i][7], scale)};
-        uint32_t bytes = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          bytes |= (uint32_t)(4 * word + j < kb ? __builtin_amdgcn_readlane(s, 16 * j) : 127) << 8 * j;
-        if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + row * kbp + 4 * word) = bytes;
-      }
+      for (int j = 0; j < 4; ++j)
+        bytes |= (uint32_t)(4 * word + j < kb ? __builtin_amdgcn_readlane(s, 16 * j) : 127) << 8 * j;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + row * kbp + 4 * word) = bytes;
     }
   }
 }
@@ -167,20 +167,40 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
 template <typename T, int CH, int W>
 hipError_t launch(const NormParams& p, hipStream_t s) {
   if ((int64_t)512 * CH * W < p.D) return hipErrorInvalidValue;
-  const int64_t groups = W == 1 ? (p.rows + 3) / 4 : p.rows;
-  const unsigned grid = (unsigned)std::min<int64_t>(groups, 1 << 16);
-  if (p.D % 8 == 0) add_norm_kernel<T, CH, W, true><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(p);
-  else add_norm_kernel<T, CH, W, false><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(p);
+  constexpr int64_t most = 1 << 22;  // rows of a launch: a grid's threads fit 32 bits
+  auto behind = [](auto* q, int64_t n) { return q ? q + n : q; };
+  auto rows = [&](const void* q, DType dt, int64_t n) { return const_cast<char*>(behind((const char*)q, n * (dt == kBF16 ? 2 : 4))); };
+  const int64_t kb = (p.D + 127) / 128, kbp = (kb + 3) / 4 * 4;
+  for (int64_t r = 0; r < p.rows; r += most) {
+    NormParams q = p;
+    q.rows = std::min(most, p.rows - r);
+    q.x = rows(p.x, p.dt, r * p.ldx);
+    q.delta = rows(p.delta, p.dt, r * p.ldd);
+    q.sum = rows(p.sum, p.dt, r * p.lds);
+    q.out = rows(p.out, p.out_dt, r * p.ldo);
+    q.codes = behind(p.codes, r * kb * 128);
+    q.scales = behind(p.scales, r * kbp);
+    const unsigned grid = (unsigned)(W == 1 ? (q.rows + 3) / 4 : q.rows);
+    if (p.D % 8 == 0) add_norm_kernel<T, CH, W, true><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(q);
+    else add_norm_kernel<T, CH, W, false><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(q);
+  }
   return hipGetLastError();
 }
 
+// As many waves as the row fills with one run of 8 a lane, up to 16: with half the
+// waves and two runs a row of 1024, 4096 and 8192 bf16 takes 2.8, 3.1 and 3.7 us
+// instead of 2.5, 2.9 and 3.6, 2^25 values in such rows 39.8, 40.0 and 41.0 instead
+// of 38.9, 39.6 and 40.3; with twice the waves 2^25 values in rows of 512 take 45
+// instead of 39. A row per wave or workgroup, no loop over rows: the compiler took
+// addresses out of one and spilled (2^25 values in rows of 32768: 102 us instead of
+// 48).
 template <typename T>
 hipError_t by_width(const NormParams& p, hipStream_t s) {
   if (p.D <= 512) return launch<T, 1, 1>(p, s);
-  if (p.D <= 1024) return launch<T, 2, 1>(p, s);
+  if (p.D <= 1024) return launch<T, 1, 2>(p, s);
   if (p.D <= 2048) return launch<T, 1, 4>(p, s);
-  if (p.D <= 4096) return launch<T, 2, 4>(p, s);
-  if (p.D <= 8192) return launch<T, 2, 8>(p, s);
+  if (p.D <= 4096) return launch<T, 1, 8>(p, s);
+  if (p.D <= 8192) return launch<T, 1, 16>(p, s);
   return p.D <= 16384 ? launch<T, 2, 16>(p, s) : launch<T, 4, 16>(p, s);
 }
 
