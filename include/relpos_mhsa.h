@@ -589,8 +589,8 @@ void mhsa_adapters_destroy(mhsa_adapters* adapters);
 /* Adapter `slot`: a [rank, in_dim], b [out_dim, rank] in data_dtype (MHSA_F32 /
  * MHSA_BF16 / MHSA_F16; host or device memory), finite after their rounding to
  * bf16; rank 0 (a and b NULL) empties the slot, as all are before their first
- * load. Waits for the GPU; no call that reads the adapters may run at the same
- * time, other slots' either. A refused load leaves the slot as it was. */
+ * load. Waits for the GPU; no other call on the adapters may run at the same
+ * time, of other slots either. A refused load leaves the slot as it was. */
 int32_t mhsa_adapters_load(mhsa_adapters* adapters, int32_t slot, int32_t rank, int32_t data_dtype, const void* a,
                            const void* b, float scale);
 /* Workspace bytes of a call with adapters of `rows` rows or fewer, on floats or

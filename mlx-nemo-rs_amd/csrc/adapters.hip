@@ -29,8 +29,7 @@
 namespace mhsa {
 namespace {
 
-// VEC: rows of whole runs of 8 inputs.
-template <typename TX, int RT, bool VEC>
+template <typename TX, int RT, RowForm FORM>
 __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
   constexpr bool CODES = std::is_same_v<TX, uint8_t>, F32 = std::is_same_v<TX, float>;
   using TL = std::conditional_t<F32, float, bf16>;  // in LDS
@@ -49,7 +48,7 @@ __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
   const uint64_t some = __ballot(mine >= 0);
   // Run u of a block: row 4 u + lane / 16 (past the last: the last), 8 inputs.
   // (Rows' addresses are made again for each block, which takes no registers.)
-  Run<TL, VEC> x[4];  // (codes: two words of it, and their scale)
+  Run<TL, FORM> x[4];  // (codes: two words of it, and their scale)
   auto fetch = [&](int b) {
     int at = c4;
     asm volatile("" : "+v"(at));
@@ -188,8 +187,12 @@ __global__ __launch_bounds__(256) void adapter_weights_kernel(const T* from, int
 template <typename TX, int RT>
 hipError_t go(const AdapterRows& p, hipStream_t s) {
   const unsigned grid = (unsigned)((p.rows + 127) / 128 * 8);
-  if (std::is_same_v<TX, uint8_t> || p.K % 8 == 0) adapter_rows_kernel<TX, RT, true><<<grid, 512, 0, s>>>(p);
-  else if constexpr (!std::is_same_v<TX, uint8_t>) adapter_rows_kernel<TX, RT, false><<<grid, 512, 0, s>>>(p);
+  const RowForm form = std::is_same_v<TX, uint8_t> ? kWhole : row_form(p.K);
+  if (form == kWhole) adapter_rows_kernel<TX, RT, kWhole><<<grid, 512, 0, s>>>(p);
+  else if constexpr (!std::is_same_v<TX, uint8_t>) {
+    if (form == kRagged) adapter_rows_kernel<TX, RT, kRagged><<<grid, 512, 0, s>>>(p);
+    else adapter_rows_kernel<TX, RT, kTiny><<<grid, 512, 0, s>>>(p);
+  }
   return hipGetLastError();
 }
 template <typename TX>

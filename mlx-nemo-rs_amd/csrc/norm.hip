@@ -12,7 +12,7 @@
 // and sum of 15001 x 4096 bf16 with codes, 431 MB, take 76 us (5.7 TB/s); one row of
 // 1024 takes 2.5, a launch and one chain of loads and sums.
 // Rows that are no whole runs of 8 pay for unaligned accesses and for putting the
-// row's end in place (2^25 bf16 in rows of 2047: 84 us, of 2048: 39).
+// row's end in place (2^25 bf16 in rows of 2047: 42 us, of 2048: 39).
 #include <algorithm>
 
 #include "fp8_common.hpp"
@@ -23,22 +23,21 @@ namespace mhsa {
 namespace {
 
 // 8 values to columns [c, c + 8) of a row of D.
-template <bool VEC, typename T>
+template <RowForm FORM, typename T>
 __device__ __forceinline__ void store8(T* row, int c, int D, const float v[8]) {
   T t[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
   if (c + 8 <= D) {
     __builtin_memcpy(row + c, t, sizeof t);
-  } else if constexpr (!VEC) {
+  } else if constexpr (FORM != kWhole) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (c + e < D) row[c + e] = t[e];
   }
 }
 
-// VEC: rows of whole runs of 8 columns.
-template <typename T, int CH, int W, bool VEC>
+template <typename T, int CH, int W, RowForm FORM>
 __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormParams p) {
   __shared__ float red[2][W];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = W == 1 ? 0 : wv;
@@ -46,9 +45,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
   if (row >= p.rows) return;
   const int kb = (p.D + 127) / 128, kbp = (kb + 3) / 4 * 4;
   auto col = [&](int i) { return 8 * (64 * (wr + W * i) + lane); };
-  auto in = [&](int i, int e) { return VEC ? col(i) < p.D : col(i) + e < p.D; };
+  auto in = [&](int i, int e) { return FORM == kWhole ? col(i) < p.D : col(i) + e < p.D; };
   constexpr bool HOLD = CH <= 2;  // registers for all that is read, at once
-  Run<float, VEC> w[CH], b[CH];
+  Run<float, FORM> w[CH], b[CH];
   auto weights = [&](int i) {
     if (p.w) {
       w[i].load(p.w, col(i), p.D);
@@ -84,7 +83,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
   };
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* d = static_cast<const T*>(p.delta) + row * p.ldd;
-  Run<T, VEC> tx[CH], td[CH];
+  Run<T, FORM> tx[CH], td[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) tx[i].load(x, col(i), p.D);
   if (HOLD && p.delta) {
@@ -94,7 +93,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
-      for (int e = 0; e < Run<T, VEC>::N; ++e) td[i].u[e] = 0;
+      for (int e = 0; e < Run<T, FORM>::N; ++e) td[i].u[e] = 0;
   }
   float v[CH][8];
 #pragma unroll
@@ -108,7 +107,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
   }
   if (p.sum) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) store8<VEC>(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
+    for (int i = 0; i < CH; ++i) store8<FORM>(static_cast<T*>(p.sum) + row * p.lds, col(i), p.D, v[i]);
   }
   if (p.layer) {
     float s = 0.f;
@@ -138,8 +137,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
   if (p.out) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if (p.out_dt == kBF16) store8<VEC>(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
-      else store8<VEC>(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+      if (p.out_dt == kBF16) store8<FORM>(static_cast<bf16*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
+      else store8<FORM>(static_cast<float*>(p.out) + row * p.ldo, col(i), p.D, v[i]);
     }
   }
   if (p.codes) {
@@ -181,8 +180,11 @@ hipError_t launch(const NormParams& p, hipStream_t s) {
     q.codes = behind(p.codes, r * kb * 128);
     q.scales = behind(p.scales, r * kbp);
     const unsigned grid = (unsigned)(W == 1 ? (q.rows + 3) / 4 : q.rows);
-    if (p.D % 8 == 0) add_norm_kernel<T, CH, W, true><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(q);
-    else add_norm_kernel<T, CH, W, false><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(q);
+    auto run = [&](auto form) { add_norm_kernel<T, CH, W, decltype(form)::value><<<grid, W == 1 ? 256 : W * 64, 0, s>>>(q); };
+    const RowForm form = row_form(p.D);
+    if (form == kWhole) run(std::integral_constant<RowForm, kWhole>());
+    else if (form == kRagged) run(std::integral_constant<RowForm, kRagged>());
+    else if constexpr (CH * W == 1) run(std::integral_constant<RowForm, kTiny>());
   }
   return hipGetLastError();
 }
