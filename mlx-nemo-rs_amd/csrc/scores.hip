@@ -16,12 +16,17 @@
 // see a key that q = ceil(k / NW) of its values reach; k of the row then reach the
 // ceil(k / q)-th largest of these keys, and a value below it is none of the k
 // best. A chunk whose maximum is below costs one comparison. The keys start from
-// the lanes' maxima of the first chunk (some 50 candidates of 16384 for 20 best;
-// with a border of each wave's own it was 140, and ranking them took longer than
-// reading the row) and rise with the lists; they are read without a barrier, for
-// an old one is only lower. At the end the candidates that reach the border, and
+// the lanes' maxima of the first chunk and rise with the lists; they are read
+// without a barrier, for an old one is only lower. (With a border of each wave's
+// own there were three times as many candidates, 140 of 16384 values for 20 best,
+// and ranking them took longer than reading the row.) At the end the candidates that reach the border, and
 // then those of a long row's parts, are ranked by counting the larger ones. Rows
 // of up to 8 loads to a lane stay in one wave's registers as a single chunk.
+//
+// Bound: HBM over long rows of many (4001 x 50001 f32, 5 best: 146 us, 5.5 TB/s),
+// else the vector unit's 12 instructions a value and the candidates' bookkeeping:
+// 3000 x 9848 f32 take 21 us without the k best (5.6 TB/s), 30 with 5, 35 with 20;
+// 64 x 128000 bf16, 20 best, 16.5, of which the join of the parts is 5.
 #include <algorithm>
 
 #include "fp8_common.hpp"
@@ -245,28 +250,36 @@ __device__ __host__ inline int64_t partial_bytes(int k) { return (int64_t)sizeof
 
 // L loads of a lane from x + base on (values up to v1, the first FULL loads of all
 // lanes below it) as they lie in memory, into the statistics; the largest value.
-template <typename T, int L, int FULL>
-__device__ __forceinline__ float load_chunk(const T* x, int base, int v1, float c, uint32_t raw[4 * L], Stats& a) {
+// A lane whose load would pass the end of the row (of V >= kPer values, or TINY)
+// loads the row's last values, and what is not its own, or past v1, is -inf: no
+// branch keeps a load waiting for another.
+template <typename T, int L, int FULL, bool TINY = false>
+__device__ __forceinline__ float load_chunk(const T* x, int base, int v1, int V, float c, uint32_t raw[4 * L], Stats& a) {
   constexpr int E = kPer<T>;
   const int lane = threadIdx.x & 63;
+  if constexpr (TINY) {
+    T t[E];
 #pragma unroll
-  for (int u = 0; u < L; ++u) {
-    const int at = base + (u * 64 + lane) * E;
-    if (u < FULL || base + (u + 1) * 64 * E <= v1) {
-      __builtin_memcpy(raw + 4 * u, x + at, 16);
-    } else if (base + u * 64 * E >= v1) {
-      T t[E];
+    for (int e = 0; e < E; ++e) t[e] = x[min(base + lane * E + e, V - 1)];
 #pragma unroll
-      for (int e = 0; e < E; ++e) t[e] = (T)-__builtin_inff();
-      __builtin_memcpy(raw + 4 * u, t, 16);
-    } else {
-      T t[E];
+    for (int e = 0; e < E; ++e)
+      if (base + lane * E + e >= V) t[e] = (T)-__builtin_inff();
+    __builtin_memcpy(raw, t, 16);
+  } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) t[e] = x[min(at + e, v1 - 1)];
+    for (int u = 0; u < L; ++u) {
+      const int at = base + (u * 64 + lane) * E;
+      __builtin_memcpy(raw + 4 * u, x + (u < FULL ? at : min(at, V - E)), 16);
+    }
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (at + e >= v1) t[e] = (T)-__builtin_inff();
-      __builtin_memcpy(raw + 4 * u, t, 16);
+    for (int u = FULL; u < L; ++u) {
+      const int from = base + (u * 64 + lane + 1) * E - v1;  // values that are not its own, if positive
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t& r = raw[4 * u + i];
+        if constexpr (sizeof(T) == 4) r = from > i ? 0xFF800000u : r;
+        else r = from > 2 * i + 1 ? 0xFF80FF80u : from > 2 * i ? (r & 0xFFFF0000u) | 0xFF80u : r;
+      }
     }
   }
   float top = -__builtin_inff();
@@ -289,9 +302,10 @@ __device__ __forceinline__ bool any_candidate(const Best& b, int base, float top
 }
 
 // Those that the border lets through join the list, one of each lane at a time;
-// `stash` (LDS of the wave) takes the chunk, for registers have no index.
+// `stash` (LDS of the wave) takes the chunk, for registers have no index. `last`:
+// where the row's last load begins.
 template <typename T, int L>
-__device__ __forceinline__ void collect(Best& b, int base, const uint32_t raw[4 * L], T* stash) {
+__device__ __forceinline__ void collect(Best& b, int base, int last, const uint32_t raw[4 * L], T* stash) {
   constexpr int E = kPer<T>, G = L * E;
   const int lane = threadIdx.x & 63;
   const uint64_t below = ((uint64_t)1 << lane) - 1;
@@ -304,11 +318,12 @@ __device__ __forceinline__ void collect(Best& b, int base, const uint32_t raw[4 
   for (int u = 0; u < L; ++u)
     *reinterpret_cast<u32x4*>(stash + (u * 64 + lane) * E) = u32x4{raw[4 * u], raw[4 * u + 1], raw[4 * u + 2], raw[4 * u + 3]};
   while (__ballot(bits != 0)) {
-    const int i = bits ? __builtin_ctzll((uint64_t)bits) : 0, at = (i / E * 64 + lane) * E + i % E;
-    const float v = (float)stash[at];
-    const bool in = bits && (v > b.low || (v == b.low && base + at < b.before));
+    const int i = bits ? __builtin_ctzll((uint64_t)bits) : 0, load = (i / E * 64 + lane) * E;
+    const float v = (float)stash[load + i % E];
+    const int at = min(base + load, last) + i % E;
+    const bool in = bits && (v > b.low || (v == b.low && at < b.before));
     const uint64_t mask = __ballot(in);
-    if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, base + at);
+    if (in) b.list[b.n + __popcll(mask & below)] = key_of(v, at);
     b.n += __popcll(mask);
     bits &= bits - 1;
     if (b.n > 64) shrink(b);
@@ -336,14 +351,15 @@ __global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
   given.fetch(p, row, lane);
   Stats a;
   uint32_t raw[4 * L];
-  const float top = load_chunk<T, L, L - 1>(x, 0, p.V, c, raw, a);
+  const bool tiny = L == 1 && p.V < kPer<T>;
+  const float top = tiny ? load_chunk<T, 1, 0, true>(x, 0, p.V, p.V, c, raw, a) : load_chunk<T, L, L - 1>(x, 0, p.V, p.V, c, raw, a);
   a = wave_stats(a, c);
   write_row(p, row, a, given);
   if (p.k == 0) return;
   Best b{lists[w]};
   b.k = p.k;
   b.raise(lanes_border(top, p.k));
-  if (any_candidate<T>(b, 0, top)) collect<T, L>(b, 0, raw, stash[w]);
+  if (any_candidate<T>(b, 0, top)) collect<T, L>(b, 0, tiny ? 0 : p.V - kPer<T>, raw, stash[w]);
   const RowOut o(a, p.inv_t);
   rank_keys(b.list, b.n, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
 }
@@ -352,6 +368,7 @@ __global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
 template <typename T, int NW>
 __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int parts, int per) {
   constexpr int E = kPer<T>, L = kLoads, CHUNK = 64 * L * E;
+  static_assert(L == 4, "the parts of a chunk");
   __shared__ uint64_t lists[NW][kList];
   __shared__ uint64_t all[NW * 64];
   __shared__ __attribute__((aligned(16))) T stash[NW][CHUNK];
@@ -365,8 +382,8 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
   const int64_t item = blockIdx.x;
   const int64_t row = item / parts;
   // a wave's values, as many as another's: with chunks dealt out in turn the last
-  // wave's few values gave a border far too low (128 rows x 50000, 20 best: 37 us
-  // instead of 13)
+  // wave's few values gave a border far too low (128 rows x 50000 bf16, 20 best, by
+  // eight waves: 37 us instead of 13)
   const int p0 = (int)(item % parts) * per, p1 = min(p.V, p0 + per), each = ((p1 - p0 + NW - 1) / NW + E - 1) / E * E;
   const int v0 = min(p1, p0 + w * each), v1 = min(p1, v0 + each);
   const T* x = static_cast<const T*>(p.x) + row * p.ld;
@@ -384,46 +401,40 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
     const uint64_t key = reached(b, nth);
     if (lane == 0 && key > border[w]) __hip_atomic_store(&border[w], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   };
-  int base = v0, known = 0;  // candidates when the wave's border was last made
-  {
+  int known = 0;  // candidates when the wave's border was last made
+  bool first = true;
+#pragma unroll 1
+  for (int base = v0; base < v1; base += CHUNK) {
     uint32_t raw[4 * L];
-    float top = -__builtin_inff();
-    if (base < v1) top = load_chunk<T, L, 0>(x, base, v1, c, raw, a);
-    if (p.k) {
+    float top;
+    auto part = [&](auto loads) {
+      constexpr int M = decltype(loads)::value;
+#pragma unroll
+      for (int i = 4 * M; i < 4 * L; ++i) raw[i] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+      top = load_chunk<T, M, M - 1>(x, base, v1, p.V, c, raw, a);
+    };
+    if (base + CHUNK <= v1) top = load_chunk<T, L, L>(x, base, v1, p.V, c, raw, a);
+    else if (base + 3 * 64 * E < v1) part(std::integral_constant<int, 4>());
+    else if (base + 2 * 64 * E < v1) part(std::integral_constant<int, 3>());
+    else if (base + 64 * E < v1) part(std::integral_constant<int, 2>());
+    else part(std::integral_constant<int, 1>());
+    if (p.k == 0) continue;
+    if (first) {  // (every wave has values)
       const uint64_t mine = lanes_border(top, nth);
       if (lane == 0) border[w] = mine;
       __syncthreads();
-      uint64_t key = common();
-      if (key == 0) key = lanes_border(top, p.k);  // (too few waves have values)
-      b.raise(key);
-      if (base < v1 && any_candidate<T>(b, base, top)) {
-        collect<T, L>(b, base, raw, stash[w]);
-        if (base + CHUNK < v1) {
-          publish();
-          known = b.n;
-        }
+    }
+    if (!first && !any_candidate<T>(b, base, top)) continue;
+    b.raise(common());
+    if (any_candidate<T>(b, base, top)) {
+      collect<T, L>(b, base, p.V - E, raw, stash[w]);
+      if (first || b.n < known || 2 * b.n >= 3 * known + 2) {  // (a new border costs more than a candidate)
+        if (base + CHUNK < v1) publish();
+        known = b.n;
       }
     }
-    base += CHUNK;
+    first = false;
   }
-  // whole chunks, then single loads
-  auto follow = [&](auto loads) {
-    constexpr int M = decltype(loads)::value;
-    uint32_t raw[4 * M];
-    const float top = load_chunk<T, M, M == L ? L : 0>(x, base, v1, c, raw, a);
-    if (p.k == 0 || !any_candidate<T>(b, base, top)) return;
-    b.raise(common());
-    if (!any_candidate<T>(b, base, top)) return;
-    collect<T, M>(b, base, raw, stash[w]);
-    if (b.n < known || 2 * b.n >= 3 * known + 2) {  // (a new border costs more than a candidate)
-      publish();
-      known = b.n;
-    }
-  };
-#pragma unroll 1
-  for (; base + CHUNK <= v1; base += CHUNK) follow(std::integral_constant<int, L>());
-#pragma unroll 1
-  for (; base < v1; base += 64 * E) follow(std::integral_constant<int, 1>());
 
   a = wave_stats(a, c);
   if (lane == 0) stats[w][0] = a.m, stats[w][1] = a.s, stats[w][2] = a.u, found[w] = b.n;
@@ -515,13 +526,15 @@ __global__ __launch_bounds__(64) void join_kernel(ScoresParams p, int parts) {
   rank_keys(list, n, p.k, [&](int rank, uint64_t k) { write_top(p, row, o, rank, k); });
 }
 
-int64_t max_parts(int V) { return std::clamp<int64_t>(V / 8192, 1, kMaxParts); }
+int64_t max_parts(int V) { return std::clamp<int64_t>(V / 4096, 1, kMaxParts); }
 
-// Parts of 8192 values or more while there are fewer of them than 2 to a CU: 64
-// rows of 128000 bf16, 20 best, take 13.2 us in 8 parts each, 17.5 in 4, 19.3 in 12
-// (which also leave more to join).
+// Fewer rows than 2 to a CU are cut into parts of 4096 values or more, of which
+// there are about 4 to a CU: with 2 to a CU 400 rows of 100000 f32, 20 best, take 44
+// us instead of 40 and 300 of 30000 bf16 18.3 instead of 16.7 (64 of 128000 alike).
+// Eight waves to a part instead of four, 2 to a CU: 48, 18.9.
 int64_t parts_of(int64_t rows, int V) {
-  return std::clamp<int64_t>((2 * device_cus() + rows - 1) / rows, 1, max_parts(V));
+  const int64_t cus = device_cus();
+  return rows >= 2 * cus ? 1 : std::clamp<int64_t>((4 * cus + rows - 1) / rows, 1, max_parts(V));
 }
 
 template <typename T>
@@ -544,12 +557,18 @@ hipError_t go(const ScoresParams& p, hipStream_t s) {
     return hipGetLastError();
   }
   const int parts = (int)parts_of(p.rows, p.V), per = ((p.V + parts - 1) / parts + 63) / 64 * 64;
+  // every wave has values (they take a multiple of kPer each, the last what is left)
+  if (p.V - (parts - 1) * per <= 16 * kPer<T>) return hipErrorInvalidValue;
   if (parts > 1) {
     if (!p.ws) return hipErrorInvalidValue;
-    scores_kernel<T, 8><<<(unsigned)(p.rows * parts), 512, 0, s>>>(p, parts, per);
+    scores_kernel<T, 4><<<(unsigned)(p.rows * parts), 256, 0, s>>>(p, parts, per);
     join_kernel<T><<<(unsigned)p.rows, 64, 0, s>>>(p, parts);
     return hipGetLastError();
   }
+  // Waves by the vocabulary alone, so that a row's bits do not depend on how many
+  // rows come with it: two up to 32 loads a lane, four beyond. 30000 rows of 5000
+  // bf16, 20 best, take 132 us with two waves, 172 with four, 407 with eight; 4001
+  // of 50001 f32, 5 best, 154, 145 and 144; 771 of 20000 f32, 20 best, 28, 21, 27.
   constexpr int64_t most = 1 << 22;  // rows of a launch: a grid's threads fit 32 bits
   for (int64_t r = 0; r < p.rows; r += most) {
     ScoresParams q = p;
@@ -560,18 +579,19 @@ hipError_t go(const ScoresParams& p, hipStream_t s) {
     q.entropy = p.entropy ? p.entropy + r : nullptr;
     q.top = p.top ? p.top + r * p.k : nullptr;
     q.top_lp = p.top_lp ? p.top_lp + r * p.k : nullptr;
-    scores_kernel<T, 8><<<(unsigned)q.rows, 512, 0, s>>>(q, 1, per);
+    if (loads <= 32) scores_kernel<T, 2><<<(unsigned)q.rows, 128, 0, s>>>(q, 1, per);
+    else scores_kernel<T, 4><<<(unsigned)q.rows, 256, 0, s>>>(q, 1, per);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-// (for any number of rows up to `rows`: r rows in p parts have r p < 2 CUs + r
+// (for any number of rows up to `rows`: r rows in p parts have r p < 4 CUs + r
 // and p <= most, and none have parts from 2 CUs on)
 int64_t scores_workspace(int64_t rows, int V, int k) {
-  const int64_t most = max_parts(V), want = 2 * device_cus(), r = std::min(rows, want - 1);
-  return most > 1 ? std::min(r * most, want - 1 + r) * partial_bytes(k) : 0;
+  const int64_t most = max_parts(V), cus = device_cus(), r = std::min(rows, 2 * cus - 1);
+  return most > 1 ? std::min(r * most, 4 * cus - 1 + r) * partial_bytes(k) : 0;
 }
 
 hipError_t token_scores(const ScoresParams& p, hipStream_t s) {
