@@ -19,6 +19,13 @@
 // adapter (184 MB), 62 with adapters of rank 64 (480 MB more). 32 or 64 rows to a
 // workgroup read A less often, but leave fewer waves (40 and 54 us without an
 // adapter) and make more of the rows where one request ends (67 and 83 us with).
+//
+// Up to 4 rows a CU are 4 to a workgroup, of 16 waves: there a wave's blocks and the
+// adapters of its rows, one behind the other, are what the launch lasts. With the
+// projection 16 rows of 4096 -> 1024 with 16 adapters of rank 16 take 18 us instead
+// of 37, 256 rows with 64 of rank 64 30 instead of 53, 1000 rows of 1024 -> 1024 f32
+// with 10 14.1 instead of 15.4; 3000 rows of 1024 -> 4096 would take 31.2 instead of
+// 30.0, for A is read four times as often.
 #include <algorithm>
 #include <type_traits>
 
@@ -29,31 +36,32 @@
 namespace mhsa {
 namespace {
 
-template <typename TX, int RT, RowForm FORM>
-__global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
+template <typename TX, int RT, RowForm FORM, bool FEW>
+__global__ __launch_bounds__(FEW ? 1024 : 512, 4) void adapter_rows_kernel(AdapterRows p) {
+  constexpr int NW = FEW ? 16 : 8, ROWS = FEW ? 4 : 16;
   constexpr bool CODES = std::is_same_v<TX, uint8_t>, F32 = std::is_same_v<TX, float>;
   using TL = std::conditional_t<F32, float, bf16>;  // in LDS
-  constexpr int PITCH = 128 * (int)sizeof(TL) + 16, BUF = 16 * PITCH, RED = 8 * RT * 1024;
-  __shared__ __attribute__((aligned(16))) char smem[8 * BUF > RED ? 8 * BUF : RED];
+  constexpr int PITCH = 128 * (int)sizeof(TL) + 16, BUF = ROWS * PITCH, RED = NW * RT * 1024;
+  __shared__ __attribute__((aligned(16))) char smem[NW * BUF > RED ? NW * BUF : RED];
   const int lane = threadIdx.x & 63, r = lane & 15, c4 = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kb = (p.K + 127) / 128, kp = kb * 128, kbp = (kb + 3) / 4 * 4;
   // a stretch of rows to each XCD, whose L2 then holds few adapters' A
   const unsigned per = gridDim.x / 8;
-  const int64_t group = blockIdx.x % 8 * per + blockIdx.x / 8, row0 = group * 16;
+  const int64_t group = blockIdx.x % 8 * per + blockIdx.x / 8, row0 = group * ROWS;
   if (row0 >= p.rows) return;
-  const int rows = (int)min<int64_t>(p.rows - row0, 16);
+  const int rows = (int)min<int64_t>(p.rows - row0, ROWS);
   int mine = r < rows ? p.which[row0 + r] : -1;
   if (mine >= p.n) mine = -1;
   const uint64_t some = __ballot(mine >= 0);
   // Run u of a block: row 4 u + lane / 16 (past the last: the last), 8 inputs.
   // (Rows' addresses are made again for each block, which takes no registers.)
-  Run<TL, FORM> x[4];  // (codes: two words of it, and their scale)
+  Run<TL, FORM> x[ROWS / 4];  // (codes: two words of it, and their scale)
   auto fetch = [&](int b) {
     int at = c4;
     asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < ROWS / 4; ++u) {
       const int64_t row = row0 + min(4 * u + at, rows - 1);
       if constexpr (CODES) {
         __builtin_memcpy(x[u].u, p.codes + row * kp + b * 128 + 8 * r, 8);
@@ -70,16 +78,16 @@ __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
   // Workgroups begin at different blocks: with rows of some KB, the same ones of
   // all rows lie on few of the memory's channels (15001 rows x 4096 without an
   // adapter 58 -> 36 us).
-  const int turn = (int)(group % ((kb + 7) / 8)) * 8;
+  const int turn = (int)(group % ((kb + NW - 1) / NW)) * NW;
   auto block = [&](int i) { return i + turn < kb ? i + turn : i + turn - kb; };
   if (w < kb) fetch(block(w));
 #pragma unroll 1
-  for (int i = w; i < kb; i += 8) {
+  for (int i = w; i < kb; i += NW) {
     const int b = block(i);
     int at = c4;
     asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < ROWS / 4; ++u) {
       char* to = buf + (4 * u + c4) * PITCH + 8 * r * (int)sizeof(TL);
       if constexpr (CODES) {
         *reinterpret_cast<bf16x8*>(to) = fp8_to_bf16(x[u].u[0], x[u].u[1], fp8_scale((int)x[u].u[2]));
@@ -99,7 +107,7 @@ __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
         }
       }
     }
-    if (i + 8 < kb) fetch(block(i + 8));
+    if (i + NW < kb) fetch(block(i + NW));
     for (uint64_t todo = some; todo;) {
       const int d = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
       todo &= ~__ballot(mine == d);
@@ -114,7 +122,7 @@ __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         if (AHEAD == 2 ? st < 3 : st > 0) fetch_a(st + AHEAD - 1);
-        const char* from = buf + r * PITCH + (32 * st + 8 * c4) * (int)sizeof(TL);
+        const char* from = buf + r % ROWS * PITCH + (32 * st + 8 * c4) * (int)sizeof(TL);
         u32x4 f[F32 ? 3 : 1];
         if constexpr (F32) {
           const floatx4 lo = *reinterpret_cast<const floatx4*>(from), hi = *reinterpret_cast<const floatx4*>(from + 16);
@@ -150,10 +158,10 @@ __global__ __launch_bounds__(512, 4) void adapter_rows_kernel(AdapterRows p) {
   if (r >= rows) return;
   const int ext = p.parts * p.rank;
   const float s = mine >= 0 ? p.scale[mine] : 0.f;  // (of no adapter: the sums are 0)
-  for (int j = w; j < RT; j += 8) {
+  for (int j = w; j < RT; j += NW) {
     floatx4 v = red[j * 64 + lane];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += red[(i * RT + j) * 64 + lane];
+    for (int i = 1; i < NW; ++i) v += red[(i * RT + j) * 64 + lane];
     uint16_t* t = p.t + (row0 + r) * ext + 16 * j + 4 * c4;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= s;
@@ -186,12 +194,17 @@ __global__ __launch_bounds__(256) void adapter_weights_kernel(const T* from, int
 
 template <typename TX, int RT>
 hipError_t go(const AdapterRows& p, hipStream_t s) {
-  const unsigned grid = (unsigned)((p.rows + 127) / 128 * 8);
+  const bool few = p.rows <= 4 * device_cus();
+  const unsigned grid = (unsigned)((p.rows + (few ? 31 : 127)) / (few ? 32 : 128) * 8);
+  auto run = [&](auto form) {
+    if (few) adapter_rows_kernel<TX, RT, decltype(form)::value, true><<<grid, 1024, 0, s>>>(p);
+    else adapter_rows_kernel<TX, RT, decltype(form)::value, false><<<grid, 512, 0, s>>>(p);
+  };
   const RowForm form = std::is_same_v<TX, uint8_t> ? kWhole : row_form(p.K);
-  if (form == kWhole) adapter_rows_kernel<TX, RT, kWhole><<<grid, 512, 0, s>>>(p);
+  if (form == kWhole) run(std::integral_constant<RowForm, kWhole>());
   else if constexpr (!std::is_same_v<TX, uint8_t>) {
-    if (form == kRagged) adapter_rows_kernel<TX, RT, kRagged><<<grid, 512, 0, s>>>(p);
-    else adapter_rows_kernel<TX, RT, kTiny><<<grid, 512, 0, s>>>(p);
+    if (form == kRagged) run(std::integral_constant<RowForm, kRagged>());
+    else run(std::integral_constant<RowForm, kTiny>());
   }
   return hipGetLastError();
 }
