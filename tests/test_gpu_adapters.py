@@ -111,6 +111,19 @@ def test_many_rows(rows, k, n, count, yd):
     made.check(got[at], x[at], which[at])
 
 
+@pytest.mark.parametrize("rows,k,n,ranks", [(1100, 5, 40, [3, 16]), (1030, 1001, 96, [40, 7]), (1024, 520, 64, [100]),
+                                            (6, 4100, 64, [16, 9, 2]), (203, 2600, 130, [60, 30, 5, 1])])
+@pytest.mark.parametrize("xd,yd", [("bf16", "bf16"), ("f32", "f32")])
+def test_requests_of_every_length(rows, k, n, ranks, xd, yd):
+    """Adapters that change from row to row, and rows of no whole runs of 8, few and many."""
+    rng = np.random.default_rng(rows + n)
+    made = Made(rng, k, n, ranks, max(ranks))
+    x = tensor(rng.standard_normal((rows, k)), xd)
+    for which in (requests(rng, rows, len(ranks), rows), rng.integers(-1, len(ranks), rows).astype(np.int32)):
+        got = made.layer.forward(x, out_dtype=DTYPES[yd], adapters=made.adapters, which=torch.from_numpy(which).cuda())
+        made.check(got, x, which)
+
+
 @pytest.mark.parametrize("rows,k,n", [(1, 128, 64), (5, 100, 40), (16, 1000, 130), (40, 512, 2048), (300, 384, 333), (3000, 512, 2050),
                                       (2, 2200, 96)])
 @pytest.mark.parametrize("yd", ["bf16", "f32"])

@@ -82,6 +82,35 @@ def test_against_oracle(rows, v, dtype):
         check(x, tokens, k, [1.0, 0.5, 1.7][k % 3])
 
 
+@pytest.mark.parametrize("v", [2049, 2052, 4095, 4097, 4104, 8192, 8193, 9002, 12301, 16384, 16391])
+@pytest.mark.parametrize("rows", [6, 530])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_ends_of_rows(rows, v, dtype):
+    """The largest logits where a row, its waves' shares and their chunks begin and end."""
+    rng = np.random.default_rng(v)
+    few = logits(rng, 6, v)
+    for i in range(6):
+        for n, at in enumerate((v - 1, 0, v - 2 - i, v // 2 - i, v // 4 + i, 1024 + i, v - 9 - i)):
+            few[i, at] = 40.0 + (n + i) % 7
+    x = tensor(few, dtype)
+    tokens = np.stack([np.full(6, v - 1), np.arange(6), v - 1 - np.arange(6), rng.integers(0, v, 6)], 1).astype(np.int32)
+    if rows == 6:
+        check(x, tokens, 9)
+        check(x, tokens, 0)
+        return
+    whole = x.repeat(-(-rows // 6), 1)[:rows]
+    got = M.token_log_probs(whole, torch.from_numpy(np.tile(tokens, (-(-rows // 6), 1))[:rows]).cuda(), 9)
+    lp, h, idx, top, sizes = R.scores(f64(x), tokens, 9)
+    # every logit is within 60 of the largest; as in check() otherwise
+    n, (m1, m2, ls) = v / 64 + 66, sizes.T
+    far = STEP * (n + 4 * m1 + 6 * ls + 8 * 60)[:, None]
+    for i in (0, rows - rows % 6 - 6):
+        assert np.array_equal(got.top_indices[i:i + 6].cpu().numpy(), idx)
+        close(got.log_probs[i:i + 6], lp, far)
+        close(got.top_log_probs[i:i + 6], top, far)
+        close(got.entropy[i:i + 6], h, STEP * (n * (1 + 2 * m1 + ls) + 8 * m2))
+
+
 @pytest.mark.parametrize("rows,v", [(2500, 1025), (1200, 5000)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_many_rows(rows, v, dtype):
