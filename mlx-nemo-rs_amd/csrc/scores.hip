@@ -24,7 +24,8 @@
 // of up to 8 loads to a lane stay in one wave's registers as a single chunk.
 //
 // Bound: HBM over long rows of many (4001 x 50001 f32, 5 best: 146 us, 5.5 TB/s),
-// else the vector unit's 12 instructions a value and the candidates' bookkeeping:
+// else the vector unit (15 instructions a value there, 27 in short rows) and the
+// candidates' bookkeeping, some 500 of a wave and one chain of LDS reads:
 // 3000 x 9848 f32 take 21 us without the k best (5.6 TB/s), 30 with 5, 35 with 20;
 // 64 x 128000 bf16, 20 best, 16.5, of which the join of the parts is 5.
 #include <algorithm>
