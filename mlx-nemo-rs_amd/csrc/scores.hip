@@ -26,7 +26,7 @@
 // Bound: HBM over long rows of many (4001 x 50001 f32, 5 best: 146 us, 5.5 TB/s),
 // else the vector unit (15 instructions a value there, 27 in short rows) and the
 // candidates' bookkeeping, some 500 of a wave and one chain of LDS reads:
-// 3000 x 9848 f32 take 21 us without the k best (5.6 TB/s), 30 with 5, 35 with 20;
+// 3000 x 9848 f32 take 21 us without the k best (5.6 TB/s), 29 with 5, 34 with 20;
 // 64 x 128000 bf16, 20 best, 16.5, of which the join of the parts is 5.
 #include <algorithm>
 
@@ -365,9 +365,12 @@ __global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
   rank_keys(b.list, b.n, p.k, [&](int rank, uint64_t key) { write_top(p, row, o, rank, key); });
 }
 
-// NW waves to a row, or to each of its `parts` parts of `per` values.
+// NW waves to a row, or to each of its `parts` parts of `per` values. Registers for 6
+// waves a SIMD, which costs one of bf16 a place in scratch (30000 rows of 5000, 5
+// best: 104 us; with 100 registers, 4 waves a SIMD, 122, and without the k best of
+// 4001 x 50001 89 instead of 97).
 template <typename T, int NW>
-__global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int parts, int per) {
+__global__ __launch_bounds__(NW * 64, 6) void scores_kernel(ScoresParams p, int parts, int per) {
   constexpr int E = kPer<T>, L = kLoads, CHUNK = 64 * L * E;
   static_assert(L == 4, "the parts of a chunk");
   __shared__ uint64_t lists[NW][kList];
@@ -420,16 +423,28 @@ __global__ __launch_bounds__(NW * 64, 4) void scores_kernel(ScoresParams p, int 
     else if (base + 64 * E < v1) part(std::integral_constant<int, 2>());
     else part(std::integral_constant<int, 1>());
     if (p.k == 0) continue;
+    uint64_t key = 0;
     if (first) {  // (every wave has values)
-      const uint64_t mine = lanes_border(top, nth);
-      if (lane == 0) border[w] = mine;
-      __syncthreads();
+      // the wave's own border where another's values do not reach one, as in a mask
+      // that leaves one stretch (3000 x 9848 f32, 7 of 8 ruled out: 42 -> 24 us)
+#pragma unroll 1
+      for (int turn = 0; turn < 2 && key == 0; ++turn) {
+        key = lanes_border(top, turn ? p.k : nth);
+        if (turn) break;
+        if (lane == 0) border[w] = key;
+        __syncthreads();
+        key = common();
+      }
+    } else {
+      if (!any_candidate<T>(b, base, top)) continue;
+      key = common();
     }
-    if (!first && !any_candidate<T>(b, base, top)) continue;
-    b.raise(common());
+    b.raise(key);
     if (any_candidate<T>(b, base, top)) {
       collect<T, L>(b, base, p.V - E, raw, stash[w]);
-      if (first || b.n < known || 2 * b.n >= 3 * known + 2) {  // (a new border costs more than a candidate)
+      if (first) {
+        known = b.n;
+      } else if (b.n < known || 2 * b.n >= 3 * known + 2) {  // (a new border costs more than a candidate)
         if (base + CHUNK < v1) publish();
         known = b.n;
       }
@@ -568,7 +583,7 @@ hipError_t go(const ScoresParams& p, hipStream_t s) {
   }
   // Waves by the vocabulary alone, so that a row's bits do not depend on how many
   // rows come with it: two up to 32 loads a lane, four beyond. 30000 rows of 5000
-  // bf16, 20 best, take 132 us with two waves, 172 with four, 407 with eight; 4001
+  // bf16, 20 best, took 132 us with two waves, 172 with four, 407 with eight; 4001
   // of 50001 f32, 5 best, 154, 145 and 144; 771 of 20000 f32, 20 best, 28, 21, 27.
   constexpr int64_t most = 1 << 22;  // rows of a launch: a grid's threads fit 32 bits
   for (int64_t r = 0; r < p.rows; r += most) {

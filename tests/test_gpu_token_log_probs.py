@@ -224,3 +224,20 @@ def test_refusals():
                 lambda: M.token_log_probs(x, tok[:, None].expand(4, 2)), lambda: M.token_log_probs(x[:, :0])):
         with pytest.raises(M.MhsaError):
             bad()
+
+
+@pytest.mark.parametrize("rows,v", [(3, 5000), (520, 9848), (2, 40001)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masks_that_leave_a_stretch(rows, v, dtype):
+    """Some waves have no token at all, or fewer than are asked for."""
+    rng = np.random.default_rng(v)
+    few = logits(rng, 3, v)
+    for i, (lo, hi) in enumerate(((0, v // 9), (v // 2 + 5, v // 2 + 12), (v - v // 7, v))):
+        few[i, :lo] = few[i, hi:] = -np.inf
+    x = tensor(few[:rows], dtype)
+    tokens = rng.integers(-1, v, (len(x), 2)).astype(np.int32)
+    check(x, tokens, 20)
+    if rows > 3:
+        whole = x.repeat(-(-rows // 3), 1)[:rows]
+        got, want = M.token_log_probs(whole, top_k=20), M.token_log_probs(x, top_k=20)
+        assert torch.equal(got.top_indices[-3 - rows % 3:][:3], want.top_indices)
