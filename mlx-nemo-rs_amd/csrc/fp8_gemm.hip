@@ -340,23 +340,56 @@ __device__ __forceinline__ void few_inner(const Fp8Gemm& p, int w, int to, int m
 // Adds the adapters' products of this lane's row, of which t is given, and 16 RC
 // columns from n0 on to acc, as few_block its block's. The distinct adapters of
 // the 16 rows, 32 ranks at a time, are shared out to the waves; a row of another
-// adapter counts as zero.
+// adapter counts as zero. Four items' operands are on their way at a time (64 rows
+// of 1024 -> 4096 with 64 adapters of rank 16: 13.3 -> 10.6 us, 8.1 with none).
 template <int NW, int RC>
 __device__ __forceinline__ void few_adapters(const Fp8Gemm& p, int w, int mine, const uint16_t* t, int n0, floatx4 acc[RC]) {
   const int lane = threadIdx.x & 63, r = lane & 15, c4 = lane >> 4, ext = p.ad.parts * p.ad.rank;
-  int item = 0;
-  each_adapter(mine, [&](int d) {
-    for (int k0 = 0; k0 < ext; k0 += 32, ++item) {
-      if (item % NW != w) continue;
-      const int k = k0 + 8 * c4;
-      const bf16x8 ft = load16<bf16x8>(t + k, mine == d && k < ext);
+  w = __builtin_amdgcn_readfirstlane(w);
+  uint64_t todo = __ballot(mine >= 0);
+  int d = -1, k0 = 0, item = -1;
+  auto advance = [&]() {  // to this wave's next item; whether there is one
+    do {
+      k0 += 32;
+      if (d < 0 || k0 >= ext) {
+        if (!todo) return false;
+        d = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+        todo &= ~__ballot(mine == d);
+        k0 = 0;
+      }
+    } while (++item % NW != w);
+    return true;
+  };
+  constexpr int AHEAD = 4;
+  bf16x8 ft[AHEAD], fb[AHEAD][RC];
+  bool more = advance();
+  while (more) {
+    bool live[AHEAD];
 #pragma unroll
-      for (int c = 0; c < RC; ++c) {
-        const int64_t row = (int64_t)d * p.N + min(n0 + 16 * c + r, p.N - 1);
-        acc[c] = mma16(load16<bf16x8>(p.ad.b + row * p.ad.rank + (k & (p.ad.rank - 1)), k < ext), ft, acc[c]);
+    for (int u = 0; u < AHEAD; ++u) {
+      live[u] = more;
+      if (more) {
+        const int k = k0 + 8 * c4;
+        const bool ok = mine == d && k < ext;
+        u32x4 v = *reinterpret_cast<const u32x4*>(t + (ok ? k : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ok ? v[e] : 0;
+        ft[u] = __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          const int64_t row = (int64_t)d * p.N + min(n0 + 16 * c + r, p.N - 1);
+          fb[u][c] = *reinterpret_cast<const bf16x8*>(p.ad.b + row * p.ad.rank + (k & (p.ad.rank - 1)));
+        }
+        more = advance();
       }
     }
-  });
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (live[u]) {
+#pragma unroll
+        for (int c = 0; c < RC; ++c) acc[c] = mma16(fb[u][c], ft[u], acc[c]);
+      }
+  }
 }
 
 // The adapters of a projection: none, with t from memory, with t formed here.
