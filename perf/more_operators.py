@@ -150,7 +150,7 @@ def _rank(case, i):
 
 def prepare(case, seed):
     g = _generator(seed)
-    s = {"case": case, "library": _library() if own else None}
+    s = {"case": case}
     rows = case["rows"]
     if case["op"] == "norm":
         d, t = case["d"], DTYPES[case["x"]]
@@ -176,7 +176,7 @@ def prepare(case, seed):
         which[torch.rand(case["requests"], device="cuda", generator=g) < 0.125] = -1
         s["which"] = which[of].to(torch.int32)
         if own:
-            m = s["library"]
+            m = _library()
             s["layer"] = m.Fp8Linear(k, n, case["bias"])
             s["layer"].load_codes(s["codes"], s["scales"], s["bias"])
             s["adapters"] = m.LowRankAdapters(k, n, na, r)
@@ -280,7 +280,7 @@ def run(state):
     c = state["case"]
     if not own:
         return {"norm": _plain_norm, "adapters": _plain_adapters, "scores": _plain_scores}[c["op"]](state)
-    m = state["library"]
+    m = _library()
     if c["op"] == "norm":
         codes = c["out"] == "codes"
         r = m.add_norm(state["x"], state["delta"], state["w"], state["b"], kind=c["kind"], eps=EPS, scale=0.5,
