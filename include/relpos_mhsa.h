@@ -580,10 +580,11 @@ int32_t mhsa_fp8_linear_forward_rounded(const mhsa_fp8_linear* linear, const uin
  *   y_r = W q(x_r) + b + s_a B_a (A_a x_r), a = which[r],
  * A_a [rank, in_dim], B_a [out_dim, rank] held in bf16, which [rows] device
  * int32; a row whose a is outside [0, n_adapters) has none. x enters A_a x
- * unrounded. The inner sums are f32, and are rounded to bf16 for a bf16 y. Up to
- * 4096 adapters of up to max_rank <= 128 each, side by side in memory that the
- * first load takes: n_adapters * (in_dim + out_dim) * 2 bytes * (max_rank rounded
- * up to 16, 32, 64 or 128). */
+ * unrounded. The inner sums are f32, and enter the second product as they are for
+ * an f32 y, off by at most 2^-15 of each for a bf16 one. Up to 4096 adapters of up
+ * to max_rank <= 128 each, side by side in memory that the first load takes:
+ * n_adapters * (in_dim + out_dim) * 2 bytes * (max_rank rounded up to 16, 32, 64 or
+ * 128). */
 int32_t mhsa_adapters_create(int32_t in_dim, int32_t out_dim, int32_t n_adapters, int32_t max_rank, mhsa_adapters** out);
 void mhsa_adapters_destroy(mhsa_adapters* adapters);
 /* Adapter `slot`: a [rank, in_dim], b [out_dim, rank] in data_dtype (MHSA_F32 /

@@ -165,16 +165,12 @@ __global__ __launch_bounds__(FEW ? 1024 : 512, 4) void adapter_rows_kernel(Adapt
     uint16_t* t = p.t + (row0 + r) * ext + 16 * j + 4 * c4;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= s;
-    if (p.parts == 1) {
-      *reinterpret_cast<u32x2*>(t) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-    } else {
-      uint32_t h[2], m[2], l[2];
-      split_pair(v[0], v[1], h[0], m[0], l[0]);
-      split_pair(v[2], v[3], h[1], m[1], l[1]);
-      *reinterpret_cast<u32x2*>(t) = u32x2{h[0], h[1]};
-      *reinterpret_cast<u32x2*>(t + p.rank) = u32x2{m[0], m[1]};
-      *reinterpret_cast<u32x2*>(t + 2 * p.rank) = u32x2{l[0], l[1]};
-    }
+    uint32_t h[2], m[2], l[2];
+    split_pair(v[0], v[1], h[0], m[0], l[0]);
+    split_pair(v[2], v[3], h[1], m[1], l[1]);
+    *reinterpret_cast<u32x2*>(t) = u32x2{h[0], h[1]};
+    *reinterpret_cast<u32x2*>(t + p.rank) = u32x2{m[0], m[1]};
+    if (p.parts == 3) *reinterpret_cast<u32x2*>(t + 2 * p.rank) = u32x2{l[0], l[1]};
   }
 }
 
@@ -223,7 +219,7 @@ hipError_t by_rank(const AdapterRows& p, hipStream_t s) {
 
 hipError_t adapter_rows(const AdapterRows& p, hipStream_t s) {
   if (p.rows <= 0 || p.rows > (int64_t)1 << 26 || p.K <= 0 || p.K > kFp8MaxK || p.n <= 0 || !p.which || !p.a || !p.scale || !p.t ||
-      (p.parts != 1 && p.parts != 3) || (!p.x && (!p.codes || !p.scales || p.q_codes)) || !p.q_codes != !p.q_scales)
+      (p.parts != 2 && p.parts != 3) || (!p.x && (!p.codes || !p.scales || p.q_codes)) || !p.q_codes != !p.q_scales)
     return hipErrorInvalidValue;
   if (!p.x) return by_rank<uint8_t>(p, s);
   return p.x_dt == kBF16 ? by_rank<bf16>(p, s) : by_rank<float>(p, s);

@@ -192,7 +192,7 @@ int32_t linear_run(const Fp8Weights& w, const LinearInput& in, int32_t rows, con
     p.ad.which = which;
     p.ad.n = ad->n;
     p.ad.rank = ad->rank;
-    p.ad.parts = od == mhsa::kBF16 ? 1 : 3;
+    p.ad.parts = od == mhsa::kBF16 ? 2 : 3;
     p.ad.a = static_cast<const uint16_t*>(ad->a.p);
     p.ad.scale = static_cast<const float*>(ad->scale.p);
     p.ad.b = static_cast<const uint16_t*>(ad->b.p);

@@ -324,13 +324,13 @@ __device__ __forceinline__ void few_inner(const Fp8Gemm& p, int w, int to, int m
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= s;
       uint32_t* out = reinterpret_cast<uint32_t*>(t + r * ext + 16 * j + 4 * c4);
-      if (p.ad.parts == 1) {
-        out[0] = pack_bf16(v[0], v[1]);
-        out[1] = pack_bf16(v[2], v[3]);
-      } else {
-        const int next = p.ad.rank / 2;
-        split_pair(v[0], v[1], out[0], out[next], out[2 * next]);
-        split_pair(v[2], v[3], out[1], out[next + 1], out[2 * next + 1]);
+      const int next = p.ad.rank / 2;
+      uint32_t l[2];
+      split_pair(v[0], v[1], out[0], out[next], l[0]);
+      split_pair(v[2], v[3], out[1], out[next + 1], l[1]);
+      if (p.ad.parts == 3) {
+        out[2 * next] = l[0];
+        out[2 * next + 1] = l[1];
       }
     }
     __syncthreads();
@@ -1301,7 +1301,7 @@ hipError_t launch_dense(const Fp8Gemm& p, hipStream_t s) {
 
 bool bad_gemm(const Fp8Gemm& p) {
   const Fp8Adapted& a = p.ad;
-  if (a.which && ((!a.t && (!a.a || !a.scale)) || !a.b || a.n <= 0 || (a.parts != 1 && a.parts != 3) || p.g.tile || p.g.idx || p.epilogue != kFp8Out ||
+  if (a.which && ((!a.t && (!a.a || !a.scale)) || !a.b || a.n <= 0 || (a.parts != 2 && a.parts != 3) || p.g.tile || p.g.idx || p.epilogue != kFp8Out ||
                   (a.rank != 16 && a.rank != 32 && a.rank != 64 && a.rank != 128)))
     return true;
   return p.N <= 0 || p.K <= 0 || !p.bias || p.K > kFp8MaxK || !p.w || !p.ws || (!p.out && p.epilogue != kFp8HiddenQ);

@@ -67,11 +67,16 @@ struct Fp8Groups {
 // Low-rank adapters beside a dense product (null `which`: none): out row r gets
 // B_a t_r, a = which[r], nothing for a outside [0, n). t_r = s_a A_a x_r comes
 // as `parts` bf16 numbers that add up to it, [rows, parts * rank], from
-// adapter_rows: one part, rounded, for a bf16 result, whose own rounding
-// is as coarse, and three, which hold f32, for an f32 one. B_a [N, rank] bf16.
+// adapter_rows. Three hold f32, for an f32 result. Two are off by 2^-15 at most,
+// 1/128 of a bf16 result's own rounding and under what the fp8 matrix unit drops
+// of the projection's sums beside them. (One, off by 2^-8, would add as much as
+// the store does: results 1.2e-3 in the 2-norm from f32 sums stored once instead of
+// 2.6e-4, which the fp8 unit's sums leave. 3000 x 1024 -> 4096, rank 32, takes
+// 29.7, 32.3 and 34.3 us with one, two and three, 15001 x 4096 -> 1024, rank 64,
+// 126, 133 and 140.) B_a [N, rank] bf16.
 struct Fp8Adapted {
   const int* which = nullptr;
-  int n = 0, rank = 0, parts = 1;  // rank 16, 32, 64 or 128
+  int n = 0, rank = 0, parts = 2;  // rank 16, 32, 64 or 128
   const uint16_t* t = nullptr;  // null: formed in the few-row kernel (fp8_few_inner) from
   const uint16_t* a = nullptr;  // A and the scales, as AdapterRows has them
   const float* scale = nullptr;
@@ -166,7 +171,7 @@ struct AdapterRows {
   const uint8_t* codes = nullptr;
   const uint8_t* scales = nullptr;
   const int* which = nullptr;
-  int n = 0, rank = 0, parts = 1;
+  int n = 0, rank = 0, parts = 2;
   const uint16_t* a = nullptr;
   const float* scale = nullptr;
   uint16_t* t = nullptr;
