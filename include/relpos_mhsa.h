@@ -669,7 +669,8 @@ int32_t mhsa_experts_forward(const mhsa_experts* experts, const void* x, int32_t
  * x, delta and sum in dtype, y in out (NULL without) in out_dtype (MHSA_F32 or
  * MHSA_BF16 each), rows a stride apart; weight and bias [dim] device f32 (NULL:
  * ones, zeros). y is taken from v before sum's rounding, all in f32, whose
- * squares are to have a sum below 2^127.
+ * squares are to have a sum below 2^127; they may be as small as they like, also
+ * with eps 0 (a row of zeros is NaN then, 0 over 0).
  * codes and scales (NULL without): y as mhsa_fp8_linear_forward would round it,
  * for mhsa_fp8_linear_forward_rounded: codes [rows, ceil(dim/128) * 128], zeros
  * past dim, scales [rows, ceil(dim/128) rounded up to 4], 127 past the last

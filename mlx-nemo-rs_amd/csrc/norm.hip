@@ -121,12 +121,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = in(i, e) ? v[i][e] - mean : 0.f;
   }
-  float q = 0.f;
+  auto squares = [&](int which) {
+    float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q = __builtin_fmaf(v[i][e], v[i][e], q);
-  const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(total(q, 1), n, p.eps));
+      for (int e = 0; e < 8; ++e) q = __builtin_fmaf(v[i][e], v[i][e], q);
+    return total(q, which);
+  };
+  float m = __builtin_fmaf(squares(1), n, p.eps);
+  if (m < 0x1p-100f) {  // (the same in all of the row's threads)
+    // Squares near f32's end lose their bits or all of themselves, and the root's
+    // instruction takes what is under 2^-126 for 0: such a row times 2^96 (its values
+    // are under 2^-42), and eps times the square of that.
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] *= 0x1p96f;
+    m = __builtin_fmaf(squares(0), n, p.eps * 0x1p96f * 0x1p96f);
+  }
+  const float r = __builtin_amdgcn_rsqf(m);
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     if constexpr (!HOLD) weights(i);
