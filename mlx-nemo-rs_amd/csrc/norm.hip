@@ -180,7 +180,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
 template <typename T, int CH, int W>
 hipError_t launch(const NormParams& p, hipStream_t s) {
   if ((int64_t)512 * CH * W < p.D) return hipErrorInvalidValue;
-  constexpr int64_t most = 1 << 22;  // rows of a launch: a grid's threads fit 32 bits
+  constexpr int64_t most = 1 << 21;  // rows of a launch: a grid's threads fit 32 bits
+  static_assert(most * 64 * W < (int64_t)1 << 32, "a wave takes a row or a part of it");
   auto behind = [](auto* q, int64_t n) { return q ? q + n : q; };
   auto rows = [&](const void* q, DType dt, int64_t n) { return const_cast<char*>(behind((const char*)q, n * (dt == kBF16 ? 2 : 4))); };
   const int64_t kb = (p.D + 127) / 128, kbp = (kb + 3) / 4 * 4;
