@@ -118,6 +118,7 @@ struct mhsa_fp8_linear {
 struct mhsa_adapters {
   int n = 0, K = 0, N = 0, rank = 0;  // rank: 16, 32, 64 or 128
   int max_rank = 0, device = -1;
+  int flag_device = -1;  // a refused first load binds the adapters to no GPU
   bool loaded = false;
   DevBuf a, b, scale, flag;
   int64_t a_stride() const { return (int64_t)rank * mhsa::fp8_kp(K); }
@@ -426,6 +427,8 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
       src[i] = stage[i].p;
     }
     int found = 0;
+    if (h->flag_device != now) h->flag.release();
+    h->flag_device = now;
     HIPCHK(h->flag.ensure(sizeof found));
     int* flag = static_cast<int*>(h->flag.p);
     HIPCHK(hipMemcpy(flag, &found, sizeof found, hipMemcpyHostToDevice));
@@ -436,13 +439,13 @@ int32_t mhsa_adapters_load(mhsa_adapters* h, int32_t slot, int32_t rank, int32_t
   }
   if (!h->loaded) {
     const int64_t na = h->n * h->a_stride() * 2, nb = h->n * h->b_stride() * 2;
+    h->device = now;  // (memory that a load takes before it fails is there)
     HIPCHK(h->a.ensure(na));
     HIPCHK(h->b.ensure(nb));
     HIPCHK(h->scale.ensure((size_t)h->n * 4));
     HIPCHK(hipMemset(h->a.p, 0, na));
     HIPCHK(hipMemset(h->b.p, 0, nb));
     HIPCHK(hipMemset(h->scale.p, 0, (size_t)h->n * 4));
-    h->device = now;
     h->loaded = true;
   }
   uint16_t* ta = static_cast<uint16_t*>(h->a.p) + slot * h->a_stride();
