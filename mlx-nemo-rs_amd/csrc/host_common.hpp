@@ -26,11 +26,15 @@ inline int32_t fail(int32_t code, const char* fmt, ...) {
   return mhsa::set_error(code, buf);
 }
 
+// (An error that is returned is taken out of the thread's last error, where the
+// next launch of anybody's would find it.)
 #define HIPCHK(expr)                                                                               \
   do {                                                                                             \
     hipError_t e_ = (expr);                                                                        \
-    if (e_ != hipSuccess) return fail(MHSA_EHIP, "%s: %s (%s:%d)", #expr, hipGetErrorString(e_), \
-                                      __FILE__, __LINE__);                                         \
+    if (e_ != hipSuccess) {                                                                        \
+      (void)hipGetLastError();                                                                     \
+      return fail(MHSA_EHIP, "%s: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); \
+    }                                                                                              \
   } while (0)
 
 inline float bits_to_f32(uint32_t u) {
