@@ -89,11 +89,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void add_norm_kernel(NormPar
   if (HOLD && p.delta) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) td[i].load(d, col(i), p.D);
-  } else {
+  } else {  // (negative zeros, which leave a negative zero of x what it is)
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
-      for (int e = 0; e < Run<T, FORM>::N; ++e) td[i].u[e] = 0;
+      for (int e = 0; e < Run<T, FORM>::N; ++e) td[i].u[e] = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
   }
   float v[CH][8];
 #pragma unroll
@@ -188,6 +188,7 @@ hipError_t launch(const NormParams& p, hipStream_t s) {
   for (int64_t r = 0; r < p.rows; r += most) {
     NormParams q = p;
     q.rows = std::min(most, p.rows - r);
+    if (!p.delta) q.scale = 1.f;
     q.x = rows(p.x, p.dt, r * p.ldx);
     q.delta = rows(p.delta, p.dt, r * p.ldd);
     q.sum = rows(p.sum, p.dt, r * p.lds);
