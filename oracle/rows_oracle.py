@@ -49,7 +49,7 @@ def scores(logits, tokens, top_k, temperature=1.0):
     under p, its square's, log sum)."""
     x = np.asarray(logits, np.float64)
     rows, v = x.shape
-    t = np.float64(np.float32(1.0) / np.float32(temperature))
+    t = 1.0 / np.float64(np.float32(temperature))
     lp = np.zeros(tokens.shape)
     h, idx, top = np.zeros(rows), np.full((rows, top_k), -1, np.int32), np.full((rows, top_k), -np.inf)
     sizes = np.zeros((rows, 3))
