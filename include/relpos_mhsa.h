@@ -581,7 +581,8 @@ int32_t mhsa_fp8_linear_forward_rounded(const mhsa_fp8_linear* linear, const uin
  * A_a [rank, in_dim], B_a [out_dim, rank] held in bf16, which [rows] device
  * int32; a row whose a is outside [0, n_adapters) has none. x enters A_a x
  * unrounded. The inner sums are f32, and enter the second product as they are for
- * an f32 y, off by at most 2^-15 of each for a bf16 one. Up to 4096 adapters of up
+ * an f32 y, off by at most 2^-15 of each for a bf16 one; a result's last bits
+ * depend on its row's place and on the number of rows. Up to 4096 adapters of up
  * to max_rank <= 128 each, side by side in memory that the first load takes:
  * n_adapters * (in_dim + out_dim) * 2 bytes * (max_rank rounded up to 16, 32, 64 or
  * 128). */
@@ -590,8 +591,9 @@ void mhsa_adapters_destroy(mhsa_adapters* adapters);
 /* Adapter `slot`: a [rank, in_dim], b [out_dim, rank] in data_dtype (MHSA_F32 /
  * MHSA_BF16 / MHSA_F16; host or device memory), finite after their rounding to
  * bf16; rank 0 (a and b NULL) empties the slot, as all are before their first
- * load. Waits for the GPU; no other call on the adapters may run at the same
- * time, of other slots either. A refused load leaves the slot as it was. */
+ * load (a call with adapters before any load at all is refused). Waits for the
+ * GPU; no other call on the adapters may run at the same time, of other slots
+ * either. A refused load leaves the slot as it was. */
 int32_t mhsa_adapters_load(mhsa_adapters* adapters, int32_t slot, int32_t rank, int32_t data_dtype, const void* a,
                            const void* b, float scale);
 /* Workspace bytes of a call with adapters of `rows` rows or fewer, on floats or
@@ -693,7 +695,10 @@ int32_t mhsa_add_norm(const void* x, int32_t dtype, int32_t rows, int32_t dim, i
  *     logits, largest first, ties to the lower index, and their log p. Logits of
  *     -inf and NaN are not among them: where fewer are left, -1 and -inf.
  * A row whose logits are all -inf has log_probs -inf and entropy 0; a row that
- * holds a NaN or +inf has NaN for both and for its alternatives' log p. All in f32.
+ * holds a NaN or +inf has NaN for both and for its alternatives' log p. All in f32:
+ * log p is -inf where a logit's distance from the largest, over temperature, is no
+ * f32 (for temperatures below 1 that of the type's lowest value as a mask). The last
+ * bits of log_probs and entropy over 8192 tokens or more depend on the number of rows.
  * vocab <= 2^24, top_k <= 32, n_tokens <= 1024, both may be 0, as may rows.
  * Results and the workspace overlap nothing. */
 int32_t mhsa_token_log_probs(const void* logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t stride,

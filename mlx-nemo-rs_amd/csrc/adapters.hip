@@ -26,6 +26,10 @@
 // of 37, 256 rows with 64 of rank 64 30 instead of 53, 1000 rows of 1024 -> 1024 f32
 // with 10 14.1 instead of 15.4; 3000 rows of 1024 -> 4096 would take 31.2 instead of
 // 30.0, for A is read four times as often.
+//
+// The sums' order, and with it t's last bits, go by the row's place in the call and
+// by the number of rows: which block a workgroup begins with, and how many waves it
+// has.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,6 +40,8 @@
 namespace mhsa {
 namespace {
 
+// Registers for 4 waves a SIMD: at rank 128 f32 rows have 16 to 20 bytes a lane in
+// scratch.
 template <typename TX, int RT, RowForm FORM, bool FEW>
 __global__ __launch_bounds__(FEW ? 1024 : 512, 4) void adapter_rows_kernel(AdapterRows p) {
   constexpr int NW = FEW ? 16 : 8, ROWS = FEW ? 4 : 16;

@@ -144,26 +144,26 @@ __device__ __forceinline__ void few_block(const uint8_t* wrow, const int off[RC]
       s = xsc[b];
     }
   } else {
-  float v[32];
+    float v[32];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (VEC) {
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VEC) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 * i + e] = 0.f;
-      if (c0 + 8 * i < K) load_run(xrow + c0 + 8 * i, v + 8 * i);
-    } else {
-      load8(xrow, c0 + 8 * i, K, v + 8 * i);
+        for (int e = 0; e < 8; ++e) v[8 * i + e] = 0.f;
+        if (c0 + 8 * i < K) load_run(xrow + c0 + 8 * i, v + 8 * i);
+      } else {
+        load8(xrow, c0 + 8 * i, K, v + 8 * i);
+      }
     }
-  }
-  float m = 0.f;
+    float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) m = fmaxf(m, fp8_mag(v[i]));
-  m = fmaxf(m, __shfl_xor(m, 16, 64));
-  m = fmaxf(m, __shfl_xor(m, 32, 64));
-  s = fp8_scale_byte(m);
-  const float scale = fp8_scale(s);
+    for (int i = 0; i < 32; ++i) m = fmaxf(m, fp8_mag(v[i]));
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    s = fp8_scale_byte(m);
+    const float scale = fp8_scale(s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = (int)fp8_pack4_scaled(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
+    for (int i = 0; i < 8; ++i) q[i] = (int)fp8_pack4_scaled(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], scale);
   }
 #pragma unroll
   for (int c = 0; c < RC; ++c) {
@@ -395,6 +395,7 @@ __device__ __forceinline__ void few_adapters(const Fp8Gemm& p, int w, int mine, 
 // The adapters of a projection: none, with t from memory, with t formed here.
 enum FewAdd { kFewPlain = 0, kFewAdd, kFewInner };
 
+// (With t formed here, f32 rows and 16 waves, 8 bytes a lane are in scratch.)
 template <typename TX, int NW, int RC, bool EXACT, bool VEC, int ADD>
 __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(Fp8Gemm p) {
   __shared__ __attribute__((aligned(16))) float red[NW][RC][16][20];

@@ -103,7 +103,8 @@ extern "C" int32_t mhsa_token_log_probs(const void* logits, int32_t dtype, int32
   if (!act_dtype(dtype, &p.dt)) return fail(MHSA_ENOTSUP, "dtype %d not supported (f32, bf16)", dtype);
   if (rows < 0 || vocab <= 0) return fail(MHSA_EINVAL, "bad shape: %d rows of %d", rows, vocab);
   if (vocab > mhsa::kScoresMaxV) return fail(MHSA_ENOTSUP, "a vocabulary of %d exceeds %d", vocab, mhsa::kScoresMaxV);
-  // (0.01: the largest logit's distance from the lowest, over it, is a float)
+  // (down to 0.01 distances of up to 2^120, times log2 e / T, are floats; farther ones
+  // are infinite there, and their exponential 0 all the same)
   if (!(temperature >= 0.01f) || !(temperature <= 100.f)) return fail(MHSA_EINVAL, "temperature is to be in [0.01, 100]");
   if (top_k < 0 || top_k > vocab) return fail(MHSA_EINVAL, "top_k %d is not in [0, %d]", top_k, vocab);
   if (top_k > mhsa::kScoresMaxK) return fail(MHSA_ENOTSUP, "top_k %d exceeds %d", top_k, mhsa::kScoresMaxK);

@@ -40,8 +40,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kLoads = 4;  // of 16 bytes, of a lane and chunk
 
-template <typename T> constexpr int kPer = 16 / (int)sizeof(T);      // values of a load
-template <typename T> constexpr int kChunk = 64 * kLoads * kPer<T>;  // values of a wave's chunk
+template <typename T> constexpr int kPer = 16 / (int)sizeof(T);  // values of a load
 
 // The order of floats as that of unsigned integers; -0 counts as 0.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -338,7 +337,8 @@ __device__ __forceinline__ uint64_t lanes_border(float top, int k) {
   return t > ordered(-__builtin_inff()) ? (uint64_t)t << 32 | kAnyIndex : 0;
 }
 
-// Rows of L loads to a lane, a wave to each.
+// Rows of L loads to a lane, a wave to each. (bf16 rows of 6 to 8 loads take 132 to
+// 172 registers, values unpacked, and run 3 and 2 waves a SIMD.)
 template <typename T, int L>
 __global__ __launch_bounds__(256) void scores_small_kernel(ScoresParams p) {
   __shared__ uint64_t lists[4][kList];
@@ -581,10 +581,12 @@ hipError_t go(const ScoresParams& p, hipStream_t s) {
     join_kernel<T><<<(unsigned)p.rows, 64, 0, s>>>(p, parts);
     return hipGetLastError();
   }
-  // Waves by the vocabulary alone, so that a row's bits do not depend on how many
-  // rows come with it: two up to 32 loads a lane, four beyond. 30000 rows of 5000
-  // bf16, 20 best, took 132 us with two waves, 172 with four, 407 with eight; 4001
-  // of 50001 f32, 5 best, 154, 145 and 144; 771 of 20000 f32, 20 best, 28, 21, 27.
+  // Waves by the vocabulary alone: two up to 32 loads a lane, four beyond. 30000
+  // rows of 5000 bf16, 20 best, took 132 us with two waves, 172 with four, 407 with
+  // eight; 4001 of 50001 f32, 5 best, 154, 145 and 144; 771 of 20000 f32, 20 best,
+  // 28, 21, 27. Rows that are not cut into parts so have the same bits however many
+  // come with them; those of fewer than 2 to a CU, of 8192 values or more, are summed
+  // in as many parts as their number gives.
   constexpr int64_t most = 1 << 22;  // rows of a launch: a grid's threads fit 32 bits
   for (int64_t r = 0; r < p.rows; r += most) {
     ScoresParams q = p;
