@@ -745,6 +745,8 @@ class LowRankAdapters:
     def __init__(self, in_dim: int, out_dim: int, n_adapters: int, max_rank: int):
         lib = library()
         h = ctypes.c_void_p()
+        if max(in_dim, out_dim, n_adapters, max_rank) > 0x7FFFFFFF:  # (an int32 would be cut off)
+            raise MhsaError(MHSA_ENOTSUP, f"adapters of {in_dim} -> {out_dim}, {n_adapters} of rank {max_rank}")
         _check(lib.mhsa_adapters_create(in_dim, out_dim, n_adapters, max_rank, ctypes.byref(h)))
         self._h, self._lib = h, lib
         self.in_dim, self.out_dim, self.n_adapters, self.max_rank = in_dim, out_dim, n_adapters, max_rank
@@ -755,20 +757,26 @@ class LowRankAdapters:
             self._lib.mhsa_adapters_destroy(h)
             self._h = None
 
+    def _check_slot(self, slot) -> None:
+        if not isinstance(slot, (int, np.integer)) or not 0 <= slot < self.n_adapters:
+            raise MhsaError(MHSA_EINVAL, f"slot {slot} is not in [0, {self.n_adapters})")
+
     def load(self, slot: int, a, b, scale: float = 1.0) -> None:
         """a [rank, in] and b [out, rank] of one dtype (float32, bfloat16 or
         float16), finite; rank <= max_rank."""
+        self._check_slot(slot)
         rank = a.shape[0] if getattr(a, "ndim", 0) == 2 else 0
         if rank == 0:
             raise MhsaError(MHSA_EINVAL, f"a: expected [rank, {self.in_dim}]")
         keep, ptrs, dtype = _load_floats([((a, (rank, self.in_dim), "a"), (b, (self.out_dim, rank), "b"))])
         if ptrs[1] is None:
             raise MhsaError(MHSA_EINVAL, f"b: expected [{self.out_dim}, {rank}]")
-        _check(self._lib.mhsa_adapters_load(self._h, slot, rank, dtype, *ptrs, float(scale)))
+        _check(self._lib.mhsa_adapters_load(self._h, int(slot), rank, dtype, *ptrs, float(scale)))
 
     def clear(self, slot: int) -> None:
         """Empties a slot: its rows get the projection alone."""
-        _check(self._lib.mhsa_adapters_load(self._h, slot, 0, F32, None, None, 0.0))
+        self._check_slot(slot)
+        _check(self._lib.mhsa_adapters_load(self._h, int(slot), 0, F32, None, None, 0.0))
 
 
 ROUTE_SCORES = {"softmax": 0, "sigmoid": 1}
@@ -887,6 +895,8 @@ class Fp8Rows:
         """Raises unless codes and scales are as said (those that a caller has
         put together)."""
         torch = _torch()
+        if not self.shape or not all(isinstance(n, int) and n >= 0 for n in self.shape):
+            raise MhsaError(MHSA_EINVAL, f"shape {self.shape}: expected [..., width]")
         rows, kb = int(np.prod(self.shape[:-1], dtype=np.int64)), _blocks(self.shape[-1])
         for t, n, name in ((self.codes, kb * 128, "codes"), (self.scales, (kb + 3) // 4 * 4, "scales")):
             if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous()
