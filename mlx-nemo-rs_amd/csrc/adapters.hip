@@ -23,9 +23,9 @@
 // Up to 4 rows a CU are 4 to a workgroup, of 16 waves: there a wave's blocks and the
 // adapters of its rows, one behind the other, are what the launch lasts. With the
 // projection 16 rows of 4096 -> 1024 with 16 adapters of rank 16 take 18 us instead
-// of 37, 256 rows with 64 of rank 64 30 instead of 53, 1000 rows of 1024 -> 1024 f32
-// with 10 14.1 instead of 15.4; 3000 rows of 1024 -> 4096 would take 31.2 instead of
-// 30.0, for A is read four times as often.
+// of 37, 256 rows with 64 of rank 64 37 instead of 60, 1000 rows of 1024 -> 1024 f32
+// with 10 14.0 instead of 15.3; 3000 rows of 1024 -> 4096, rank 32, would take 32.2
+// instead of 30.7, for A is read four times as often.
 //
 // The sums' order, and with it t's last bits, go by the row's place in the call and
 // by the number of rows: which block a workgroup begins with, and how many waves it

@@ -341,7 +341,8 @@ __device__ __forceinline__ void few_inner(const Fp8Gemm& p, int w, int to, int m
 // columns from n0 on to acc, as few_block its block's. The distinct adapters of
 // the 16 rows, 32 ranks at a time, are shared out to the waves; a row of another
 // adapter counts as zero. Four items' operands are on their way at a time (64 rows
-// of 1024 -> 4096 with 64 adapters of rank 16: 13.3 -> 10.6 us, 8.1 with none).
+// of 1024 -> 4096 with 64 adapters of rank 16: this launch 13.3 -> 10.6 us, 8.1 where
+// no row has one).
 template <int NW, int RC>
 __device__ __forceinline__ void few_adapters(const Fp8Gemm& p, int w, int mine, const uint16_t* t, int n0, floatx4 acc[RC]) {
   const int lane = threadIdx.x & 63, r = lane & 15, c4 = lane >> 4, ext = p.ad.parts * p.ad.rank;
@@ -937,9 +938,10 @@ __device__ __forceinline__ void fp8_tile_body(const Fp8Gemm& p, char* smem) {
   // of the wave's rows one by one, 16 ranks at a time, the next ones' operands on
   // their way meanwhile. A row of another adapter counts as zero (its offset
   // lies past the buffer's end; branches around the MFMAs would have the sums
-  // copied from register to register: 15001 x 4096 -> 1024 with rank 64 124 us,
-  // 67 so, and 60 without adapters). Rows' adapters looked up a tile ahead, or two
-  // steps ahead of the ring's loads, gained nothing.
+  // copied from register to register: 15001 x 4096 -> 1024 with rank 64 and one bf16
+  // number to an inner sum 124 us, 67 so, and 60 without adapters; with two numbers
+  // 75). Rows' adapters looked up a tile ahead, or two steps ahead of the ring's
+  // loads, gained nothing.
   auto adapters = [&](const Tile& t) {
     const int ext = p.ad.parts * p.ad.rank;
     const auto rt = rsrc(reinterpret_cast<const uint8_t*>(p.ad.t + (int64_t)t.m0 * ext), (uint32_t)(t.rows * ext * 2));
